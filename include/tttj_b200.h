@@ -39,6 +39,7 @@ extern "C" {
 
 #define TTTJ_DTYPE_F16 0
 #define TTTJ_DTYPE_F32 1
+#define TTTJ_DTYPE_BF16 2 /* serving operators only */
 
 /* Mirrors TransformerConfig (benchmarks/torch_transformer_benchmark.py:29-56). */
 typedef struct tttj_config {
@@ -312,6 +313,88 @@ int tttj_attention(const void* qkv, void* ctx, int qkv_rows, const uint8_t* vali
 int tttj_attention_noalloc(const void* qkv, void* ctx, int qkv_rows, const uint8_t* valid_mask,
                            int batch, int seq_len, int d_model, int num_heads, int causal,
                            void* stream);
+
+/* ---- serving operators: packed prompts, a paged key/value cache ----
+ *
+ * Causal attention with grouped heads (heads = kv_heads x group, query head h reads
+ * key/value head h / group) for prompts, and for chunks of new tokens or single tokens
+ * over a cache, with what keeps such a cache: append, the attention mass that each slot
+ * gathers, eviction.  No counterpart in the reference (it runs whole sequences only).
+ *
+ * fp16 or bf16 (TTTJ_DTYPE_F16 / TTTJ_DTYPE_BF16) in and out, fp32 products, softmax
+ * statistics and masses.  head_dim 32, 64, 128 or 256; group 1 .. 64; at most 2048
+ * sequences.  Rows are given by element strides, head_dim contiguous, all strides
+ * positive multiples of 8, pointers 16-byte aligned; tokens x heads < 2^31.
+ *
+ * Tokens of all sequences are packed: those of sequence b are rows seq_offsets[b] ..
+ * seq_offsets[b+1].  Rows behind the last sequence are left as they were, so a batch may
+ * be padded.  In a cache, cache_lens[b] counts the tokens of sequence b with the new ones
+ * included: new token i of n is at slot len - n + i and sees the slots up to its own.  A
+ * row that sees no key (len < n) gets output 0 and log-sum-exp -inf.  Offsets, lengths
+ * and page numbers are device memory that no entry point reads on the host, so a call
+ * can be captured into a CUDA graph and replayed with new ones.  They are bounds-checked
+ * on the device: offsets and lengths are clamped to the call's tensors, an entry of the
+ * page table outside the cache stands for a page of zeros (nothing is written to it),
+ * and `status` (nullable) records TTTJ_DEV_BAD_LENS / TTTJ_DEV_BAD_PAGE.  Infinite or NaN
+ * values reach only rows that see them. */
+typedef struct tttj_rows { /* [tokens][heads][head_dim] */
+  const void* data;
+  int64_t token_stride, head_stride;
+} tttj_rows;
+typedef struct tttj_pages { /* [num_pages][page_size][kv_heads][head_dim], any stride order */
+  void* data;
+  int64_t page_stride, slot_stride, head_stride;
+} tttj_pages;
+typedef struct tttj_seqs {
+  const int32_t* seq_offsets; /* device [batch + 1] */
+  const int32_t* cache_lens;  /* device [batch]; NULL without a cache */
+  const int32_t* page_table;  /* device [batch][table_stride], pages_per_seq used; NULL without a cache */
+  int64_t table_stride;
+  int32_t batch, tokens;      /* sequences; rows allocated in q and out */
+  int32_t pages_per_seq, page_size, num_pages; /* page_size 16, 32, 64, 128 or 256 */
+  int32_t dtype, heads, kv_heads, head_dim;
+  int32_t* status;            /* device status word, nullable */
+} tttj_seqs;
+#define TTTJ_DEV_BAD_PAGE 0x401    /* status: a live page-table entry is outside the cache */
+#define TTTJ_DEV_BAD_LENS 0x402    /* status: lengths or offsets outside the call's tensors */
+#define TTTJ_DEV_SERVE_TIMEOUT 0x403 /* status: a bounded device wait gave up */
+
+/* out = softmax(scale q k^T) v inside every sequence (causal: token i sees tokens <= i),
+ * lse (nullable) [tokens][heads] = log sum exp of the scaled scores.  The workspace
+ * (tttj_serve_workspace_bytes with cache_lens = NULL; 256-byte aligned, any contents) must
+ * not be shared by calls that may overlap. */
+size_t tttj_serve_workspace_bytes(const tttj_seqs* s);
+int tttj_prompt_attention(const tttj_seqs* s, const tttj_rows* q, const tttj_rows* k,
+                          const tttj_rows* v, const tttj_rows* out, float* lse, int causal,
+                          float scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The same for new tokens over the cache (their own keys and values appended before).
+ * max_new: an upper bound of the new tokens of any sequence if the caller knows one (it
+ * only picks kernels; longer sequences are still computed), else 0. */
+int tttj_cache_attention(const tttj_seqs* s, const tttj_rows* q, const tttj_pages* k_cache,
+                         const tttj_pages* v_cache, const tttj_rows* out, float* lse, int max_new,
+                         float scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Write the new tokens' keys and values to their slots.  With positions / mass (nullable,
+ * [batch][kv_heads][pages_per_seq * page_size], contiguous) a new slot's position becomes
+ * seen[b] - n + i (seen: tokens the sequence has had, new ones included; NULL =
+ * cache_lens, which differ once tokens were evicted) and its mass 0. */
+int tttj_cache_append(const tttj_seqs* s, const tttj_rows* k, const tttj_rows* v,
+                      const tttj_pages* k_cache, const tttj_pages* v_cache, int32_t* positions,
+                      float* mass, const int32_t* seen, void* stream);
+
+/* Evict down to `keep` slots per sequence and key/value head.  A slot's value is its mass
+ * (NaN counts as -inf), +inf for positions within `recent` of the head's newest; the
+ * `keep` largest stay, equal ones by lower slot.  Slots that stay behind the budget move
+ * into the freed ones in front, the i-th into the i-th; the others keep their place.
+ * Written: mass_out, positions_out (0 and -1 behind the new length; may not alias the
+ * inputs), lens_out = min(len, keep), and the moved rows of the caches.  The sequence's
+ * pages must be its own.  Workspace: tttj_cache_evict_workspace_bytes. */
+size_t tttj_cache_evict_workspace_bytes(const tttj_seqs* s, int keep);
+int tttj_cache_evict(const tttj_seqs* s, const tttj_pages* k_cache, const tttj_pages* v_cache,
+                     const float* mass, const int32_t* positions, int keep, int recent,
+                     float* mass_out, int32_t* positions_out, int32_t* lens_out, void* workspace,
+                     size_t workspace_bytes, void* stream);
 
 /* Failure-detection self test: launches a kernel whose bounded wait on an mbarrier
  * that is never signalled gives up after limit_ns and writes 0x1ff into *status_dev.

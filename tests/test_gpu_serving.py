@@ -1,0 +1,452 @@
+"""GPU: the serving operators against their 64-bit definitions (serving_reference.py).
+
+Tolerances.  With u half a step of the type (2^-11 fp16, 2^-8 bf16), one output element is
+off by at most u A for the rounding of the probabilities (A = sum p |v|), u |o| for the store,
+2 ds A for scores that are off by ds, and a few fp32 roundings (2^-18 A covers the sums and
+the exponentials' 2^-22); fp16 probabilities under 2^-14 round absolutely, by 2^-25 each.
+ds: an fp32 sum of d products is off by at most d 2^-24 sum |q k| scale.  The log-sum-exp is
+off by ds and a few roundings of its own size."""
+import math
+
+import pytest
+import torch
+
+from serving_reference import (attention_block, attention_rows, cache_rows, evict_choice,
+                               lengths_to_offsets)
+from tttj_2026_b200 import ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+TYPES = [torch.float16, torch.bfloat16]
+
+
+def _gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def _check(out, lse, q, k, v, n, length, scale, causal=True, rows=False):
+    """One sequence: out / lse [n, H, ...] of its last n of `length` tokens."""
+    f = attention_rows if rows else attention_block
+    ref, ref_lse = f(q, k, v, n, length, scale, causal)
+    d, u = q.shape[2], torch.finfo(q.dtype).eps / 2
+    g = q.shape[1] // k.shape[1]
+    qn = torch.nan_to_num(q.double().abs()).amax((0, 1)) if n else torch.zeros(d, device=DEV, dtype=torch.float64)
+    kn = torch.nan_to_num(k.double().abs(), posinf=0).amax((0, 1))
+    ds = d * 2.0**-24 * float((qn * kn).sum()) * scale
+    vabs = torch.nan_to_num(v.double().abs(), posinf=0)
+    a, _ = f(q, torch.nan_to_num(k, posinf=0, neginf=0), vabs.to(v.dtype), n, length, scale, causal)
+    tol = (u + 2 * ds + 2.0**-18) * a + u * ref.abs() + (2.0**-25 * (1 + vabs.sum(0)).repeat_interleave(g, 0)
+                                                          if q.dtype == torch.float16 else 0)
+    fin = torch.isfinite(ref)
+    assert torch.equal(torch.isnan(out.double()), torch.isnan(ref))
+    assert torch.equal(torch.isposinf(out.double()), torch.isposinf(ref))
+    assert torch.equal(torch.isneginf(out.double()), torch.isneginf(ref))
+    err = (out.double() - ref).abs()
+    assert bool((err <= tol)[fin].all()), f"out: {float((err / tol)[fin].max()):.2f} times the tolerance"
+    lfin = torch.isfinite(ref_lse)
+    assert torch.equal(torch.isneginf(lse.double()), torch.isneginf(ref_lse))
+    lerr = (lse.double() - ref_lse).abs()[lfin]
+    ltol = (ds + 2.0**-20 * (1 + ref_lse.abs()))[lfin]
+    assert bool((lerr <= ltol).all()), f"lse: {float((lerr / ltol).max()):.2f} times the tolerance"
+
+
+# ------------------------------------------------------------------------------- prompts
+def _prompt(lens, heads, kv, d, dtype, seed, spread=1.5):
+    t = sum(lens)
+    qkv = torch.randn(t, (heads + 2 * kv) * d, device=DEV, generator=_gen(seed)).to(dtype)
+    q, k, v = qkv.split((heads * d, kv * d, kv * d), 1)
+    q.mul_(spread)
+    return q.view(t, heads, d), k.view(t, kv, d), v.view(t, kv, d)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [32, 64, 128, 256])
+@pytest.mark.parametrize("heads,kv", [(2, 2), (6, 2), (8, 1), (5, 1)])
+@pytest.mark.parametrize("lens", [[1], [77, 0, 200, 1, 129], [513, 2, 255]])
+def test_prompt_attention(dtype, d, heads, kv, lens):
+    q, k, v = _prompt(lens, heads, kv, d, dtype, sum(lens) + d)
+    off = lengths_to_offsets(lens)
+    for causal in (True, False):
+        out, lse = ops.prompt_attention(q, k, v, off, causal=causal, return_lse=True)
+        at = 0
+        for n in lens:
+            s = slice(at, at + n)
+            if n:
+                _check(out[s], lse[s], q[s], k[s], v[s], n, n, d**-0.5, causal)
+            at += n
+
+
+@pytest.mark.parametrize("group", [7, 16, 33, 64])
+def test_prompt_attention_wide_groups(group):
+    lens = [3, 150, 40]
+    q, k, v = _prompt(lens, 2 * group, 2, 64, torch.float16, group)
+    out, lse = ops.prompt_attention(q, k, v, lengths_to_offsets(lens), return_lse=True, scale=0.2)
+    at = 0
+    for n in lens:
+        s = slice(at, at + n)
+        _check(out[s], lse[s], q[s], k[s], v[s], n, n, 0.2)
+        at += n
+
+
+def test_prompt_attention_long_and_sharp():
+    """A long prompt whose scores reach far: running maxima that keep growing."""
+    q, k, v = _prompt([2500], 4, 2, 128, torch.bfloat16, 5, spread=8.0)
+    k.mul_(torch.linspace(0.2, 2, 2500, device=DEV)[:, None, None])
+    out, lse = ops.prompt_attention(q, k, v, lengths_to_offsets([2500]), return_lse=True)
+    _check(out, lse, q, k, v, 2500, 2500, 128**-0.5)
+
+
+def test_prompt_attention_rows_behind_the_last_sequence_stay():
+    q, k, v = _prompt([40, 30, 58], 4, 2, 64, torch.float16, 3)
+    k[70:], v[70:], q[70:] = math.nan, math.inf, math.nan
+    out = torch.full((128, 4, 64), 7.0, dtype=torch.float16, device=DEV)
+    got = ops.prompt_attention(q, k, v, lengths_to_offsets([40, 30]), out=out)
+    assert got is out
+    assert bool((out[70:] == 7).all())
+    for s in (slice(0, 40), slice(40, 70)):
+        ref, _ = attention_block(q[s], k[s], v[s], s.stop - s.start, s.stop - s.start, 64**-0.5)
+        assert float((out[s].double() - ref).abs().max()) < 0.01
+
+
+def test_prompt_attention_strided_rows():
+    base = torch.randn(90, 3, 5, 96, device=DEV, generator=_gen(1)).half()
+    q, k, v = base[:, 0, :4, 8:72], base[:, 1, 1:3, 16:80], base[:, 2, ::2, 32:][:, :2]
+    big = torch.zeros(90, 8, 72, dtype=torch.float16, device=DEV)
+    out = ops.prompt_attention(q, k, v, lengths_to_offsets([33, 57]), out=big[:, ::2, 8:])
+    for s in (slice(0, 33), slice(33, 90)):
+        n = s.stop - s.start
+        lse = attention_block(q[s], k[s], v[s], n, n, 0.125)[1]
+        _check(out[s], lse, q[s], k[s], v[s], n, n, 0.125)
+    assert bool((big[:, 1::2] == 0).all()) and bool((big[:, :, :8] == 0).all())
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_prompt_attention_nonfinite_values_reach_only_rows_that_see_them(d, dtype):
+    lens = [140, 9, 300]
+    q, k, v = _prompt(lens, 4, 2, d, dtype, 11)
+    v[37, 0, 3], v[100, 1, 5], v[101, 1, 5] = math.nan, math.inf, -math.inf
+    v[145, 0, 0] = -math.inf
+    k[148, 1] = math.nan  # the last token of the second sequence: only its own row sees it
+    v[149 + 200, 1, d - 1] = math.inf
+    out, lse = ops.prompt_attention(q, k, v, lengths_to_offsets(lens), return_lse=True)
+    at = 0
+    for n in lens:
+        s = slice(at, at + n)
+        _check(out[s], lse[s], q[s], k[s], v[s], n, n, d**-0.5, rows=True)
+        at += n
+
+
+# -------------------------------------------------------------------------- paged cache
+class Cache:
+    def __init__(self, lens, kv, d, page, dtype, seed, spare=5, heads_first=False, extra_pages=0):
+        b = len(lens)
+        self.per = max(1, -(-max(lens) // page)) + extra_pages
+        pages = b * self.per + spare
+        shape = (pages, kv, page, d) if heads_first else (pages, page, kv, d)
+        g = _gen(seed)
+        self.k = torch.full(shape, math.nan, dtype=dtype, device=DEV)
+        self.v = torch.full(shape, math.inf, dtype=dtype, device=DEV)
+        if heads_first:
+            self.k, self.v = self.k.transpose(1, 2), self.v.transpose(1, 2)
+        order = torch.randperm(pages, generator=g, device=DEV)[: b * self.per]
+        self.table = order.to(torch.int32).view(b, self.per).contiguous()
+        self.lens = torch.tensor(lens, dtype=torch.int32, device=DEV)
+        for i, n in enumerate(lens):  # only live slots hold finite values
+            j = torch.arange(n, device=DEV)
+            at = self.table[i].long()[j // page]
+            self.k[at, j % page] = torch.randn(n, kv, d, device=DEV, generator=g).to(dtype)
+            self.v[at, j % page] = torch.randn(n, kv, d, device=DEV, generator=g).to(dtype)
+
+
+def _check_cache(out, lse, q, c, new, lens, scale, rows=False):
+    at = 0
+    for b, (n, m) in enumerate(zip(new, lens)):
+        if n:
+            s = slice(at, at + n)
+            if m == 0:
+                assert bool((out[s] == 0).all()) and bool(torch.isneginf(lse[s]).all())
+            else:
+                _check(out[s], lse[s], q[s], cache_rows(c.k, c.table, b, m), cache_rows(c.v, c.table, b, m), n, m,
+                       scale, rows=rows or m < n)
+        at += n
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [32, 64, 128, 256])
+@pytest.mark.parametrize("page", [16, 64, 256])
+@pytest.mark.parametrize("heads,kv", [(8, 2), (3, 3), (10, 2)])
+def test_cache_attention_single_tokens(dtype, d, page, heads, kv):
+    lens = [1, 15, 16, 17, 63, 64, 65, 300, 129, 1000]
+    c = Cache(lens, kv, d, page, dtype, d + page)
+    q = (1.5 * torch.randn(len(lens), heads, d, device=DEV, generator=_gen(2))).to(dtype)
+    new = [1] * len(lens)
+    out, lse = ops.cache_attention(q, c.k, c.v, c.table, lengths_to_offsets(new), c.lens, max_new=1, return_lse=True)
+    _check_cache(out, lse, q, c, new, lens, d**-0.5)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [32, 64, 128, 256])
+@pytest.mark.parametrize("heads,kv,page", [(8, 2, 16), (3, 3, 32), (10, 2, 128), (16, 1, 64)])
+def test_cache_attention_chunks(dtype, d, heads, kv, page):
+    new = [5, 0, 1, 130, 33, 64]
+    lens = [5, 40, 700, 130, 500, 257]
+    c = Cache(lens, kv, d, page, dtype, d + page)
+    q = (1.5 * torch.randn(sum(new), heads, d, device=DEV, generator=_gen(2))).to(dtype)
+    for hint in (None, max(new), 1):
+        out, lse = ops.cache_attention(q, c.k, c.v, c.table, lengths_to_offsets(new), c.lens, max_new=hint,
+                                       return_lse=True)
+        _check_cache(out, lse, q, c, new, lens, d**-0.5)
+
+
+@pytest.mark.parametrize("new", [1, 3, 200])
+def test_cache_attention_long_axis_is_split(new):
+    """One sequence, many keys: the work of its few rows is shared between CTAs and joined."""
+    lens = [20011]
+    c = Cache(lens, 2, 128, 64, torch.bfloat16, 4)
+    q = (2 * torch.randn(new, 8, 128, device=DEV, generator=_gen(5))).bfloat16()
+    args = (q, c.k, c.v, c.table, lengths_to_offsets([new]), c.lens)
+    out, lse = ops.cache_attention(*args, max_new=new, return_lse=True)
+    _check_cache(out, lse, q, c, [new], lens, 128**-0.5)
+    again = ops.cache_attention(*args, max_new=new)
+    assert torch.equal(out, again)  # joined in a fixed order
+
+
+def test_cache_attention_heads_first_pages():
+    new, lens = [1, 40, 1], [90, 333, 64]
+    c = Cache(lens, 3, 64, 32, torch.float16, 8, heads_first=True)
+    q = torch.randn(sum(new), 6, 64, device=DEV, generator=_gen(5)).half()
+    out, lse = ops.cache_attention(q, c.k, c.v, c.table, lengths_to_offsets(new), c.lens, return_lse=True)
+    _check_cache(out, lse, q, c, new, lens, 0.125)
+
+
+def test_cache_attention_rows_that_see_nothing():
+    """More new tokens than cached ones: the first of them see no key; an empty cache."""
+    new, lens = [4, 3, 70], [2, 0, 69]
+    c = Cache(lens, 2, 64, 16, torch.float16, 8)
+    q = torch.randn(sum(new), 4, 64, device=DEV, generator=_gen(5)).half()
+    out, lse = ops.cache_attention(q, c.k, c.v, c.table, lengths_to_offsets(new), c.lens, return_lse=True)
+    assert bool((out[:2] == 0).all()) and bool(torch.isneginf(lse[:2]).all())
+    assert bool((out[7] == 0).all()) and bool(torch.isneginf(lse[7]).all())
+    _check_cache(out, lse, q, c, new, lens, 0.125)
+
+
+@pytest.mark.parametrize("new", [[3, 1], [60, 50]])
+def test_cache_attention_nonfinite_values_reach_only_rows_that_see_them(new):
+    lens = [131, 80]
+    c = Cache(lens, 2, 128, 16, torch.bfloat16, 8)
+    last = cache_rows  # noqa: F841
+    j = 129  # seen by the last two new tokens of the first sequence only
+    c.v[c.table[0, j // 16].long(), j % 16, 1, 77] = math.nan
+    c.v[c.table[0, (j + 1) // 16].long(), (j + 1) % 16, 0, 3] = -math.inf
+    c.k[c.table[1, 79 // 16].long(), 79 % 16, 0] = math.nan
+    q = torch.randn(sum(new), 4, 128, device=DEV, generator=_gen(5)).bfloat16()
+    out, lse = ops.cache_attention(q, c.k, c.v, c.table, lengths_to_offsets(new), c.lens, return_lse=True)
+    _check_cache(out, lse, q, c, new, lens, 128**-0.5, rows=True)
+
+
+def test_cache_attention_wrong_pages_and_lengths_are_contained():
+    """Page numbers outside the cache stand for zeros, lengths for the table's slots."""
+    lens = [100, 64, 30]
+    c = Cache(lens, 2, 64, 16, torch.float16, 8)
+    c.table[0, 2] = -7
+    c.table[1, 1] = 1 << 30
+    q = torch.randn(3, 4, 64, device=DEV, generator=_gen(5)).half()
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    off = lengths_to_offsets([1, 1, 1])
+    out = ops.cache_attention(q, c.k, c.v, c.table, off, c.lens, status=status)
+    assert int(status) == 0x401
+    for b, (bad, m) in enumerate([(2, 100), (1, 64), (None, 30)]):
+        table = c.table.clone().clamp_(0, c.k.shape[0] - 1)
+        k, v = cache_rows(c.k, table, b, m).clone(), cache_rows(c.v, table, b, m).clone()
+        if bad is not None:
+            k[bad * 16:(bad + 1) * 16], v[bad * 16:(bad + 1) * 16] = 0, 0
+        ref, _ = attention_block(q[b:b + 1], k, v, 1, m, 0.125)
+        assert float((out[b] - ref).abs().max()) < 0.01
+    status.zero_()
+    c = Cache([112, 64, 30], 2, 64, 16, torch.float16, 8)
+    lens = torch.tensor([1 << 30, 64, -5], dtype=torch.int32, device=DEV)
+    out = ops.cache_attention(q, c.k, c.v, c.table, off, lens, status=status)
+    assert int(status) == 0x402
+    ref, _ = attention_block(q[:1], cache_rows(c.k, c.table, 0, 112), cache_rows(c.v, c.table, 0, 112), 1, 112, 0.125)
+    assert float((out[0] - ref).abs().max()) < 0.01
+    assert bool((out[2] == 0).all())
+    status.zero_()
+    bad_off = torch.tensor([-3, 1, 90, 3], dtype=torch.int32, device=DEV)
+    ops.cache_attention(q, c.k, c.v, c.table, bad_off, c.lens, status=status)
+    assert int(status) == 0x402
+
+
+@pytest.mark.parametrize("new", [1, 100])
+def test_cache_attention_behind_2_31_elements(new):
+    """Pages whose elements lie beyond 32-bit offsets."""
+    pages, page, kv, d = 70000, 64, 4, 128
+    k = torch.empty(pages, page, kv, d, dtype=torch.float16, device=DEV)
+    v = torch.empty_like(k)
+    c = Cache([150], kv, d, page, torch.float16, 3)
+    table = torch.tensor([[69999, 66001, 65537]], dtype=torch.int32, device=DEV)
+    k[table[0].long()], v[table[0].long()] = c.k[c.table[0].long()], c.v[c.table[0].long()]
+    q = torch.randn(new, 8, d, device=DEV, generator=_gen(5)).half()
+    out, lse = ops.cache_attention(q, k, v, table, lengths_to_offsets([new]), c.lens, return_lse=True)
+    _check_cache(out, lse, q, c, [new], [150], d**-0.5)
+    nk = torch.randn(new, kv, d, device=DEV, generator=_gen(6)).half()
+    ops.cache_append(nk, nk + 1, k, v, table, lengths_to_offsets([new]), c.lens)
+    c.k, c.v, c.table = k, v, table
+    assert torch.equal(cache_rows(k, table, 0, 150)[150 - new:], nk)
+    assert torch.equal(cache_rows(v, table, 0, 150)[150 - new:], nk + 1)
+
+
+def test_captured_calls_follow_new_lengths():
+    """One graph of append + attention, replayed with other lengths, pages and tokens."""
+    kv, heads, d, page = 2, 8, 64, 16
+    c = Cache([200, 200, 200], kv, d, page, torch.float16, 3)
+    off = lengths_to_offsets([1, 1, 1])
+    q = torch.zeros(3, heads, d, dtype=torch.float16, device=DEV)
+    nk, nv = torch.zeros(3, kv, d, dtype=torch.float16, device=DEV), torch.zeros(3, kv, d, dtype=torch.float16, device=DEV)
+
+    def step():
+        ops.cache_append(nk, nv, c.k, c.v, c.table, off, c.lens)
+        return ops.cache_attention(q, c.k, c.v, c.table, off, c.lens, max_new=1, return_lse=True)
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = step()
+    for i, lens in enumerate([[3, 77, 200], [1, 16, 17], [100, 0, 64]]):
+        g = _gen(20 + i)
+        q.copy_(torch.randn(q.shape, device=DEV, generator=g))
+        nk.copy_(torch.randn(nk.shape, device=DEV, generator=g))
+        nv.copy_(torch.randn(nk.shape, device=DEV, generator=g))
+        c.lens.copy_(torch.tensor(lens))
+        c.table.copy_(c.table.flatten()[torch.randperm(c.table.numel(), device=DEV, generator=g)].view_as(c.table))
+        c.k.copy_(torch.randn(c.k.shape, device=DEV, generator=g))
+        c.v.copy_(torch.randn(c.v.shape, device=DEV, generator=g))
+        graph.replay()
+        torch.cuda.synchronize()
+        for b, m in enumerate(lens):
+            if m:
+                assert torch.equal(cache_rows(c.k, c.table, b, m)[-1], nk[b])
+        _check_cache(out, lse, q, c, [1, 1, 1], lens, 0.125)
+
+
+def test_serving_on_another_stream():
+    lens = [100, 300]
+    c = Cache(lens, 2, 64, 16, torch.float16, 3)
+    q = torch.randn(2, 4, 64, device=DEV, generator=_gen(5)).half()
+    off = lengths_to_offsets([1, 1])
+    want = ops.cache_attention(q, c.k, c.v, c.table, off, c.lens)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = [ops.cache_attention(q, c.k, c.v, c.table, off, c.lens) for _ in range(20)]
+    side.synchronize()
+    assert all(torch.equal(want, g) for g in got)
+
+
+# -------------------------------------------------------------------------------- append
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d,page,kv", [(32, 16, 3), (64, 64, 1), (128, 32, 8), (256, 256, 2)])
+def test_cache_append(dtype, d, page, kv):
+    new, lens = [1, 0, 17, 300, 5], [1, 9, 40, 300, 3]
+    c = Cache([300] * 5, kv, d, page, dtype, 3, extra_pages=1)
+    c.lens = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    k0, v0 = c.k.clone(), c.v.clone()
+    rows = torch.randn(sum(new) + 4, 2 * kv + 1, d, device=DEV, generator=_gen(1)).to(dtype)
+    k, v = rows[:, :kv], rows[:, kv:2 * kv]
+    cap = c.table.shape[1] * page
+    pos = torch.full((5, kv, cap), 77, dtype=torch.int32, device=DEV)
+    mass = torch.full((5, kv, cap), 5.0, device=DEV)
+    seen = torch.tensor([11, 12, 1000, 300, 1 << 20], dtype=torch.int32, device=DEV)
+    ops.cache_append(k, v, c.k, c.v, c.table, lengths_to_offsets(new), c.lens, positions=pos, mass=mass, seen=seen)
+    at = 0
+    want_pos, want_mass = torch.full_like(pos, 77), torch.full_like(mass, 5.0)
+    for b, (n, m) in enumerate(zip(new, lens)):
+        skip = max(0, n - m)  # tokens before the cache's first slot are dropped
+        for i in range(skip, n):
+            slot = m - n + i
+            page_at = int(c.table[b, slot // page])
+            k0[page_at, slot % page], v0[page_at, slot % page] = k[at + i], v[at + i]
+            want_pos[b, :, slot], want_mass[b, :, slot] = int(seen[b]) - n + i, 0
+        at += n
+    # compared as bits: most of the cache is NaN here
+    assert torch.equal(c.k.contiguous().view(torch.int16), k0.contiguous().view(torch.int16))
+    assert torch.equal(c.v.contiguous().view(torch.int16), v0.contiguous().view(torch.int16))
+    assert torch.equal(pos, want_pos) and torch.equal(mass, want_mass)
+
+
+def test_cache_append_drops_tokens_of_wrong_pages():
+    c = Cache([64, 64], 2, 64, 16, torch.float16, 3)
+    k0 = c.k.clone()
+    c.table[0, 3] = 10**6
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    k = torch.randn(3, 2, 64, device=DEV, generator=_gen(1)).half()
+    ops.cache_append(k, k, c.k, c.v, c.table, lengths_to_offsets([1, 2]), c.lens, status=status)
+    assert int(status) == 0x401
+    at = c.table[1, 3].long()
+    k0[at, 14], k0[at, 15] = k[1], k[2]
+    assert torch.equal(c.k.view(torch.int16), k0.view(torch.int16))
+
+
+# ----------------------------------------------------------------------------- eviction
+def _evict_case(lens, kv, d, page, dtype, seed, heads_first=False):
+    c = Cache(lens, kv, d, page, dtype, seed, heads_first=heads_first)
+    b, cap = len(lens), c.table.shape[1] * page
+    g = _gen(seed + 1)
+    mass = torch.exp(torch.randn(b, kv, cap, device=DEV, generator=g))
+    mass = (mass * 8).round() / 8  # many equal ones
+    pos = torch.rand(b, kv, cap, device=DEV, generator=g).argsort(2).to(torch.int32)
+    return c, mass, pos
+
+
+def _check_evict(c, mass, pos, lens, keep, recent):
+    k0, v0 = c.k.clone(), c.v.clone()
+    page = c.k.shape[1]
+    got_mass, got_pos, got_lens = ops.cache_evict(mass, pos, c.k, c.v, c.table, c.lens, keep, recent=recent)
+    want_mass, want_pos = mass.clone(), pos.clone()
+    for b, m in enumerate(lens):
+        t = c.table[b].long()
+        for h in range(c.k.shape[2]):
+            hole, mover = evict_choice(mass[b, h], pos[b, h], m, keep, recent)
+            assert len(hole) == len(mover)
+            if hole:
+                hole, mover = torch.tensor(hole, device=DEV), torch.tensor(mover, device=DEV)
+                for cache in (k0, v0):
+                    cache[t[hole // page], hole % page, h] = cache[t[mover // page], mover % page, h]
+                want_mass[b, h, hole], want_pos[b, h, hole] = mass[b, h, mover], pos[b, h, mover]
+        want_mass[b, :, min(m, keep):], want_pos[b, :, min(m, keep):] = 0, -1
+    assert got_lens.tolist() == [min(m, keep) for m in lens]
+    assert torch.equal(got_pos, want_pos)
+    assert torch.equal(got_mass.view(torch.int32), want_mass.view(torch.int32))
+    assert torch.equal(c.k.contiguous().view(torch.int16), k0.contiguous().view(torch.int16))
+    assert torch.equal(c.v.contiguous().view(torch.int16), v0.contiguous().view(torch.int16))
+    return got_mass, got_pos, got_lens
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d,page,kv", [(32, 16, 3), (64, 64, 1), (128, 32, 2), (256, 128, 2)])
+@pytest.mark.parametrize("keep,recent", [(1, 0), (1, 1), (100, 30), (64, 64), (511, 0), (5000, 9)])
+def test_cache_evict(dtype, d, page, kv, keep, recent):
+    lens = [0, 1, 64, 100, 101, 700, 512]
+    c, mass, pos = _evict_case(lens, kv, d, page, dtype, 9)
+    _check_evict(c, mass, pos, lens, keep, recent)
+
+
+def test_cache_evict_special_masses():
+    """NaN, infinities, both zeros, negative numbers, denormals, all equal."""
+    lens = [300, 300, 200]
+    c, mass, pos = _evict_case(lens, 2, 64, 16, torch.float16, 9, heads_first=True)
+    odd = torch.tensor([math.nan, math.inf, -math.inf, 0.0, -0.0, -1.0, 1e-42, -1e-42, 3e38], device=DEV)
+    mass[0] = odd[torch.randint(0, 9, mass[0].shape, device=DEV, generator=_gen(1))]
+    mass[1] = 0.25
+    _check_evict(c, mass, pos, lens, 128, 16)
+
+
+@pytest.mark.parametrize("length", [40000, 70000])
+def test_cache_evict_long(length):
+    """Longer than what the selection holds in shared memory, and just below."""
+    lens = [length, 30000]
+    c, mass, pos = _evict_case(lens, 1, 32, 256, torch.float16, 9)
+    _check_evict(c, mass, pos, lens, 8000, 100)

@@ -20,6 +20,7 @@ TTTJ_ERR_DEVICE_TIMEOUT = 3
 
 DTYPE_F16 = 0
 DTYPE_F32 = 1
+DTYPE_BF16 = 2
 
 EPI_BIAS = 0
 EPI_BIAS_GELU = 1
@@ -101,6 +102,19 @@ _SIGNATURES = {
         _c.c_int, [_vp, _vp, _c.c_int, _vp, _vp, _c.c_int, _c.c_int, _vp, _vp]
     ),
     "tttj_plan_path": (_c.c_int, [_vp]),
+    "tttj_serve_workspace_bytes": (_c.c_size_t, [_vp]),
+    "tttj_prompt_attention": (
+        _c.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _c.c_int, _c.c_float, _vp, _c.c_size_t, _vp]
+    ),
+    "tttj_cache_attention": (
+        _c.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _c.c_int, _c.c_float, _vp, _c.c_size_t, _vp]
+    ),
+    "tttj_cache_append": (_c.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "tttj_cache_evict_workspace_bytes": (_c.c_size_t, [_vp, _c.c_int]),
+    "tttj_cache_evict": (
+        _c.c_int,
+        [_vp, _vp, _vp, _vp, _vp, _c.c_int, _c.c_int, _vp, _vp, _vp, _vp, _c.c_size_t, _vp],
+    ),
 }
 
 KCLASS_COUNT = 9
@@ -134,6 +148,40 @@ class TttjConfig(ctypes.Structure):
             int(cfg.num_layers),
             1 if cfg.causal else 0,
         )
+
+
+class TttjRows(ctypes.Structure):
+    """C mirror of tttj_rows: [tokens][heads][head_dim] by element strides."""
+
+    _fields_ = [("data", ctypes.c_void_p), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
+
+
+class TttjPages(ctypes.Structure):
+    """C mirror of tttj_pages: [pages][page_size][kv_heads][head_dim] by element strides."""
+
+    _fields_ = [("data", ctypes.c_void_p), ("page_stride", ctypes.c_int64),
+                ("slot_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
+
+
+class TttjSeqs(ctypes.Structure):
+    """C mirror of tttj_seqs: the sequences of a serving call."""
+
+    _fields_ = [
+        ("seq_offsets", ctypes.c_void_p),
+        ("cache_lens", ctypes.c_void_p),
+        ("page_table", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("batch", ctypes.c_int32),
+        ("tokens", ctypes.c_int32),
+        ("pages_per_seq", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("status", ctypes.c_void_p),
+    ]
 
 
 _lock = threading.Lock()

@@ -11,6 +11,7 @@
 #include <vector>
 
 #include "../../include/tttj_b200.h"
+#include "capi_util.h"
 #include "launch.h"
 
 using namespace tttj;
@@ -1485,3 +1486,22 @@ extern "C" int tttj_attention_noalloc(const void* qkv, void* ctx, int qkv_rows,
   TTTJ_CUDA(attention_tc_launch(tm, ap, hd, causal, grid, seq_len, s));
   return TTTJ_OK;
 }
+
+// ---------------------------------------------------------------------------
+// capi_util.h: the helpers of this file that other entry points share.
+// ---------------------------------------------------------------------------
+namespace tttj {
+
+int capi_fail(int code, const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof(buf), fmt, ap);
+  va_end(ap);
+  return fail(code, "%s", buf);
+}
+int capi_cuda_fail(cudaError_t e, const char* what) { return cuda_fail(e, what); }
+PFN_cuTensorMapEncodeTiled_v12000 capi_encode_fn() { return encode_fn(); }
+int capi_sm_count(int device) { return sm_count(device); }
+
+}  // namespace tttj

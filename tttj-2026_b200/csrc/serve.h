@@ -1,0 +1,124 @@
+// Parameter blocks, device helpers and launchers of the serving operators (prompt
+// attention, paged-cache append / attention / gathered mass / eviction).
+#pragma once
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "params.h"
+
+namespace tttj {
+
+constexpr int SRV_MAX_BATCH = 2048;  // sequences of a call (prefix sums in shared memory)
+constexpr int SRV_MAX_GROUP = 64;    // query heads per key / value head
+constexpr int SRV_DEV_BAD_PAGE = 0x401;   // a live page-table entry outside the cache
+constexpr int SRV_DEV_BAD_LENS = 0x402;   // lengths or offsets outside the call's tensors
+constexpr int SRV_DEV_TIMEOUT = 0x403;    // a bounded device wait gave up
+
+// Where the tokens of a call live: packed new tokens, and keys / values either packed
+// the same way (table == nullptr: prompts) or in the pages of a cache.
+struct SrvSeqs {
+  const int* seq_off;  // [batch + 1] first packed row of each sequence
+  const int* lens;     // [batch] cached tokens, new ones included (nullptr: prompts)
+  const int* table;    // [batch][table_stride] page numbers (nullptr: prompts)
+  long table_stride;
+  int pages_per_seq;
+  int page_shift;      // log2 of the page size
+  int num_pages;
+  int batch;
+  int tokens;          // rows allocated in q / out
+  int causal;
+  int* status;         // device status word (nullable)
+};
+
+struct SrvSeq {
+  int row0, n, len;  // first packed row, new tokens, keys
+};
+
+// Offsets and lengths come from device memory and are never trusted: whatever they
+// hold, rows stay inside [0, tokens) and slots inside the table.
+__device__ __forceinline__ SrvSeq srv_seq(const SrvSeqs& s, int b) {
+  SrvSeq r;
+  const int o0 = s.seq_off[b], o1 = s.seq_off[b + 1];
+  r.row0 = min(max(o0, 0), s.tokens);
+  const int end = min(max(o1, r.row0), s.tokens);
+  r.n = end - r.row0;
+  bool bad = r.row0 != o0 || end != o1;
+  if (s.lens != nullptr) {
+    const int len = s.lens[b];
+    const long cap = (long)s.pages_per_seq << s.page_shift;
+    r.len = (int)min((long)max(len, 0), cap);
+    bad |= r.len != len;
+  } else {
+    r.len = r.n;
+  }
+  if (bad && s.status != nullptr) atomicCAS(s.status, 0, SRV_DEV_BAD_LENS);
+  return r;
+}
+
+// Page holding `slot` of sequence b; num_pages (a page that TMA fills with zeros and
+// that plain accesses skip) for entries outside the cache.
+__device__ __forceinline__ int srv_page(const SrvSeqs& s, int b, int slot) {
+  const int page = s.table[(long)b * s.table_stride + (slot >> s.page_shift)];
+  if (page >= 0 && page < s.num_pages) return page;
+  if (s.status != nullptr) atomicCAS(s.status, 0, SRV_DEV_BAD_PAGE);
+  return s.num_pages;
+}
+
+// ---- attention of few query rows per sequence (serve_step.cuh) ----
+struct StepParams {
+  SrvSeqs s;
+  const void* q;
+  long q_tok, q_head;  // element strides
+  void* out;
+  long o_tok, o_head;
+  float* lse;          // [tokens][heads] or nullptr
+  int heads, kv_heads, group;
+  float scale_log2;
+  float* part_o;       // [2 * grid][STEP_ROWS][head_dim] partial outputs
+  float2* part_ml;     // [2 * grid][STEP_ROWS] their (max, sum)
+  int most_rows;       // sequences with more rows (tokens x group) are not handled here
+  unsigned long long wait_limit_ns;
+};
+constexpr int STEP_ROWS = 16;   // query rows of one mma tile
+constexpr int STEP_KEYS = 64;   // keys per pipeline stage
+constexpr int step_ctas_per_sm(int hd) { return hd == 256 ? 1 : 2; }
+cudaError_t step_launch(const CUtensorMap& tm_k, const CUtensorMap& tm_v, const StepParams& p,
+                        int head_dim, int bf16, int grid, cudaStream_t stream);
+
+// ---- cache append / evict (serve_cache.cu) ----
+struct CacheView {
+  void* data;
+  long page, slot, head;  // element strides
+};
+struct AppendParams {
+  SrvSeqs s;
+  const void* k;
+  const void* v;
+  long k_tok, k_head, v_tok, v_head;
+  CacheView kc, vc;
+  int kv_heads, head_dim;
+  int* positions;    // [batch][kv_heads][cap] or nullptr
+  float* mass;       // the same shape, or nullptr
+  const int* seen;   // [batch] tokens seen by each sequence, or nullptr (= lens)
+};
+cudaError_t append_launch(const AppendParams& p, cudaStream_t stream);
+
+struct EvictParams {
+  SrvSeqs s;  // seq_off is unused
+  CacheView kc, vc;
+  int kv_heads, head_dim;
+  const float* mass;
+  const int* positions;
+  float* mass_out;
+  int* positions_out;
+  int* lens_out;
+  int keep, recent;
+  long cap;       // slots per sequence (row length of mass / positions)
+  int2* moves;    // [batch * kv_heads][most_moves] (from, to) slots
+  int* n_moves;   // [batch * kv_heads]
+  int most_moves;
+};
+cudaError_t evict_launch(const EvictParams& p, cudaStream_t stream);
+
+}  // namespace tttj

@@ -1,0 +1,305 @@
+// C entry points of the serving operators (include/tttj_b200.h): argument checks,
+// tensor maps and launches.  Nothing here reads device memory or synchronises.
+#include <math.h>
+
+#include "capi_util.h"
+#include "serve.h"
+
+using namespace tttj;
+
+namespace {
+
+constexpr size_t kAlign = 256;
+inline size_t up(size_t v) { return (v + kAlign - 1) / kAlign * kAlign; }
+inline bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
+
+int check_seqs(const char* what, const tttj_seqs* s, bool cache, bool offsets) {
+  if (!s) return capi_fail(TTTJ_ERR_INVALID, "%s: null argument", what);
+  if (s->dtype != TTTJ_DTYPE_F16 && s->dtype != TTTJ_DTYPE_BF16)
+    return capi_fail(TTTJ_ERR_INVALID, "%s: dtype must be fp16 or bf16", what);
+  if (s->head_dim != 32 && s->head_dim != 64 && s->head_dim != 128 && s->head_dim != 256)
+    return capi_fail(TTTJ_ERR_INVALID, "%s: head_dim=%d unsupported (32, 64, 128, 256)", what, s->head_dim);
+  if (s->kv_heads <= 0 || s->heads <= 0 || s->heads % s->kv_heads || s->heads / s->kv_heads > SRV_MAX_GROUP)
+    return capi_fail(TTTJ_ERR_INVALID, "%s: heads=%d must be kv_heads=%d times a group of 1 .. %d", what,
+                     s->heads, s->kv_heads, SRV_MAX_GROUP);
+  if (s->batch <= 0 || s->batch > SRV_MAX_BATCH)
+    return capi_fail(TTTJ_ERR_INVALID, "%s: batch=%d outside 1 .. %d", what, s->batch, SRV_MAX_BATCH);
+  if (s->tokens < 0 || (long)s->tokens * s->heads >= (1l << 31))
+    return capi_fail(TTTJ_ERR_INVALID, "%s: tokens=%d x heads=%d out of range", what, s->tokens, s->heads);
+  if (offsets && !s->seq_offsets) return capi_fail(TTTJ_ERR_INVALID, "%s: null seq_offsets", what);
+  if (cache) {
+    if (!s->cache_lens || !s->page_table) return capi_fail(TTTJ_ERR_INVALID, "%s: null cache_lens or page_table", what);
+    const int ps = s->page_size;
+    if (ps < 16 || ps > 256 || (ps & (ps - 1)))
+      return capi_fail(TTTJ_ERR_INVALID, "%s: page_size=%d unsupported (16, 32, 64, 128, 256)", what, ps);
+    if (s->pages_per_seq <= 0 || s->num_pages <= 0 || (long)s->pages_per_seq * ps >= (1l << 30))
+      return capi_fail(TTTJ_ERR_INVALID, "%s: pages_per_seq=%d, num_pages=%d out of range", what,
+                       s->pages_per_seq, s->num_pages);
+    if (s->table_stride < s->pages_per_seq)
+      return capi_fail(TTTJ_ERR_INVALID, "%s: page_table rows overlap", what);
+  }
+  return TTTJ_OK;
+}
+
+int check_rows(const char* what, const char* name, const tttj_rows* r, const tttj_seqs* s, int heads) {
+  if (!r || (!r->data && s->tokens > 0)) return capi_fail(TTTJ_ERR_INVALID, "%s: null %s", what, name);
+  if (misaligned(r->data)) return capi_fail(TTTJ_ERR_INVALID, "%s: %s must be 16-byte aligned", what, name);
+  if ((s->tokens > 1 && r->token_stride <= 0) || r->token_stride % 8 || (heads > 1 && r->head_stride <= 0) ||
+      r->head_stride % 8)
+    return capi_fail(TTTJ_ERR_INVALID, "%s: %s strides must be positive multiples of 8 elements", what, name);
+  return TTTJ_OK;
+}
+
+int check_pages(const char* what, const char* name, const tttj_pages* c, const tttj_seqs* s) {
+  if (!c || !c->data) return capi_fail(TTTJ_ERR_INVALID, "%s: null %s", what, name);
+  if (misaligned(c->data)) return capi_fail(TTTJ_ERR_INVALID, "%s: %s must be 16-byte aligned", what, name);
+  if ((s->num_pages > 1 && c->page_stride <= 0) || c->page_stride % 8 || c->slot_stride <= 0 || c->slot_stride % 8 ||
+      (s->kv_heads > 1 && c->head_stride <= 0) || c->head_stride % 8)
+    return capi_fail(TTTJ_ERR_INVALID, "%s: %s strides must be positive multiples of 8 elements", what, name);
+  return TTTJ_OK;
+}
+
+#define TRY(call)             \
+  do {                        \
+    const int rc_ = (call);   \
+    if (rc_) return rc_;      \
+  } while (0)
+
+SrvSeqs seqs_of(const tttj_seqs* s, bool cache, int causal) {
+  SrvSeqs r{};
+  r.seq_off = s->seq_offsets;
+  r.batch = s->batch;
+  r.tokens = s->tokens;
+  r.causal = causal;
+  r.status = s->status;
+  if (cache) {
+    r.lens = s->cache_lens;
+    r.table = s->page_table;
+    r.table_stride = s->table_stride;
+    r.pages_per_seq = s->pages_per_seq;
+    while ((1 << r.page_shift) < s->page_size) ++r.page_shift;
+    r.num_pages = s->num_pages;
+  }
+  return r;
+}
+
+// 4-D map {head_dim, slots, heads, pages} of keys or values, moved in boxes of one
+// head's `box_rows` slots x min(head_dim, 64) columns, swizzled by the box's row width.
+int kv_map(CUtensorMap* m, const char* what, const tttj_seqs* s, const void* data, long page_stride,
+           long slot_stride, long head_stride, int slots, int pages, int box_rows) {
+  auto fn = capi_encode_fn();
+  if (!fn) return capi_fail(TTTJ_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  const int cols = s->head_dim < 64 ? s->head_dim : 64;
+  cuuint64_t dims[4] = {(cuuint64_t)s->head_dim, (cuuint64_t)slots, (cuuint64_t)s->kv_heads, (cuuint64_t)pages};
+  // The stride of a dimension of size one is never used; it still has to be valid.
+  const long one = s->head_dim;
+  cuuint64_t strides[3] = {(cuuint64_t)(slots > 1 ? slot_stride : one) * 2,
+                           (cuuint64_t)(s->kv_heads > 1 ? head_stride : one) * 2,
+                           (cuuint64_t)(pages > 1 ? page_stride : one) * 2};
+  cuuint32_t box[4] = {(cuuint32_t)cols, (cuuint32_t)box_rows, 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUresult r =
+      fn(m, s->dtype == TTTJ_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+         const_cast<void*>(data), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+         cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return capi_fail(TTTJ_ERR_INVALID, "%s: strides out of range (%d)", what, (int)r);
+  return TTTJ_OK;
+}
+
+int sm_count_here(int* sms) {
+  int dev = 0;
+  CAPI_CUDA(cudaGetDevice(&dev));
+  *sms = capi_sm_count(dev);
+  if (*sms <= 0) return capi_fail(TTTJ_ERR_CUDA, "no multiprocessor count");
+  return TTTJ_OK;
+}
+
+constexpr int kMostSms = 256;  // workspace sizes hold for any device of at most this many
+
+struct ServeWs {
+  size_t part_o, part_ml, total;
+};
+ServeWs serve_ws(const tttj_seqs* s) {
+  ServeWs w{};
+  const size_t parts = 2ul * kMostSms * step_ctas_per_sm(s->head_dim) * STEP_ROWS;
+  w.part_o = 0;
+  w.part_ml = up(parts * s->head_dim * 4);
+  w.total = w.part_ml + up(parts * 8);
+  return w;
+}
+
+int check_attention(const char* what, const tttj_seqs* s, float scale, const void* workspace,
+                    size_t workspace_bytes) {
+  const size_t need = serve_ws(s).total;
+  if (!workspace || workspace_bytes < need)
+    return capi_fail(TTTJ_ERR_INVALID, "%s: workspace too small: %zu < %zu", what, workspace ? workspace_bytes : 0,
+                     need);
+  if (reinterpret_cast<uintptr_t>(workspace) & (kAlign - 1))
+    return capi_fail(TTTJ_ERR_INVALID, "%s: workspace must be 256-byte aligned", what);
+  if (!(scale > 0.f) || !isfinite(scale))
+    return capi_fail(TTTJ_ERR_INVALID, "%s: scale must be positive and finite", what);
+  return TTTJ_OK;
+}
+
+int attention(const tttj_seqs* s, const tttj_rows* q, const tttj_rows* out, float* lse, int causal, float scale,
+              void* workspace, bool cache, const CUtensorMap& tm_k, const CUtensorMap& tm_v, cudaStream_t stream) {
+  const ServeWs w = serve_ws(s);
+  int sms = 0;
+  TRY(sm_count_here(&sms));
+  if (sms > kMostSms) sms = kMostSms;
+  uint8_t* base = static_cast<uint8_t*>(workspace);
+  StepParams p{};
+  p.s = seqs_of(s, cache, causal);
+  p.q = q->data;
+  p.q_tok = q->token_stride;
+  p.q_head = q->head_stride;
+  p.out = const_cast<void*>(out->data);
+  p.o_tok = out->token_stride;
+  p.o_head = out->head_stride;
+  p.lse = lse;
+  p.heads = s->heads;
+  p.kv_heads = s->kv_heads;
+  p.group = s->heads / s->kv_heads;
+  p.scale_log2 = scale * 1.44269504088896341f;
+  p.part_o = reinterpret_cast<float*>(base + w.part_o);
+  p.part_ml = reinterpret_cast<float2*>(base + w.part_ml);
+  p.most_rows = INT32_MAX;
+  p.wait_limit_ns = TTTJ_WAIT_LIMIT_NS;
+  CAPI_CUDA(step_launch(tm_k, tm_v, p, s->head_dim, s->dtype == TTTJ_DTYPE_BF16,
+                        sms * step_ctas_per_sm(s->head_dim), stream));
+  return TTTJ_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t tttj_serve_workspace_bytes(const tttj_seqs* s) {
+  if (check_seqs("serve_workspace_bytes", s, false, false)) return 0;
+  return serve_ws(s).total;
+}
+
+int tttj_prompt_attention(const tttj_seqs* s, const tttj_rows* q, const tttj_rows* k, const tttj_rows* v,
+                          const tttj_rows* out, float* lse, int causal, float scale, void* workspace,
+                          size_t workspace_bytes, void* stream) {
+  const char* what = "prompt_attention";
+  TRY(check_seqs(what, s, false, true));
+  TRY(check_rows(what, "q", q, s, s->heads));
+  TRY(check_rows(what, "k", k, s, s->kv_heads));
+  TRY(check_rows(what, "v", v, s, s->kv_heads));
+  TRY(check_rows(what, "out", out, s, s->heads));
+  if (s->tokens == 0) return TTTJ_OK;
+  TRY(check_attention(what, s, scale, workspace, workspace_bytes));
+  CUtensorMap tm_k, tm_v;
+  TRY(kv_map(&tm_k, what, s, k->data, 0, k->token_stride, k->head_stride, s->tokens, 1, STEP_KEYS));
+  TRY(kv_map(&tm_v, what, s, v->data, 0, v->token_stride, v->head_stride, s->tokens, 1, STEP_KEYS));
+  return attention(s, q, out, lse, causal ? 1 : 0, scale, workspace, false, tm_k, tm_v,
+                   static_cast<cudaStream_t>(stream));
+}
+
+int tttj_cache_attention(const tttj_seqs* s, const tttj_rows* q, const tttj_pages* k_cache,
+                         const tttj_pages* v_cache, const tttj_rows* out, float* lse, int max_new, float scale,
+                         void* workspace, size_t workspace_bytes, void* stream) {
+  const char* what = "cache_attention";
+  TRY(check_seqs(what, s, true, true));
+  TRY(check_rows(what, "q", q, s, s->heads));
+  TRY(check_rows(what, "out", out, s, s->heads));
+  TRY(check_pages(what, "k_cache", k_cache, s));
+  TRY(check_pages(what, "v_cache", v_cache, s));
+  if (max_new < 0) return capi_fail(TTTJ_ERR_INVALID, "%s: max_new=%d is negative", what, max_new);
+  if (s->tokens == 0) return TTTJ_OK;
+  TRY(check_attention(what, s, scale, workspace, workspace_bytes));
+  const int box = s->page_size < STEP_KEYS ? s->page_size : STEP_KEYS;
+  CUtensorMap tm_k, tm_v;
+  TRY(kv_map(&tm_k, what, s, k_cache->data, k_cache->page_stride, k_cache->slot_stride, k_cache->head_stride,
+             s->page_size, s->num_pages, box));
+  TRY(kv_map(&tm_v, what, s, v_cache->data, v_cache->page_stride, v_cache->slot_stride, v_cache->head_stride,
+             s->page_size, s->num_pages, box));
+  return attention(s, q, out, lse, 1, scale, workspace, true, tm_k, tm_v, static_cast<cudaStream_t>(stream));
+}
+
+int tttj_cache_append(const tttj_seqs* s, const tttj_rows* k, const tttj_rows* v, const tttj_pages* k_cache,
+                      const tttj_pages* v_cache, int32_t* positions, float* mass, const int32_t* seen,
+                      void* stream) {
+  const char* what = "cache_append";
+  TRY(check_seqs(what, s, true, true));
+  TRY(check_rows(what, "k", k, s, s->kv_heads));
+  TRY(check_rows(what, "v", v, s, s->kv_heads));
+  TRY(check_pages(what, "k_cache", k_cache, s));
+  TRY(check_pages(what, "v_cache", v_cache, s));
+  if (s->tokens == 0) return TTTJ_OK;
+  AppendParams p{};
+  p.s = seqs_of(s, true, 1);
+  p.k = k->data;
+  p.v = v->data;
+  p.k_tok = k->token_stride;
+  p.k_head = k->head_stride;
+  p.v_tok = v->token_stride;
+  p.v_head = v->head_stride;
+  p.kc = {k_cache->data, k_cache->page_stride, k_cache->slot_stride, k_cache->head_stride};
+  p.vc = {v_cache->data, v_cache->page_stride, v_cache->slot_stride, v_cache->head_stride};
+  p.kv_heads = s->kv_heads;
+  p.head_dim = s->head_dim;
+  p.positions = positions;
+  p.mass = mass;
+  p.seen = seen;
+  CAPI_CUDA(append_launch(p, static_cast<cudaStream_t>(stream)));
+  return TTTJ_OK;
+}
+
+static int evict_most_moves(const tttj_seqs* s, int keep) {
+  const long cap = (long)s->pages_per_seq * s->page_size;
+  const long behind = cap - keep;
+  return behind <= 0 ? 0 : (int)(behind < keep ? behind : keep);
+}
+
+size_t tttj_cache_evict_workspace_bytes(const tttj_seqs* s, int keep) {
+  if (check_seqs("cache_evict", s, true, false) || keep <= 0) return 0;
+  const size_t bh = (size_t)s->batch * s->kv_heads;
+  return up(bh * evict_most_moves(s, keep) * sizeof(int2)) + up(bh * 4);
+}
+
+int tttj_cache_evict(const tttj_seqs* s, const tttj_pages* k_cache, const tttj_pages* v_cache, const float* mass,
+                     const int32_t* positions, int keep, int recent, float* mass_out, int32_t* positions_out,
+                     int32_t* lens_out, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* what = "cache_evict";
+  TRY(check_seqs(what, s, true, false));
+  TRY(check_pages(what, "k_cache", k_cache, s));
+  TRY(check_pages(what, "v_cache", v_cache, s));
+  if (!mass || !positions || !mass_out || !positions_out || !lens_out)
+    return capi_fail(TTTJ_ERR_INVALID, "%s: null argument", what);
+  if (mass == mass_out || positions == positions_out || s->cache_lens == lens_out)
+    return capi_fail(TTTJ_ERR_INVALID, "%s: outputs may not be the inputs", what);
+  if (keep <= 0) return capi_fail(TTTJ_ERR_INVALID, "%s: keep=%d must be positive", what, keep);
+  if (recent < 0 || recent > keep)
+    return capi_fail(TTTJ_ERR_INVALID, "%s: recent=%d outside 0 .. keep=%d", what, recent, keep);
+  const size_t need = tttj_cache_evict_workspace_bytes(s, keep);
+  if (!workspace || workspace_bytes < need)
+    return capi_fail(TTTJ_ERR_INVALID, "%s: workspace too small: %zu < %zu", what, workspace ? workspace_bytes : 0,
+                     need);
+  if (reinterpret_cast<uintptr_t>(workspace) & (kAlign - 1))
+    return capi_fail(TTTJ_ERR_INVALID, "%s: workspace must be 256-byte aligned", what);
+  EvictParams p{};
+  p.s = seqs_of(s, true, 1);
+  p.kc = {k_cache->data, k_cache->page_stride, k_cache->slot_stride, k_cache->head_stride};
+  p.vc = {v_cache->data, v_cache->page_stride, v_cache->slot_stride, v_cache->head_stride};
+  p.kv_heads = s->kv_heads;
+  p.head_dim = s->head_dim;
+  p.mass = mass;
+  p.positions = positions;
+  p.mass_out = mass_out;
+  p.positions_out = positions_out;
+  p.lens_out = lens_out;
+  p.keep = keep;
+  p.recent = recent;
+  p.cap = (long)s->pages_per_seq * s->page_size;
+  p.most_moves = evict_most_moves(s, keep);
+  const size_t bh = (size_t)s->batch * s->kv_heads;
+  p.moves = reinterpret_cast<int2*>(workspace);
+  p.n_moves = reinterpret_cast<int*>(static_cast<uint8_t*>(workspace) + up(bh * p.most_moves * sizeof(int2)));
+  CAPI_CUDA(evict_launch(p, static_cast<cudaStream_t>(stream)));
+  return TTTJ_OK;
+}
+
+}  // extern "C"

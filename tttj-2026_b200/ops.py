@@ -101,3 +101,235 @@ def selftest_wait_timeout(status: torch.Tensor, limit_ns: int) -> None:
     """Launch the bounded-wait self test (writes 0x1ff into ``status`` on timeout)."""
     _need(status.dtype == torch.int32 and status.is_cuda, "selftest: status must be a CUDA int32 tensor")
     _lib.check(_lib.lib().tttj_selftest_wait_timeout(_ptr(status), int(limit_ns), _stream(status.device)), "selftest")
+
+
+# ------------------------------------------------------------------ serving operators
+# Prompts with grouped heads, and a paged key/value cache: append, attention of new tokens,
+# the attention mass each slot gathers, eviction.  Common to all of them:
+#
+# * Tokens of all sequences are packed: sequence b owns rows seq_offsets[b] ..
+#   seq_offsets[b + 1] (int32 [B + 1] on the device).  Rows behind the last sequence are left
+#   as they were, so a batch may be padded.
+# * q [T, heads, head_dim], k / v [T, kv_heads, head_dim], fp16 or bf16, head_dim 32, 64, 128
+#   or 256, the last dimension contiguous, other strides any positive multiples of 8 (views
+#   of one packed projection will do).  Query head h reads key/value head
+#   h // (heads // kv_heads).
+# * A cache is [pages, page_size, kv_heads, head_dim] for k and for v (any stride order: pass a
+#   transposed view for heads-first pages), page_size 16 .. 256; page_table int32 [B, P] holds
+#   each sequence's pages in order, cache_lens int32 [B] its tokens, the new ones included.
+#   New token i of n is at slot len - n + i.
+# * Lengths, offsets and page numbers are read on the device only: calls can be captured into
+#   CUDA graphs and replayed with new ones.  They are bounds-checked there; ``status`` (int32
+#   [1], zeroed by the caller) records a wrong one (include/tttj_b200.h, TTTJ_DEV_BAD_*).
+# * Launches go to the current stream of the tensors' device, whichever device is current.
+# * Inference only: tensors that require gradients are refused while gradients are enabled.
+
+_SERVE_DTYPES = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
+
+
+def _call(device: torch.device, fn, *args) -> int:
+    """Run a C entry point with ``device`` current, its current stream as last argument."""
+    if torch.cuda.current_device() == device.index:
+        return fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    with torch.cuda.device(device):
+        return fn(*args, torch.cuda.current_stream(device).cuda_stream)
+
+
+def _serve_rows(what: str, name: str, t: torch.Tensor, like: torch.Tensor, heads: Optional[int] = None) -> _lib.TttjRows:
+    if t.dim() != 3 or t.dtype != like.dtype or t.device != like.device:
+        raise ValueError(f"{what}: {name} must be [tokens, heads, head_dim], {like.dtype} on {like.device}")
+    if t.shape[0] != like.shape[0] or t.shape[2] != like.shape[2] or (heads is not None and t.shape[1] != heads):
+        raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}")
+    s = t.stride()
+    if s[2] != 1:
+        raise ValueError(f"{what}: head_dim of {name} must be contiguous")
+    return _lib.TttjRows(t.data_ptr(), s[0], s[1])
+
+
+def _serve_ints(what: str, name: str, t: torch.Tensor, shape: tuple, device: torch.device) -> int:
+    if t.dtype != torch.int32 or t.shape != shape or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{what}: {name} must be a contiguous int32 tensor {list(shape)} on {device}")
+    return t.data_ptr()
+
+
+def _serve_pages(what: str, name: str, t: torch.Tensor, like: torch.Tensor) -> _lib.TttjPages:
+    if t.dim() != 4 or t.dtype != like.dtype or t.device != like.device or t.shape != like.shape:
+        raise ValueError(f"{what}: {name} must be [pages, page_size, kv_heads, head_dim], {like.dtype} on {like.device}")
+    s = t.stride()
+    if s[3] != 1:
+        raise ValueError(f"{what}: head_dim of {name} must be contiguous")
+    return _lib.TttjPages(t.data_ptr(), s[0], s[1], s[2])
+
+
+def _serve_seqs(what: str, rows: torch.Tensor, seq_offsets: Optional[torch.Tensor], heads: int, kv_heads: int,
+                cache: Optional[torch.Tensor] = None, page_table: Optional[torch.Tensor] = None,
+                cache_lens: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None,
+                tokens: int = 0) -> _lib.TttjSeqs:
+    """The call's tttj_seqs; ``rows`` gives dtype, device and head_dim (its last dimension)."""
+    dtype = _SERVE_DTYPES.get(rows.dtype)
+    if dtype is None:
+        raise ValueError(f"{what}: dtype {rows.dtype} unsupported (float16, bfloat16)")
+    device = rows.device
+    if device.type != "cuda":
+        raise ValueError(f"{what}: tensors must be on a CUDA device")
+    if torch.is_grad_enabled() and rows.requires_grad:
+        raise ValueError(f"{what}: inference only (no gradient)")
+    stat = None if status is None else _serve_ints(what, "status", status, (1,), device)
+    if seq_offsets is not None:
+        if seq_offsets.dim() != 1 or seq_offsets.shape[0] < 2:
+            raise ValueError(f"{what}: seq_offsets must be [sequences + 1]")
+        batch = seq_offsets.shape[0] - 1
+        off = _serve_ints(what, "seq_offsets", seq_offsets, (batch + 1,), device)
+    else:
+        batch, off = cache_lens.shape[0], None
+    if cache is None:
+        return _lib.TttjSeqs(off, None, None, 0, batch, tokens, 0, 0, 0, dtype, heads, kv_heads, rows.shape[-1], stat)
+    if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.device != device or \
+            page_table.shape[0] != batch or page_table.stride(1) != 1:
+        raise ValueError(f"{what}: page_table must be int32 [{batch}, pages per sequence] on {device}, rows contiguous")
+    lens = _serve_ints(what, "cache_lens", cache_lens, (batch,), device)
+    stride = page_table.stride(0) if batch > 1 else page_table.shape[1]
+    return _lib.TttjSeqs(off, lens, page_table.data_ptr(), stride, batch, tokens, page_table.shape[1],
+                         cache.shape[1], cache.shape[0], dtype, heads, kv_heads, rows.shape[-1], stat)
+
+
+def _serve_workspace(what: str, workspace: Optional[torch.Tensor], nbytes: int, device: torch.device) -> torch.Tensor:
+    if nbytes == 0:
+        _lib.check(_lib.TTTJ_ERR_INVALID, what)
+    if workspace is None:
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    if workspace.dtype != torch.uint8 or workspace.device != device or not workspace.is_contiguous():
+        raise ValueError(f"{what}: workspace must be a contiguous uint8 tensor on {device}")
+    return workspace
+
+
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_offsets: torch.Tensor, *,
+                     causal: bool = True, scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                     return_lse: bool = False, workspace: Optional[torch.Tensor] = None,
+                     status: Optional[torch.Tensor] = None):
+    """Attention inside each packed sequence: out[i] = softmax(scale q[i] k^T) v over the
+    tokens j <= i of the same sequence (all of them with ``causal=False``).
+
+    scale defaults to head_dim^-0.5.  Returns out [T, heads, head_dim] in q's dtype (``out``
+    may be given; it must not overlap the inputs), with ``return_lse`` also the fp32 [T, heads]
+    log-sum-exp of the scaled scores.  ``workspace`` (uint8,
+    ``serve_workspace_bytes(...)``) may be kept between calls that do not overlap."""
+    what = "prompt_attention"
+    if q.dim() != 3 or k.dim() != 3:
+        raise ValueError(f"{what}: q and k must be [tokens, heads, head_dim]")
+    heads, kv_heads = q.shape[1], k.shape[1]
+    s = _serve_seqs(what, q, seq_offsets, heads, kv_heads, status=status, tokens=q.shape[0])
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    rq, rk = _serve_rows(what, "q", q, q), _serve_rows(what, "k", k, q)
+    rv, ro = _serve_rows(what, "v", v, q, kv_heads), _serve_rows(what, "out", out, q, heads)
+    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
+    L = _lib.lib()
+    p = ctypes.byref(s)
+    ws = _serve_workspace(what, workspace, L.tttj_serve_workspace_bytes(p), q.device)
+    rc = _call(q.device, L.tttj_prompt_attention, p, ctypes.byref(rq), ctypes.byref(rk), ctypes.byref(rv),
+               ctypes.byref(ro), lse.data_ptr() if return_lse else None, 1 if causal else 0,
+               q.shape[2] ** -0.5 if scale is None else float(scale), ws.data_ptr(), ws.numel())
+    if rc:
+        _lib.check(rc, what)
+    return (out, lse) if return_lse else out
+
+
+def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+                    seq_offsets: torch.Tensor, cache_lens: torch.Tensor, *, max_new: Optional[int] = None,
+                    scale: Optional[float] = None, out: Optional[torch.Tensor] = None, return_lse: bool = False,
+                    workspace: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None):
+    """Attention of each sequence's new tokens over its cache (their own keys and values
+    appended before): new token i of n sees slots 0 .. len - n + i.
+
+    ``max_new``: the most new tokens a sequence of this call has, if known (1 for a decode
+    step); it picks the kernels and need not be exact.  Returns as ``prompt_attention``."""
+    what = "cache_attention"
+    if q.dim() != 3 or k_cache.dim() != 4:
+        raise ValueError(f"{what}: q must be [tokens, heads, head_dim], k_cache [pages, page_size, kv_heads, head_dim]")
+    heads, kv_heads = q.shape[1], k_cache.shape[2]
+    s = _serve_seqs(what, q, seq_offsets, heads, kv_heads, k_cache, page_table, cache_lens, status, q.shape[0])
+    if k_cache.dtype != q.dtype or k_cache.device != q.device or k_cache.shape[3] != q.shape[2]:
+        raise ValueError(f"{what}: the cache must be {q.dtype} on {q.device} with head_dim {q.shape[2]}")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    rq, ro = _serve_rows(what, "q", q, q), _serve_rows(what, "out", out, q, heads)
+    ck, cv = _serve_pages(what, "k_cache", k_cache, k_cache), _serve_pages(what, "v_cache", v_cache, k_cache)
+    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
+    L = _lib.lib()
+    p = ctypes.byref(s)
+    ws = _serve_workspace(what, workspace, L.tttj_serve_workspace_bytes(p), q.device)
+    rc = _call(q.device, L.tttj_cache_attention, p, ctypes.byref(rq), ctypes.byref(ck), ctypes.byref(cv),
+               ctypes.byref(ro), lse.data_ptr() if return_lse else None, 0 if max_new is None else max_new,
+               q.shape[2] ** -0.5 if scale is None else float(scale), ws.data_ptr(), ws.numel())
+    if rc:
+        _lib.check(rc, what)
+    return (out, lse) if return_lse else out
+
+
+def _slot_tensor(what: str, name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple, device: torch.device) -> int:
+    if t.dtype != dtype or t.shape != shape or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{what}: {name} must be a contiguous {dtype} tensor {list(shape)} "
+                         f"(sequences, kv_heads, slots) on {device}")
+    return t.data_ptr()
+
+
+def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                 page_table: torch.Tensor, seq_offsets: torch.Tensor, cache_lens: torch.Tensor, *,
+                 positions: Optional[torch.Tensor] = None, mass: Optional[torch.Tensor] = None,
+                 seen: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> None:
+    """Write the new tokens' keys and values to their slots of the cache.
+
+    With ``positions`` (int32) / ``mass`` (fp32), both [B, kv_heads, P * page_size], a new
+    slot's position becomes seen[b] - n + i and its mass 0; ``seen`` int32 [B] counts the tokens
+    of each sequence, new ones included (default cache_lens; they differ once tokens were
+    evicted)."""
+    what = "cache_append"
+    if k.dim() != 3 or k_cache.dim() != 4:
+        raise ValueError(f"{what}: k must be [tokens, kv_heads, head_dim], k_cache [pages, page_size, kv_heads, head_dim]")
+    kv_heads = k.shape[1]
+    s = _serve_seqs(what, k, seq_offsets, kv_heads, kv_heads, k_cache, page_table, cache_lens, status, k.shape[0])
+    if k_cache.dtype != k.dtype or k_cache.device != k.device or k_cache.shape[2:] != k.shape[1:]:
+        raise ValueError(f"{what}: the cache must be {k.dtype} on {k.device} with rows {list(k.shape[1:])}")
+    rk, rv = _serve_rows(what, "k", k, k), _serve_rows(what, "v", v, k, kv_heads)
+    ck, cv = _serve_pages(what, "k_cache", k_cache, k_cache), _serve_pages(what, "v_cache", v_cache, k_cache)
+    slots = (s.batch, kv_heads, s.pages_per_seq * s.page_size)
+    pos = None if positions is None else _slot_tensor(what, "positions", positions, torch.int32, slots, k.device)
+    ms = None if mass is None else _slot_tensor(what, "mass", mass, torch.float32, slots, k.device)
+    sn = None if seen is None else _serve_ints(what, "seen", seen, (s.batch,), k.device)
+    rc = _call(k.device, _lib.lib().tttj_cache_append, ctypes.byref(s), ctypes.byref(rk), ctypes.byref(rv),
+               ctypes.byref(ck), ctypes.byref(cv), pos, ms, sn)
+    if rc:
+        _lib.check(rc, what)
+
+
+def cache_evict(mass: torch.Tensor, positions: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                page_table: torch.Tensor, cache_lens: torch.Tensor, keep: int, *, recent: int = 0,
+                status: Optional[torch.Tensor] = None):
+    """Evict down to ``keep`` slots per sequence and key/value head, those of least mass.
+
+    mass fp32 and positions int32 [B, kv_heads, P * page_size].  Slots whose position is among
+    the head's ``recent`` newest stay; of the others the largest masses (equal ones: the
+    lower slot; NaN counts as -inf).  Kept slots behind the budget move into the freed ones in
+    front of it, the i-th into the i-th, in both caches (whose pages must be the sequence's own);
+    all others keep their place, so the cache is no longer in the tokens' order.  Returns new
+    (mass, positions, cache_lens): 0 and -1 behind the new lengths min(len, keep)."""
+    what = "cache_evict"
+    if k_cache.dim() != 4 or cache_lens.dim() != 1 or cache_lens.shape[0] < 1:
+        raise ValueError(f"{what}: k_cache must be [pages, page_size, kv_heads, head_dim], cache_lens [sequences]")
+    kv_heads = k_cache.shape[2]
+    s = _serve_seqs(what, k_cache, None, kv_heads, kv_heads, k_cache, page_table, cache_lens, status)
+    ck, cv = _serve_pages(what, "k_cache", k_cache, k_cache), _serve_pages(what, "v_cache", v_cache, k_cache)
+    slots = (s.batch, kv_heads, s.pages_per_seq * s.page_size)
+    ms = _slot_tensor(what, "mass", mass, torch.float32, slots, k_cache.device)
+    pos = _slot_tensor(what, "positions", positions, torch.int32, slots, k_cache.device)
+    L = _lib.lib()
+    p = ctypes.byref(s)
+    ws = _serve_workspace(what, None, L.tttj_cache_evict_workspace_bytes(p, keep), k_cache.device)
+    mass_out, pos_out = torch.empty_like(mass), torch.empty_like(positions)
+    lens_out = torch.empty_like(cache_lens)
+    rc = _call(k_cache.device, L.tttj_cache_evict, p, ctypes.byref(ck), ctypes.byref(cv), ms, pos, keep, recent,
+               mass_out.data_ptr(), pos_out.data_ptr(), lens_out.data_ptr(), ws.data_ptr(), ws.numel())
+    if rc:
+        _lib.check(rc, what)
+    return mass_out, pos_out, lens_out
