@@ -503,9 +503,10 @@ __device__ __forceinline__ uint64_t desc_mnmajor_sw64(uint32_t smem_addr, uint32
 // Instruction descriptor for kind::f16 with fp16 A and B, fp32 D, both operands
 // K-major unless flagged: D format bits [4,6) = 1 (F32), A/B format bits [7,10) and
 // [10,13) = 0 (F16), A major bit 15, B major bit 16, N >> 3 in [17,23), M >> 4 in [24,29).
+// bf16 = 1: both operands bf16 (format 1).
 __host__ __device__ constexpr uint32_t idesc_f16_f32(int M, int N, int a_mn_major = 0,
-                                                     int b_mn_major = 0) {
-  return (1u << 4) | ((uint32_t)a_mn_major << 15) | ((uint32_t)b_mn_major << 16) |
+                                                     int b_mn_major = 0, int bf16 = 0) {
+  return (1u << 4) | ((uint32_t)bf16 << 7) | ((uint32_t)bf16 << 10) | ((uint32_t)a_mn_major << 15) | ((uint32_t)b_mn_major << 16) |
          ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 

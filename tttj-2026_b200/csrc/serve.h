@@ -65,6 +65,11 @@ __device__ __forceinline__ int srv_page(const SrvSeqs& s, int b, int slot) {
   return s.num_pages;
 }
 
+struct CacheView {
+  void* data;
+  long page, slot, head;  // element strides
+};
+
 // ---- attention of few query rows per sequence (serve_step.cuh) ----
 struct StepParams {
   SrvSeqs s;
@@ -77,7 +82,6 @@ struct StepParams {
   float scale_log2;
   float* part_o;       // [2 * grid][STEP_ROWS][head_dim] partial outputs
   float2* part_ml;     // [2 * grid][STEP_ROWS] their (max, sum)
-  int most_rows;       // sequences with more rows (tokens x group) are not handled here
   unsigned long long wait_limit_ns;
 };
 constexpr int STEP_ROWS = 16;   // query rows of one mma tile
@@ -86,11 +90,46 @@ constexpr int step_ctas_per_sm(int hd) { return hd == 256 ? 1 : 2; }
 cudaError_t step_launch(const CUtensorMap& tm_k, const CUtensorMap& tm_v, const StepParams& p,
                         int head_dim, int bf16, int grid, cudaStream_t stream);
 
-// ---- cache append / evict (serve_cache.cu) ----
-struct CacheView {
-  void* data;
-  long page, slot, head;  // element strides
+// ---- attention of many query rows per sequence (serve_tile.cuh) ----
+// Query rows of a key/value head: row = token x group + head of the group; a tile takes
+// the rows of floor(128 / group) tokens, an item NT tiles (two; one at head_dim 256).
+struct TileEntry {    // one item of every key/value head
+  int b, q;           // sequence, item of the sequence
+  int j0, j1;         // key tiles [j0, j1)
+  int part;           // first of kv_heads partial-result slots, or -1: whole items
+  int pad[3];
 };
+struct TileJoin {     // an entry whose keys were split
+  int b, q, pieces, part;  // piece i of head h is slot part + i * kv_heads + h
+};
+struct TilePlan {     // in the workspace, rebuilt by every call
+  int* counters;      // [4]: items taken, entries, joins, items to redo
+  TileEntry* entries; // [most_entries]
+  TileJoin* joins;    // [most_entries]
+  int* redo;          // [2 * most_entries * kv_heads][3]: b, q, h
+  int most_entries;
+  int most_parts;     // partial-result slots
+};
+struct TileParams {
+  SrvSeqs s;
+  const void* q;       // for rows computed again
+  long q_tok, q_head;
+  CacheView k, v;      // the same (prompts: page 0)
+  void* out;
+  long o_tok, o_head;
+  float* lse;
+  int heads, kv_heads, group, tile_tokens;
+  float scale_log2;
+  TilePlan plan;
+  float* part_o;       // [most_parts][NT * 128][head_dim]
+  float2* part_ml;     // [most_parts][NT * 128]
+  unsigned long long wait_limit_ns;
+};
+constexpr int tile_nt(int hd) { return hd == 256 ? 1 : 2; }
+cudaError_t tile_launch(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v,
+                        const TileParams& p, int head_dim, int bf16, int grid, cudaStream_t stream);
+
+// ---- cache append / evict (serve_cache.cu) ----
 struct AppendParams {
   SrvSeqs s;
   const void* k;

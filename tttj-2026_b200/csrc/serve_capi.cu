@@ -83,6 +83,8 @@ SrvSeqs seqs_of(const tttj_seqs* s, bool cache, int causal) {
   return r;
 }
 
+CacheView view_of(const tttj_pages* c) { return {c->data, c->page_stride, c->slot_stride, c->head_stride}; }
+
 // 4-D map {head_dim, slots, heads, pages} of keys or values, moved in boxes of one
 // head's `box_rows` slots x min(head_dim, 64) columns, swizzled by the box's row width.
 int kv_map(CUtensorMap* m, const char* what, const tttj_seqs* s, const void* data, long page_stride,
@@ -107,6 +109,27 @@ int kv_map(CUtensorMap* m, const char* what, const tttj_seqs* s, const void* dat
   return TTTJ_OK;
 }
 
+// 3-D map {head_dim, heads, tokens} of queries, moved in boxes of one key/value head's
+// group x `tokens` tokens x min(head_dim, 64) columns.
+int q_map(CUtensorMap* m, const char* what, const tttj_seqs* s, const tttj_rows* q, int tokens) {
+  auto fn = capi_encode_fn();
+  if (!fn) return capi_fail(TTTJ_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  const int cols = s->head_dim < 64 ? s->head_dim : 64;
+  const long one = s->head_dim;
+  cuuint64_t dims[3] = {(cuuint64_t)s->head_dim, (cuuint64_t)s->heads, (cuuint64_t)s->tokens};
+  cuuint64_t strides[2] = {(cuuint64_t)(s->heads > 1 ? q->head_stride : one) * 2,
+                           (cuuint64_t)(s->tokens > 1 ? q->token_stride : one) * 2};
+  cuuint32_t box[3] = {(cuuint32_t)cols, (cuuint32_t)(s->heads / s->kv_heads), (cuuint32_t)tokens};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r =
+      fn(m, s->dtype == TTTJ_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+         const_cast<void*>(q->data), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+         cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return capi_fail(TTTJ_ERR_INVALID, "%s: strides out of range (%d)", what, (int)r);
+  return TTTJ_OK;
+}
+
 int sm_count_here(int* sms) {
   int dev = 0;
   CAPI_CUDA(cudaGetDevice(&dev));
@@ -115,12 +138,18 @@ int sm_count_here(int* sms) {
   return TTTJ_OK;
 }
 
-constexpr int kMostSms = 256;  // workspace sizes hold for any device of at most this many
+constexpr int kMostSms = 160;  // multiprocessors that a call uses at most (workspace sizes)
+// Sequences of at most this many query rows per key/value head (new tokens x group) run on
+// the few-row kernel, chunks of more on the tile kernel.
+constexpr int kStepMostRows = 16;
 
+// Workspace of either attention kernel.
 struct ServeWs {
-  size_t part_o, part_ml, total;
+  size_t part_o, part_ml, entries, joins, redo, counters, total;
+  int most_entries, most_parts;
 };
-ServeWs serve_ws(const tttj_seqs* s) {
+int tile_tokens(const tttj_seqs* s) { return ATC_BM / (s->heads / s->kv_heads); }
+ServeWs step_ws(const tttj_seqs* s) {
   ServeWs w{};
   const size_t parts = 2ul * kMostSms * step_ctas_per_sm(s->head_dim) * STEP_ROWS;
   w.part_o = 0;
@@ -128,10 +157,36 @@ ServeWs serve_ws(const tttj_seqs* s) {
   w.total = w.part_ml + up(parts * 8);
   return w;
 }
+ServeWs tile_ws(const tttj_seqs* s) {
+  ServeWs w{};
+  // Bounds of tile_plan_kernel: cut items leave at most 4 pieces per CTA (and one per head).
+  w.most_parts = 4 * kMostSms + s->kv_heads;
+  w.most_entries = s->tokens / (tile_nt(s->head_dim) * tile_tokens(s)) + s->batch + w.most_parts;
+  const size_t rows = (size_t)w.most_parts * tile_nt(s->head_dim) * ATC_BM;
+  w.counters = 0;
+  w.entries = up(16);
+  w.joins = w.entries + up((size_t)w.most_entries * sizeof(TileEntry));
+  w.redo = w.joins + up((size_t)w.most_entries * sizeof(TileJoin));
+  w.part_ml = w.redo + up((size_t)w.most_entries * s->kv_heads * 2 * 3 * 4);
+  w.part_o = w.part_ml + up(rows * 8);
+  w.total = w.part_o + up(rows * s->head_dim * 4);
+  return w;
+}
+bool step_runs(const tttj_seqs* s, bool cache, int max_new) {
+  const long new_tokens = max_new > 0 && max_new < s->tokens ? max_new : s->tokens;
+  return cache && new_tokens * (s->heads / s->kv_heads) <= kStepMostRows;
+}
+size_t serve_bytes(const tttj_seqs* s) {
+  const size_t a = step_ws(s).total, b = tile_ws(s).total;
+  return a > b ? a : b;
+}
 
-int check_attention(const char* what, const tttj_seqs* s, float scale, const void* workspace,
-                    size_t workspace_bytes) {
-  const size_t need = serve_ws(s).total;
+// One call of either attention: packed keys / values (cache = false; page strides unused,
+// slots are tokens) or a cache.
+int attention(const char* what, const tttj_seqs* s, const tttj_rows* q, const CacheView& k, const CacheView& v,
+              const tttj_rows* out, float* lse, int causal, int max_new, float scale, void* workspace,
+              size_t workspace_bytes, bool cache, cudaStream_t stream) {
+  const size_t need = serve_bytes(s);
   if (!workspace || workspace_bytes < need)
     return capi_fail(TTTJ_ERR_INVALID, "%s: workspace too small: %zu < %zu", what, workspace ? workspace_bytes : 0,
                      need);
@@ -139,21 +194,48 @@ int check_attention(const char* what, const tttj_seqs* s, float scale, const voi
     return capi_fail(TTTJ_ERR_INVALID, "%s: workspace must be 256-byte aligned", what);
   if (!(scale > 0.f) || !isfinite(scale))
     return capi_fail(TTTJ_ERR_INVALID, "%s: scale must be positive and finite", what);
-  return TTTJ_OK;
-}
-
-int attention(const tttj_seqs* s, const tttj_rows* q, const tttj_rows* out, float* lse, int causal, float scale,
-              void* workspace, bool cache, const CUtensorMap& tm_k, const CUtensorMap& tm_v, cudaStream_t stream) {
-  const ServeWs w = serve_ws(s);
   int sms = 0;
   TRY(sm_count_here(&sms));
   if (sms > kMostSms) sms = kMostSms;
+  const bool step = step_runs(s, cache, max_new);
+  const int keys = step ? STEP_KEYS : ATC_BN;
+  const int slots = cache ? s->page_size : s->tokens, pages = cache ? s->num_pages : 1;
+  const int box = cache && s->page_size < keys ? s->page_size : keys;
+  CUtensorMap tm_k, tm_v;
+  TRY(kv_map(&tm_k, what, s, k.data, k.page, k.slot, k.head, slots, pages, box));
+  TRY(kv_map(&tm_v, what, s, v.data, v.page, v.slot, v.head, slots, pages, box));
   uint8_t* base = static_cast<uint8_t*>(workspace);
-  StepParams p{};
+  const int bf16 = s->dtype == TTTJ_DTYPE_BF16;
+  const float scale_log2 = scale * 1.44269504088896341f;
+  if (step) {
+    const ServeWs w = step_ws(s);
+    StepParams p{};
+    p.s = seqs_of(s, cache, causal);
+    p.q = q->data;
+    p.q_tok = q->token_stride;
+    p.q_head = q->head_stride;
+    p.out = const_cast<void*>(out->data);
+    p.o_tok = out->token_stride;
+    p.o_head = out->head_stride;
+    p.lse = lse;
+    p.heads = s->heads;
+    p.kv_heads = s->kv_heads;
+    p.group = s->heads / s->kv_heads;
+    p.scale_log2 = scale_log2;
+    p.part_o = reinterpret_cast<float*>(base + w.part_o);
+    p.part_ml = reinterpret_cast<float2*>(base + w.part_ml);
+    p.wait_limit_ns = TTTJ_WAIT_LIMIT_NS;
+    CAPI_CUDA(step_launch(tm_k, tm_v, p, s->head_dim, bf16, sms * step_ctas_per_sm(s->head_dim), stream));
+    return TTTJ_OK;
+  }
+  const ServeWs w = tile_ws(s);
+  TileParams p{};
   p.s = seqs_of(s, cache, causal);
   p.q = q->data;
   p.q_tok = q->token_stride;
   p.q_head = q->head_stride;
+  p.k = k;
+  p.v = v;
   p.out = const_cast<void*>(out->data);
   p.o_tok = out->token_stride;
   p.o_head = out->head_stride;
@@ -161,13 +243,20 @@ int attention(const tttj_seqs* s, const tttj_rows* q, const tttj_rows* out, floa
   p.heads = s->heads;
   p.kv_heads = s->kv_heads;
   p.group = s->heads / s->kv_heads;
-  p.scale_log2 = scale * 1.44269504088896341f;
+  p.tile_tokens = tile_tokens(s);
+  p.scale_log2 = scale_log2;
+  p.plan.counters = reinterpret_cast<int*>(base + w.counters);
+  p.plan.entries = reinterpret_cast<TileEntry*>(base + w.entries);
+  p.plan.joins = reinterpret_cast<TileJoin*>(base + w.joins);
+  p.plan.redo = reinterpret_cast<int*>(base + w.redo);
+  p.plan.most_entries = w.most_entries;
+  p.plan.most_parts = w.most_parts;
   p.part_o = reinterpret_cast<float*>(base + w.part_o);
   p.part_ml = reinterpret_cast<float2*>(base + w.part_ml);
-  p.most_rows = INT32_MAX;
   p.wait_limit_ns = TTTJ_WAIT_LIMIT_NS;
-  CAPI_CUDA(step_launch(tm_k, tm_v, p, s->head_dim, s->dtype == TTTJ_DTYPE_BF16,
-                        sms * step_ctas_per_sm(s->head_dim), stream));
+  CUtensorMap tm_q;
+  TRY(q_map(&tm_q, what, s, q, p.tile_tokens));
+  CAPI_CUDA(tile_launch(tm_q, tm_k, tm_v, p, s->head_dim, bf16, sms, stream));
   return TTTJ_OK;
 }
 
@@ -177,7 +266,7 @@ extern "C" {
 
 size_t tttj_serve_workspace_bytes(const tttj_seqs* s) {
   if (check_seqs("serve_workspace_bytes", s, false, false)) return 0;
-  return serve_ws(s).total;
+  return serve_bytes(s);
 }
 
 int tttj_prompt_attention(const tttj_seqs* s, const tttj_rows* q, const tttj_rows* k, const tttj_rows* v,
@@ -190,11 +279,9 @@ int tttj_prompt_attention(const tttj_seqs* s, const tttj_rows* q, const tttj_row
   TRY(check_rows(what, "v", v, s, s->kv_heads));
   TRY(check_rows(what, "out", out, s, s->heads));
   if (s->tokens == 0) return TTTJ_OK;
-  TRY(check_attention(what, s, scale, workspace, workspace_bytes));
-  CUtensorMap tm_k, tm_v;
-  TRY(kv_map(&tm_k, what, s, k->data, 0, k->token_stride, k->head_stride, s->tokens, 1, STEP_KEYS));
-  TRY(kv_map(&tm_v, what, s, v->data, 0, v->token_stride, v->head_stride, s->tokens, 1, STEP_KEYS));
-  return attention(s, q, out, lse, causal ? 1 : 0, scale, workspace, false, tm_k, tm_v,
+  const CacheView kv{const_cast<void*>(k->data), 0, k->token_stride, k->head_stride};
+  const CacheView vv{const_cast<void*>(v->data), 0, v->token_stride, v->head_stride};
+  return attention(what, s, q, kv, vv, out, lse, causal ? 1 : 0, 0, scale, workspace, workspace_bytes, false,
                    static_cast<cudaStream_t>(stream));
 }
 
@@ -209,14 +296,8 @@ int tttj_cache_attention(const tttj_seqs* s, const tttj_rows* q, const tttj_page
   TRY(check_pages(what, "v_cache", v_cache, s));
   if (max_new < 0) return capi_fail(TTTJ_ERR_INVALID, "%s: max_new=%d is negative", what, max_new);
   if (s->tokens == 0) return TTTJ_OK;
-  TRY(check_attention(what, s, scale, workspace, workspace_bytes));
-  const int box = s->page_size < STEP_KEYS ? s->page_size : STEP_KEYS;
-  CUtensorMap tm_k, tm_v;
-  TRY(kv_map(&tm_k, what, s, k_cache->data, k_cache->page_stride, k_cache->slot_stride, k_cache->head_stride,
-             s->page_size, s->num_pages, box));
-  TRY(kv_map(&tm_v, what, s, v_cache->data, v_cache->page_stride, v_cache->slot_stride, v_cache->head_stride,
-             s->page_size, s->num_pages, box));
-  return attention(s, q, out, lse, 1, scale, workspace, true, tm_k, tm_v, static_cast<cudaStream_t>(stream));
+  return attention(what, s, q, view_of(k_cache), view_of(v_cache), out, lse, 1, max_new, scale, workspace,
+                   workspace_bytes, true, static_cast<cudaStream_t>(stream));
 }
 
 int tttj_cache_append(const tttj_seqs* s, const tttj_rows* k, const tttj_rows* v, const tttj_pages* k_cache,
@@ -237,8 +318,8 @@ int tttj_cache_append(const tttj_seqs* s, const tttj_rows* k, const tttj_rows* v
   p.k_head = k->head_stride;
   p.v_tok = v->token_stride;
   p.v_head = v->head_stride;
-  p.kc = {k_cache->data, k_cache->page_stride, k_cache->slot_stride, k_cache->head_stride};
-  p.vc = {v_cache->data, v_cache->page_stride, v_cache->slot_stride, v_cache->head_stride};
+  p.kc = view_of(k_cache);
+  p.vc = view_of(v_cache);
   p.kv_heads = s->kv_heads;
   p.head_dim = s->head_dim;
   p.positions = positions;
@@ -282,8 +363,8 @@ int tttj_cache_evict(const tttj_seqs* s, const tttj_pages* k_cache, const tttj_p
     return capi_fail(TTTJ_ERR_INVALID, "%s: workspace must be 256-byte aligned", what);
   EvictParams p{};
   p.s = seqs_of(s, true, 1);
-  p.kc = {k_cache->data, k_cache->page_stride, k_cache->slot_stride, k_cache->head_stride};
-  p.vc = {v_cache->data, v_cache->page_stride, v_cache->slot_stride, v_cache->head_stride};
+  p.kc = view_of(k_cache);
+  p.vc = view_of(v_cache);
   p.kv_heads = s->kv_heads;
   p.head_dim = s->head_dim;
   p.mass = mass;

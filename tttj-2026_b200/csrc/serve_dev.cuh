@@ -1,0 +1,86 @@
+// Device helpers shared by the serving kernels.
+#pragma once
+#include <cuda_bf16.h>
+
+#include "common.cuh"
+#include "serve.h"
+
+namespace tttj {
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t srv_pack(float a, float b) {
+  if constexpr (BF16) {
+    __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&h);
+  } else {
+    return pack_half2(a, b);
+  }
+}
+
+template <bool BF16>
+__device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                          uint32_t b1) {
+  if constexpr (BF16) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  } else {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+}
+
+__device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm_x4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* tmap, uint32_t bar, int c0, int c1,
+                                            int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+
+// Whether one of the two 16-bit floats of a word is infinite or NaN.
+template <bool BF16>
+__device__ __forceinline__ bool srv_nonfinite(uint32_t w) {
+  constexpr uint32_t e = BF16 ? 0x7f80u : 0x7c00u;
+  return (w & e) == e || ((w >> 16) & e) == e;
+}
+template <bool BF16>
+__device__ __forceinline__ float srv_to_float(uint32_t half_bits) {
+  if constexpr (BF16) return __uint_as_float(half_bits << 16);
+  return __half2float(__ushort_as_half((unsigned short)half_bits));
+}
+
+// max(a, b, c), NaN if any of them is.
+__device__ __forceinline__ float srv_max3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// Natural log-sum-exp of a row from its maximum (log2 domain) and sum: -inf for a row that
+// sees no key, NaN where its scores hold one.
+__device__ __forceinline__ float srv_lse(float top, float sum) {
+  if (top == -INFINITY) return sum == 0.f ? -INFINITY : sum;
+  return (top + log2f(sum)) * 0.69314718055994531f;
+}
+
+}  // namespace tttj

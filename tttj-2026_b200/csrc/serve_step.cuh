@@ -15,81 +15,9 @@
 //   * a run that does not cover a row block's whole key range leaves (max, sum, O) in
 //     the workspace, and a second small kernel joins the runs of each row in order.
 #pragma once
-#include <cuda_bf16.h>
-
-#include "common.cuh"
-#include "serve.h"
+#include "serve_dev.cuh"
 
 namespace tttj {
-
-template <bool BF16>
-__device__ __forceinline__ uint32_t srv_pack(float a, float b) {
-  if constexpr (BF16) {
-    __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<uint32_t*>(&h);
-  } else {
-    return pack_half2(a, b);
-  }
-}
-
-template <bool BF16>
-__device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
-                                          uint32_t b1) {
-  if constexpr (BF16) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-        "{%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  } else {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-        "{%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  }
-}
-
-__device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
-}
-__device__ __forceinline__ void ldsm_x4_trans(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
-}
-
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* tmap, uint32_t bar, int c0, int c1,
-                                            int c2, int c3) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
-      : "memory");
-}
-
-// Whether one of the two 16-bit floats of a word is infinite or NaN.
-template <bool BF16>
-__device__ __forceinline__ bool srv_nonfinite(uint32_t w) {
-  constexpr uint32_t e = BF16 ? 0x7f80u : 0x7c00u;
-  return (w & e) == e || ((w >> 16) & e) == e;
-}
-template <bool BF16>
-__device__ __forceinline__ float srv_to_float(uint32_t half_bits) {
-  if constexpr (BF16) return __uint_as_float(half_bits << 16);
-  return __half2float(__ushort_as_half((unsigned short)half_bits));
-}
-
-// Natural log-sum-exp of a row from its maximum (log2 domain) and sum: -inf for a row that
-// sees no key, NaN where its scores hold one.
-__device__ __forceinline__ float srv_lse(float top, float sum) {
-  if (top == -INFINITY) return sum == 0.f ? -INFINITY : sum;
-  return (top + log2f(sum)) * 0.69314718055994531f;
-}
 
 template <int HD>
 struct StepSmem {
@@ -115,16 +43,16 @@ constexpr int STEP_MIN_UNITS = 2;
 struct StepBlocks {  // row blocks and key tiles of a sequence
   int blocks, tiles;
 };
-__device__ __forceinline__ StepBlocks step_blocks(const SrvSeq& q, int group, int most_rows) {
+__device__ __forceinline__ StepBlocks step_blocks(const SrvSeq& q, int group) {
   StepBlocks r;
   const long rows = (long)q.n * group;
-  r.blocks = rows > most_rows ? 0 : (int)((rows + STEP_ROWS - 1) / STEP_ROWS);
+  r.blocks = (int)((rows + STEP_ROWS - 1) / STEP_ROWS);
   r.tiles = max(1, (q.len + STEP_KEYS - 1) / STEP_KEYS);
   return r;
 }
 __device__ __forceinline__ long step_units(const StepParams& p, int b) {
   const SrvSeq q = srv_seq(p.s, b);
-  const StepBlocks k = step_blocks(q, p.group, p.most_rows);
+  const StepBlocks k = step_blocks(q, p.group);
   return (long)k.blocks * k.tiles * p.kv_heads;
 }
 
@@ -169,7 +97,7 @@ __device__ __forceinline__ StepRun step_run(const StepParams& p, const long* pre
   StepRun r;
   r.b = lo;
   r.q = srv_seq(p.s, lo);
-  const StepBlocks k = step_blocks(r.q, p.group, p.most_rows);
+  const StepBlocks k = step_blocks(r.q, p.group);
   const long at = u - pre[lo];
   const long blk = at / k.tiles;
   r.tiles = k.tiles;
@@ -540,7 +468,7 @@ __global__ void __launch_bounds__(32 * STEP_JOIN_WARPS)
       if (p.s.seq_off[mid] <= tok) lo = mid; else hi = mid - 1;
     }
     const SrvSeq q = srv_seq(p.s, lo);
-    const StepBlocks k = step_blocks(q, p.group, p.most_rows);
+    const StepBlocks k = step_blocks(q, p.group);
     work = tok >= q.row0 && tok < q.row0 + q.n && k.blocks > 0;
     if (work) {
       const int qrow = (tok - q.row0) * p.group + head % p.group;

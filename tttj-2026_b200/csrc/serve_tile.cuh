@@ -1,0 +1,937 @@
+// Attention of many query rows per sequence -- prompts and chunks of new tokens -- on the
+// 5th-generation tensor cores: S = Q K^T and O += P V by tcgen05, S, P and O in TMEM.
+//
+// The query rows of one key/value head are packed into tiles of 128: row = token x group
+// + head of the group (floor(128 / group) tokens per tile), so the heads of a group share
+// every K / V tile and a chunk of few tokens still fills the tensor core's 128 lanes.
+// Keys come in tiles of 128 from packed rows or from the pages of a cache (one TMA box per
+// page piece and 64 columns).
+//
+// Three kernels:
+//   tile_plan_kernel  one block turns the device-side offsets and lengths into a work list,
+//                     longest items first.  An item is NT query tiles of one head.  Items
+//                     that would leave CTAs idle -- those of a last, partial wave, and any
+//                     longer than a CTA's fair share -- are cut along the keys.
+//   tile_kernel       persistent CTAs (1 per SM) of 11 warps take items in turn: a TMA
+//                     loader, one MMA-issuing warp and four softmax warps per query tile
+//                     (one thread per row), running statistics in fp32, O rescaled only
+//                     when a row's maximum grew by more than 2^8.
+//   tile_join_kernel  joins the pieces of cut items in the order of their keys.
+//
+// Hidden keys.  Scores of keys a row does not see are replaced by -inf.  Their values still
+// meet P = 0 in the product, and 0 x NaN is NaN: V rows behind the last key are zeroed in
+// shared memory, and a tile that some row sees only in part is searched for infinite or NaN
+// values while the softmax works on its scores.  Where one is found the item is noted, and
+// the joining kernel computes its rows again, one warp per row, key by key.
+//
+// Every wait is bounded; a role that gives up records SRV_DEV_TIMEOUT and unwinds.
+#pragma once
+#include "attention_tc.cuh"
+#include "serve_dev.cuh"
+
+namespace tttj {
+
+struct TileInfo {  // one decoded item, in shared memory
+  int b, q, h, row0, n, len, tok0, part;
+  int j0;     // first key tile of this piece
+  int n_kv;   // key tiles of this piece; -1: no more items
+  int nt[2];  // key tiles of query tile 0 / 1 inside this piece
+};
+static_assert(sizeof(TileInfo) <= 64, "item info slot is 64 bytes");
+
+constexpr int TILE_MIN_PIECE = 4;  // key tiles (512 keys) a cut piece has at least
+
+// Keys that the tokens [tok0, tok0 + tokens) of a sequence see (their last one's limit).
+__device__ __forceinline__ int tile_kv_end(const SrvSeq& q, int causal, int tok0, int tokens) {
+  if (!causal) return q.len;
+  const int last = min(tok0 + tokens, q.n) - 1;
+  return max(0, min(q.len, q.len - q.n + last + 1));
+}
+__device__ __forceinline__ int tile_kv_tiles(int kv_end) { return max(1, (kv_end + ATC_BN - 1) / ATC_BN); }
+
+// ------------------------------------------------------------------------------ plan
+constexpr int TILE_PLAN_THREADS = 1024;
+constexpr int TILE_BUCKETS = 1024;
+
+__global__ void __launch_bounds__(TILE_PLAN_THREADS) tile_plan_kernel(const TileParams p, int nt, int grid) {
+  __shared__ int s_pre[SRV_MAX_BATCH + 1];  // items before each sequence
+  __shared__ int s_n[SRV_MAX_BATCH], s_len[SRV_MAX_BATCH];
+  __shared__ int s_hist[TILE_BUCKETS];
+  __shared__ int s_warp[32];
+  __shared__ unsigned long long s_all, s_rest;
+  __shared__ int s_joins, s_parts, s_entries;
+  griddep_wait();
+  griddep_launch();
+  const int tid = threadIdx.x, batch = p.s.batch;
+  const int item_tokens = nt * p.tile_tokens;
+  if (tid == 0) {
+    s_all = s_rest = 0;
+    s_joins = s_parts = s_entries = 0;
+  }
+  s_hist[tid] = 0;
+  // Two sequences per thread: items, then their prefix sums.
+  int cnt[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int b = 2 * tid + i;
+    if (b < batch) {
+      const SrvSeq q = srv_seq(p.s, b);
+      s_n[b] = q.n;
+      s_len[b] = q.len;
+      cnt[i] = (q.n + item_tokens - 1) / item_tokens;
+    }
+  }
+  // Sums saturate: offsets that do not rise may claim more items than there are rows for.
+  constexpr int FULL_SUM = 1 << 29;
+  int x = min(cnt[0], FULL_SUM / 2) + min(cnt[1], FULL_SUM / 2);
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int o = __shfl_up_sync(0xffffffffu, x, d);
+    if ((tid & 31) >= d) x = min(x + o, FULL_SUM);
+  }
+  if ((tid & 31) == 31) s_warp[tid >> 5] = x;
+  __syncthreads();
+  if (tid < 32) {
+    int w = s_warp[tid];
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, w, d);
+      if (tid >= d) w = min(w + o, FULL_SUM);
+    }
+    s_warp[tid] = w;
+  }
+  __syncthreads();
+  const bool rising = s_warp[31] <= p.s.tokens / item_tokens + batch;
+  if (!rising) {
+    if (tid == 0) {
+      report_status(p.s.status, SRV_DEV_BAD_LENS);
+      p.plan.counters[0] = p.plan.counters[1] = p.plan.counters[2] = p.plan.counters[3] = 0;
+    }
+    return;
+  }
+  const int before = (tid >= 32 ? s_warp[(tid >> 5) - 1] : 0) + x - cnt[0] - cnt[1];
+  if (2 * tid <= batch) s_pre[2 * tid] = before;
+  if (2 * tid + 1 <= batch) s_pre[2 * tid + 1] = before + cnt[0];
+  if (tid == 0) s_pre[batch] = s_warp[31];
+  __syncthreads();
+  const int items = s_pre[batch];  // per key/value head
+  auto locate = [&](int e, int* b) {
+    int lo = 0, hi = batch - 1;  // last b with s_pre[b] <= e
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (s_pre[mid] <= e) lo = mid; else hi = mid - 1;
+    }
+    *b = lo;
+    return e - s_pre[lo];
+  };
+  auto tiles_of = [&](int b, int q) {
+    SrvSeq s;
+    s.n = s_n[b];
+    s.len = s_len[b];
+    return tile_kv_tiles(tile_kv_end(s, p.s.causal, q * item_tokens, item_tokens));
+  };
+  // Whole waves of items stay whole; with at least four waves the last one is short
+  // against the rest.  Which items are cut depends on their number alone, not on the
+  // order in which threads run: results repeat exactly.
+  const long all_items = (long)items * p.kv_heads;
+  const long waves = all_items / grid;
+  const int whole = waves >= 4 ? items : (int)(waves * grid / p.kv_heads);
+  unsigned long long sum = 0, rest = 0;
+  for (int e = tid; e < items; e += TILE_PLAN_THREADS) {
+    int b;
+    const int q = locate(e, &b);
+    const int t = tiles_of(b, q);
+    sum += t;
+    if (e >= whole) rest += t;
+  }
+  if (sum) atomicAdd(&s_all, sum);
+  if (rest) atomicAdd(&s_rest, rest);
+  __syncthreads();
+  const long share = (long)(s_all * p.kv_heads + grid - 1) / grid;
+  const int most = (int)max(share, (long)TILE_MIN_PIECE);
+  const int most_rest = (int)max((long)(s_rest * p.kv_heads + grid - 1) / grid, (long)TILE_MIN_PIECE);
+  auto pieces_of = [&](int e, int t) {
+    const int c = e >= whole ? min(most, most_rest) : most;
+    return (t + c - 1) / c;
+  };
+  auto bucket = [&](int len) { return TILE_BUCKETS - min(len, TILE_BUCKETS); };  // longest first
+  for (int e = tid; e < items; e += TILE_PLAN_THREADS) {
+    int b;
+    const int q = locate(e, &b);
+    const int t = tiles_of(b, q), n = pieces_of(e, t);
+    atomicAdd(&s_hist[bucket((t + n - 1) / n)], n);
+  }
+  __syncthreads();
+  {
+    const int v = s_hist[tid];
+    int y = v;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, y, d);
+      if ((tid & 31) >= d) y += o;
+    }
+    if ((tid & 31) == 31) s_warp[tid >> 5] = y;
+    __syncthreads();
+    if (tid < 32) {
+      int w = s_warp[tid];
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, w, d);
+        if (tid >= d) w += o;
+      }
+      s_warp[tid] = w;
+    }
+    __syncthreads();
+    const int base = (tid >= 32 ? s_warp[(tid >> 5) - 1] : 0) + y - v;
+    s_hist[tid] = base;
+    if (tid == TILE_PLAN_THREADS - 1) s_entries = base + v;
+  }
+  __syncthreads();
+  for (int e = tid; e < items; e += TILE_PLAN_THREADS) {
+    TileEntry out{};
+    out.q = locate(e, &out.b);
+    const int t = tiles_of(out.b, out.q), n = pieces_of(e, t);
+    int part = -1;
+    if (n > 1) {
+      part = atomicAdd(&s_parts, n * p.kv_heads);
+      p.plan.joins[atomicAdd(&s_joins, 1)] = TileJoin{out.b, out.q, n, part};
+    }
+    const int at = atomicAdd(&s_hist[bucket((t + n - 1) / n)], n);
+    for (int i = 0; i < n; ++i) {
+      out.j0 = (int)((long)t * i / n);
+      out.j1 = (int)((long)t * (i + 1) / n);
+      out.part = n > 1 ? part + i * p.kv_heads : -1;
+      p.plan.entries[at + i] = out;
+    }
+  }
+  __syncthreads();
+  if (tid == 0) {
+    p.plan.counters[0] = 0;
+    p.plan.counters[1] = s_entries;
+    p.plan.counters[2] = s_joins;
+    p.plan.counters[3] = 0;
+  }
+}
+
+// -------------------------------------------------------------------------- attention
+template <int HD, bool BF16>
+__global__ void __launch_bounds__(ATC_THREADS, 1)
+    tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                const __grid_constant__ CUtensorMap tmV, const TileParams p) {
+  using SM = AtcSmem<HD>;
+  constexpr int STAGES = SM::STAGES;
+  constexpr int NT = SM::NT;
+  constexpr int QBUF = SM::QBUF;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t pad = (1024u - (raw & 1023u)) & 1023u;
+  uint8_t* smem = smem_raw + pad;
+  const uint32_t sQ = smem_u32(smem);
+  const uint32_t sKV = sQ + SM::Q_BYTES;
+  const uint32_t bar0 = sKV + SM::KV_BYTES;
+  const uint32_t bar_q_full = bar0;                        // [QS]
+  const uint32_t bar_q_empty = bar0 + 8 * SM::QS;          // [QS]
+  const uint32_t bar_kv_full = bar0 + 16 * SM::QS;         // [STAGES]
+  const uint32_t bar_kv_empty = bar_kv_full + 8 * STAGES;  // [STAGES]
+  const uint32_t bar_s_full = bar_kv_empty + 8 * STAGES;   // [2]
+  const uint32_t bar_p_full = bar_s_full + 16;             // [2]
+  const uint32_t bar_o_full = bar_p_full + 16;             // [2]
+  const uint32_t bar_o_free = bar_o_full + 16;             // [2]
+  const uint32_t bar_s_free = bar_o_free + 16;             // [2] scores read by softmax
+  const uint32_t bar_pv_done = bar_s_free + 16;            // [2] P V complete
+  const uint32_t bar_drain = bar_pv_done + 16;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + SM::Q_BYTES + SM::KV_BYTES + SM::NBAR * 8);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  TileInfo* info = reinterpret_cast<TileInfo*>(smem + SM::Q_BYTES + SM::KV_BYTES + SM::NBAR * 8 + 16);
+  const uint32_t sEpi = smem_u32(smem + SM::Q_BYTES + SM::KV_BYTES + SM::NBAR * 8 + 16 + SM::INFO_BYTES);
+
+  const int warp = warp_id();
+  const int lane = lane_id();
+  const uint64_t limit = p.wait_limit_ns;
+  const int TOK = p.tile_tokens;
+  const bool paged = p.s.table != nullptr;
+
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+    for (int i = 0; i < SM::QS; ++i) {
+      mbar_init(bar_q_full + 8 * i, 1);
+      mbar_init(bar_q_empty + 8 * i, NT + NT * ATC_BM);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar_s_full + 8 * i, 1);
+      mbar_init(bar_p_full + 8 * i, ATC_BM);
+      mbar_init(bar_o_full + 8 * i, 1);
+      mbar_init(bar_o_free + 8 * i, ATC_BM);
+      mbar_init(bar_s_free + 8 * i, ATC_BM);
+      mbar_init(bar_pv_done + 8 * i, 1);
+    }
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(bar_kv_full + 8 * s, 1);
+      mbar_init(bar_kv_empty + 8 * s, NT);
+    }
+    mbar_init(bar_drain, 1);
+    mbar_init(bar_drain + 8, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    fence_proxy_async_smem();
+  }
+  if (warp == 9) {
+    tmem_alloc(smem_u32(tmem_slot), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  griddep_wait();
+  griddep_launch();
+  const long n_items = (long)p.plan.counters[1] * p.kv_heads;
+
+  if (warp == 8) {
+    // ------------------------------------------------------------ TMA loader
+    // The whole warp runs the loop: each lane issues the boxes of its page pieces.
+    const int cr = paged ? min(ATC_BN, 1 << p.s.page_shift) : ATC_BN;
+    const int boxes = (ATC_BN / cr) * SM::NBOX * 2;  // <= 64
+    const uint32_t q_bytes = (uint32_t)(TOK * p.group * HD * 2);
+    bool ok = true;
+    long kvc = 0;  // KV tiles issued
+    int k = 0;     // items issued (including the final "no more items" marker)
+    for (;; ++k) {
+      int it = 0;
+      if (lane == 0) it = atomicAdd(p.plan.counters, 1);
+      it = __shfl_sync(0xffffffffu, it, 0);
+      const bool stop = it >= n_items;
+      TileInfo w{};
+      w.n_kv = -1;
+      if (!stop) {
+        const TileEntry e = p.plan.entries[it / p.kv_heads];
+        const SrvSeq s = srv_seq(p.s, e.b);
+        w.b = e.b;
+        w.q = e.q;
+        w.h = it % p.kv_heads;
+        w.row0 = s.row0;
+        w.n = s.n;
+        w.len = s.len;
+        w.tok0 = e.q * NT * TOK;
+        w.j0 = e.j0;
+        w.part = e.part < 0 ? -1 : e.part + w.h;
+        w.n_kv = 0;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const int t0 = w.tok0 + t * TOK;
+          const int tiles = tile_kv_tiles(tile_kv_end(s, p.s.causal, t0, TOK));
+          w.nt[t] = t0 < s.n ? max(0, min(tiles, e.j1) - e.j0) : 0;
+          w.n_kv = max(w.n_kv, w.nt[t]);
+        }
+      }
+      const int qb = k % QBUF;
+      ok = __all_sync(0xffffffffu, mbar_wait(bar_q_empty + 8 * qb, ((k / QBUF) & 1) ^ 1u, abort_flag, limit));
+      if (!ok) break;
+      if (lane == 0) {
+        info[qb] = w;  // published by the release of the arrive below
+        if (stop) {
+          mbar_arrive(bar_q_full + 8 * qb);
+        } else {
+          const int nq = w.tok0 + TOK < w.n && NT == 2 ? 2 : 1;
+          mbar_arrive_expect_tx(bar_q_full + 8 * qb, nq * q_bytes);
+          for (int t = 0; t < nq; ++t)
+            for (int x = 0; x < SM::NBOX; ++x)
+              tma_load_3d(sQ + (qb * NT + t) * SM::Q_TILE + x * SM::BOX_BYTES, &tmQ, bar_q_full + 8 * qb,
+                          x * SM::BOX_COLS, w.h * p.group, w.row0 + w.tok0 + t * TOK);
+        }
+      }
+      __syncwarp();
+      if (stop) break;
+      for (int j = 0; j < w.n_kv; ++j, ++kvc) {
+        const int st = (int)(kvc % STAGES);
+        const int base = (w.j0 + j) * ATC_BN;
+        // Page numbers are fetched before the wait for the stage.
+        int page[2] = {0, 0}, c1[2] = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int id = lane + 32 * i;
+          const int slot = base + (id / (2 * SM::NBOX)) * cr;
+          c1[i] = w.row0 + slot;
+          if (paged && id < boxes) {
+            page[i] = slot < w.len ? srv_page(p.s, w.b, slot) : p.s.num_pages;
+            c1[i] = slot & ((1 << p.s.page_shift) - 1);
+          }
+        }
+        ok = __all_sync(0xffffffffu, mbar_wait(bar_kv_empty + 8 * st, (uint32_t)((kvc / STAGES) & 1) ^ 1u,
+                                               abort_flag, limit));
+        if (!ok) break;
+        const uint32_t dst = sKV + st * 2 * SM::KV_TILE;
+        const uint32_t bar = bar_kv_full + 8 * st;
+        if (lane == 0) mbar_arrive_expect_tx(bar, 2 * SM::KV_TILE);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int id = lane + 32 * i;
+          if (id < boxes) {
+            const int kv = id & 1, x = (id >> 1) % SM::NBOX, c = id / (2 * SM::NBOX);
+            tma_load_4d(dst + kv * SM::KV_TILE + x * SM::BOX_BYTES + c * cr * SM::BOX_COLS * 2, kv ? &tmV : &tmK,
+                        bar, x * SM::BOX_COLS, c1[i], w.h, page[i]);
+          }
+        }
+        __syncwarp();
+      }
+      if (!ok) break;
+    }
+    if (!ok && lane == 0) {
+      *abort_flag = 1;
+      report_status(p.s.status, SRV_DEV_TIMEOUT);
+      // Let issued loads land before the CTA can exit.
+      for (long j = kvc > STAGES ? kvc - STAGES : 0; j < kvc; ++j)
+        mbar_wait(bar_kv_full + 8 * (int)(j % STAGES), (uint32_t)((j / STAGES) & 1), nullptr, limit);
+      for (int i = k > QBUF ? k - QBUF : 0; i < k; ++i)
+        mbar_wait(bar_q_full + 8 * (i % QBUF), (uint32_t)((i / QBUF) & 1), nullptr, limit);
+    }
+  } else if (warp == 9 || (warp == 10 && NT == 2)) {
+    // ------------------------------------------------------------ MMA issuers
+    // One warp per query tile, as in attention_tc.cuh: the whole warp runs the loop, one
+    // elected lane issues.
+    constexpr unsigned FULL = 0xffffffffu;
+    const int t = warp - 9;
+    constexpr uint32_t idesc_s = idesc_f16_f32(ATC_BM, ATC_BN, 0, 0, BF16);
+    constexpr uint32_t idesc_o = idesc_f16_f32(ATC_BM, HD, 0, 1, BF16);
+    constexpr uint32_t v_step = HD == 32 ? (1024u >> 4) : (2048u >> 4);
+    const uint32_t s_col = t == 0 ? SM::TMEM_S0 : SM::TMEM_S1;
+    const uint32_t p_col = t == 0 ? SM::TMEM_P0 : SM::TMEM_P1;
+    const uint32_t o_col = t == 0 ? SM::TMEM_O0 : SM::TMEM_O1;
+    bool ok = true;
+    bool issued = false;
+    long kvc = 0;         // KV tiles of all items so far
+    long kv_waited = -1;  // highest KV tile index whose arrival this warp observed
+    long pc = 0, sfc = 0, oc = 0, pvc = 0;
+    int k = 0;
+    auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
+      if (!__all_sync(FULL, mbar_wait(bar, parity, abort_flag, limit))) {
+        ok = false;
+        return false;
+      }
+      tc_fence_after();
+      return true;
+    };
+    auto ensure_kv = [&](long idx) -> bool {
+      while (kv_waited < idx) {
+        ++kv_waited;
+        if (!wait(bar_kv_full + 8 * (int)(kv_waited % STAGES), (uint32_t)((kv_waited / STAGES) & 1))) return false;
+      }
+      return true;
+    };
+    for (; ok; ++k) {
+      const int qb = k % QBUF;
+      if (!wait(bar_q_full + 8 * qb, (k / QBUF) & 1)) break;
+      const int n_kv = __shfl_sync(FULL, info[qb].n_kv, 0);
+      if (n_kv < 0) break;  // no more items
+      const int tq = atc_query_tile<NT>(t, k);
+      const int n = __shfl_sync(FULL, info[qb].nt[tq], 0);
+      const int len = __shfl_sync(FULL, info[qb].len, 0);
+      const int j0 = __shfl_sync(FULL, info[qb].j0, 0);
+      // Keys from here on are hidden from some row of the tile.
+      const int all_see = p.s.causal
+                              ? len - __shfl_sync(FULL, info[qb].n, 0) + __shfl_sync(FULL, info[qb].tok0, 0) + tq * TOK + 1
+                              : len;
+      bool noted = false;
+      const uint32_t qaddr = sQ + (qb * NT + tq) * SM::Q_TILE;
+      auto issue_s = [&](long kv_idx) {
+        const uint32_t kaddr = sKV + (int)(kv_idx % STAGES) * 2 * SM::KV_TILE;
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk)
+          mma_f16_ss_warp(tmem + s_col, atc_desc_qk<HD>(qaddr, kk), atc_desc_qk<HD>(kaddr, kk), idesc_s,
+                          kk > 0 ? 1u : 0u);
+        mma_commit_warp(bar_s_full + 8 * t);
+        issued = true;
+      };
+      // While the softmax works on the scores of item key tile j: V rows behind the last
+      // key become zeros (both warps may write the same ones), and a partly hidden tile
+      // is searched for values that a product with P = 0 would not hide.
+      auto clean_v = [&](long kv_idx, int j) {
+        const int base = (j0 + j) * ATC_BN;
+        if (base + ATC_BN <= all_see) return;  // warp-uniform
+        const int keep = max(0, min(ATC_BN, len - base));
+        constexpr int ROW_BYTES = SM::BOX_COLS * 2;
+        constexpr int CH = ROW_BYTES / 16;
+        const uint32_t vaddr = sKV + (int)(kv_idx % STAGES) * 2 * SM::KV_TILE + SM::KV_TILE;
+        bool odd = false;
+#pragma unroll 1
+        for (int x = 0; x < SM::NBOX; ++x) {
+          const uint32_t vx = vaddr + (uint32_t)(x * SM::BOX_BYTES);
+#pragma unroll 4
+          for (int i = lane; i < (p.s.causal ? keep * CH : 0); i += 32) {
+            uint32_t w[4];
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                         : "r"(vx + (uint32_t)(i * 16))
+                         : "memory");
+            odd |= srv_nonfinite<BF16>(w[0]) | srv_nonfinite<BF16>(w[1]) | srv_nonfinite<BF16>(w[2]) |
+                   srv_nonfinite<BF16>(w[3]);
+          }
+          for (int i = keep * CH + lane; i < ATC_BN * CH; i += 32)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(vx + (uint32_t)(i * 16)), "r"(0u)
+                         : "memory");
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (__any_sync(FULL, odd) && !noted) {
+          noted = true;
+          if (lane == 0) {
+            const int at = atomicAdd(p.plan.counters + 3, 1);
+            if (at < 2 * p.plan.most_entries * p.kv_heads) {
+              p.plan.redo[3 * at] = info[qb].b;
+              p.plan.redo[3 * at + 1] = info[qb].q;
+              p.plan.redo[3 * at + 2] = info[qb].h;
+            }
+          }
+          __syncwarp();
+        }
+      };
+      auto issue_pv = [&](long kv_idx, bool accumulate) {
+        const uint32_t vaddr = sKV + (int)(kv_idx % STAGES) * 2 * SM::KV_TILE + SM::KV_TILE;
+        const uint64_t vd = atc_desc_v<HD>(vaddr);
+#pragma unroll
+        for (int kk = 0; kk < ATC_BN / 16; ++kk)
+          mma_f16_ts_warp(tmem + o_col, tmem + p_col + (uint32_t)(kk * 8), vd + (uint64_t)(kk * v_step), idesc_o,
+                          (accumulate || kk > 0) ? 1u : 0u);
+        mma_commit_warp(bar_pv_done + 8 * t);
+        issued = true;
+      };
+      if (n > 0) {
+        if (!ensure_kv(kvc)) break;
+        issue_s(kvc);
+        clean_v(kvc, 0);
+      }
+      for (int j = 0; j < n_kv && ok; ++j) {
+        const long kv_j = kvc + j;
+        if (j < n) {
+          if (!SM::P_ALIAS && j + 1 < n) {
+            if (!wait(bar_s_free + 8 * t, (uint32_t)(sfc++ & 1))) break;
+            if (!ensure_kv(kv_j + 1)) break;
+            issue_s(kv_j + 1);
+            clean_v(kv_j + 1, j + 1);
+          }
+          if (!wait(bar_p_full + 8 * t, (uint32_t)(pc++ & 1))) break;
+          // The first P V of an item overwrites O: the previous item's O must be read.
+          if (j == 0 && !wait(bar_o_free + 8 * t, (uint32_t)(oc++ & 1) ^ 1u)) break;
+          issue_pv(kv_j, j > 0);
+          if (j + 1 == n) mma_commit_warp(bar_o_full + 8 * t);
+          mma_commit_warp(bar_kv_empty + 8 * (int)(kv_j % STAGES));
+          if (SM::P_ALIAS) {
+            // The next S of this tile overwrites P(j): P V(j) must have completed.
+            if (!wait(bar_pv_done + 8 * t, (uint32_t)(pvc & 1))) break;
+            if (j + 1 < n) {
+              if (!ensure_kv(kv_j + 1)) break;
+              issue_s(kv_j + 1);
+              clean_v(kv_j + 1, j + 1);
+            }
+          }
+          ++pvc;
+        } else {
+          // Not used by this query tile: release it once it has landed.
+          if (!ensure_kv(kv_j)) break;
+          if (lane == 0) mbar_arrive(bar_kv_empty + 8 * (int)(kv_j % STAGES));
+          __syncwarp();
+        }
+      }
+      if (!ok) break;
+      kvc += n_kv;
+      mma_commit_warp(bar_q_empty + 8 * qb);
+    }
+    if (!ok) {
+      if (lane == 0) {
+        *abort_flag = 1;
+        report_status(p.s.status, SRV_DEV_TIMEOUT);
+      }
+      if (issued) {
+        mma_commit_warp(bar_drain + 8 * t);
+        mbar_wait(bar_drain + 8 * t, 0, nullptr, limit);
+      }
+    }
+  } else if (warp < 4 * NT) {
+    // ------------------------------------------------------------ softmax, warps 0-7
+    const int t = warp >> 2;
+    const int quad = warp & 3;
+    const int row = quad * 32 + lane;  // row inside the query tile
+    const int rtok = row / p.group;    // its token inside the tile, its head in the group
+    const int rhead = row - rtok * p.group;
+    const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
+    const uint32_t s_addr = tmem + lane_base + (t == 0 ? SM::TMEM_S0 : SM::TMEM_S1);
+    const uint32_t p_addr = tmem + lane_base + (t == 0 ? SM::TMEM_P0 : SM::TMEM_P1);
+    const uint32_t o_addr = tmem + lane_base + (t == 0 ? SM::TMEM_O0 : SM::TMEM_O1);
+    const float scale = p.scale_log2;
+    long sc = 0, ofc = 0;
+    long pv_before = 0;
+    bool ok = true;
+    int k = 0;
+    for (; ok; ++k) {
+      const int qb = k % QBUF;
+      if (!mbar_wait(bar_q_full + 8 * qb, (uint32_t)((k / QBUF) & 1), abort_flag, limit)) {
+        ok = false;
+        break;
+      }
+      const TileInfo& wi = info[qb];
+      if (wi.n_kv < 0) break;  // no more items
+      const int tq = atc_query_tile<NT>(t, k);
+      const int n = tq == 0 ? wi.nt[0] : wi.nt[1];
+      const int j0 = wi.j0, len = wi.len, part = wi.part, h = wi.h;
+      const int tok0 = wi.tok0 + tq * TOK;  // first token of the tile
+      const int tokens = wi.n;
+      const int token = wi.row0 + tok0 + rtok;   // packed row of this thread's token
+      const int first = p.s.causal ? len - tokens + tok0 : len - 1;  // last key of the tile's first row
+      mbar_arrive(bar_q_empty + 8 * qb);  // this thread no longer needs the info slot
+      const bool live = rtok < TOK && tok0 + rtok < tokens;
+      const long prow = part < 0 ? 0 : (long)part * (NT * ATC_BM) + tq * ATC_BM + row;
+      if (n == 0) {
+        // No key of this piece for this tile: an empty partial result.
+        if (part >= 0 && live) p.part_ml[prow] = make_float2(-INFINITY, 0.f);
+        continue;
+      }
+      const int row_lim = p.s.causal ? min(len - 1, first + rtok) : len - 1;
+      float m_run = -INFINITY;  // running max (log2 domain) used as the exp base
+      float l_run = 0.f;
+      for (int j = 0; j < n; ++j) {
+        if (!mbar_wait(bar_s_full + 8 * t, (uint32_t)(sc++ & 1), abort_flag, limit)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        uint32_t sv[ATC_BN];  // raw fp32 scores of this thread's row
+#pragma unroll
+        for (int c = 0; c < ATC_BN / 32; ++c) {
+          uint32_t chunk[32];
+          tmem_ld_32x32b_x32(s_addr + (uint32_t)(c * 32), chunk);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) sv[c * 32 + e] = chunk[e];
+        }
+        tmem_wait_ld();
+        if (!SM::P_ALIAS && j + 1 < n) {
+          tc_fence_before();
+          mbar_arrive(bar_s_free + 8 * t);
+        }
+        const int k0 = (j0 + j) * ATC_BN;
+        if (k0 + ATC_BN - 1 > first) {
+          // Column c of this tile is hidden when c > lim.
+          const int lim = row_lim - k0;
+#pragma unroll
+          for (int c = 0; c < ATC_BN; ++c)
+            if (c > lim) sv[c] = __float_as_uint(-INFINITY);
+        }
+        // Row max: 8 independent chains of three-input maxima.
+        float pm[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) pm[i] = __uint_as_float(sv[i]);
+#pragma unroll
+        for (int c = 8; c < ATC_BN; c += 2)
+          pm[(c >> 1) & 7] = srv_max3(pm[(c >> 1) & 7], __uint_as_float(sv[c]), __uint_as_float(sv[c + 1]));
+        const float mx =
+            srv_max3(srv_max3(pm[0], pm[1], pm[2]), srv_max3(pm[3], pm[4], pm[5]), srv_max3(pm[6], pm[7], pm[7]));
+        const float m_tile = mx * scale;
+        float alpha = 1.f;
+        bool rescale = false;
+        if (j == 0) {
+          m_run = m_tile;
+        } else {
+          // Lazy rescale: keep the old base unless the max grew by more than 2^8.  Rows
+          // that no token owns do not vote.
+          const bool grow = live && m_tile > m_run + 8.0f;
+          if (__any_sync(0xffffffff, grow)) {
+            const float m_new = fmaxf(m_run, m_tile);
+            alpha = (m_run == -INFINITY) ? 0.f : ex2_approx(m_run - m_new);
+            m_run = m_new;
+            rescale = true;  // warp-uniform
+          }
+        }
+        // A NaN or +inf score makes the whole row NaN (exp2_fma2 alone would lose it).
+        const float base = !(m_tile < INFINITY) ? NAN : m_run == -INFINITY ? 0.f : m_run;
+        const float2 sc2 = make_float2(scale, scale), nb2 = make_float2(-base, -base);
+        unsigned long long ps2[2] = {0ull, 0ull};  // partial row sums, f32x2 pairs
+        uint32_t pk[4][16];
+        auto exp_chunk = [&](int q) {
+#pragma unroll
+          for (int cc = 0; cc < 16; ++cc) {
+            const int c = q * 16 + cc;
+            const float2 x =
+                ffma2(make_float2(__uint_as_float(sv[2 * c]), __uint_as_float(sv[2 * c + 1])), sc2, nb2);
+            float p0, p1;
+            if ((c & 3) == 3) {
+              const float2 e = exp2_fma2(x);
+              p0 = e.x;
+              p1 = e.y;
+            } else {
+              p0 = ex2_approx(x.x);
+              p1 = ex2_approx(x.y);
+            }
+            ps2[c & 1] = add2p(ps2[c & 1], pk2(p0, p1));
+            pk[q][cc] = srv_pack<BF16>(p0, p1);
+          }
+        };
+#pragma unroll
+        for (int q = 0; q < ATC_P_EARLY; ++q) exp_chunk(q);
+        // P(j) replaces P(j-1), and O is rescaled below: P V(j-1) must be complete (see
+        // attention_tc.cuh).
+        if (!SM::P_ALIAS && j > 0) {
+          if (!mbar_wait(bar_pv_done + 8 * t, (uint32_t)((pv_before + j - 1) & 1), abort_flag, limit)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if (q >= ATC_P_EARLY) exp_chunk(q);
+          tmem_st_32x32b_x16(p_addr + (uint32_t)(q * 16), pk[q]);
+        }
+        const float2 rs2 = upk2(add2p(ps2[0], ps2[1]));
+        l_run = l_run * alpha + (rs2.x + rs2.y);
+        if (rescale) {
+#pragma unroll
+          for (int c = 0; c < HD / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld_32x32b_x32(o_addr + (uint32_t)(c * 32), o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_st_32x32b_x32(o_addr + (uint32_t)(c * 32), o);
+          }
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(bar_p_full + 8 * t);
+      }
+      pv_before += n;
+      if (!ok) break;
+      // A row that saw no key: exp2_fma2 leaves 2^-126 where the exponential of -inf is 0.
+      if (m_run == -INFINITY && l_run == l_run) l_run = 0.f;
+      if (!mbar_wait(bar_o_full + 8 * t, (uint32_t)(ofc++ & 1), abort_flag, limit)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      if (part >= 0) {
+        // A piece: raw sums, joined later.
+        float* dst = p.part_o + prow * HD;
+        if (live) p.part_ml[prow] = make_float2(m_run, l_run);
+#pragma unroll 1
+        for (int c = 0; c < HD / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld_32x32b_x32(o_addr + (uint32_t)(c * 32), o);
+          tmem_wait_ld();
+          if (live) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              *reinterpret_cast<uint4*>(dst + c * 32 + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          }
+        }
+      } else {
+        const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
+        if (live && p.lse != nullptr)
+          p.lse[(long)token * p.heads + h * p.group + rhead] = srv_lse(m_run, l_run);
+        uint16_t* out = static_cast<uint16_t*>(p.out);
+        if constexpr (SM::STAGED_EPI) {
+          // The warp's 32 rows go through shared memory so that the stores cover whole
+          // row segments (16-byte chunk j of row r staged at slot j ^ (r % NCH)).
+          constexpr int NCH = SM::EPI_ROW / 16;
+          const uint32_t stage = sEpi + (uint32_t)(warp * 32 * SM::EPI_ROW);
+#pragma unroll
+          for (int c = 0; c < HD / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld_32x32b_x32(o_addr + (uint32_t)(c * 32), o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const int j = c * 4 + q;
+              const uint32_t a = stage + (uint32_t)(lane * SM::EPI_ROW + ((j ^ (lane % NCH)) << 4));
+              uint32_t w[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                w[e] = srv_pack<BF16>(__uint_as_float(o[8 * q + 2 * e]) * inv, __uint_as_float(o[8 * q + 2 * e + 1]) * inv);
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                           "r"(w[3])
+                           : "memory");
+            }
+          }
+          __syncwarp();
+          constexpr int RPI = 32 / NCH;  // rows per store instruction
+          const int j = lane % NCH;
+#pragma unroll
+          for (int it = 0; it < 32 / RPI; ++it) {
+            const int rr = it * RPI + lane / NCH;
+            const uint32_t a = stage + (uint32_t)(rr * SM::EPI_ROW + ((j ^ (rr % NCH)) << 4));
+            uint4 v;
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                         : "r"(a)
+                         : "memory");
+            const int r2 = quad * 32 + rr;
+            const int tk = r2 / p.group, hd = r2 - tk * p.group;
+            if (tk < TOK && tok0 + tk < tokens)
+              *reinterpret_cast<uint4*>(out + (long)(token - rtok + tk) * p.o_tok +
+                                        (long)(h * p.group + hd) * p.o_head + j * 8) = v;
+          }
+        } else {
+          // Wide heads: each thread stores its own row, 64 bytes per 32 columns.
+          uint16_t* dst = out + (long)token * p.o_tok + (long)(h * p.group + rhead) * p.o_head;
+#pragma unroll 1
+          for (int c = 0; c < HD / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld_32x32b_x32(o_addr + (uint32_t)(c * 32), o);
+            tmem_wait_ld();
+            if (live) {
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                uint32_t w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  w[e] = srv_pack<BF16>(__uint_as_float(o[8 * q + 2 * e]) * inv,
+                                        __uint_as_float(o[8 * q + 2 * e + 1]) * inv);
+                *reinterpret_cast<uint4*>(dst + c * 32 + q * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+              }
+            }
+          }
+        }
+      }
+      __syncwarp();
+      tc_fence_before();
+      mbar_arrive(bar_o_free + 8 * t);
+    }
+    if (!ok) {
+      *abort_flag = 1;
+      report_status(p.s.status, SRV_DEV_TIMEOUT);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ------------------------------------------------------------------------------- join
+template <int HD, bool BF16>
+__device__ __forceinline__ void tile_store_row(const TileParams& p, int token, int head,
+                                               const float (&acc)[HD / 32], float inv, float top, float sum) {
+  const int lane = lane_id();
+  const long at = (long)token * p.o_tok + (long)head * p.o_head + lane * (HD / 32);
+  if constexpr (HD == 32) {
+    if constexpr (BF16)
+      static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16(acc[0] * inv);
+    else
+      static_cast<__half*>(p.out)[at] = __float2half(acc[0] * inv);
+  } else {
+    uint32_t* dst = static_cast<uint32_t*>(p.out) + at / 2;
+#pragma unroll
+    for (int i = 0; i < HD / 64; ++i) dst[i] = srv_pack<BF16>(acc[2 * i] * inv, acc[2 * i + 1] * inv);
+  }
+  if (p.lse != nullptr && lane == 0) p.lse[(long)token * p.heads + head] = srv_lse(top, sum);
+}
+
+constexpr int TILE_JOIN_WARPS = 8;
+
+// One row key by key, hidden keys left out: for items in which a hidden value is infinite
+// or NaN.
+template <int HD, bool BF16>
+__device__ void tile_redo_row(const TileParams& p, const SrvSeq& s, int b, int tok, int kvh, int g) {
+  const int lane = lane_id();
+  constexpr int E = HD / 32;
+  const int token = s.row0 + tok, head = kvh * p.group + g;
+  const uint16_t* q = static_cast<const uint16_t*>(p.q) + (long)token * p.q_tok + (long)head * p.q_head + lane * E;
+  float qv[E], acc[E], m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    qv[i] = srv_to_float<BF16>(q[i]);
+    acc[i] = 0.f;
+  }
+  const int keys = p.s.causal ? min(s.len, s.len - s.n + tok + 1) : s.len;
+  for (int j = 0; j < keys; ++j) {
+    long at_k, at_v;
+    bool there = true;
+    if (p.s.table != nullptr) {
+      const int page = srv_page(p.s, b, j), in = j & ((1 << p.s.page_shift) - 1);
+      there = page < p.s.num_pages;
+      at_k = page * p.k.page + in * p.k.slot;
+      at_v = page * p.v.page + in * p.v.slot;
+    } else {
+      at_k = (long)(s.row0 + j) * p.k.slot;
+      at_v = (long)(s.row0 + j) * p.v.slot;
+    }
+    const uint16_t* kr = static_cast<const uint16_t*>(p.k.data) + at_k + kvh * p.k.head + lane * E;
+    const uint16_t* vr = static_cast<const uint16_t*>(p.v.data) + at_v + kvh * p.v.head + lane * E;
+    float dot = 0.f;
+    if (there)
+#pragma unroll
+      for (int i = 0; i < E; ++i) dot = fmaf(qv[i], srv_to_float<BF16>(kr[i]), dot);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
+    const float x = dot * p.scale_log2;
+    const float m_new = fmaxf(m, x);
+    const float base = m_new == -INFINITY ? 0.f : m_new;
+    const float alpha = m == m_new ? 1.f : ex2_approx(m - m_new);
+    const float e = ex2_approx(x - base);
+    m = m_new;
+    l = l * alpha + e;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      if (alpha != 1.f) acc[i] *= alpha;
+      if (there) acc[i] = fmaf(e, srv_to_float<BF16>(vr[i]), acc[i]);
+    }
+  }
+  tile_store_row<HD, BF16>(p, token, head, acc, l == 0.f ? 0.f : 1.f / l, m, l);
+}
+
+template <int HD, bool BF16>
+__global__ void __launch_bounds__(32 * TILE_JOIN_WARPS) tile_join_kernel(const TileParams p) {
+  constexpr int NT = AtcSmem<HD>::NT;
+  constexpr int ROWS = NT * ATC_BM;
+  griddep_wait();
+  const int joins = p.plan.counters[2];
+  const int redo = min(p.plan.counters[3], 2 * p.plan.most_entries * p.kv_heads);
+  const int lane = lane_id();
+  const long w0 = (long)blockIdx.x * TILE_JOIN_WARPS + warp_id(), step = (long)gridDim.x * TILE_JOIN_WARPS;
+  for (long i = w0; i < (long)joins * p.kv_heads * ROWS; i += step) {
+    const int r = (int)(i % ROWS);
+    const int h = (int)(i / ROWS % p.kv_heads);
+    const TileJoin e = p.plan.joins[i / ROWS / p.kv_heads];
+    const int rtok = (r % ATC_BM) / p.group, g = (r % ATC_BM) - rtok * p.group;
+    const int tok = (e.q * NT + r / ATC_BM) * p.tile_tokens + rtok;
+    const SrvSeq s = srv_seq(p.s, e.b);
+    if (rtok >= p.tile_tokens || tok >= s.n) continue;
+    bool noted = false;
+    for (int c = 0; c < redo; ++c)
+      noted |= p.plan.redo[3 * c] == e.b && p.plan.redo[3 * c + 1] == e.q && p.plan.redo[3 * c + 2] == h;
+    if (noted) continue;
+    auto at = [&](int piece) { return ((long)e.part + (long)piece * p.kv_heads + h) * ROWS + r; };
+    float top = -INFINITY;
+    for (int c = lane; c < e.pieces; c += 32) top = fmaxf(top, p.part_ml[at(c)].x);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    float acc[HD / 32], sum = 0.f;
+#pragma unroll
+    for (int x = 0; x < HD / 32; ++x) acc[x] = 0.f;
+    for (int c = 0; c < e.pieces; ++c) {
+      const float2 ml = p.part_ml[at(c)];
+      const float f = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - top);
+      sum += ml.y * f;
+      if (ml.x == -INFINITY && ml.y == 0.f) continue;  // nothing was stored for it
+#pragma unroll
+      for (int x = 0; x < HD / 32; ++x) acc[x] += p.part_o[at(c) * HD + lane * (HD / 32) + x] * f;
+    }
+    tile_store_row<HD, BF16>(p, s.row0 + tok, h * p.group + g, acc, sum == 0.f ? 0.f : 1.f / sum, top, sum);
+  }
+  // Items with a hidden infinite or NaN value (left out above where they were also cut).
+  for (long i = w0; i < (long)redo * ROWS; i += step) {
+    const int* e = p.plan.redo + 3 * (i / ROWS);
+    const int r = (int)(i % ROWS);
+    const int rtok = (r % ATC_BM) / p.group, g = (r % ATC_BM) - rtok * p.group;
+    const int tok = (e[1] * NT + r / ATC_BM) * p.tile_tokens + rtok;
+    const SrvSeq s = srv_seq(p.s, e[0]);
+    if (rtok >= p.tile_tokens || tok >= s.n) continue;
+    tile_redo_row<HD, BF16>(p, s, e[0], tok, e[2], g);
+  }
+}
+
+}  // namespace tttj
