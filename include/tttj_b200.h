@@ -383,6 +383,14 @@ int tttj_cache_append(const tttj_seqs* s, const tttj_rows* k, const tttj_rows* v
                       const tttj_pages* k_cache, const tttj_pages* v_cache, int32_t* positions,
                       float* mass, const int32_t* seen, void* stream);
 
+/* Attention mass: mass_out[b][g][j] = mass + sum over the new tokens i that see slot j and
+ * the query heads h of key/value head g of exp(scale q_ih k_jg - lse_ih), with the lse
+ * [tokens][heads] that the attention of the same queries returned.  mass, mass_out
+ * [batch][kv_heads][pages_per_seq * page_size] contiguous; mass_out may be mass; slots
+ * behind a sequence's length are copied.  max_new as in tttj_cache_attention. */
+int tttj_cache_mass(const tttj_seqs* s, const tttj_rows* q, const float* lse, const tttj_pages* k_cache,
+                    const float* mass, float* mass_out, int max_new, float scale, void* stream);
+
 /* Evict down to `keep` slots per sequence and key/value head.  A slot's value is its mass
  * (NaN counts as -inf), +inf for positions within `recent` of the head's newest; the
  * `keep` largest stay, equal ones by lower slot.  Slots that stay behind the budget move

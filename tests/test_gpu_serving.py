@@ -450,3 +450,169 @@ def test_cache_evict_long(length):
     lens = [length, 30000]
     c, mass, pos = _evict_case(lens, 1, 32, 256, torch.float16, 9)
     _check_evict(c, mass, pos, lens, 8000, 100)
+
+
+# -------------------------------------------------------------------------- gathered mass
+def _check_mass(got, mass, q, lse, c, new, lens, scale):
+    """Each probability is off by its score's error ds (see above), the log-sum-exp's
+    rounding in the log2 domain (2^-23 of its size) and the exponential's 2^-22; sums of m
+    terms by m 2^-24 relative, taken as one."""
+    d = q.shape[2]
+    at = 0
+    want, tol = mass.double(), torch.zeros_like(mass, dtype=torch.float64)
+    for b, (n, m) in enumerate(zip(new, lens)):
+        if n and m:
+            k = cache_rows(c.k, c.table, b, m)
+            g = q.shape[1] // k.shape[1]
+            s = torch.einsum("nhd,mhd->hnm", q[at:at + n].double(), k.double().repeat_interleave(g, 1)) * scale
+            sa = torch.einsum("nhd,mhd->hnm", q[at:at + n].double().abs(), k.double().abs().repeat_interleave(g, 1))
+            hidden = torch.ones(n, m, dtype=torch.bool, device=DEV).triu(m - n + 1)
+            w = torch.exp(s - lse[at:at + n].double().t()[:, :, None]).masked_fill(hidden, 0)
+            e = w * (d * 2.0**-24 * sa * scale + 2.0**-21 * (1 + s.abs() + lse[at:at + n].double().t().abs()[:, :, None]))
+            want[b, :, :m] += w.view(k.shape[1], -1, m).sum(1)
+            tol[b, :, :m] += e.view(k.shape[1], -1, m).sum(1)
+        at += n
+    tol += (sum(new) * q.shape[1] + 2) * 2.0**-24 * want.abs()
+    err = (got.double() - want).abs()
+    assert bool((err <= tol + 1e-30).all()), f"{float((err / (tol + 1e-30)).max()):.2f} times the tolerance"
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [32, 64, 128, 256])
+@pytest.mark.parametrize("heads,kv,page", [(8, 2, 16), (3, 3, 32), (10, 2, 128), (16, 1, 256), (6, 2, 64)])
+@pytest.mark.parametrize("new,lens", [([1, 1, 1, 1, 1], [1, 16, 127, 129, 1000]),
+                                      ([5, 0, 1, 130, 33, 300], [5, 40, 700, 130, 500, 301])])
+def test_cache_mass(dtype, d, heads, kv, page, new, lens):
+    c = Cache(lens, kv, d, page, dtype, d + page)
+    q = (1.5 * torch.randn(sum(new), heads, d, device=DEV, generator=_gen(2))).to(dtype)
+    off, scale = lengths_to_offsets(new), d**-0.5
+    mass = torch.rand(len(lens), kv, c.table.shape[1] * page, device=DEV, generator=_gen(3))
+    _, lse = ops.cache_attention(q, c.k, c.v, c.table, off, c.lens, max_new=max(new), return_lse=True)
+    for hint in (None, max(new), 1):
+        got = ops.cache_mass(q, lse, c.k, c.table, off, c.lens, mass, max_new=hint)
+        _check_mass(got, mass, q, lse, c, new, lens, scale)
+    again = mass.clone()
+    assert ops.cache_mass(q, lse, c.k, c.table, off, c.lens, again, max_new=max(new), out=again) is again
+    assert torch.equal(again, ops.cache_mass(q, lse, c.k, c.table, off, c.lens, mass, max_new=max(new)))
+
+
+def test_cache_mass_hidden_and_empty():
+    """Rows that see nothing, padded rows, NaN keys and queries that others do not see."""
+    new, lens = [4, 3, 70, 2], [2, 0, 69, 40]
+    c = Cache(lens, 2, 64, 16, torch.float16, 8)
+    q = torch.randn(sum(new) + 5, 4, 64, device=DEV, generator=_gen(5)).half()
+    off = lengths_to_offsets(new)
+    _, lse = ops.cache_attention(q, c.k, c.v, c.table, off, c.lens, return_lse=True)
+    lse[sum(new):] = math.nan
+    q[sum(new):] = math.nan
+    mass = torch.rand(4, 2, c.table.shape[1] * 16, device=DEV, generator=_gen(3))
+    got = ops.cache_mass(q, lse, c.k, c.table, off, c.lens, mass)
+    want = mass.double()
+    at = 0
+    for b, (n, m) in enumerate(zip(new, lens)):
+        for i in range(n):
+            see = max(0, m - n + i + 1)
+            k = cache_rows(c.k, c.table, b, m)[:see].double()
+            for h in range(4):
+                s = k[:, h // 2] @ q[at + i, h].double() * 0.125
+                want[b, h // 2, :see] += torch.exp(s - lse[at + i, h].double())
+        at += n
+    assert float((got - want).abs().max()) < 1e-4
+    # the last token's key is NaN: only its own slot may become NaN
+    c.k[c.table[3, 39 // 16].long(), 39 % 16, 1] = math.nan
+    got2 = ops.cache_mass(q, lse, c.k, c.table, off, c.lens, mass)
+    bad = torch.isnan(got2)
+    assert bool(bad[3, 1, 39]) and int(bad.sum()) == 1
+    assert torch.equal(got2[~bad], got[~bad])
+
+
+def test_cache_mass_of_no_tokens_copies():
+    c = Cache([5], 2, 64, 16, torch.float16, 8)
+    mass = torch.rand(1, 2, 16, device=DEV)
+    q = torch.zeros(0, 4, 64, dtype=torch.float16, device=DEV)
+    lse = torch.zeros(0, 4, device=DEV)
+    got = ops.cache_mass(q, lse, c.k, c.table, lengths_to_offsets([0]), c.lens, mass)
+    assert torch.equal(got, mass)
+
+
+# ---------------------------------------------------------------------------- all together
+@pytest.mark.parametrize("dtype", TYPES)
+def test_prompt_then_steps_with_a_budget(dtype):
+    """A user's loop: attend to the prompts, cache them, gather their mass, cut the cache to
+    a budget, then single tokens -- append, attend, gather, evict -- against a plain model of
+    the same cache that holds 64-bit masses and Python lists of kept tokens."""
+    heads, kv, d, page, keep, recent = 6, 2, 64, 16, 48, 8
+    lens = [100, 30, 61]
+    b, g, scale = len(lens), 3, 64**-0.5
+    gen = _gen(77)
+    per = 8
+    kc = torch.zeros(b * per, page, kv, d, dtype=dtype, device=DEV)
+    vc = torch.zeros_like(kc)
+    table = torch.randperm(b * per, device=DEV, generator=gen).to(torch.int32).view(b, per)
+    cap = per * page
+    mass, pos = torch.zeros(b, kv, cap, device=DEV), torch.full((b, kv, cap), -1, dtype=torch.int32, device=DEV)
+    seen = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    cache_lens = seen.clone()
+    rand = lambda t, h: torch.randn(t, h, d, device=DEV, generator=gen).to(dtype)  # noqa: E731
+    # model: per (sequence, head) the keys and values that are kept, by position
+    model = [[{} for _ in range(kv)] for _ in range(b)]
+
+    def attend_model(q, i, hh):
+        h = hh // g
+        items = model[i][h]
+        k = torch.stack([items[p][0] for p in sorted(items)]).double()
+        v = torch.stack([items[p][1] for p in sorted(items)]).double()
+        w = torch.softmax(k @ q.double() * scale, 0)
+        return w @ v, dict(zip(sorted(items), w.tolist()))
+
+    t = sum(lens)
+    q, k, v = rand(t, heads), rand(t, kv), rand(t, kv)
+    off = lengths_to_offsets(lens)
+    out, lse = ops.prompt_attention(q, k, v, off, return_lse=True)
+    ops.cache_append(k, v, kc, vc, table, off, cache_lens, positions=pos, mass=mass, seen=seen)
+    chunk, chunk_lse = ops.cache_attention(q, kc, vc, table, off, cache_lens, max_new=max(lens), return_lse=True)
+    u = torch.finfo(dtype).eps
+    assert float((chunk.double() - out.double()).abs().max()) <= 4 * u * float(v.abs().max())
+    assert float((chunk_lse - lse).abs().max()) < 1e-4
+    mass = ops.cache_mass(q, lse, kc, table, off, cache_lens, mass, out=mass)
+    at = 0
+    for i, n in enumerate(lens):
+        for h in range(kv):
+            for p in range(n):
+                model[i][h][p] = (k[at + p, h], v[at + p, h])
+        at += n
+    assert float((mass.sum(2).cpu() - torch.tensor([[n * g] * kv for n in lens], dtype=torch.float32)).abs().max()) < 0.01
+    step_off = lengths_to_offsets([1] * b)
+    for step in range(12):
+        # cut to the budget; the model follows the choice that the operator reports
+        old_pos, old_mass, old_lens = pos.clone(), mass.clone(), cache_lens.tolist()
+        mass, pos, cache_lens = ops.cache_evict(mass, pos, kc, vc, table, cache_lens, keep, recent=recent)
+        for i in range(b):
+            for h in range(kv):
+                hole, mover = evict_choice(old_mass[i, h], old_pos[i, h], old_lens[i], keep, recent)
+                gone = {int(old_pos[i, h, j]) for j in hole}
+                gone |= {int(old_pos[i, h, j]) for j in range(keep, old_lens[i])} - {int(old_pos[i, h, j]) for j in mover}
+                for p in gone:
+                    del model[i][h][p]
+                n = int(cache_lens[i])
+                assert sorted(pos[i, h, :n].tolist()) == sorted(model[i][h])
+        q, k, v = rand(b, heads), rand(b, kv), rand(b, kv)
+        seen += 1
+        cache_lens = cache_lens + 1
+        ops.cache_append(k, v, kc, vc, table, step_off, cache_lens, positions=pos, mass=mass, seen=seen)
+        out, lse = ops.cache_attention(q, kc, vc, table, step_off, cache_lens, max_new=1, return_lse=True)
+        before = mass.clone()
+        ops.cache_mass(q, lse, kc, table, step_off, cache_lens, mass, max_new=1, out=mass)
+        for i in range(b):
+            for h in range(kv):
+                model[i][h][int(seen[i]) - 1] = (k[i, h], v[i, h])
+            gained = {}
+            for hh in range(heads):
+                ref, w = attend_model(q[i, hh], i, hh)
+                assert float((out[i, hh].double() - ref).abs().max()) <= 2 * u * float(vc.abs().max())
+                for p, x in w.items():
+                    gained[(hh // g, p)] = gained.get((hh // g, p), 0) + x
+            for h in range(kv):
+                for j in range(int(cache_lens[i])):
+                    p = int(pos[i, h, j])
+                    assert abs(float(mass[i, h, j] - before[i, h, j]) - gained[(h, p)]) < 1e-4

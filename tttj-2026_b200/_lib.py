@@ -110,6 +110,7 @@ _SIGNATURES = {
         _c.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _c.c_int, _c.c_float, _vp, _c.c_size_t, _vp]
     ),
     "tttj_cache_append": (_c.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "tttj_cache_mass": (_c.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _c.c_int, _c.c_float, _vp]),
     "tttj_cache_evict_workspace_bytes": (_c.c_size_t, [_vp, _c.c_int]),
     "tttj_cache_evict": (
         _c.c_int,

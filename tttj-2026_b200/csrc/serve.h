@@ -129,6 +129,20 @@ constexpr int tile_nt(int hd) { return hd == 256 ? 1 : 2; }
 cudaError_t tile_launch(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v,
                         const TileParams& p, int head_dim, int bf16, int grid, cudaStream_t stream);
 
+// ---- attention mass of cached keys (serve_mass.cuh) ----
+struct MassParams {
+  SrvSeqs s;
+  const float* lse;   // [tokens][heads], natural
+  const float* mass;  // [batch][kv_heads][cap]
+  float* out;         // the same shape (may be mass)
+  long cap;
+  int heads, kv_heads, group, tile_tokens;
+  float scale_log2;
+  unsigned long long wait_limit_ns;
+};
+cudaError_t mass_launch(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const MassParams& p, int head_dim,
+                        int bf16, int grid, cudaStream_t stream);
+
 // ---- cache append / evict (serve_cache.cu) ----
 struct AppendParams {
   SrvSeqs s;

@@ -59,6 +59,12 @@ int check_pages(const char* what, const char* name, const tttj_pages* c, const t
   return TTTJ_OK;
 }
 
+int check_scale(const char* what, float scale) {
+  if (!(scale > 0.f) || !isfinite(scale))
+    return capi_fail(TTTJ_ERR_INVALID, "%s: scale must be positive and finite", what);
+  return TTTJ_OK;
+}
+
 #define TRY(call)             \
   do {                        \
     const int rc_ = (call);   \
@@ -192,8 +198,7 @@ int attention(const char* what, const tttj_seqs* s, const tttj_rows* q, const Ca
                      need);
   if (reinterpret_cast<uintptr_t>(workspace) & (kAlign - 1))
     return capi_fail(TTTJ_ERR_INVALID, "%s: workspace must be 256-byte aligned", what);
-  if (!(scale > 0.f) || !isfinite(scale))
-    return capi_fail(TTTJ_ERR_INVALID, "%s: scale must be positive and finite", what);
+  TRY(check_scale(what, scale));
   int sms = 0;
   TRY(sm_count_here(&sms));
   if (sms > kMostSms) sms = kMostSms;
@@ -326,6 +331,47 @@ int tttj_cache_append(const tttj_seqs* s, const tttj_rows* k, const tttj_rows* v
   p.mass = mass;
   p.seen = seen;
   CAPI_CUDA(append_launch(p, static_cast<cudaStream_t>(stream)));
+  return TTTJ_OK;
+}
+
+int tttj_cache_mass(const tttj_seqs* s, const tttj_rows* q, const float* lse, const tttj_pages* k_cache,
+                    const float* mass, float* mass_out, int max_new, float scale, void* stream) {
+  const char* what = "cache_mass";
+  TRY(check_seqs(what, s, true, true));
+  TRY(check_rows(what, "q", q, s, s->heads));
+  TRY(check_pages(what, "k_cache", k_cache, s));
+  if (!mass || !mass_out || (!lse && s->tokens > 0)) return capi_fail(TTTJ_ERR_INVALID, "%s: null argument", what);
+  TRY(check_scale(what, scale));
+  if (max_new < 0) return capi_fail(TTTJ_ERR_INVALID, "%s: max_new=%d is negative", what, max_new);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const long cap = (long)s->pages_per_seq * s->page_size;
+  if (s->tokens == 0) {
+    if (mass != mass_out)
+      CAPI_CUDA(cudaMemcpyAsync(mass_out, mass, (size_t)s->batch * s->kv_heads * cap * 4, cudaMemcpyDeviceToDevice, st));
+    return TTTJ_OK;
+  }
+  int sms = 0;
+  TRY(sm_count_here(&sms));
+  MassParams p{};
+  p.s = seqs_of(s, true, 1);
+  p.lse = lse;
+  p.mass = mass;
+  p.out = mass_out;
+  p.cap = cap;
+  p.heads = s->heads;
+  p.kv_heads = s->kv_heads;
+  p.group = s->heads / s->kv_heads;
+  // Query tiles no larger than the tokens a sequence has: single tokens load one each.
+  p.tile_tokens = tile_tokens(s);
+  const int most = max_new > 0 && max_new < s->tokens ? max_new : s->tokens;
+  if (most < p.tile_tokens) p.tile_tokens = most;
+  p.scale_log2 = scale * 1.44269504088896341f;
+  p.wait_limit_ns = TTTJ_WAIT_LIMIT_NS;
+  CUtensorMap tm_q, tm_k;
+  TRY(q_map(&tm_q, what, s, q, p.tile_tokens));
+  TRY(kv_map(&tm_k, what, s, k_cache->data, k_cache->page_stride, k_cache->slot_stride, k_cache->head_stride,
+             s->page_size, s->num_pages, s->page_size < ATC_BM ? s->page_size : ATC_BM));
+  CAPI_CUDA(mass_launch(tm_q, tm_k, p, s->head_dim, s->dtype == TTTJ_DTYPE_BF16, sms, st));
   return TTTJ_OK;
 }
 

@@ -1,0 +1,32 @@
+// Instantiations and launcher of the attention mass (serve_mass.cuh).
+#include "launch.h"
+#include "serve_mass.cuh"
+
+namespace tttj {
+
+namespace {
+template <int HD, bool BF16>
+cudaError_t launch(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const MassParams& p, int grid,
+                   cudaStream_t stream) {
+  auto kern = mass_kernel<HD, BF16>;
+  static_assert(MassSmem<HD>::FIXED + SRV_MAX_BATCH * (int)sizeof(SrvSeq) <= 232448,
+                "shared memory exceeds the 227 KB per-CTA limit");
+  const int smem = MassSmem<HD>::FIXED + p.s.batch * (int)sizeof(SrvSeq);
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(kern, dim3(grid), dim3(MASS_THREADS), smem, stream, tm_q, tm_k, p);
+}
+}  // namespace
+
+cudaError_t mass_launch(const CUtensorMap& q, const CUtensorMap& k, const MassParams& p, int head_dim, int bf16,
+                        int grid, cudaStream_t stream) {
+  switch (head_dim) {
+    case 32: return bf16 ? launch<32, true>(q, k, p, grid, stream) : launch<32, false>(q, k, p, grid, stream);
+    case 64: return bf16 ? launch<64, true>(q, k, p, grid, stream) : launch<64, false>(q, k, p, grid, stream);
+    case 128: return bf16 ? launch<128, true>(q, k, p, grid, stream) : launch<128, false>(q, k, p, grid, stream);
+    case 256: return bf16 ? launch<256, true>(q, k, p, grid, stream) : launch<256, false>(q, k, p, grid, stream);
+  }
+  return cudaErrorInvalidValue;
+}
+
+}  // namespace tttj

@@ -333,3 +333,37 @@ def cache_evict(mass: torch.Tensor, positions: torch.Tensor, k_cache: torch.Tens
     if rc:
         _lib.check(rc, what)
     return mass_out, pos_out, lens_out
+
+
+def cache_mass(q: torch.Tensor, lse: torch.Tensor, k_cache: torch.Tensor, page_table: torch.Tensor,
+               seq_offsets: torch.Tensor, cache_lens: torch.Tensor, mass: torch.Tensor, *,
+               max_new: Optional[int] = None, scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+               status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """mass plus the attention weight that the new tokens give to every slot: for key/value
+    head g and slot j, the sum over the tokens that see j and the heads of g of
+    exp(scale q k_j - lse), with the ``lse`` that ``cache_attention`` (or
+    ``prompt_attention``) returned for the same queries.
+
+    mass fp32 [B, kv_heads, P * page_size]; returns a new tensor, or ``out``, which may be
+    ``mass`` itself.  ``max_new`` and ``scale`` as for ``cache_attention``."""
+    what = "cache_mass"
+    if q.dim() != 3 or k_cache.dim() != 4:
+        raise ValueError(f"{what}: q must be [tokens, heads, head_dim], k_cache [pages, page_size, kv_heads, head_dim]")
+    heads, kv_heads = q.shape[1], k_cache.shape[2]
+    s = _serve_seqs(what, q, seq_offsets, heads, kv_heads, k_cache, page_table, cache_lens, status, q.shape[0])
+    if k_cache.dtype != q.dtype or k_cache.device != q.device or k_cache.shape[3] != q.shape[2]:
+        raise ValueError(f"{what}: the cache must be {q.dtype} on {q.device} with head_dim {q.shape[2]}")
+    if lse.dtype != torch.float32 or lse.shape != q.shape[:2] or lse.device != q.device or not lse.is_contiguous():
+        raise ValueError(f"{what}: lse must be a contiguous float32 tensor {list(q.shape[:2])} on {q.device}")
+    slots = (s.batch, kv_heads, s.pages_per_seq * s.page_size)
+    ms = _slot_tensor(what, "mass", mass, torch.float32, slots, q.device)
+    if out is None:
+        out = torch.empty_like(mass)
+    mo = _slot_tensor(what, "out", out, torch.float32, slots, q.device)
+    rq, ck = _serve_rows(what, "q", q, q), _serve_pages(what, "k_cache", k_cache, k_cache)
+    rc = _call(q.device, _lib.lib().tttj_cache_mass, ctypes.byref(s), ctypes.byref(rq), lse.data_ptr(),
+               ctypes.byref(ck), ms, mo, 0 if max_new is None else max_new,
+               q.shape[2] ** -0.5 if scale is None else float(scale))
+    if rc:
+        _lib.check(rc, what)
+    return out
