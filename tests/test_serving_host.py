@@ -81,13 +81,24 @@ def test_evict_arguments_refused(kw, text):
     _refused(_evict(_seqs(), **kw), text)
 
 
+def test_packed_arguments_have_the_c_layout():
+    seqs = [A, 2 * A, 3 * A, 1 << 40, *range(1, 10), 4 * A]
+    assert ops._pack_seqs(*seqs) == bytes(_lib.TttjSeqs(*seqs))
+    assert ops._pack_rows(A, 1 << 40, -3) == bytes(_lib.TttjRows(A, 1 << 40, -3))
+    assert ops._pack_pages(A, 1 << 40, 5, 6) == bytes(_lib.TttjPages(A, 1 << 40, 5, 6))
+
+
 def test_workspace_sizes():
     L = _lib.lib()
     assert L.tttj_serve_workspace_bytes(ctypes.byref(_seqs())) > 0
     assert L.tttj_serve_workspace_bytes(ctypes.byref(_seqs(head_dim=40))) == 0
     s = _seqs()
-    # moves: at most min(keep, slots - keep) of 8 bytes per head, and a count per head
-    assert L.tttj_cache_evict_workspace_bytes(ctypes.byref(s), 100) >= 4 * 28 * 8 + 16
+    # moves: at most min(keep, slots - keep) of 8 bytes per head
+    assert L.tttj_cache_evict_workspace_bytes(ctypes.byref(s), 100) >= 4 * 28 * 8
+    assert L.tttj_cache_evict_workspace_bytes(ctypes.byref(s), 10**6) > 0
+    assert ops.serve_workspace_bytes(2, 5, 8, 2, 64) == L.tttj_serve_workspace_bytes(ctypes.byref(s))
+    with pytest.raises(ValueError, match="head_dim=40"):
+        ops.serve_workspace_bytes(2, 5, 8, 2, 40)
     assert L.tttj_cache_evict_workspace_bytes(ctypes.byref(s), 0) == 0
 
 

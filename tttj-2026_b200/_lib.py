@@ -192,6 +192,8 @@ _lib: ctypes.CDLL | None = None
 def lib() -> ctypes.CDLL:
     """Load libtttj_b200.so (once) and attach the C signatures."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is None:
             if not LIB_PATH.exists():

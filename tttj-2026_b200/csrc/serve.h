@@ -169,9 +169,8 @@ struct EvictParams {
   int keep, recent;
   long cap;       // slots per sequence (row length of mass / positions)
   int2* moves;    // [batch * kv_heads][most_moves] (from, to) slots
-  int* n_moves;   // [batch * kv_heads]
   int most_moves;
 };
-cudaError_t evict_launch(const EvictParams& p, cudaStream_t stream);
+cudaError_t evict_launch(const EvictParams& p, int sms, cudaStream_t stream);
 
 }  // namespace tttj

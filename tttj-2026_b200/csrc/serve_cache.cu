@@ -68,15 +68,20 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const AppendPara
 }
 
 // ------------------------------------------------------------------- evict
-// Selection, one block per (sequence, head): a radix selection finds the keep-th largest
-// value (four 8-bit digits of an order-preserving integer image of the mass, counted in
-// shared memory), then one ordered pass ranks the equal values, the holes (slots < keep
-// that go) and the movers (slots >= keep that stay), each thread owning a contiguous range
-// of slots.  The i-th mover goes to the i-th hole, so as few rows move as can: those kept
-// from behind the budget.  The integer counts make the result independent of the order in
-// which threads run.
-constexpr int EVICT_THREADS = 1024;
-constexpr int EVICT_SMEM_SLOTS = 48 * 1024;  // values held in shared memory up to this length
+// One cluster of 1 .. 8 blocks per (sequence, head); each block owns a contiguous range of
+// slots, whose masses and positions it holds in shared memory.  A radix selection over
+// an order-preserving integer image of the mass (digits of 11, 11 and 10 bits, counted in shared memory
+// and added up across the cluster) finds the keep-th largest value.  One ordered pass
+// then ranks the equal values, the holes (slots < keep that go) and the movers (slots >= keep
+// that stay); the i-th mover goes to the i-th hole, so as few rows move as can, and since
+// sources lie behind the budget and destinations in front of it, no move reads what
+// another writes.  All counts are integers: the result does not depend on the order in
+// which threads run.  Bound: for short caches latency (about twenty barriers), for long ones the bytes
+// of masses, positions and moved rows.
+constexpr int EVICT_MAX_CLUSTER = 8;
+constexpr int EVICT_MAX_THREADS = 512;
+constexpr int EVICT_BINS = 2048;
+constexpr int EVICT_HELD_SLOTS = 24 * 1024;  // slots of one block held in shared memory (8 bytes each)
 
 // Unsigned image of a mass: larger mass, larger integer; -0 as +0, NaN lowest.
 __device__ __forceinline__ uint32_t evict_key(float mass) {
@@ -85,46 +90,32 @@ __device__ __forceinline__ uint32_t evict_key(float mass) {
   return (u >> 31) ? ~u : (u | 0x80000000u);
 }
 
-// Exclusive prefix sum of one int per thread over the block; *total gets the sum.
-__device__ __forceinline__ int block_scan(int v, int* warp_sums, int* total) {
-  const int lane = lane_id(), warp = warp_id();
-  int x = v;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int o = __shfl_up_sync(0xffffffffu, x, d);
-    if (lane >= d) x += o;
-  }
-  __syncthreads();
-  if (lane == 31) warp_sums[warp] = x;
-  __syncthreads();
-  if (warp == 0) {
-    int w = lane < EVICT_THREADS / 32 ? warp_sums[lane] : 0;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int o = __shfl_up_sync(0xffffffffu, w, d);
-      if (lane >= d) w += o;
-    }
-    warp_sums[lane] = w;
-  }
-  __syncthreads();
-  *total = warp_sums[EVICT_THREADS / 32 - 1];
-  return (warp > 0 ? warp_sums[warp - 1] : 0) + x - v;
+__device__ __forceinline__ int ld_cluster(uint32_t addr) {
+  int v;
+  asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
 }
 
-__global__ void __launch_bounds__(EVICT_THREADS) evict_select_kernel(const EvictParams p) {
-  extern __shared__ uint32_t s_key[];  // [min(len, EVICT_SMEM_SLOTS)]
-  __shared__ int s_hist[256];
-  __shared__ int s_warp[32];
-  __shared__ int s_newest;
-  __shared__ uint32_t s_prefix;
-  __shared__ int s_need;
+struct EvictShared {
+  int hist[EVICT_BINS];   // counts of one digit (read by the whole cluster)
+  int total[4];           // newest position; equal, holes, movers of this block
+  int warp[2][32];
+  int digit, need;
+};
+
+__global__ void __launch_bounds__(EVICT_MAX_THREADS) evict_kernel(const EvictParams p, int cluster) {
+  extern __shared__ __align__(16) uint8_t s_dyn[];
+  __shared__ EvictShared sh;
   griddep_wait();
   griddep_launch();
-  const int bh = blockIdx.x, b = bh / p.kv_heads;
+  const int rank = cluster > 1 ? (int)cluster_ctarank() : 0;
+  const int bh = blockIdx.x / cluster, b = bh / p.kv_heads;
+  const int threads = blockDim.x, warps = threads >> 5, warp = warp_id(), lane = lane_id();
+  const unsigned below = (1u << lane) - 1;
   const long cap = p.cap;
   int len = p.s.lens[b];
   if (len < 0 || len > cap) {
-    if (threadIdx.x == 0 && p.s.status != nullptr) atomicCAS(p.s.status, 0, SRV_DEV_BAD_LENS);
+    if (threadIdx.x == 0) report_status(p.s.status, SRV_DEV_BAD_LENS);
     len = (int)min((long)max(len, 0), cap);
   }
   const float* mass = p.mass + bh * cap;
@@ -132,131 +123,190 @@ __global__ void __launch_bounds__(EVICT_THREADS) evict_select_kernel(const Evict
   float* mass_out = p.mass_out + bh * cap;
   int* pos_out = p.positions_out + bh * cap;
   const int keep = p.keep;
-  if (threadIdx.x == 0 && bh % p.kv_heads == 0) p.lens_out[b] = min(len, keep);
-  if (len <= keep) {
-    if (threadIdx.x == 0) p.n_moves[bh] = 0;
-    for (long j = threadIdx.x; j < cap; j += EVICT_THREADS) {
-      mass_out[j] = j < len ? mass[j] : 0.f;
-      pos_out[j] = j < len ? pos[j] : -1;
+  if (rank == 0 && threadIdx.x == 0 && bh % p.kv_heads == 0) p.lens_out[b] = min(len, keep);
+  const int me = rank * threads + threadIdx.x, all = cluster * threads;
+  // Slots behind the live ones (or the budget) are cleared by everyone.
+  for (long j = min(len, keep) + me; j < cap; j += all) {
+    mass_out[j] = 0.f;
+    pos_out[j] = -1;
+  }
+  if (len <= keep) {  // uniform over the cluster
+    for (int j = me; j < len; j += all) {
+      mass_out[j] = mass[j];
+      pos_out[j] = pos[j];
     }
     return;
   }
-  // The newest position; slots within `recent` of it count as +inf.
-  if (threadIdx.x == 0) s_newest = INT32_MIN;
-  __syncthreads();
-  int newest = INT32_MIN;
-  for (int j = threadIdx.x; j < len; j += EVICT_THREADS) newest = max(newest, pos[j]);
-  newest = __reduce_max_sync(0xffffffffu, newest);
-  if (lane_id() == 0) atomicMax(&s_newest, newest);
-  __syncthreads();
-  const long edge = (long)s_newest - p.recent;
-  const bool held = len <= EVICT_SMEM_SLOTS;
-  auto key_at = [&](int j) -> uint32_t {
-    return (long)pos[j] > edge ? 0xff800000u /* image of +inf */ : evict_key(mass[j]);
+  auto sync_all = [&] {
+    if (cluster > 1) cluster_sync_all(); else __syncthreads();
   };
-  if (held)
-    for (int j = threadIdx.x; j < len; j += EVICT_THREADS) s_key[j] = key_at(j);
-  uint32_t prefix = 0;
-  int need = keep;  // how many of the values matching the prefix so far are kept
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    if (threadIdx.x < 256) s_hist[threadIdx.x] = 0;
-    __syncthreads();
-    for (int j = threadIdx.x; j < len; j += EVICT_THREADS) {
-      const uint32_t key = held ? s_key[j] : key_at(j);
-      if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8)))
-        atomicAdd(&s_hist[(key >> shift) & 255u], 1);
+  auto peer = [&](const int* x, int r) {
+    return cluster > 1 ? ld_cluster(map_to_cta(smem_u32(x), (uint32_t)r)) : *x;
+  };
+  // This block's slots, a multiple of 32 per warp.
+  const int each = ((len + cluster - 1) / cluster + 31) & ~31;
+  const int lo = min(rank * each, len), hi = min(lo + each, len);
+  const bool held = each <= EVICT_HELD_SLOTS;
+  float* s_mass = reinterpret_cast<float*>(s_dyn);
+  int* s_pos = reinterpret_cast<int*>(s_dyn) + (held ? each : 0);
+  int newest = INT32_MIN;
+#pragma unroll 4
+  for (int j = lo + (int)threadIdx.x; j < hi; j += threads) {
+    const int x = pos[j];
+    const float m = held ? mass[j] : 0.f;
+    newest = max(newest, x);
+    if (held) {
+      s_mass[j - lo] = m;
+      s_pos[j - lo] = x;
     }
-    __syncthreads();
-    if (threadIdx.x < 32) {
-      // Lane l holds digits 255 - 8 l .. 248 - 8 l: counts from the largest digit down.
-      int c[8], sum = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) sum += c[i] = s_hist[255 - 8 * (int)threadIdx.x - i];
-      int inc = sum;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int o = __shfl_up_sync(0xffffffffu, inc, d);
-        if ((int)threadIdx.x >= d) inc += o;
-      }
-      int above = inc - sum;
-      if (above < need && need <= inc) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (above < need && need <= above + c[i]) {
-            s_prefix = prefix | ((uint32_t)(255 - 8 * (int)threadIdx.x - i) << shift);
-            s_need = need - above;
-          }
-          above += c[i];
-        }
-      }
-    }
-    __syncthreads();
-    prefix = s_prefix;
-    need = s_need;
   }
-  // Kept: key > prefix, and the first `need` slots with key == prefix.
-  const int each = (len + EVICT_THREADS - 1) / EVICT_THREADS;
-  const int j0 = min((int)threadIdx.x * each, len), j1 = min(j0 + each, len);
-  int equal = 0, total;
-  for (int j = j0; j < j1; ++j) equal += (held ? s_key[j] : key_at(j)) == prefix;
-  const int equal0 = block_scan(equal, s_warp, &total);
-  // Both lists start at the same length, so one scan counts holes (slots < keep) for the
-  // threads in front of the budget and movers for those behind it.
-  int holes = 0, movers = 0, rank = equal0;
-  for (int j = j0; j < j1; ++j) {
-    const uint32_t key = held ? s_key[j] : key_at(j);
-    const bool kept = key > prefix || (key == prefix && rank++ < need);
-    holes += j < keep && !kept;
-    movers += j >= keep && kept;
-  }
-  int n_holes, n_movers;
-  int hole0 = block_scan(holes, s_warp, &n_holes);
-  int mover0 = block_scan(movers, s_warp, &n_movers);
-  int2* moves = p.moves + (long)bh * p.most_moves;
-  rank = equal0;
-  for (int j = j0; j < j1; ++j) {
-    const uint32_t key = held ? s_key[j] : key_at(j);
-    const bool kept = key > prefix || (key == prefix && rank++ < need);
-    if (j < keep && !kept) moves[hole0++].y = j;
-    if (j >= keep && kept) moves[mover0++].x = j;
-  }
-  if (threadIdx.x == 0) p.n_moves[bh] = n_movers;
-  // Kept slots in place; the holes are filled below from the list.
-  for (long j = threadIdx.x; j < cap; j += EVICT_THREADS) {
-    mass_out[j] = j < keep ? mass[j] : 0.f;
-    pos_out[j] = j < keep ? pos[j] : -1;
-  }
+  newest = __reduce_max_sync(0xffffffffu, newest);
+  if (lane == 0) sh.warp[0][warp] = newest;
+  for (int i = threadIdx.x; i < EVICT_BINS; i += threads) sh.hist[i] = 0;
   __syncthreads();
-  for (int i = threadIdx.x; i < n_movers; i += EVICT_THREADS) {
+  if (warp == 0) {
+    newest = __reduce_max_sync(0xffffffffu, lane < warps ? sh.warp[0][lane] : INT32_MIN);
+    if (lane == 0) sh.total[0] = newest;
+  }
+  sync_all();
+  newest = INT32_MIN;
+  for (int r = 0; r < cluster; ++r) newest = max(newest, peer(&sh.total[0], r));
+  const long edge = (long)newest - p.recent;  // positions behind it count as +inf
+  auto key_at = [&](int j) -> uint32_t {
+    const int x = held ? s_pos[j - lo] : pos[j];
+    return (long)x > edge ? 0xff800000u /* image of +inf */ : evict_key(held ? s_mass[j - lo] : mass[j]);
+  };
+  uint32_t prefix = 0;
+  int need = keep;  // how many of the values that match the prefix so far are kept
+#pragma unroll 1
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+    const int bits = pass == 2 ? 10 : 11;
+    for (int j = lo + (int)threadIdx.x; j < hi; j += threads) {
+      const uint32_t key = key_at(j);
+      if (pass == 0 || (key >> (shift + bits)) == (prefix >> (shift + bits)))
+        atomicAdd(&sh.hist[(key >> shift) & ((1u << bits) - 1)], 1);
+    }
+    sync_all();
+    // Largest digits first: thread t takes bins top - per t .. ; counts over the cluster.
+    const int per = (1 << bits) / threads;
+    const int first = (1 << bits) - 1 - per * (int)threadIdx.x;
+    int c[EVICT_BINS / 128], sum = 0;  // at least 128 threads
+#pragma unroll
+    for (int i = 0; i < EVICT_BINS / 128; ++i) {
+      c[i] = 0;
+      if (i < per)
+        for (int r = 0; r < cluster; ++r) c[i] += peer(&sh.hist[first - i], r);
+      sum += c[i];
+    }
+    int inc = sum;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, inc, d);
+      if (lane >= d) inc += o;
+    }
+    if (lane == 31) sh.warp[0][warp] = inc;
+    __syncthreads();
+    int above = inc - sum;
+    for (int w = 0; w < warp; ++w) above += sh.warp[0][w];
+    if (above < need && need <= above + sum) {
+#pragma unroll
+      for (int i = 0; i < EVICT_BINS / 128; ++i) {
+        if (i < per && above < need && need <= above + c[i]) {
+          sh.digit = first - i;
+          sh.need = need - above;
+        }
+        above += c[i];
+      }
+    }
+    sync_all();  // digit and need are there; every block has read this one's counts
+    prefix |= (uint32_t)sh.digit << shift;
+    need = sh.need;
+    for (int i = threadIdx.x; i < EVICT_BINS; i += threads) sh.hist[i] = 0;
+    __syncthreads();
+  }
+  // Kept: key > prefix, and the first `need` slots with key == prefix.  Each warp owns a
+  // contiguous range; ranks by ballots.
+  const int per_warp = ((hi - lo + warps - 1) / warps + 31) & ~31;
+  const int w0 = min(lo + warp * per_warp, hi), w1 = min(w0 + per_warp, hi);
+  // Exclusive sum of one count per warp over the block (and the blocks before it).
+  auto offset = [&](int mine, int which) {
+    if (lane == 0) sh.warp[which & 1][warp] = mine;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      int t = 0;
+      for (int w = 0; w < warps; ++w) t += sh.warp[which & 1][w];
+      sh.total[which] = t;
+    }
+    int at = 0;
+    for (int w = 0; w < warp; ++w) at += sh.warp[which & 1][w];
+    sync_all();
+    for (int r = 0; r < rank; ++r) at += peer(&sh.total[which], r);
+    return at;
+  };
+  int equal = 0;
+  for (int j = w0; j < w1; j += 32)
+    equal += __popc(__ballot_sync(0xffffffffu, j + lane < w1 && key_at(j + lane) == prefix));
+  const int equal0 = offset(equal, 1);
+  auto kept_at = [&](int j, int* rank_eq) {  // of slots j .. j + 31, a bit per lane
+    const uint32_t key = j + lane < w1 ? key_at(j + lane) : 0u;
+    const bool live = j + lane < w1;
+    const unsigned eq = __ballot_sync(0xffffffffu, live && key == prefix);
+    const bool kept = live && (key > prefix || (key == prefix && *rank_eq + __popc(eq & below) < need));
+    *rank_eq += __popc(eq);
+    return __ballot_sync(0xffffffffu, kept);
+  };
+  auto span = [&](int j) {  // lanes of slots j .. that are live, and of those the ones < keep
+    const int n = w1 - j, f = keep - j;
+    const unsigned live = n >= 32 ? 0xffffffffu : (1u << n) - 1;
+    return make_uint2(live, f >= 32 ? live : f <= 0 ? 0u : live & ((1u << f) - 1));
+  };
+  int holes = 0, movers = 0, eq_rank = equal0;
+  for (int j = w0; j < w1; j += 32) {
+    const unsigned kept = kept_at(j, &eq_rank);
+    const uint2 sp = span(j);
+    holes += __popc(~kept & sp.y);
+    movers += __popc(kept & sp.x & ~sp.y);
+  }
+  int hole0 = offset(holes, 2);
+  int mover0 = offset(movers, 3);
+  int n_moves = 0;
+  for (int r = 0; r < cluster; ++r) n_moves += peer(&sh.total[3], r);
+  int2* moves = p.moves + (long)bh * p.most_moves;
+  eq_rank = equal0;
+  for (int j = w0; j < w1; j += 32) {
+    const unsigned kept = kept_at(j, &eq_rank);
+    const uint2 sp = span(j);
+    const unsigned hole = ~kept & sp.y, mover = kept & sp.x & ~sp.y, bit = 1u << lane;
+    if (hole & bit) moves[hole0 + __popc(hole & below)].y = j + lane;
+    if (mover & bit) moves[mover0 + __popc(mover & below)].x = j + lane;
+    if (kept & sp.y & bit) {
+      mass_out[j + lane] = held ? s_mass[j + lane - lo] : mass[j + lane];
+      pos_out[j + lane] = held ? s_pos[j + lane - lo] : pos[j + lane];
+    }
+    hole0 += __popc(hole);
+    mover0 += __popc(mover);
+  }
+  sync_all();  // the list is complete (and no block still reads another's shared memory)
+  for (int i = me; i < n_moves; i += all) {
     const int2 mv = moves[i];
     mass_out[mv.y] = mass[mv.x];
     pos_out[mv.y] = pos[mv.x];
   }
-}
-
-// Moves the listed rows of K and V: sources are slots >= keep, destinations slots < keep,
-// so no move reads what another writes.  One warp per move and cache.
-constexpr int EVICT_MOVE_WARPS = 8;
-__global__ void __launch_bounds__(32 * EVICT_MOVE_WARPS) evict_move_kernel(const EvictParams p) {
-  griddep_wait();
-  griddep_launch();
-  const int bh = blockIdx.x, b = bh / p.kv_heads, h = bh - b * p.kv_heads;
-  const int n = p.n_moves[bh];
-  const int lane = lane_id();
-  const int pieces = p.head_dim / 8;  // 16-byte pieces of a row (4 .. 32)
-  const int per_warp = 32 / pieces;   // rows of one warp step
-  const int sub = lane / pieces, c = lane - sub * pieces;
-  const int mask = (1 << p.s.page_shift) - 1;
-  const long rows = 2l * n;           // move i of K is row 2 i, of V row 2 i + 1
-  const long step = (long)gridDim.y * EVICT_MOVE_WARPS * per_warp;
-  for (long i = ((long)blockIdx.y * EVICT_MOVE_WARPS + warp_id()) * per_warp + sub; i < rows; i += step) {
-    const int2 mv = p.moves[(long)bh * p.most_moves + (i >> 1)];
+  // The rows: a 16-byte piece per thread and step; move i of K is row 2 i, of V row 2 i + 1.
+  const int pieces = p.head_dim / 8;  // 4 .. 32
+  const int c = threadIdx.x % pieces, h = bh - b * p.kv_heads;
+  const int step = all / pieces, mask = (1 << p.s.page_shift) - 1;
+#pragma unroll 4
+  for (int i = me / pieces; i < 2 * n_moves; i += step) {
+    const int2 mv = moves[i >> 1];
     const CacheView& cv = (i & 1) ? p.vc : p.kc;
     const int from = srv_page(p.s, b, mv.x), to = srv_page(p.s, b, mv.y);
-    if (from >= p.s.num_pages || to >= p.s.num_pages) continue;
-    uint16_t* base = static_cast<uint16_t*>(cv.data) + h * cv.head + c * 8;
-    const uint4 v = *reinterpret_cast<const uint4*>(base + from * cv.page + (mv.x & mask) * cv.slot);
-    *reinterpret_cast<uint4*>(base + to * cv.page + (mv.y & mask) * cv.slot) = v;
+    if (from < p.s.num_pages && to < p.s.num_pages) {
+      uint16_t* base = static_cast<uint16_t*>(cv.data) + h * cv.head + c * 8;
+      const uint4 v = *reinterpret_cast<const uint4*>(base + from * cv.page + (mv.x & mask) * cv.slot);
+      *reinterpret_cast<uint4*>(base + to * cv.page + (mv.y & mask) * cv.slot) = v;
+    }
   }
 }
 
@@ -267,20 +317,19 @@ cudaError_t append_launch(const AppendParams& p, cudaStream_t stream) {
   return launch_pdl(append_kernel, dim3(blocks), dim3(APPEND_THREADS), 0, stream, p);
 }
 
-cudaError_t evict_launch(const EvictParams& p, cudaStream_t stream) {
-  const int smem = (int)(p.cap < EVICT_SMEM_SLOTS ? p.cap : EVICT_SMEM_SLOTS) * 4;
-  cudaError_t e = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+cudaError_t evict_launch(const EvictParams& p, int sms, cudaStream_t stream) {
+  // Blocks per head: as many as keep at least 2048 slots each, while there are
+  // multiprocessors for them.  Threads: one per four slots or so.
+  const long bh = (long)p.s.batch * p.kv_heads;
+  int cluster = 1;
+  while (cluster < EVICT_MAX_CLUSTER && p.cap / (2 * cluster) >= 2048 && bh * 2 * cluster <= 2 * sms) cluster *= 2;
+  const long each = ((p.cap + cluster - 1) / cluster + 31) & ~31l;
+  const int threads = each <= 1024 ? 128 : each <= 2048 ? 256 : EVICT_MAX_THREADS;
+  const int smem = each <= EVICT_HELD_SLOTS ? (int)each * 8 : EVICT_HELD_SLOTS * 8;
+  cudaError_t e = cudaFuncSetAttribute(evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  const int bh = p.s.batch * p.kv_heads;
-  e = launch_pdl(evict_select_kernel, dim3(bh), dim3(EVICT_THREADS), smem, stream, p);
-  if (e != cudaSuccess || p.most_moves == 0) return e;
-  // Enough blocks for the most moves a call can have, in at most about eight waves.
-  const long steps = (2l * p.most_moves * (p.head_dim / 8) + 32 * EVICT_MOVE_WARPS - 1) / (32 * EVICT_MOVE_WARPS);
-  long x = 148l * 8 * 8 / bh;
-  x = x > steps ? steps : x;
-  x = x < 1 ? 1 : x;
-  return launch_pdl(evict_move_kernel, dim3((unsigned)bh, (unsigned)x), dim3(32 * EVICT_MOVE_WARPS), 0,
-                    stream, p);
+  return launch_pdl_cluster(evict_kernel, dim3((unsigned)(bh * cluster)), dim3(threads), smem, stream, cluster, p,
+                            cluster);
 }
 
 }  // namespace tttj

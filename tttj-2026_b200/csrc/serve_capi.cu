@@ -384,7 +384,7 @@ static int evict_most_moves(const tttj_seqs* s, int keep) {
 size_t tttj_cache_evict_workspace_bytes(const tttj_seqs* s, int keep) {
   if (check_seqs("cache_evict", s, true, false) || keep <= 0) return 0;
   const size_t bh = (size_t)s->batch * s->kv_heads;
-  return up(bh * evict_most_moves(s, keep) * sizeof(int2)) + up(bh * 4);
+  return up(bh * evict_most_moves(s, keep) * sizeof(int2) + 1);  // never 0: that stands for an error
 }
 
 int tttj_cache_evict(const tttj_seqs* s, const tttj_pages* k_cache, const tttj_pages* v_cache, const float* mass,
@@ -422,10 +422,10 @@ int tttj_cache_evict(const tttj_seqs* s, const tttj_pages* k_cache, const tttj_p
   p.recent = recent;
   p.cap = (long)s->pages_per_seq * s->page_size;
   p.most_moves = evict_most_moves(s, keep);
-  const size_t bh = (size_t)s->batch * s->kv_heads;
   p.moves = reinterpret_cast<int2*>(workspace);
-  p.n_moves = reinterpret_cast<int*>(static_cast<uint8_t*>(workspace) + up(bh * p.most_moves * sizeof(int2)));
-  CAPI_CUDA(evict_launch(p, static_cast<cudaStream_t>(stream)));
+  int sms = 0;
+  TRY(sm_count_here(&sms));
+  CAPI_CUDA(evict_launch(p, sms, static_cast<cudaStream_t>(stream)));
   return TTTJ_OK;
 }
 

@@ -58,16 +58,13 @@ __global__ void __launch_bounds__(TILE_PLAN_THREADS) tile_plan_kernel(const Tile
   __shared__ int s_n[SRV_MAX_BATCH], s_len[SRV_MAX_BATCH];
   __shared__ int s_hist[TILE_BUCKETS];
   __shared__ int s_warp[32];
-  __shared__ unsigned long long s_all, s_rest;
+  __shared__ unsigned long long s_sum[2][32];  // key tiles of all items / of those in the last wave
   __shared__ int s_joins, s_parts, s_entries;
   griddep_wait();
   griddep_launch();
   const int tid = threadIdx.x, batch = p.s.batch;
   const int item_tokens = nt * p.tile_tokens;
-  if (tid == 0) {
-    s_all = s_rest = 0;
-    s_joins = s_parts = s_entries = 0;
-  }
+  if (tid == 0) s_joins = s_parts = s_entries = 0;
   s_hist[tid] = 0;
   // Two sequences per thread: items, then their prefix sums.
   int cnt[2] = {0, 0};
@@ -144,12 +141,37 @@ __global__ void __launch_bounds__(TILE_PLAN_THREADS) tile_plan_kernel(const Tile
     sum += t;
     if (e >= whole) rest += t;
   }
-  if (sum) atomicAdd(&s_all, sum);
-  if (rest) atomicAdd(&s_rest, rest);
+#pragma unroll
+  for (int d = 16; d; d >>= 1) {
+    sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    rest += __shfl_xor_sync(0xffffffffu, rest, d);
+  }
+  if ((tid & 31) == 0) {
+    s_sum[0][tid >> 5] = sum;
+    s_sum[1][tid >> 5] = rest;
+  }
   __syncthreads();
-  const long share = (long)(s_all * p.kv_heads + grid - 1) / grid;
-  const int most = (int)max(share, (long)TILE_MIN_PIECE);
-  const int most_rest = (int)max((long)(s_rest * p.kv_heads + grid - 1) / grid, (long)TILE_MIN_PIECE);
+  sum = s_sum[0][tid & 31];
+  rest = s_sum[1][tid & 31];
+#pragma unroll
+  for (int d = 16; d; d >>= 1) {
+    sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    rest += __shfl_xor_sync(0xffffffffu, rest, d);
+  }
+  const int most = (int)max((long)(sum * p.kv_heads + grid - 1) / grid, (long)TILE_MIN_PIECE);
+  const int most_rest = (int)max((long)(rest * p.kv_heads + grid - 1) / grid, (long)TILE_MIN_PIECE);
+  // Adds n to a bucket, returns what it held: lanes of one bucket share one atomic.
+  auto add_to = [&](int at, int n) {
+    const unsigned active = __activemask();
+    const unsigned same = __match_any_sync(active, at);
+    if (__all_sync(active, n == 1)) {
+      const int leader = __ffs(same) - 1;
+      int base = 0;
+      if ((tid & 31) == leader) base = atomicAdd(&s_hist[at], __popc(same));
+      return __shfl_sync(active, base, leader) + __popc(same & ((1u << (tid & 31)) - 1));
+    }
+    return atomicAdd(&s_hist[at], n);
+  };
   auto pieces_of = [&](int e, int t) {
     const int c = e >= whole ? min(most, most_rest) : most;
     return (t + c - 1) / c;
@@ -159,7 +181,7 @@ __global__ void __launch_bounds__(TILE_PLAN_THREADS) tile_plan_kernel(const Tile
     int b;
     const int q = locate(e, &b);
     const int t = tiles_of(b, q), n = pieces_of(e, t);
-    atomicAdd(&s_hist[bucket((t + n - 1) / n)], n);
+    add_to(bucket((t + n - 1) / n), n);
   }
   __syncthreads();
   {
@@ -196,7 +218,7 @@ __global__ void __launch_bounds__(TILE_PLAN_THREADS) tile_plan_kernel(const Tile
       part = atomicAdd(&s_parts, n * p.kv_heads);
       p.plan.joins[atomicAdd(&s_joins, 1)] = TileJoin{out.b, out.q, n, part};
     }
-    const int at = atomicAdd(&s_hist[bucket((t + n - 1) / n)], n);
+    const int at = add_to(bucket((t + n - 1) / n), n);
     for (int i = 0; i < n; ++i) {
       out.j0 = (int)((long)t * i / n);
       out.j1 = (int)((long)t * (i + 1) / n);

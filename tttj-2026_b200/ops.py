@@ -8,6 +8,8 @@ own layer; the forward of ``B200Transformer`` runs the same kernels from C.
 from __future__ import annotations
 
 import ctypes
+import functools
+import struct
 from typing import Optional
 
 import torch
@@ -125,77 +127,97 @@ def selftest_wait_timeout(status: torch.Tensor, limit_ns: int) -> None:
 # * Inference only: tensors that require gradients are refused while gradients are enabled.
 
 _SERVE_DTYPES = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
+# tttj_rows, tttj_pages and tttj_seqs of include/tttj_b200.h as bytes in C layout: a decode
+# step's host time counts, and packing is several times cheaper than ctypes structures.
+_pack_rows = struct.Struct("@Pqq").pack
+_pack_pages = struct.Struct("@Pqqq").pack
+_pack_seqs = struct.Struct("@PPPq9iP").pack
 
 
 def _call(device: torch.device, fn, *args) -> int:
     """Run a C entry point with ``device`` current, its current stream as last argument."""
-    if torch.cuda.current_device() == device.index:
-        return fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    index = device.index
+    if torch._C._cuda_getDevice() == index:
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
     with torch.cuda.device(device):
-        return fn(*args, torch.cuda.current_stream(device).cuda_stream)
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
 
 
-def _serve_rows(what: str, name: str, t: torch.Tensor, like: torch.Tensor, heads: Optional[int] = None) -> _lib.TttjRows:
-    if t.dim() != 3 or t.dtype != like.dtype or t.device != like.device:
-        raise ValueError(f"{what}: {name} must be [tokens, heads, head_dim], {like.dtype} on {like.device}")
-    if t.shape[0] != like.shape[0] or t.shape[2] != like.shape[2] or (heads is not None and t.shape[1] != heads):
-        raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}")
-    s = t.stride()
-    if s[2] != 1:
+def _serve_rows(what: str, name: str, t: torch.Tensor, shape: tuple, dtype: torch.dtype, device: torch.device) -> bytes:
+    if t.shape != shape or t.dtype != dtype or t.device != device:
+        raise ValueError(f"{what}: {name} must be [tokens, heads, head_dim] = {list(shape)}, {dtype} on {device}, "
+                         f"got {list(t.shape)}, {t.dtype} on {t.device}")
+    tok, head, one = t.stride()
+    if one != 1:
         raise ValueError(f"{what}: head_dim of {name} must be contiguous")
-    return _lib.TttjRows(t.data_ptr(), s[0], s[1])
+    return _pack_rows(t.data_ptr(), tok, head)
 
 
-def _serve_ints(what: str, name: str, t: torch.Tensor, shape: tuple, device: torch.device) -> int:
-    if t.dtype != torch.int32 or t.shape != shape or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{what}: {name} must be a contiguous int32 tensor {list(shape)} on {device}")
+def _serve_ints(what: str, name: str, t: torch.Tensor, n: int, device: torch.device) -> int:
+    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or t.device != device or (n > 1 and t.stride(0) != 1):
+        raise ValueError(f"{what}: {name} must be a contiguous int32 tensor [{n}] on {device}")
     return t.data_ptr()
 
 
-def _serve_pages(what: str, name: str, t: torch.Tensor, like: torch.Tensor) -> _lib.TttjPages:
-    if t.dim() != 4 or t.dtype != like.dtype or t.device != like.device or t.shape != like.shape:
-        raise ValueError(f"{what}: {name} must be [pages, page_size, kv_heads, head_dim], {like.dtype} on {like.device}")
-    s = t.stride()
-    if s[3] != 1:
+def _serve_pages(what: str, name: str, t: torch.Tensor, shape: tuple, dtype: torch.dtype, device: torch.device) -> bytes:
+    if t.shape != shape or t.dtype != dtype or t.device != device:
+        raise ValueError(f"{what}: {name} must be [pages, page_size, kv_heads, head_dim] = {list(shape)}, {dtype} on "
+                         f"{device}, got {list(t.shape)}, {t.dtype} on {t.device}")
+    page, slot, head, one = t.stride()
+    if one != 1:
         raise ValueError(f"{what}: head_dim of {name} must be contiguous")
-    return _lib.TttjPages(t.data_ptr(), s[0], s[1], s[2])
+    return _pack_pages(t.data_ptr(), page, slot, head)
 
 
-def _serve_seqs(what: str, rows: torch.Tensor, seq_offsets: Optional[torch.Tensor], heads: int, kv_heads: int,
-                cache: Optional[torch.Tensor] = None, page_table: Optional[torch.Tensor] = None,
-                cache_lens: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None,
-                tokens: int = 0) -> _lib.TttjSeqs:
-    """The call's tttj_seqs; ``rows`` gives dtype, device and head_dim (its last dimension)."""
-    dtype = _SERVE_DTYPES.get(rows.dtype)
+def _serve_type(what: str, t: torch.Tensor) -> int:
+    dtype = _SERVE_DTYPES.get(t.dtype)
     if dtype is None:
-        raise ValueError(f"{what}: dtype {rows.dtype} unsupported (float16, bfloat16)")
-    device = rows.device
-    if device.type != "cuda":
+        raise ValueError(f"{what}: dtype {t.dtype} unsupported (float16, bfloat16)")
+    if not t.is_cuda:
         raise ValueError(f"{what}: tensors must be on a CUDA device")
-    if torch.is_grad_enabled() and rows.requires_grad:
+    if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{what}: inference only (no gradient)")
-    stat = None if status is None else _serve_ints(what, "status", status, (1,), device)
-    if seq_offsets is not None:
-        if seq_offsets.dim() != 1 or seq_offsets.shape[0] < 2:
-            raise ValueError(f"{what}: seq_offsets must be [sequences + 1]")
-        batch = seq_offsets.shape[0] - 1
-        off = _serve_ints(what, "seq_offsets", seq_offsets, (batch + 1,), device)
-    else:
-        batch, off = cache_lens.shape[0], None
-    if cache is None:
-        return _lib.TttjSeqs(off, None, None, 0, batch, tokens, 0, 0, 0, dtype, heads, kv_heads, rows.shape[-1], stat)
+    return dtype
+
+
+def _serve_offsets(what: str, seq_offsets: torch.Tensor, device: torch.device) -> tuple:
+    batch = seq_offsets.shape[0] - 1 if seq_offsets.dim() == 1 else 0
+    if batch < 1:
+        raise ValueError(f"{what}: seq_offsets must be [sequences + 1]")
+    return batch, _serve_ints(what, "seq_offsets", seq_offsets, batch + 1, device)
+
+
+def _cache_seqs(what: str, off: Optional[int], batch: int, tokens: int, dtype: int, heads: int, cache: torch.Tensor,
+                page_table: torch.Tensor, cache_lens: torch.Tensor, status: Optional[torch.Tensor],
+                device: torch.device) -> tuple:
+    """(tttj_seqs as bytes, slots per sequence) of a call over a cache."""
     if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.device != device or \
             page_table.shape[0] != batch or page_table.stride(1) != 1:
         raise ValueError(f"{what}: page_table must be int32 [{batch}, pages per sequence] on {device}, rows contiguous")
-    lens = _serve_ints(what, "cache_lens", cache_lens, (batch,), device)
-    stride = page_table.stride(0) if batch > 1 else page_table.shape[1]
-    return _lib.TttjSeqs(off, lens, page_table.data_ptr(), stride, batch, tokens, page_table.shape[1],
-                         cache.shape[1], cache.shape[0], dtype, heads, kv_heads, rows.shape[-1], stat)
+    pages, page, kv_heads, head_dim = cache.shape
+    per_seq = page_table.shape[1]
+    lens = _serve_ints(what, "cache_lens", cache_lens, batch, device)
+    stat = 0 if status is None else _serve_ints(what, "status", status, 1, device)
+    return _pack_seqs(off or 0, lens, page_table.data_ptr(), page_table.stride(0) if batch > 1 else per_seq, batch, tokens,
+                      per_seq, page, pages, dtype, heads, kv_heads, head_dim, stat), per_seq * page
+
+
+@functools.lru_cache(maxsize=1024)
+def _serve_workspace_bytes(batch: int, tokens: int, dtype: int, heads: int, kv_heads: int, head_dim: int) -> int:
+    return int(_lib.lib().tttj_serve_workspace_bytes(
+        _pack_seqs(0, 0, 0, 0, batch, tokens, 0, 0, 0, dtype, heads, kv_heads, head_dim, 0)))
+
+
+def serve_workspace_bytes(batch: int, tokens: int, heads: int, kv_heads: int, head_dim: int) -> int:
+    """Workspace of prompt_attention and cache_attention for this many sequences, packed
+    tokens and heads; a larger one serves smaller calls too."""
+    n = _serve_workspace_bytes(batch, tokens, _lib.DTYPE_F16, heads, kv_heads, head_dim)
+    if n == 0:
+        _lib.check(_lib.TTTJ_ERR_INVALID, "serve_workspace_bytes")
+    return n
 
 
 def _serve_workspace(what: str, workspace: Optional[torch.Tensor], nbytes: int, device: torch.device) -> torch.Tensor:
-    if nbytes == 0:
-        _lib.check(_lib.TTTJ_ERR_INVALID, what)
     if workspace is None:
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
     if workspace.dtype != torch.uint8 or workspace.device != device or not workspace.is_contiguous():
@@ -213,23 +235,25 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_offs
     scale defaults to head_dim^-0.5.  Returns out [T, heads, head_dim] in q's dtype (``out``
     may be given; it must not overlap the inputs), with ``return_lse`` also the fp32 [T, heads]
     log-sum-exp of the scaled scores.  ``workspace`` (uint8,
-    ``serve_workspace_bytes(...)``) may be kept between calls that do not overlap."""
+    ``serve_workspace_bytes``) may be kept between calls that do not overlap."""
     what = "prompt_attention"
     if q.dim() != 3 or k.dim() != 3:
         raise ValueError(f"{what}: q and k must be [tokens, heads, head_dim]")
-    heads, kv_heads = q.shape[1], k.shape[1]
-    s = _serve_seqs(what, q, seq_offsets, heads, kv_heads, status=status, tokens=q.shape[0])
+    dtype, device, kind = q.dtype, q.device, _serve_type(what, q)
+    tokens, heads, d = q.shape
+    kv_heads = k.shape[1]
+    batch, off = _serve_offsets(what, seq_offsets, device)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    rq, rk = _serve_rows(what, "q", q, q), _serve_rows(what, "k", k, q)
-    rv, ro = _serve_rows(what, "v", v, q, kv_heads), _serve_rows(what, "out", out, q, heads)
-    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
-    L = _lib.lib()
-    p = ctypes.byref(s)
-    ws = _serve_workspace(what, workspace, L.tttj_serve_workspace_bytes(p), q.device)
-    rc = _call(q.device, L.tttj_prompt_attention, p, ctypes.byref(rq), ctypes.byref(rk), ctypes.byref(rv),
-               ctypes.byref(ro), lse.data_ptr() if return_lse else None, 1 if causal else 0,
-               q.shape[2] ** -0.5 if scale is None else float(scale), ws.data_ptr(), ws.numel())
+        out = torch.empty((tokens, heads, d), dtype=dtype, device=device)
+    rows, kv_rows = (tokens, heads, d), (tokens, kv_heads, d)
+    s = _pack_seqs(off, 0, 0, 0, batch, tokens, 0, 0, 0, kind, heads, kv_heads, d,
+                   0 if status is None else _serve_ints(what, "status", status, 1, device))
+    rq, rk = _serve_rows(what, "q", q, rows, dtype, device), _serve_rows(what, "k", k, kv_rows, dtype, device)
+    rv, ro = _serve_rows(what, "v", v, kv_rows, dtype, device), _serve_rows(what, "out", out, rows, dtype, device)
+    lse = torch.empty((tokens, heads), dtype=torch.float32, device=device) if return_lse else None
+    ws = _serve_workspace(what, workspace, _serve_workspace_bytes(batch, tokens, kind, heads, kv_heads, d), device)
+    rc = _call(device, _lib.lib().tttj_prompt_attention, s, rq, rk, rv, ro, lse.data_ptr() if return_lse else None,
+               1 if causal else 0, d ** -0.5 if scale is None else scale, ws.data_ptr(), ws.shape[0])
     if rc:
         _lib.check(rc, what)
     return (out, lse) if return_lse else out
@@ -247,21 +271,24 @@ def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     what = "cache_attention"
     if q.dim() != 3 or k_cache.dim() != 4:
         raise ValueError(f"{what}: q must be [tokens, heads, head_dim], k_cache [pages, page_size, kv_heads, head_dim]")
-    heads, kv_heads = q.shape[1], k_cache.shape[2]
-    s = _serve_seqs(what, q, seq_offsets, heads, kv_heads, k_cache, page_table, cache_lens, status, q.shape[0])
-    if k_cache.dtype != q.dtype or k_cache.device != q.device or k_cache.shape[3] != q.shape[2]:
-        raise ValueError(f"{what}: the cache must be {q.dtype} on {q.device} with head_dim {q.shape[2]}")
+    dtype, device, kind = q.dtype, q.device, _serve_type(what, q)
+    tokens, heads, d = q.shape
+    pages = k_cache.shape
+    kv_heads = pages[2]
+    if pages[3] != d:
+        raise ValueError(f"{what}: the cache has head_dim {pages[3]}, q {d}")
+    batch, off = _serve_offsets(what, seq_offsets, device)
+    s, _ = _cache_seqs(what, off, batch, tokens, kind, heads, k_cache, page_table, cache_lens, status, device)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    rq, ro = _serve_rows(what, "q", q, q), _serve_rows(what, "out", out, q, heads)
-    ck, cv = _serve_pages(what, "k_cache", k_cache, k_cache), _serve_pages(what, "v_cache", v_cache, k_cache)
-    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
-    L = _lib.lib()
-    p = ctypes.byref(s)
-    ws = _serve_workspace(what, workspace, L.tttj_serve_workspace_bytes(p), q.device)
-    rc = _call(q.device, L.tttj_cache_attention, p, ctypes.byref(rq), ctypes.byref(ck), ctypes.byref(cv),
-               ctypes.byref(ro), lse.data_ptr() if return_lse else None, 0 if max_new is None else max_new,
-               q.shape[2] ** -0.5 if scale is None else float(scale), ws.data_ptr(), ws.numel())
+        out = torch.empty((tokens, heads, d), dtype=dtype, device=device)
+    rows = (tokens, heads, d)
+    rq, ro = _serve_rows(what, "q", q, rows, dtype, device), _serve_rows(what, "out", out, rows, dtype, device)
+    ck = _serve_pages(what, "k_cache", k_cache, pages, dtype, device)
+    cv = _serve_pages(what, "v_cache", v_cache, pages, dtype, device)
+    lse = torch.empty((tokens, heads), dtype=torch.float32, device=device) if return_lse else None
+    ws = _serve_workspace(what, workspace, _serve_workspace_bytes(batch, tokens, kind, heads, kv_heads, d), device)
+    rc = _call(device, _lib.lib().tttj_cache_attention, s, rq, ck, cv, ro, lse.data_ptr() if return_lse else None,
+               max_new or 0, d ** -0.5 if scale is None else scale, ws.data_ptr(), ws.shape[0])
     if rc:
         _lib.check(rc, what)
     return (out, lse) if return_lse else out
@@ -287,18 +314,21 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     what = "cache_append"
     if k.dim() != 3 or k_cache.dim() != 4:
         raise ValueError(f"{what}: k must be [tokens, kv_heads, head_dim], k_cache [pages, page_size, kv_heads, head_dim]")
-    kv_heads = k.shape[1]
-    s = _serve_seqs(what, k, seq_offsets, kv_heads, kv_heads, k_cache, page_table, cache_lens, status, k.shape[0])
-    if k_cache.dtype != k.dtype or k_cache.device != k.device or k_cache.shape[2:] != k.shape[1:]:
-        raise ValueError(f"{what}: the cache must be {k.dtype} on {k.device} with rows {list(k.shape[1:])}")
-    rk, rv = _serve_rows(what, "k", k, k), _serve_rows(what, "v", v, k, kv_heads)
-    ck, cv = _serve_pages(what, "k_cache", k_cache, k_cache), _serve_pages(what, "v_cache", v_cache, k_cache)
-    slots = (s.batch, kv_heads, s.pages_per_seq * s.page_size)
-    pos = None if positions is None else _slot_tensor(what, "positions", positions, torch.int32, slots, k.device)
-    ms = None if mass is None else _slot_tensor(what, "mass", mass, torch.float32, slots, k.device)
-    sn = None if seen is None else _serve_ints(what, "seen", seen, (s.batch,), k.device)
-    rc = _call(k.device, _lib.lib().tttj_cache_append, ctypes.byref(s), ctypes.byref(rk), ctypes.byref(rv),
-               ctypes.byref(ck), ctypes.byref(cv), pos, ms, sn)
+    dtype, device, kind = k.dtype, k.device, _serve_type(what, k)
+    tokens, kv_heads, d = rows = k.shape
+    pages = k_cache.shape
+    if pages[2:] != rows[1:]:
+        raise ValueError(f"{what}: the cache has rows {list(pages[2:])}, k {list(rows[1:])}")
+    batch, off = _serve_offsets(what, seq_offsets, device)
+    s, cap = _cache_seqs(what, off, batch, tokens, kind, kv_heads, k_cache, page_table, cache_lens, status, device)
+    rk, rv = _serve_rows(what, "k", k, rows, dtype, device), _serve_rows(what, "v", v, rows, dtype, device)
+    ck = _serve_pages(what, "k_cache", k_cache, pages, dtype, device)
+    cv = _serve_pages(what, "v_cache", v_cache, pages, dtype, device)
+    slots = (batch, kv_heads, cap)
+    pos = None if positions is None else _slot_tensor(what, "positions", positions, torch.int32, slots, device)
+    ms = None if mass is None else _slot_tensor(what, "mass", mass, torch.float32, slots, device)
+    sn = None if seen is None else _serve_ints(what, "seen", seen, batch, device)
+    rc = _call(device, _lib.lib().tttj_cache_append, s, rk, rv, ck, cv, pos, ms, sn)
     if rc:
         _lib.check(rc, what)
 
@@ -317,19 +347,24 @@ def cache_evict(mass: torch.Tensor, positions: torch.Tensor, k_cache: torch.Tens
     what = "cache_evict"
     if k_cache.dim() != 4 or cache_lens.dim() != 1 or cache_lens.shape[0] < 1:
         raise ValueError(f"{what}: k_cache must be [pages, page_size, kv_heads, head_dim], cache_lens [sequences]")
-    kv_heads = k_cache.shape[2]
-    s = _serve_seqs(what, k_cache, None, kv_heads, kv_heads, k_cache, page_table, cache_lens, status)
-    ck, cv = _serve_pages(what, "k_cache", k_cache, k_cache), _serve_pages(what, "v_cache", v_cache, k_cache)
-    slots = (s.batch, kv_heads, s.pages_per_seq * s.page_size)
-    ms = _slot_tensor(what, "mass", mass, torch.float32, slots, k_cache.device)
-    pos = _slot_tensor(what, "positions", positions, torch.int32, slots, k_cache.device)
+    dtype, device, kind = k_cache.dtype, k_cache.device, _serve_type(what, k_cache)
+    pages = k_cache.shape
+    batch, kv_heads = cache_lens.shape[0], pages[2]
+    s, cap = _cache_seqs(what, None, batch, 0, kind, kv_heads, k_cache, page_table, cache_lens, status, device)
+    ck = _serve_pages(what, "k_cache", k_cache, pages, dtype, device)
+    cv = _serve_pages(what, "v_cache", v_cache, pages, dtype, device)
+    slots = (batch, kv_heads, cap)
+    ms = _slot_tensor(what, "mass", mass, torch.float32, slots, device)
+    pos = _slot_tensor(what, "positions", positions, torch.int32, slots, device)
     L = _lib.lib()
-    p = ctypes.byref(s)
-    ws = _serve_workspace(what, None, L.tttj_cache_evict_workspace_bytes(p, keep), k_cache.device)
+    nbytes = L.tttj_cache_evict_workspace_bytes(s, keep)
+    if nbytes == 0:
+        _lib.check(_lib.TTTJ_ERR_INVALID, what)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
     mass_out, pos_out = torch.empty_like(mass), torch.empty_like(positions)
     lens_out = torch.empty_like(cache_lens)
-    rc = _call(k_cache.device, L.tttj_cache_evict, p, ctypes.byref(ck), ctypes.byref(cv), ms, pos, keep, recent,
-               mass_out.data_ptr(), pos_out.data_ptr(), lens_out.data_ptr(), ws.data_ptr(), ws.numel())
+    rc = _call(device, L.tttj_cache_evict, s, ck, cv, ms, pos, keep, recent, mass_out.data_ptr(), pos_out.data_ptr(),
+               lens_out.data_ptr(), ws.data_ptr(), nbytes)
     if rc:
         _lib.check(rc, what)
     return mass_out, pos_out, lens_out
@@ -349,21 +384,24 @@ def cache_mass(q: torch.Tensor, lse: torch.Tensor, k_cache: torch.Tensor, page_t
     what = "cache_mass"
     if q.dim() != 3 or k_cache.dim() != 4:
         raise ValueError(f"{what}: q must be [tokens, heads, head_dim], k_cache [pages, page_size, kv_heads, head_dim]")
-    heads, kv_heads = q.shape[1], k_cache.shape[2]
-    s = _serve_seqs(what, q, seq_offsets, heads, kv_heads, k_cache, page_table, cache_lens, status, q.shape[0])
-    if k_cache.dtype != q.dtype or k_cache.device != q.device or k_cache.shape[3] != q.shape[2]:
-        raise ValueError(f"{what}: the cache must be {q.dtype} on {q.device} with head_dim {q.shape[2]}")
-    if lse.dtype != torch.float32 or lse.shape != q.shape[:2] or lse.device != q.device or not lse.is_contiguous():
-        raise ValueError(f"{what}: lse must be a contiguous float32 tensor {list(q.shape[:2])} on {q.device}")
-    slots = (s.batch, kv_heads, s.pages_per_seq * s.page_size)
-    ms = _slot_tensor(what, "mass", mass, torch.float32, slots, q.device)
+    dtype, device, kind = q.dtype, q.device, _serve_type(what, q)
+    tokens, heads, d = rows = q.shape
+    pages = k_cache.shape
+    if pages[3] != d:
+        raise ValueError(f"{what}: the cache has head_dim {pages[3]}, q {d}")
+    batch, off = _serve_offsets(what, seq_offsets, device)
+    s, cap = _cache_seqs(what, off, batch, tokens, kind, heads, k_cache, page_table, cache_lens, status, device)
+    if lse.dtype != torch.float32 or lse.shape != rows[:2] or lse.device != device or not lse.is_contiguous():
+        raise ValueError(f"{what}: lse must be a contiguous float32 tensor [{tokens}, {heads}] on {device}")
+    slots = (batch, pages[2], cap)
+    ms = _slot_tensor(what, "mass", mass, torch.float32, slots, device)
     if out is None:
         out = torch.empty_like(mass)
-    mo = _slot_tensor(what, "out", out, torch.float32, slots, q.device)
-    rq, ck = _serve_rows(what, "q", q, q), _serve_pages(what, "k_cache", k_cache, k_cache)
-    rc = _call(q.device, _lib.lib().tttj_cache_mass, ctypes.byref(s), ctypes.byref(rq), lse.data_ptr(),
-               ctypes.byref(ck), ms, mo, 0 if max_new is None else max_new,
-               q.shape[2] ** -0.5 if scale is None else float(scale))
+    mo = _slot_tensor(what, "out", out, torch.float32, slots, device)
+    rq = _serve_rows(what, "q", q, rows, dtype, device)
+    ck = _serve_pages(what, "k_cache", k_cache, pages, dtype, device)
+    rc = _call(device, _lib.lib().tttj_cache_mass, s, rq, lse.data_ptr(), ck, ms, mo, max_new or 0,
+               d ** -0.5 if scale is None else scale)
     if rc:
         _lib.check(rc, what)
     return out
