@@ -155,7 +155,7 @@ struct AppendParams {
   float* mass;       // the same shape, or nullptr
   const int* seen;   // [batch] tokens seen by each sequence, or nullptr (= lens)
 };
-cudaError_t append_launch(const AppendParams& p, cudaStream_t stream);
+cudaError_t append_launch(const AppendParams& p, int sms, cudaStream_t stream);
 
 struct EvictParams {
   SrvSeqs s;  // seq_off is unused

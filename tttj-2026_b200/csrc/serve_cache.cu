@@ -8,19 +8,22 @@ namespace tttj {
 namespace {
 
 // ------------------------------------------------------------------ append
-// One 16-byte piece of one head's key or value row per thread and step: the bytes of k,
-// v and of the cache rows they become bound it.  A warp's pieces are consecutive, so both
-// sides move whole sectors.  Blocks take APPEND_TOKENS tokens; a token's sequence is found by a
-// binary search of the offsets, uniform in the block's small groups of threads.
+// The bytes of k, v and of the cache rows they become bound it.  A thread keeps one 16-byte
+// piece of a token's k | v rows and copies it for U tokens, all loads before the first
+// store, so a block has 256 x U pieces in flight; a warp's pieces are consecutive, so
+// both sides move whole sectors.  The block's tokens are located (sequence, slot, page) once, by
+// a binary search of the offsets per token.
 constexpr int APPEND_THREADS = 256;
-constexpr int APPEND_TOKENS = 4;
+constexpr int APPEND_MOST_TOKENS = 256;  // of one block: U x groups, at least 8 threads a token
 
-__global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const AppendParams p) {
-  __shared__ int s_b[APPEND_TOKENS], s_slot[APPEND_TOKENS], s_page[APPEND_TOKENS], s_first[APPEND_TOKENS];
+template <int U>
+__global__ void __launch_bounds__(APPEND_THREADS, 5) append_kernel(const AppendParams p, int lanes, int per_block) {
+  __shared__ int s_b[APPEND_MOST_TOKENS], s_slot[APPEND_MOST_TOKENS], s_page[APPEND_MOST_TOKENS];
+  __shared__ int s_first[APPEND_MOST_TOKENS];
   griddep_wait();
   griddep_launch();
-  const long t0 = (long)blockIdx.x * APPEND_TOKENS;
-  const int tokens = (int)min((long)APPEND_TOKENS, p.s.tokens - t0);
+  const long t0 = (long)blockIdx.x * per_block;
+  const int tokens = (int)min((long)per_block, p.s.tokens - t0);
   if ((int)threadIdx.x < tokens) {
     const int t = (int)t0 + threadIdx.x;
     int lo = 0, hi = p.s.batch - 1;  // the sequence of this token, if any
@@ -38,27 +41,37 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const AppendPara
     s_first[threadIdx.x] = (p.seen != nullptr ? p.seen[lo] : q.len) - q.n + (t - q.row0);
   }
   __syncthreads();
-  const int per_head = p.head_dim / 8;
-  const int per_tok = 2 * p.kv_heads * per_head;
-  for (int i = threadIdx.x; i < tokens * per_tok; i += APPEND_THREADS) {
-    const int j = i / per_tok;
-    int x = i - j * per_tok;
-    const int page = s_page[j];
-    if (page >= p.s.num_pages) continue;
-    const bool is_v = x >= p.kv_heads * per_head;
-    if (is_v) x -= p.kv_heads * per_head;
-    const int h = x / per_head, c = x - h * per_head;
-    const int in_page = s_slot[j] & ((1 << p.s.page_shift) - 1);
-    const uint16_t* src = static_cast<const uint16_t*>(is_v ? p.v : p.k) +
-                          (t0 + j) * (is_v ? p.v_tok : p.k_tok) + h * (is_v ? p.v_head : p.k_head) + c * 8;
+  const int per_head = p.head_dim / 8, per_tensor = p.kv_heads * per_head;
+  const int groups = APPEND_THREADS / lanes, group = threadIdx.x / lanes;
+  const int page_mask = (1 << p.s.page_shift) - 1;
+  for (int x = threadIdx.x - group * lanes; group < groups && x < 2 * per_tensor; x += lanes) {
+    const bool is_v = x >= per_tensor;
+    const int y = is_v ? x - per_tensor : x;
+    const int h = y / per_head, c = y - h * per_head;
+    const long tok = is_v ? p.v_tok : p.k_tok;
+    const uint16_t* src = static_cast<const uint16_t*>(is_v ? p.v : p.k) + h * (is_v ? p.v_head : p.k_head) + c * 8;
     const CacheView& to = is_v ? p.vc : p.kc;
-    uint16_t* dst = static_cast<uint16_t*>(to.data) + page * to.page + in_page * to.slot + h * to.head + c * 8;
-    *reinterpret_cast<uint4*>(dst) = __ldg(reinterpret_cast<const uint4*>(src));
+    uint16_t* dst = static_cast<uint16_t*>(to.data) + h * to.head + c * 8;
+    const long page_stride = to.page, slot_stride = to.slot;
+    uint4 v[U];
+    bool there[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = group + u * groups;
+      there[u] = j < tokens && s_page[j] < p.s.num_pages;
+      if (there[u]) v[u] = __ldg(reinterpret_cast<const uint4*>(src + (t0 + j) * tok));
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = group + u * groups;
+      if (there[u])
+        *reinterpret_cast<uint4*>(dst + s_page[j] * page_stride + (s_slot[j] & page_mask) * slot_stride) = v[u];
+    }
   }
   if (p.positions != nullptr || p.mass != nullptr) {
     const long cap = (long)p.s.pages_per_seq << p.s.page_shift;
     for (int i = threadIdx.x; i < tokens * p.kv_heads; i += APPEND_THREADS) {
-      const int j = i / p.kv_heads, h = i - j * p.kv_heads;
+      const int h = i / tokens, j = i - h * tokens;  // neighbours write neighbouring slots
       if (s_page[j] >= p.s.num_pages) continue;
       const long at = ((long)s_b[j] * p.kv_heads + h) * cap + s_slot[j];
       if (p.positions != nullptr) p.positions[at] = s_first[j];
@@ -81,6 +94,7 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const AppendPara
 constexpr int EVICT_MAX_CLUSTER = 8;
 constexpr int EVICT_MAX_THREADS = 512;
 constexpr int EVICT_BINS = 2048;
+constexpr int EVICT_BATCH = 4;
 constexpr int EVICT_HELD_SLOTS = 24 * 1024;  // slots of one block held in shared memory (8 bytes each)
 
 // Unsigned image of a mass: larger mass, larger integer; -0 as +0, NaN lowest.
@@ -88,12 +102,6 @@ __device__ __forceinline__ uint32_t evict_key(float mass) {
   if (mass != mass) return 0x007fffffu;  // the image of -inf
   const uint32_t u = __float_as_uint(mass + 0.f);
   return (u >> 31) ? ~u : (u | 0x80000000u);
-}
-
-__device__ __forceinline__ int ld_cluster(uint32_t addr) {
-  int v;
-  asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-  return v;
 }
 
 struct EvictShared {
@@ -140,8 +148,8 @@ __global__ void __launch_bounds__(EVICT_MAX_THREADS) evict_kernel(const EvictPar
   auto sync_all = [&] {
     if (cluster > 1) cluster_sync_all(); else __syncthreads();
   };
-  auto peer = [&](const int* x, int r) {
-    return cluster > 1 ? ld_cluster(map_to_cta(smem_u32(x), (uint32_t)r)) : *x;
+  auto peer = [&](int* x, int r) -> int {
+    return cluster > 1 ? *static_cast<int*>(__cluster_map_shared_rank(x, (unsigned)r)) : *x;
   };
   // This block's slots, a multiple of 32 per warp.
   const int each = ((len + cluster - 1) / cluster + 31) & ~31;
@@ -193,12 +201,14 @@ __global__ void __launch_bounds__(EVICT_MAX_THREADS) evict_kernel(const EvictPar
     const int first = (1 << bits) - 1 - per * (int)threadIdx.x;
     int c[EVICT_BINS / 128], sum = 0;  // at least 128 threads
 #pragma unroll
-    for (int i = 0; i < EVICT_BINS / 128; ++i) {
-      c[i] = 0;
-      if (i < per)
-        for (int r = 0; r < cluster; ++r) c[i] += peer(&sh.hist[first - i], r);
-      sum += c[i];
+    for (int i = 0; i < EVICT_BINS / 128; ++i) c[i] = 0;
+    for (int r = 0; r < cluster; ++r) {
+#pragma unroll
+      for (int i = 0; i < EVICT_BINS / 128; ++i)
+        if (i < per) c[i] += peer(&sh.hist[first - i], r);
     }
+#pragma unroll
+    for (int i = 0; i < EVICT_BINS / 128; ++i) sum += c[i];
     int inc = sum;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -289,32 +299,62 @@ __global__ void __launch_bounds__(EVICT_MAX_THREADS) evict_kernel(const EvictPar
   }
   sync_all();  // the list is complete (and no block still reads another's shared memory)
   for (int i = me; i < n_moves; i += all) {
-    const int2 mv = moves[i];
+    const int2 mv = __ldcg(moves + i);
     mass_out[mv.y] = mass[mv.x];
     pos_out[mv.y] = pos[mv.x];
   }
-  // The rows: a 16-byte piece per thread and step; move i of K is row 2 i, of V row 2 i + 1.
+  // The rows: one 16-byte piece of K and of V per thread and move, EVICT_BATCH moves' loads
+  // before their stores.
   const int pieces = p.head_dim / 8;  // 4 .. 32
   const int c = threadIdx.x % pieces, h = bh - b * p.kv_heads;
   const int step = all / pieces, mask = (1 << p.s.page_shift) - 1;
-#pragma unroll 4
-  for (int i = me / pieces; i < 2 * n_moves; i += step) {
-    const int2 mv = moves[i >> 1];
-    const CacheView& cv = (i & 1) ? p.vc : p.kc;
-    const int from = srv_page(p.s, b, mv.x), to = srv_page(p.s, b, mv.y);
-    if (from < p.s.num_pages && to < p.s.num_pages) {
-      uint16_t* base = static_cast<uint16_t*>(cv.data) + h * cv.head + c * 8;
-      const uint4 v = *reinterpret_cast<const uint4*>(base + from * cv.page + (mv.x & mask) * cv.slot);
-      *reinterpret_cast<uint4*>(base + to * cv.page + (mv.y & mask) * cv.slot) = v;
+  uint16_t* kbase = static_cast<uint16_t*>(p.kc.data) + h * p.kc.head + c * 8;
+  uint16_t* vbase = static_cast<uint16_t*>(p.vc.data) + h * p.vc.head + c * 8;
+  for (int i0 = me / pieces; i0 < n_moves; i0 += EVICT_BATCH * step) {
+    int2 mv[EVICT_BATCH];
+    int from[EVICT_BATCH], to[EVICT_BATCH];
+    uint4 kv[EVICT_BATCH], vv[EVICT_BATCH];
+#pragma unroll
+    for (int u = 0; u < EVICT_BATCH; ++u)
+      mv[u] = i0 + u * step < n_moves ? __ldcg(moves + i0 + u * step) : make_int2(-1, -1);
+#pragma unroll
+    for (int u = 0; u < EVICT_BATCH; ++u) {
+      from[u] = to[u] = p.s.num_pages;
+      if (mv[u].x >= 0) {
+        from[u] = srv_page(p.s, b, mv[u].x);
+        to[u] = srv_page(p.s, b, mv[u].y);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < EVICT_BATCH; ++u) {
+      if (from[u] < p.s.num_pages && to[u] < p.s.num_pages) {
+        kv[u] = *reinterpret_cast<const uint4*>(kbase + from[u] * p.kc.page + (mv[u].x & mask) * p.kc.slot);
+        vv[u] = *reinterpret_cast<const uint4*>(vbase + from[u] * p.vc.page + (mv[u].x & mask) * p.vc.slot);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < EVICT_BATCH; ++u) {
+      if (from[u] < p.s.num_pages && to[u] < p.s.num_pages) {
+        *reinterpret_cast<uint4*>(kbase + to[u] * p.kc.page + (mv[u].y & mask) * p.kc.slot) = kv[u];
+        *reinterpret_cast<uint4*>(vbase + to[u] * p.vc.page + (mv[u].y & mask) * p.vc.slot) = vv[u];
+      }
     }
   }
 }
 
 }  // namespace
 
-cudaError_t append_launch(const AppendParams& p, cudaStream_t stream) {
-  const int blocks = (p.s.tokens + APPEND_TOKENS - 1) / APPEND_TOKENS;
-  return launch_pdl(append_kernel, dim3(blocks), dim3(APPEND_THREADS), 0, stream, p);
+cudaError_t append_launch(const AppendParams& p, int sms, cudaStream_t stream) {
+  const long pieces = 2l * p.kv_heads * (p.head_dim / 8);
+  const int lanes = (int)(pieces < APPEND_THREADS ? pieces : APPEND_THREADS);
+  const int groups = APPEND_THREADS / lanes;
+  // Four tokens per thread where that still gives every multiprocessor four blocks, else
+  // one (a decode step: latency counts, not bytes in flight).
+  const bool many = p.s.tokens / (4 * groups) >= 4 * sms;
+  const int per_block = groups * (many ? 4 : 1);
+  const unsigned blocks = (unsigned)((p.s.tokens + per_block - 1) / per_block);
+  return launch_pdl(many ? append_kernel<4> : append_kernel<1>, dim3(blocks), dim3(APPEND_THREADS), 0, stream, p,
+                    lanes, per_block);
 }
 
 cudaError_t evict_launch(const EvictParams& p, int sms, cudaStream_t stream) {

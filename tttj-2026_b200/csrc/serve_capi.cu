@@ -330,7 +330,9 @@ int tttj_cache_append(const tttj_seqs* s, const tttj_rows* k, const tttj_rows* v
   p.positions = positions;
   p.mass = mass;
   p.seen = seen;
-  CAPI_CUDA(append_launch(p, static_cast<cudaStream_t>(stream)));
+  int sms = 0;
+  TRY(sm_count_here(&sms));
+  CAPI_CUDA(append_launch(p, sms, static_cast<cudaStream_t>(stream)));
   return TTTJ_OK;
 }
 

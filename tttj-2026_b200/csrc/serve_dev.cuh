@@ -7,6 +7,23 @@
 
 namespace tttj {
 
+// mbar_wait with the timer read only every 64 polls: reading it between polls costs more than
+// the hand-over that is waited for.  Bounded like mbar_wait (limit_ns, or *abort).
+__device__ __forceinline__ bool srv_wait(uint32_t bar, uint32_t parity, volatile int* abort, uint64_t limit_ns) {
+#pragma unroll 1
+  for (int i = 0; i < 64; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+#pragma unroll 1
+  while (true) {
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i)
+      if (mbar_try_wait(bar, parity)) return true;
+    if (abort != nullptr && *abort) return false;
+    if (globaltimer_ns() - t0 > limit_ns) return false;
+  }
+}
+
 template <bool BF16>
 __device__ __forceinline__ uint32_t srv_pack(float a, float b) {
   if constexpr (BF16) {
@@ -74,6 +91,18 @@ __device__ __forceinline__ float srv_max3(float a, float b, float c) {
   float d;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
+}
+
+// tmem_wait_ld for a load whose registers are first used after other work: naming them keeps
+// the compiler from moving a use in front of the wait.
+__device__ __forceinline__ void tmem_wait_ld_of(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+      : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+        "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+        "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+        "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+      :
+      : "memory");
 }
 
 // Natural log-sum-exp of a row from its maximum (log2 domain) and sum: -inf for a row that

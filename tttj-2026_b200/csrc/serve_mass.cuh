@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(MASS_THREADS, 1)
       int page = p.s.num_pages;
       if (lane < boxes && slot < w.q.len) page = srv_page(p.s, w.b, slot);
       const int kb = (int)(kc % SM::KBUF);
-      ok = __all_sync(0xffffffffu, mbar_wait(bar_k_empty + 8 * kb, (uint32_t)((kc / SM::KBUF) & 1) ^ 1u, abort_flag, limit));
+      ok = __all_sync(0xffffffffu, srv_wait(bar_k_empty + 8 * kb, (uint32_t)((kc / SM::KBUF) & 1) ^ 1u, abort_flag, limit));
       if (!ok) break;
       if (lane == 0) mbar_arrive_expect_tx(bar_k_full + 8 * kb, NT * SM::TILE);
       __syncwarp();
@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(MASS_THREADS, 1)
           lim[e] = live ? w.q.len - w.q.n + tok0 + tk : -1;
         }
         const int st = (int)(qc % SM::STAGES);
-        ok = __all_sync(0xffffffffu, mbar_wait(bar_q_empty + 8 * st, (uint32_t)((qc / SM::STAGES) & 1) ^ 1u, abort_flag, limit));
+        ok = __all_sync(0xffffffffu, srv_wait(bar_q_empty + 8 * st, (uint32_t)((qc / SM::STAGES) & 1) ^ 1u, abort_flag, limit));
         if (!ok) break;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -185,9 +185,9 @@ __global__ void __launch_bounds__(MASS_THREADS, 1)
       *abort_flag = 1;
       report_status(p.s.status, SRV_DEV_TIMEOUT);
       for (long j = kc > SM::KBUF ? kc - SM::KBUF : 0; j < kc; ++j)
-        mbar_wait(bar_k_full + 8 * (int)(j % SM::KBUF), (uint32_t)((j / SM::KBUF) & 1), nullptr, limit);
+        srv_wait(bar_k_full + 8 * (int)(j % SM::KBUF), (uint32_t)((j / SM::KBUF) & 1), nullptr, limit);
       for (long j = qc > SM::STAGES ? qc - SM::STAGES : 0; j < qc; ++j)
-        mbar_wait(bar_q_full + 8 * (int)(j % SM::STAGES), (uint32_t)((j / SM::STAGES) & 1), nullptr, limit);
+        srv_wait(bar_q_full + 8 * (int)(j % SM::STAGES), (uint32_t)((j / SM::STAGES) & 1), nullptr, limit);
     }
   } else if (warp == 9 || (warp == 10 && NT == 2)) {
     // ------------------------------------------------------------ MMA issuers
@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(MASS_THREADS, 1)
     bool ok = true, issued = false;
     long kc = 0, qc = 0;
     auto wait = [&](uint32_t bar, uint32_t parity) {
-      ok = __all_sync(FULL, mbar_wait(bar, parity, abort_flag, limit));
+      ok = __all_sync(FULL, srv_wait(bar, parity, abort_flag, limit));
       tc_fence_after();
       return ok;
     };
@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(MASS_THREADS, 1)
       }
       if (issued) {
         mma_commit_warp(bar_drain + 8 * t);
-        mbar_wait(bar_drain + 8 * t, 0, nullptr, limit);
+        srv_wait(bar_drain + 8 * t, 0, nullptr, limit);
       }
     }
   } else if (warp < 4 * NT) {
@@ -256,8 +256,8 @@ __global__ void __launch_bounds__(MASS_THREADS, 1)
         const int rows = min(TOK, w.q.n - tok0) * p.group;
         // Some row of this tile does not see some key of this one.
         const bool partly = tile0 + ATC_BM - 1 > w.q.len - w.q.n + tok0;
-        if (!mbar_wait(bar_q_full + 8 * st, (uint32_t)((qc / SM::STAGES) & 1), abort_flag, limit) ||
-            !mbar_wait(bar_s_full + 8 * (2 * t + buf), (uint32_t)((qc >> 1) & 1), abort_flag, limit)) {
+        if (!srv_wait(bar_q_full + 8 * st, (uint32_t)((qc / SM::STAGES) & 1), abort_flag, limit) ||
+            !srv_wait(bar_s_full + 8 * (2 * t + buf), (uint32_t)((qc >> 1) & 1), abort_flag, limit)) {
           ok = false;
           break;
         }

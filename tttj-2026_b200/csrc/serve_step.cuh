@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(STEP_THREADS, step_ctas_per_sm(HD))
           c1 = slot & ((1 << p.s.page_shift) - 1);
         }
         const int st = (int)(it % SM::STAGES);
-        ok = mbar_wait(bar_empty + 8 * st, (uint32_t)((it / SM::STAGES) & 1) ^ 1u, abort_flag,
+        ok = srv_wait(bar_empty + 8 * st, (uint32_t)((it / SM::STAGES) & 1) ^ 1u, abort_flag,
                        p.wait_limit_ns);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(STEP_THREADS, step_ctas_per_sm(HD))
     // Issued loads land before the CTA may exit.
     if (!ok)
       for (long j = it > SM::STAGES ? it - SM::STAGES : 0; j < it; ++j)
-        mbar_wait(bar_full + 8 * (int)(j % SM::STAGES), (uint32_t)((j / SM::STAGES) & 1), nullptr,
+        srv_wait(bar_full + 8 * (int)(j % SM::STAGES), (uint32_t)((j / SM::STAGES) & 1), nullptr,
                   p.wait_limit_ns);
     return;
   }
@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(STEP_THREADS, step_ctas_per_sm(HD))
 
     for (int t = r.t0; t < r.t1; ++t, ++it) {
       const int st = (int)(it % SM::STAGES);
-      ok = mbar_wait(bar_full + 8 * st, (uint32_t)((it / SM::STAGES) & 1), abort_flag, p.wait_limit_ns);
+      ok = srv_wait(bar_full + 8 * st, (uint32_t)((it / SM::STAGES) & 1), abort_flag, p.wait_limit_ns);
       if (!__all_sync(0xffffffffu, ok)) {
         ok = false;
         break;

@@ -9,13 +9,13 @@ template <int HD, bool BF16>
 cudaError_t launch(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v, const TileParams& p,
                    int grid, cudaStream_t stream) {
   auto kern = tile_kernel<HD, BF16>;
-  constexpr int smem = AtcSmem<HD>::TOTAL;
+  constexpr int smem = TileSmem<HD>::ALL;
   static_assert(smem <= 232448, "shared memory exceeds the 227 KB per-CTA limit");
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   e = launch_pdl(tile_plan_kernel, dim3(1), dim3(TILE_PLAN_THREADS), 0, stream, p, tile_nt(HD), grid);
   if (e != cudaSuccess) return e;
-  e = launch_pdl(kern, dim3(grid), dim3(ATC_THREADS), smem, stream, tm_q, tm_k, tm_v, p);
+  e = launch_pdl(kern, dim3(grid), dim3(tile_threads(tile_nt(HD))), smem, stream, tm_q, tm_k, tm_v, p);
   if (e != cudaSuccess) return e;
   return launch_pdl(tile_join_kernel<HD, BF16>, dim3(4 * grid), dim3(32 * TILE_JOIN_WARPS), 0, stream, p);
 }

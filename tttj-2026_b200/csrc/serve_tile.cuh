@@ -12,10 +12,11 @@
 //                     longest items first.  An item is NT query tiles of one head.  Items
 //                     that would leave CTAs idle -- those of a last, partial wave, and any
 //                     longer than a CTA's fair share -- are cut along the keys.
-//   tile_kernel       persistent CTAs (1 per SM) of 11 warps take items in turn: a TMA
+//   tile_kernel       persistent CTAs (1 per SM) of 12 warps take items in turn: a TMA
 //                     loader, one MMA-issuing warp and four softmax warps per query tile
-//                     (one thread per row), running statistics in fp32, O rescaled only
-//                     when a row's maximum grew by more than 2^8.
+//                     (one thread per row), and a warp that prepares V tiles; running
+//                     statistics in fp32, O rescaled only when a row's maximum grew by
+//                     more than 2^8.
 //   tile_join_kernel  joins the pieces of cut items in the order of their keys.
 //
 // Hidden keys.  Scores of keys a row does not see are replaced by -inf.  Their values still
@@ -35,9 +36,37 @@ struct TileInfo {  // one decoded item, in shared memory
   int b, q, h, row0, n, len, tok0, part;
   int j0;     // first key tile of this piece
   int n_kv;   // key tiles of this piece; -1: no more items
-  int nt[2];  // key tiles of query tile 0 / 1 inside this piece
+  int ns[2];  // softmax steps of query tile 0 / 1 inside this piece
 };
 static_assert(sizeof(TileInfo) <= 64, "item info slot is 64 bytes");
+
+// Warps: four softmax warps per query tile (their number modulo four is their TMEM quadrant),
+// the loader, one MMA issuer per query tile, the cleaner.
+constexpr int tile_threads(int nt) { return 32 * (4 * nt + 1 + nt + 1); }
+
+// Keys per step of the softmax.  TMEM (512 columns) holds, per query tile, the scores (fp32, one
+// column per key), the probabilities (16 bits, half a column per key, PBUF buffers) and O
+// (head_dim columns).  With head_dim 128 the two O take 256 columns, so a step is 64 keys
+// there; then nothing shares columns and S of the next step is computed while the softmax
+// works on this one.  (128 keys with P written over S, as in attention_tc.cuh, make the
+// next S wait for P V: 4500 - 4900 cycles per 128 keys of both tiles, measured on prompts of 4096.)
+template <int HD>
+struct TileSmem : AtcSmem<HD> {  // tile sizes and stages as there
+  using B = AtcSmem<HD>;
+  static constexpr int KT = HD == 128 ? 64 : 128;
+  static constexpr int SUB = ATC_BN / KT;  // steps per loaded key tile
+  static constexpr int PBUF = HD == 128 ? 2 : 1;
+  __host__ __device__ static constexpr uint32_t s_col(int t) { return (uint32_t)(t * KT); }
+  __host__ __device__ static constexpr uint32_t p_col(int t) { return (uint32_t)(B::NT * KT + t * PBUF * KT / 2); }
+  __host__ __device__ static constexpr uint32_t o_col(int t) { return t == 0 ? B::TMEM_O0 : B::TMEM_O1; }
+  static_assert(B::NT * (KT + PBUF * KT / 2) <= (int)B::TMEM_O0, "TMEM columns overlap");
+  static constexpr int BARS = 4 * B::QS + 5 * B::STAGES + 10 + 4 + 2;
+  static constexpr int BAR_AT = B::Q_BYTES + B::KV_BYTES;
+  static constexpr int SLOT_AT = BAR_AT + BARS * 8;  // TMEM base, abort flag
+  static constexpr int INFO_AT = SLOT_AT + 16;       // [side][QS] items
+  static constexpr int EPI_AT = (INFO_AT + 2 * B::QS * 64 + 127) / 128 * 128;
+  static constexpr int ALL = EPI_AT + B::EPI_BYTES + 1024;
+};
 
 constexpr int TILE_MIN_PIECE = 4;  // key tiles (512 keys) a cut piece has at least
 
@@ -237,35 +266,39 @@ __global__ void __launch_bounds__(TILE_PLAN_THREADS) tile_plan_kernel(const Tile
 
 // -------------------------------------------------------------------------- attention
 template <int HD, bool BF16>
-__global__ void __launch_bounds__(ATC_THREADS, 1)
+__global__ void __launch_bounds__(tile_threads(tile_nt(HD)), 1)
     tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                 const __grid_constant__ CUtensorMap tmV, const TileParams p) {
-  using SM = AtcSmem<HD>;
+  using SM = TileSmem<HD>;
   constexpr int STAGES = SM::STAGES;
   constexpr int NT = SM::NT;
   constexpr int QBUF = SM::QBUF;
+  constexpr int LOADER = 4 * NT, ISSUER = LOADER + 1, CLEANER = ISSUER + NT;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t pad = (1024u - (raw & 1023u)) & 1023u;
   uint8_t* smem = smem_raw + pad;
-  const uint32_t sQ = smem_u32(smem);
-  const uint32_t sKV = sQ + SM::Q_BYTES;
-  const uint32_t bar0 = sKV + SM::KV_BYTES;
-  const uint32_t bar_q_full = bar0;                        // [QS]
-  const uint32_t bar_q_empty = bar0 + 8 * SM::QS;          // [QS]
-  const uint32_t bar_kv_full = bar0 + 16 * SM::QS;         // [STAGES]
-  const uint32_t bar_kv_empty = bar_kv_full + 8 * STAGES;  // [STAGES]
-  const uint32_t bar_s_full = bar_kv_empty + 8 * STAGES;   // [2]
-  const uint32_t bar_p_full = bar_s_full + 16;             // [2]
-  const uint32_t bar_o_full = bar_p_full + 16;             // [2]
-  const uint32_t bar_o_free = bar_o_full + 16;             // [2]
-  const uint32_t bar_s_free = bar_o_free + 16;             // [2] scores read by softmax
-  const uint32_t bar_pv_done = bar_s_free + 16;            // [2] P V complete
-  const uint32_t bar_drain = bar_pv_done + 16;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + SM::Q_BYTES + SM::KV_BYTES + SM::NBAR * 8);
+  const uint32_t sQ = smem_u32(smem);     // [side][QBUF]
+  const uint32_t sK = sQ + SM::Q_BYTES;   // [STAGES]
+  const uint32_t sV = sK + STAGES * SM::KV_TILE;
+  const uint32_t bar_q_full = sQ + SM::BAR_AT;              // [side][QS]
+  const uint32_t bar_q_empty = bar_q_full + 16 * SM::QS;    // [side][QS]
+  const uint32_t bar_k_full = bar_q_empty + 16 * SM::QS;    // [STAGES]
+  const uint32_t bar_k_empty = bar_k_full + 8 * STAGES;     // [STAGES]
+  const uint32_t bar_v_full = bar_k_empty + 8 * STAGES;     // [STAGES]
+  const uint32_t bar_v_ready = bar_v_full + 8 * STAGES;     // [STAGES] landed and cleaned
+  const uint32_t bar_v_empty = bar_v_ready + 8 * STAGES;    // [STAGES]
+  const uint32_t bar_s_full = bar_v_empty + 8 * STAGES;     // [side] ...
+  const uint32_t bar_p_full = bar_s_full + 16;
+  const uint32_t bar_o_full = bar_p_full + 16;
+  const uint32_t bar_o_free = bar_o_full + 16;
+  const uint32_t bar_s_free = bar_o_free + 16;              // scores read by softmax
+  const uint32_t bar_pv_done = bar_s_free + 16;             // [side][2] P V of P buffer 0 / 1 complete
+  const uint32_t bar_drain = bar_pv_done + 32;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + SM::SLOT_AT);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  TileInfo* info = reinterpret_cast<TileInfo*>(smem + SM::Q_BYTES + SM::KV_BYTES + SM::NBAR * 8 + 16);
-  const uint32_t sEpi = smem_u32(smem + SM::Q_BYTES + SM::KV_BYTES + SM::NBAR * 8 + 16 + SM::INFO_BYTES);
+  TileInfo* info = reinterpret_cast<TileInfo*>(smem + SM::INFO_AT);  // [side][QS]
+  const uint32_t sEpi = sQ + SM::EPI_AT;
 
   const int warp = warp_id();
   const int lane = lane_id();
@@ -277,29 +310,33 @@ __global__ void __launch_bounds__(ATC_THREADS, 1)
     tma_prefetch_desc(&tmQ);
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
-    for (int i = 0; i < SM::QS; ++i) {
+    for (int i = 0; i < 2 * SM::QS; ++i) {
       mbar_init(bar_q_full + 8 * i, 1);
-      mbar_init(bar_q_empty + 8 * i, NT + NT * ATC_BM);
+      // The side's issuer and softmax warps, and for side 0 the cleaner.
+      mbar_init(bar_q_empty + 8 * i, i < SM::QS ? 6 : 5);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(bar_k_full + 8 * i, 1);
+      mbar_init(bar_k_empty + 8 * i, NT);
+      mbar_init(bar_v_full + 8 * i, 1);
+      mbar_init(bar_v_ready + 8 * i, 1);
+      mbar_init(bar_v_empty + 8 * i, NT);
+    }
+    for (int i = 0; i < 2; ++i) {  // softmax side: one arrival per warp
       mbar_init(bar_s_full + 8 * i, 1);
-      mbar_init(bar_p_full + 8 * i, ATC_BM);
+      mbar_init(bar_p_full + 8 * i, 4);
       mbar_init(bar_o_full + 8 * i, 1);
-      mbar_init(bar_o_free + 8 * i, ATC_BM);
-      mbar_init(bar_s_free + 8 * i, ATC_BM);
-      mbar_init(bar_pv_done + 8 * i, 1);
+      mbar_init(bar_o_free + 8 * i, 4);
+      mbar_init(bar_s_free + 8 * i, 4);
+      mbar_init(bar_pv_done + 16 * i, 1);
+      mbar_init(bar_pv_done + 16 * i + 8, 1);
+      mbar_init(bar_drain + 8 * i, 1);
     }
-    for (int s = 0; s < STAGES; ++s) {
-      mbar_init(bar_kv_full + 8 * s, 1);
-      mbar_init(bar_kv_empty + 8 * s, NT);
-    }
-    mbar_init(bar_drain, 1);
-    mbar_init(bar_drain + 8, 1);
     *abort_flag = 0;
     fence_barrier_init();
     fence_proxy_async_smem();
   }
-  if (warp == 9) {
+  if (warp == ISSUER) {
     tmem_alloc(smem_u32(tmem_slot), 512);
     tmem_relinquish();
   }
@@ -312,19 +349,26 @@ __global__ void __launch_bounds__(ATC_THREADS, 1)
   griddep_launch();
   const long n_items = (long)p.plan.counters[1] * p.kv_heads;
 
-  if (warp == 8) {
+  if (warp == LOADER) {
     // ------------------------------------------------------------ TMA loader
     // The whole warp runs the loop: each lane issues the boxes of its page pieces.
+    constexpr unsigned FULL = 0xffffffffu;
     const int cr = paged ? min(ATC_BN, 1 << p.s.page_shift) : ATC_BN;
-    const int boxes = (ATC_BN / cr) * SM::NBOX * 2;  // <= 64
+    const int boxes = (ATC_BN / cr) * SM::NBOX;  // of K or of V, <= 32
+    const int box_x = lane % SM::NBOX, piece = lane / SM::NBOX;
+    const uint32_t box_at = (uint32_t)(box_x * SM::BOX_BYTES + piece * cr * SM::BOX_COLS * 2);
     const uint32_t q_bytes = (uint32_t)(TOK * p.group * HD * 2);
     bool ok = true;
-    long kvc = 0;  // KV tiles issued
-    int k = 0;     // items issued (including the final "no more items" marker)
+    long kc = 0, vc = 0;  // K / V tiles issued
+    int k = 0, sides = 0;  // items (including the final "no more items" marker), sides of it published
+    auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
+      ok = __all_sync(FULL, srv_wait(bar, parity, abort_flag, limit));
+      return ok;
+    };
     for (;; ++k) {
       int it = 0;
       if (lane == 0) it = atomicAdd(p.plan.counters, 1);
-      it = __shfl_sync(0xffffffffu, it, 0);
+      it = __shfl_sync(FULL, it, 0);
       const bool stop = it >= n_items;
       TileInfo w{};
       w.n_kv = -1;
@@ -344,223 +388,178 @@ __global__ void __launch_bounds__(ATC_THREADS, 1)
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           const int t0 = w.tok0 + t * TOK;
-          const int tiles = tile_kv_tiles(tile_kv_end(s, p.s.causal, t0, TOK));
-          w.nt[t] = t0 < s.n ? max(0, min(tiles, e.j1) - e.j0) : 0;
-          w.n_kv = max(w.n_kv, w.nt[t]);
+          const int steps = max(1, (tile_kv_end(s, p.s.causal, t0, TOK) + SM::KT - 1) / SM::KT);
+          w.ns[t] = t0 < s.n ? max(0, min(steps, e.j1 * SM::SUB) - e.j0 * SM::SUB) : 0;
+          w.n_kv = max(w.n_kv, (w.ns[t] + SM::SUB - 1) / SM::SUB);
         }
       }
       const int qb = k % QBUF;
-      ok = __all_sync(0xffffffffu, mbar_wait(bar_q_empty + 8 * qb, ((k / QBUF) & 1) ^ 1u, abort_flag, limit));
-      if (!ok) break;
-      if (lane == 0) {
-        info[qb] = w;  // published by the release of the arrive below
-        if (stop) {
-          mbar_arrive(bar_q_full + 8 * qb);
-        } else {
-          const int nq = w.tok0 + TOK < w.n && NT == 2 ? 2 : 1;
-          mbar_arrive_expect_tx(bar_q_full + 8 * qb, nq * q_bytes);
-          for (int t = 0; t < nq; ++t)
+      // Hand the item to a side: its query tile and the item's fields.
+      auto publish = [&](int t) -> bool {
+        const uint32_t full = bar_q_full + 8 * (t * SM::QS + qb);
+        if (!wait(bar_q_empty + 8 * (t * SM::QS + qb), ((k / QBUF) & 1) ^ 1u)) return false;
+        if (lane == 0) {
+          info[t * SM::QS + qb] = w;  // published by the release of the arrive below
+          const int tok0 = w.tok0 + atc_query_tile<NT>(t, k) * TOK;
+          if (stop || tok0 >= w.n) {
+            mbar_arrive(full);
+          } else {
+            mbar_arrive_expect_tx(full, q_bytes);
             for (int x = 0; x < SM::NBOX; ++x)
-              tma_load_3d(sQ + (qb * NT + t) * SM::Q_TILE + x * SM::BOX_BYTES, &tmQ, bar_q_full + 8 * qb,
-                          x * SM::BOX_COLS, w.h * p.group, w.row0 + w.tok0 + t * TOK);
-        }
-      }
-      __syncwarp();
-      if (stop) break;
-      for (int j = 0; j < w.n_kv; ++j, ++kvc) {
-        const int st = (int)(kvc % STAGES);
-        const int base = (w.j0 + j) * ATC_BN;
-        // Page numbers are fetched before the wait for the stage.
-        int page[2] = {0, 0}, c1[2] = {0, 0};
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int id = lane + 32 * i;
-          const int slot = base + (id / (2 * SM::NBOX)) * cr;
-          c1[i] = w.row0 + slot;
-          if (paged && id < boxes) {
-            page[i] = slot < w.len ? srv_page(p.s, w.b, slot) : p.s.num_pages;
-            c1[i] = slot & ((1 << p.s.page_shift) - 1);
-          }
-        }
-        ok = __all_sync(0xffffffffu, mbar_wait(bar_kv_empty + 8 * st, (uint32_t)((kvc / STAGES) & 1) ^ 1u,
-                                               abort_flag, limit));
-        if (!ok) break;
-        const uint32_t dst = sKV + st * 2 * SM::KV_TILE;
-        const uint32_t bar = bar_kv_full + 8 * st;
-        if (lane == 0) mbar_arrive_expect_tx(bar, 2 * SM::KV_TILE);
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int id = lane + 32 * i;
-          if (id < boxes) {
-            const int kv = id & 1, x = (id >> 1) % SM::NBOX, c = id / (2 * SM::NBOX);
-            tma_load_4d(dst + kv * SM::KV_TILE + x * SM::BOX_BYTES + c * cr * SM::BOX_COLS * 2, kv ? &tmV : &tmK,
-                        bar, x * SM::BOX_COLS, c1[i], w.h, page[i]);
+              tma_load_3d(sQ + (t * QBUF + qb) * SM::Q_TILE + x * SM::BOX_BYTES, &tmQ, full, x * SM::BOX_COLS,
+                          w.h * p.group, w.row0 + tok0);
           }
         }
         __syncwarp();
+        sides = t + 1;
+        return true;
+      };
+      sides = 0;
+      if (!publish(0)) break;
+      for (int j = 0; j < w.n_kv; ++j) {
+        // K tile, then (with the item's first tile in between) the other side's queries, then
+        // the V tile.  Page numbers are fetched before the wait for the stage.
+        const int slot = (w.j0 + j) * ATC_BN + piece * cr;
+        int page = 0, c1 = w.row0 + slot;
+        if (paged) {
+          page = lane < boxes && slot < w.len ? srv_page(p.s, w.b, slot) : p.s.num_pages;
+          c1 = slot & ((1 << p.s.page_shift) - 1);
+        }
+        const int ks = (int)(kc % STAGES), vs = (int)(vc % STAGES);
+        if (!wait(bar_k_empty + 8 * ks, (uint32_t)((kc / STAGES) & 1) ^ 1u)) break;
+        if (lane == 0) mbar_arrive_expect_tx(bar_k_full + 8 * ks, SM::KV_TILE);
+        __syncwarp();
+        if (lane < boxes)
+          tma_load_4d(sK + ks * SM::KV_TILE + box_at, &tmK, bar_k_full + 8 * ks, box_x * SM::BOX_COLS, c1, w.h, page);
+        __syncwarp();
+        ++kc;
+        if (NT == 2 && j == 0 && !publish(1)) break;
+        if (!wait(bar_v_empty + 8 * vs, (uint32_t)((vc / STAGES) & 1) ^ 1u)) break;
+        if (lane == 0) mbar_arrive_expect_tx(bar_v_full + 8 * vs, SM::KV_TILE);
+        __syncwarp();
+        if (lane < boxes)
+          tma_load_4d(sV + vs * SM::KV_TILE + box_at, &tmV, bar_v_full + 8 * vs, box_x * SM::BOX_COLS, c1, w.h, page);
+        __syncwarp();
+        ++vc;
       }
       if (!ok) break;
+      if (stop) {
+        if (NT == 2) publish(1);
+        break;
+      }
     }
     if (!ok && lane == 0) {
       *abort_flag = 1;
       report_status(p.s.status, SRV_DEV_TIMEOUT);
       // Let issued loads land before the CTA can exit.
-      for (long j = kvc > STAGES ? kvc - STAGES : 0; j < kvc; ++j)
-        mbar_wait(bar_kv_full + 8 * (int)(j % STAGES), (uint32_t)((j / STAGES) & 1), nullptr, limit);
-      for (int i = k > QBUF ? k - QBUF : 0; i < k; ++i)
-        mbar_wait(bar_q_full + 8 * (i % QBUF), (uint32_t)((i / QBUF) & 1), nullptr, limit);
+      for (long j = kc > STAGES ? kc - STAGES : 0; j < kc; ++j)
+        srv_wait(bar_k_full + 8 * (int)(j % STAGES), (uint32_t)((j / STAGES) & 1), nullptr, limit);
+      for (long j = vc > STAGES ? vc - STAGES : 0; j < vc; ++j)
+        srv_wait(bar_v_full + 8 * (int)(j % STAGES), (uint32_t)((j / STAGES) & 1), nullptr, limit);
+      for (int t = 0; t < NT; ++t) {
+        const int done = k + (t < sides ? 1 : 0);  // items handed to this side
+        for (int i = done > QBUF ? done - QBUF : 0; i < done; ++i)
+          srv_wait(bar_q_full + 8 * (t * SM::QS + i % QBUF), (uint32_t)((i / QBUF) & 1), nullptr, limit);
+      }
     }
-  } else if (warp == 9 || (warp == 10 && NT == 2)) {
+  } else if (warp < CLEANER && warp >= ISSUER) {
     // ------------------------------------------------------------ MMA issuers
     // One warp per query tile, as in attention_tc.cuh: the whole warp runs the loop, one
     // elected lane issues.
     constexpr unsigned FULL = 0xffffffffu;
-    const int t = warp - 9;
-    constexpr uint32_t idesc_s = idesc_f16_f32(ATC_BM, ATC_BN, 0, 0, BF16);
+    const int t = warp - ISSUER;
+    constexpr uint32_t idesc_s = idesc_f16_f32(ATC_BM, SM::KT, 0, 0, BF16);
     constexpr uint32_t idesc_o = idesc_f16_f32(ATC_BM, HD, 0, 1, BF16);
-    constexpr uint32_t v_step = HD == 32 ? (1024u >> 4) : (2048u >> 4);
-    const uint32_t s_col = t == 0 ? SM::TMEM_S0 : SM::TMEM_S1;
-    const uint32_t p_col = t == 0 ? SM::TMEM_P0 : SM::TMEM_P1;
-    const uint32_t o_col = t == 0 ? SM::TMEM_O0 : SM::TMEM_O1;
+    constexpr uint32_t v_step = HD == 32 ? (1024u >> 4) : (2048u >> 4);  // 16 keys
+    constexpr uint32_t sub_bytes = SM::KT * SM::BOX_COLS * 2;            // a step's rows of a box
+    const uint32_t s_col = SM::s_col(t), p_col = SM::p_col(t), o_col = SM::o_col(t);
     bool ok = true;
     bool issued = false;
-    long kvc = 0;         // KV tiles of all items so far
-    long kv_waited = -1;  // highest KV tile index whose arrival this warp observed
-    long pc = 0, sfc = 0, oc = 0, pvc = 0;
-    int k = 0;
+    long kvc = 0;                   // key tiles of all items so far
+    long k_seen = -1, v_seen = -1;  // highest K / V tile whose arrival this warp observed
+    long pc = 0, sfc = 0, oc = 0;   // p_full / s_free / o_free phases used
     auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
-      if (!__all_sync(FULL, mbar_wait(bar, parity, abort_flag, limit))) {
+      if (!__all_sync(FULL, srv_wait(bar, parity, abort_flag, limit))) {
         ok = false;
         return false;
       }
       tc_fence_after();
       return true;
     };
-    auto ensure_kv = [&](long idx) -> bool {
-      while (kv_waited < idx) {
-        ++kv_waited;
-        if (!wait(bar_kv_full + 8 * (int)(kv_waited % STAGES), (uint32_t)((kv_waited / STAGES) & 1))) return false;
+    auto ensure_k = [&](long idx) -> bool {
+      while (k_seen < idx) {
+        ++k_seen;
+        if (!wait(bar_k_full + 8 * (int)(k_seen % STAGES), (uint32_t)((k_seen / STAGES) & 1))) return false;
       }
       return true;
     };
-    for (; ok; ++k) {
+    auto ensure_v = [&](long idx) -> bool {
+      while (v_seen < idx) {
+        ++v_seen;
+        if (!wait(bar_v_ready + 8 * (int)(v_seen % STAGES), (uint32_t)((v_seen / STAGES) & 1))) return false;
+      }
+      return true;
+    };
+    for (int k = 0; ok; ++k) {
       const int qb = k % QBUF;
-      if (!wait(bar_q_full + 8 * qb, (k / QBUF) & 1)) break;
-      const int n_kv = __shfl_sync(FULL, info[qb].n_kv, 0);
+      if (!wait(bar_q_full + 8 * (t * SM::QS + qb), (k / QBUF) & 1)) break;
+      const TileInfo& wi = info[t * SM::QS + qb];
+      const int n_kv = __shfl_sync(FULL, wi.n_kv, 0);
       if (n_kv < 0) break;  // no more items
-      const int tq = atc_query_tile<NT>(t, k);
-      const int n = __shfl_sync(FULL, info[qb].nt[tq], 0);
-      const int len = __shfl_sync(FULL, info[qb].len, 0);
-      const int j0 = __shfl_sync(FULL, info[qb].j0, 0);
-      // Keys from here on are hidden from some row of the tile.
-      const int all_see = p.s.causal
-                              ? len - __shfl_sync(FULL, info[qb].n, 0) + __shfl_sync(FULL, info[qb].tok0, 0) + tq * TOK + 1
-                              : len;
-      bool noted = false;
-      const uint32_t qaddr = sQ + (qb * NT + tq) * SM::Q_TILE;
-      auto issue_s = [&](long kv_idx) {
-        const uint32_t kaddr = sKV + (int)(kv_idx % STAGES) * 2 * SM::KV_TILE;
+      const int n = __shfl_sync(FULL, wi.ns[atc_query_tile<NT>(t, k)], 0);
+      const uint32_t qaddr = sQ + (t * QBUF + qb) * SM::Q_TILE;
+      // S of step i; the K stage is free after its last step.
+      auto issue_s = [&](int i) {
+        const long idx = kvc + i / SM::SUB;
+        const uint32_t kaddr = sK + (int)(idx % STAGES) * SM::KV_TILE + (uint32_t)(i % SM::SUB) * sub_bytes;
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk)
           mma_f16_ss_warp(tmem + s_col, atc_desc_qk<HD>(qaddr, kk), atc_desc_qk<HD>(kaddr, kk), idesc_s,
                           kk > 0 ? 1u : 0u);
         mma_commit_warp(bar_s_full + 8 * t);
-        issued = true;
-      };
-      // While the softmax works on the scores of item key tile j: V rows behind the last
-      // key become zeros (both warps may write the same ones), and a partly hidden tile
-      // is searched for values that a product with P = 0 would not hide.
-      auto clean_v = [&](long kv_idx, int j) {
-        const int base = (j0 + j) * ATC_BN;
-        if (base + ATC_BN <= all_see) return;  // warp-uniform
-        const int keep = max(0, min(ATC_BN, len - base));
-        constexpr int ROW_BYTES = SM::BOX_COLS * 2;
-        constexpr int CH = ROW_BYTES / 16;
-        const uint32_t vaddr = sKV + (int)(kv_idx % STAGES) * 2 * SM::KV_TILE + SM::KV_TILE;
-        bool odd = false;
-#pragma unroll 1
-        for (int x = 0; x < SM::NBOX; ++x) {
-          const uint32_t vx = vaddr + (uint32_t)(x * SM::BOX_BYTES);
-#pragma unroll 4
-          for (int i = lane; i < (p.s.causal ? keep * CH : 0); i += 32) {
-            uint32_t w[4];
-            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                         : "r"(vx + (uint32_t)(i * 16))
-                         : "memory");
-            odd |= srv_nonfinite<BF16>(w[0]) | srv_nonfinite<BF16>(w[1]) | srv_nonfinite<BF16>(w[2]) |
-                   srv_nonfinite<BF16>(w[3]);
-          }
-          for (int i = keep * CH + lane; i < ATC_BN * CH; i += 32)
-            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(vx + (uint32_t)(i * 16)), "r"(0u)
-                         : "memory");
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (__any_sync(FULL, odd) && !noted) {
-          noted = true;
-          if (lane == 0) {
-            const int at = atomicAdd(p.plan.counters + 3, 1);
-            if (at < 2 * p.plan.most_entries * p.kv_heads) {
-              p.plan.redo[3 * at] = info[qb].b;
-              p.plan.redo[3 * at + 1] = info[qb].q;
-              p.plan.redo[3 * at + 2] = info[qb].h;
-            }
-          }
-          __syncwarp();
-        }
-      };
-      auto issue_pv = [&](long kv_idx, bool accumulate) {
-        const uint32_t vaddr = sKV + (int)(kv_idx % STAGES) * 2 * SM::KV_TILE + SM::KV_TILE;
-        const uint64_t vd = atc_desc_v<HD>(vaddr);
-#pragma unroll
-        for (int kk = 0; kk < ATC_BN / 16; ++kk)
-          mma_f16_ts_warp(tmem + o_col, tmem + p_col + (uint32_t)(kk * 8), vd + (uint64_t)(kk * v_step), idesc_o,
-                          (accumulate || kk > 0) ? 1u : 0u);
-        mma_commit_warp(bar_pv_done + 8 * t);
+        if (i % SM::SUB == SM::SUB - 1 || i + 1 == n) mma_commit_warp(bar_k_empty + 8 * (int)(idx % STAGES));
         issued = true;
       };
       if (n > 0) {
-        if (!ensure_kv(kvc)) break;
-        issue_s(kvc);
-        clean_v(kvc, 0);
+        if (!ensure_k(kvc)) break;
+        issue_s(0);
       }
-      for (int j = 0; j < n_kv && ok; ++j) {
-        const long kv_j = kvc + j;
-        if (j < n) {
-          if (!SM::P_ALIAS && j + 1 < n) {
-            if (!wait(bar_s_free + 8 * t, (uint32_t)(sfc++ & 1))) break;
-            if (!ensure_kv(kv_j + 1)) break;
-            issue_s(kv_j + 1);
-            clean_v(kv_j + 1, j + 1);
-          }
-          if (!wait(bar_p_full + 8 * t, (uint32_t)(pc++ & 1))) break;
-          // The first P V of an item overwrites O: the previous item's O must be read.
-          if (j == 0 && !wait(bar_o_free + 8 * t, (uint32_t)(oc++ & 1) ^ 1u)) break;
-          issue_pv(kv_j, j > 0);
-          if (j + 1 == n) mma_commit_warp(bar_o_full + 8 * t);
-          mma_commit_warp(bar_kv_empty + 8 * (int)(kv_j % STAGES));
-          if (SM::P_ALIAS) {
-            // The next S of this tile overwrites P(j): P V(j) must have completed.
-            if (!wait(bar_pv_done + 8 * t, (uint32_t)(pvc & 1))) break;
-            if (j + 1 < n) {
-              if (!ensure_kv(kv_j + 1)) break;
-              issue_s(kv_j + 1);
-              clean_v(kv_j + 1, j + 1);
-            }
-          }
-          ++pvc;
-        } else {
-          // Not used by this query tile: release it once it has landed.
-          if (!ensure_kv(kv_j)) break;
-          if (lane == 0) mbar_arrive(bar_kv_empty + 8 * (int)(kv_j % STAGES));
-          __syncwarp();
+      for (int i = 0; i < n && ok; ++i, ++pc) {
+        // Next scores as soon as the softmax threads have read these (s_free).
+        if (i + 1 < n) {
+          if (!wait(bar_s_free + 8 * t, (uint32_t)(sfc++ & 1))) break;
+          if (!ensure_k(kvc + (i + 1) / SM::SUB)) break;
+          issue_s(i + 1);
         }
+        if (!wait(bar_p_full + 8 * t, (uint32_t)(pc & 1))) break;
+        const long idx = kvc + i / SM::SUB;
+        if (!ensure_v(idx)) break;
+        // The first P V of an item overwrites O: the previous item's O must be read.
+        if (i == 0 && !wait(bar_o_free + 8 * t, (uint32_t)(oc++ & 1) ^ 1u)) break;
+        const uint32_t pb = (uint32_t)(pc % SM::PBUF);
+        const uint64_t vd =
+            atc_desc_v<HD>(sV + (int)(idx % STAGES) * SM::KV_TILE + (uint32_t)(i % SM::SUB) * sub_bytes);
+#pragma unroll
+        for (int kk = 0; kk < SM::KT / 16; ++kk)
+          mma_f16_ts_warp(tmem + o_col, tmem + p_col + pb * (SM::KT / 2) + (uint32_t)(kk * 8),
+                          vd + (uint64_t)(kk * v_step), idesc_o, (i > 0 || kk > 0) ? 1u : 0u);
+        mma_commit_warp(bar_pv_done + 16 * t + 8 * pb);
+        issued = true;
+        if (i + 1 == n) mma_commit_warp(bar_o_full + 8 * t);
+        if (i % SM::SUB == SM::SUB - 1 || i + 1 == n) mma_commit_warp(bar_v_empty + 8 * (int)(idx % STAGES));
+      }
+      // Key tiles that only the other side uses: released once they have landed.
+      for (int j = (n + SM::SUB - 1) / SM::SUB; j < n_kv && ok; ++j) {
+        if (!ensure_k(kvc + j) || !ensure_v(kvc + j)) break;
+        if (lane == 0) {
+          mbar_arrive(bar_k_empty + 8 * (int)((kvc + j) % STAGES));
+          mbar_arrive(bar_v_empty + 8 * (int)((kvc + j) % STAGES));
+        }
+        __syncwarp();
       }
       if (!ok) break;
       kvc += n_kv;
-      mma_commit_warp(bar_q_empty + 8 * qb);
+      mma_commit_warp(bar_q_empty + 8 * (t * SM::QS + qb));
     }
     if (!ok) {
       if (lane == 0) {
@@ -569,41 +568,119 @@ __global__ void __launch_bounds__(ATC_THREADS, 1)
       }
       if (issued) {
         mma_commit_warp(bar_drain + 8 * t);
-        mbar_wait(bar_drain + 8 * t, 0, nullptr, limit);
+        srv_wait(bar_drain + 8 * t, 0, nullptr, limit);
       }
     }
+  } else if (warp == CLEANER) {
+    // ------------------------------------------------------------ cleaner
+    // Sees every V tile before the products do: rows behind the last key become zeros, and
+    // a tile that some row of the item sees only in part is searched for values that a
+    // product with P = 0 would not hide.
+    constexpr unsigned FULL = 0xffffffffu;
+    bool ok = true;
+    long vc = 0;
+    for (int k = 0; ok; ++k) {
+      const int qb = k % QBUF;
+      ok = __all_sync(FULL, srv_wait(bar_q_full + 8 * qb, (uint32_t)((k / QBUF) & 1), abort_flag, limit));
+      if (!ok) break;
+      const TileInfo wi = info[qb];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_q_empty + 8 * qb);
+      if (wi.n_kv < 0) break;  // no more items
+      const int all_see = p.s.causal ? wi.len - wi.n + wi.tok0 + 1 : wi.len;
+      bool noted = false;
+      for (int j = 0; j < wi.n_kv; ++j, ++vc) {
+        const int vs = (int)(vc % STAGES);
+        ok = __all_sync(FULL, srv_wait(bar_v_full + 8 * vs, (uint32_t)((vc / STAGES) & 1), abort_flag, limit));
+        if (!ok) break;
+        const int base = (wi.j0 + j) * ATC_BN;
+        if (base + ATC_BN > all_see) {
+          const int keep = max(0, min(ATC_BN, wi.len - base));
+          constexpr int ROW_BYTES = SM::BOX_COLS * 2;
+          constexpr int CH = ROW_BYTES / 16;
+          bool odd = false;
+#pragma unroll 1
+          for (int x = 0; x < SM::NBOX; ++x) {
+            const uint32_t vx = sV + vs * SM::KV_TILE + (uint32_t)(x * SM::BOX_BYTES);
+#pragma unroll 4
+            for (int i = lane; i < (p.s.causal ? keep * CH : 0); i += 32) {
+              uint32_t w[4];
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                           : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                           : "r"(vx + (uint32_t)(i * 16))
+                           : "memory");
+              odd |= srv_nonfinite<BF16>(w[0]) | srv_nonfinite<BF16>(w[1]) | srv_nonfinite<BF16>(w[2]) |
+                     srv_nonfinite<BF16>(w[3]);
+            }
+            for (int i = keep * CH + lane; i < ATC_BN * CH; i += 32)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(vx + (uint32_t)(i * 16)), "r"(0u)
+                           : "memory");
+          }
+          fence_proxy_async_smem();
+          if (__any_sync(FULL, odd) && !noted) {
+            noted = true;
+            if (lane == 0) {
+              const int at = atomicAdd(p.plan.counters + 3, 1);
+              if (at < 2 * p.plan.most_entries * p.kv_heads) {
+                p.plan.redo[3 * at] = wi.b;
+                p.plan.redo[3 * at + 1] = wi.q;
+                p.plan.redo[3 * at + 2] = wi.h;
+              }
+            }
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_v_ready + 8 * vs);
+      }
+    }
+    if (!ok && lane == 0) {
+      *abort_flag = 1;
+      report_status(p.s.status, SRV_DEV_TIMEOUT);
+    }
   } else if (warp < 4 * NT) {
-    // ------------------------------------------------------------ softmax, warps 0-7
+    // ------------------------------------------------------------ softmax
+    constexpr int KT = SM::KT;
     const int t = warp >> 2;
     const int quad = warp & 3;
     const int row = quad * 32 + lane;  // row inside the query tile
     const int rtok = row / p.group;    // its token inside the tile, its head in the group
     const int rhead = row - rtok * p.group;
     const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
-    const uint32_t s_addr = tmem + lane_base + (t == 0 ? SM::TMEM_S0 : SM::TMEM_S1);
-    const uint32_t p_addr = tmem + lane_base + (t == 0 ? SM::TMEM_P0 : SM::TMEM_P1);
-    const uint32_t o_addr = tmem + lane_base + (t == 0 ? SM::TMEM_O0 : SM::TMEM_O1);
+    const uint32_t s_addr = tmem + lane_base + SM::s_col(t);
+    const uint32_t p_addr0 = tmem + lane_base + SM::p_col(t);
+    const uint32_t o_addr = tmem + lane_base + SM::o_col(t);
     const float scale = p.scale_log2;
-    long sc = 0, ofc = 0;
-    long pv_before = 0;
+    long c = 0;    // steps of all items so far (phase of s_full, P buffer)
+    long ofc = 0;  // items with steps so far
     bool ok = true;
-    int k = 0;
-    for (; ok; ++k) {
+    // One arrival per warp, after every lane's reads and TMEM accesses.
+    auto arrive = [&](uint32_t bar) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+    };
+    // P V of step i of this side complete: phase i / PBUF of its buffer's barrier.
+    auto pv_done = [&](long i) -> bool {
+      const bool fine = srv_wait(bar_pv_done + 16 * t + 8 * (uint32_t)(i % SM::PBUF),
+                                 (uint32_t)((i / SM::PBUF) & 1), abort_flag, limit);
+      tc_fence_after();
+      return fine;
+    };
+    for (int k = 0; ok; ++k) {
       const int qb = k % QBUF;
-      if (!mbar_wait(bar_q_full + 8 * qb, (uint32_t)((k / QBUF) & 1), abort_flag, limit)) {
+      if (!srv_wait(bar_q_full + 8 * (t * SM::QS + qb), (uint32_t)((k / QBUF) & 1), abort_flag, limit)) {
         ok = false;
         break;
       }
-      const TileInfo& wi = info[qb];
+      const TileInfo& wi = info[t * SM::QS + qb];
       if (wi.n_kv < 0) break;  // no more items
       const int tq = atc_query_tile<NT>(t, k);
-      const int n = tq == 0 ? wi.nt[0] : wi.nt[1];
-      const int j0 = wi.j0, len = wi.len, part = wi.part, h = wi.h;
+      const int n = tq == 0 ? wi.ns[0] : wi.ns[1];
+      const int key0 = wi.j0 * ATC_BN, len = wi.len, part = wi.part, h = wi.h;
       const int tok0 = wi.tok0 + tq * TOK;  // first token of the tile
       const int tokens = wi.n;
       const int token = wi.row0 + tok0 + rtok;   // packed row of this thread's token
       const int first = p.s.causal ? len - tokens + tok0 : len - 1;  // last key of the tile's first row
-      mbar_arrive(bar_q_empty + 8 * qb);  // this thread no longer needs the info slot
+      arrive(bar_q_empty + 8 * (t * SM::QS + qb));  // the info slot is read
       const bool live = rtok < TOK && tok0 + rtok < tokens;
       const long prow = part < 0 ? 0 : (long)part * (NT * ATC_BM) + tq * ATC_BM + row;
       if (n == 0) {
@@ -614,46 +691,47 @@ __global__ void __launch_bounds__(ATC_THREADS, 1)
       const int row_lim = p.s.causal ? min(len - 1, first + rtok) : len - 1;
       float m_run = -INFINITY;  // running max (log2 domain) used as the exp base
       float l_run = 0.f;
-      for (int j = 0; j < n; ++j) {
-        if (!mbar_wait(bar_s_full + 8 * t, (uint32_t)(sc++ & 1), abort_flag, limit)) {
+      for (int i = 0; i < n; ++i, ++c) {
+        if (!srv_wait(bar_s_full + 8 * t, (uint32_t)(c & 1), abort_flag, limit)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        uint32_t sv[ATC_BN];  // raw fp32 scores of this thread's row
+        uint32_t sv[KT];  // raw fp32 scores of this thread's row
 #pragma unroll
-        for (int c = 0; c < ATC_BN / 32; ++c) {
+        for (int q = 0; q < KT / 32; ++q) {
           uint32_t chunk[32];
-          tmem_ld_32x32b_x32(s_addr + (uint32_t)(c * 32), chunk);
+          tmem_ld_32x32b_x32(s_addr + (uint32_t)(q * 32), chunk);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) sv[c * 32 + e] = chunk[e];
+          for (int e = 0; e < 32; ++e) sv[q * 32 + e] = chunk[e];
         }
         tmem_wait_ld();
-        if (!SM::P_ALIAS && j + 1 < n) {
+        // The scores are in registers: the buffer may take the next step's.
+        if (i + 1 < n) {
           tc_fence_before();
-          mbar_arrive(bar_s_free + 8 * t);
+          arrive(bar_s_free + 8 * t);
         }
-        const int k0 = (j0 + j) * ATC_BN;
-        if (k0 + ATC_BN - 1 > first) {
-          // Column c of this tile is hidden when c > lim.
+        const int k0 = key0 + i * KT;
+        if (k0 + KT - 1 > first) {
+          // Column e of this step is hidden when e > lim.
           const int lim = row_lim - k0;
 #pragma unroll
-          for (int c = 0; c < ATC_BN; ++c)
-            if (c > lim) sv[c] = __float_as_uint(-INFINITY);
+          for (int e = 0; e < KT; ++e)
+            if (e > lim) sv[e] = __float_as_uint(-INFINITY);
         }
-        // Row max: 8 independent chains of three-input maxima.
+        // Row max: independent chains of three-input maxima.
         float pm[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) pm[i] = __uint_as_float(sv[i]);
+        for (int e = 0; e < 8; ++e) pm[e] = __uint_as_float(sv[e]);
 #pragma unroll
-        for (int c = 8; c < ATC_BN; c += 2)
-          pm[(c >> 1) & 7] = srv_max3(pm[(c >> 1) & 7], __uint_as_float(sv[c]), __uint_as_float(sv[c + 1]));
+        for (int e = 8; e < KT; e += 2)
+          pm[(e >> 1) & 7] = srv_max3(pm[(e >> 1) & 7], __uint_as_float(sv[e]), __uint_as_float(sv[e + 1]));
         const float mx =
             srv_max3(srv_max3(pm[0], pm[1], pm[2]), srv_max3(pm[3], pm[4], pm[5]), srv_max3(pm[6], pm[7], pm[7]));
         const float m_tile = mx * scale;
         float alpha = 1.f;
         bool rescale = false;
-        if (j == 0) {
+        if (i == 0) {
           m_run = m_tile;
         } else {
           // Lazy rescale: keep the old base unless the max grew by more than 2^8.  Rows
@@ -670,68 +748,73 @@ __global__ void __launch_bounds__(ATC_THREADS, 1)
         const float base = !(m_tile < INFINITY) ? NAN : m_run == -INFINITY ? 0.f : m_run;
         const float2 sc2 = make_float2(scale, scale), nb2 = make_float2(-base, -base);
         unsigned long long ps2[2] = {0ull, 0ull};  // partial row sums, f32x2 pairs
-        uint32_t pk[4][16];
+        uint32_t pk[KT / 32][16];
+        // 32 keys' probabilities; one pair in four takes its exponentials from the FMA pipe
+        // (the MUFU is the tighter one).
         auto exp_chunk = [&](int q) {
 #pragma unroll
           for (int cc = 0; cc < 16; ++cc) {
-            const int c = q * 16 + cc;
+            const int e = q * 16 + cc;
             const float2 x =
-                ffma2(make_float2(__uint_as_float(sv[2 * c]), __uint_as_float(sv[2 * c + 1])), sc2, nb2);
+                ffma2(make_float2(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1])), sc2, nb2);
             float p0, p1;
-            if ((c & 3) == 3) {
-              const float2 e = exp2_fma2(x);
-              p0 = e.x;
-              p1 = e.y;
+            if ((e & 3) == 3) {
+              const float2 y = exp2_fma2(x);
+              p0 = y.x;
+              p1 = y.y;
             } else {
               p0 = ex2_approx(x.x);
               p1 = ex2_approx(x.y);
             }
-            ps2[c & 1] = add2p(ps2[c & 1], pk2(p0, p1));
+            ps2[e & 1] = add2p(ps2[e & 1], pk2(p0, p1));
             pk[q][cc] = srv_pack<BF16>(p0, p1);
           }
         };
+        // The P buffer is free once the P V that used it last is complete; with one buffer
+        // that is the previous step's, so half of the exponentials come before the wait.
+        constexpr int EARLY = SM::PBUF == 1 ? ATC_P_EARLY : 0;
 #pragma unroll
-        for (int q = 0; q < ATC_P_EARLY; ++q) exp_chunk(q);
-        // P(j) replaces P(j-1), and O is rescaled below: P V(j-1) must be complete (see
-        // attention_tc.cuh).
-        if (!SM::P_ALIAS && j > 0) {
-          if (!mbar_wait(bar_pv_done + 8 * t, (uint32_t)((pv_before + j - 1) & 1), abort_flag, limit)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
+        for (int q = 0; q < EARLY; ++q) exp_chunk(q);
+        if (c >= SM::PBUF && !pv_done(c - SM::PBUF)) {
+          ok = false;
+          break;
         }
+        const uint32_t p_addr = p_addr0 + (uint32_t)(c % SM::PBUF) * (KT / 2);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          if (q >= ATC_P_EARLY) exp_chunk(q);
+        for (int q = 0; q < KT / 32; ++q) {
+          if (q >= EARLY) exp_chunk(q);
           tmem_st_32x32b_x16(p_addr + (uint32_t)(q * 16), pk[q]);
         }
         const float2 rs2 = upk2(add2p(ps2[0], ps2[1]));
         l_run = l_run * alpha + (rs2.x + rs2.y);
         if (rescale) {
+          // O holds P V of this item's steps before this one.
+          if (SM::PBUF > 1 && !pv_done(c - 1)) {
+            ok = false;
+            break;
+          }
 #pragma unroll
-          for (int c = 0; c < HD / 32; ++c) {
+          for (int q = 0; q < HD / 32; ++q) {
             uint32_t o[32];
-            tmem_ld_32x32b_x32(o_addr + (uint32_t)(c * 32), o);
+            tmem_ld_32x32b_x32(o_addr + (uint32_t)(q * 32), o);
             tmem_wait_ld();
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-            tmem_st_32x32b_x32(o_addr + (uint32_t)(c * 32), o);
+            tmem_st_32x32b_x32(o_addr + (uint32_t)(q * 32), o);
           }
         }
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(bar_p_full + 8 * t);
+        arrive(bar_p_full + 8 * t);
       }
-      pv_before += n;
       if (!ok) break;
-      // A row that saw no key: exp2_fma2 leaves 2^-126 where the exponential of -inf is 0.
-      if (m_run == -INFINITY && l_run == l_run) l_run = 0.f;
-      if (!mbar_wait(bar_o_full + 8 * t, (uint32_t)(ofc++ & 1), abort_flag, limit)) {
+      if (!srv_wait(bar_o_full + 8 * t, (uint32_t)(ofc++ & 1), abort_flag, limit)) {
         ok = false;
         break;
       }
       tc_fence_after();
+      // A row that saw no key: exp2_fma2 leaves 2^-126 where the exponential of -inf is 0.
+      if (m_run == -INFINITY && l_run == l_run) l_run = 0.f;
       if (part >= 0) {
         // A piece: raw sums, joined later.
         float* dst = p.part_o + prow * HD;
@@ -815,9 +898,8 @@ __global__ void __launch_bounds__(ATC_THREADS, 1)
           }
         }
       }
-      __syncwarp();
       tc_fence_before();
-      mbar_arrive(bar_o_free + 8 * t);
+      arrive(bar_o_free + 8 * t);
     }
     if (!ok) {
       *abort_flag = 1;
@@ -827,7 +909,7 @@ __global__ void __launch_bounds__(ATC_THREADS, 1)
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == ISSUER) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
