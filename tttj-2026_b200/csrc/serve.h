@@ -97,8 +97,9 @@ struct TileEntry {    // one item of every key/value head
   int b, q;           // sequence, item of the sequence
   int j0, j1;         // key tiles [j0, j1)
   int part;           // first of kv_heads partial-result slots, or -1: whole items
-  int pad[3];
+  int row0, n, len;   // of the sequence (SrvSeq)
 };
+static_assert(sizeof(TileEntry) == 32, "entries are read as two 16-byte words");
 struct TileJoin {     // an entry whose keys were split
   int b, q, pieces, part;  // piece i of head h is slot part + i * kv_heads + h
 };

@@ -15,7 +15,7 @@ cudaError_t launch(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUten
   if (e != cudaSuccess) return e;
   e = launch_pdl(tile_plan_kernel, dim3(1), dim3(TILE_PLAN_THREADS), 0, stream, p, tile_nt(HD), grid);
   if (e != cudaSuccess) return e;
-  e = launch_pdl(kern, dim3(grid), dim3(tile_threads(tile_nt(HD))), smem, stream, tm_q, tm_k, tm_v, p);
+  e = launch_pdl(kern, dim3(grid), dim3(TileSmem<HD>::THREADS), smem, stream, tm_q, tm_k, tm_v, p);
   if (e != cudaSuccess) return e;
   return launch_pdl(tile_join_kernel<HD, BF16>, dim3(4 * grid), dim3(32 * TILE_JOIN_WARPS), 0, stream, p);
 }

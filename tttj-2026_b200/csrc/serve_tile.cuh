@@ -40,27 +40,31 @@ struct TileInfo {  // one decoded item, in shared memory
 };
 static_assert(sizeof(TileInfo) <= 64, "item info slot is 64 bytes");
 
-// Warps: four softmax warps per query tile (their number modulo four is their TMEM quadrant),
-// the loader, one MMA issuer per query tile, the cleaner.
-constexpr int tile_threads(int nt) { return 32 * (4 * nt + 1 + nt + 1); }
-
-// Keys per step of the softmax.  TMEM (512 columns) holds, per query tile, the scores (fp32, one
-// column per key), the probabilities (16 bits, half a column per key, PBUF buffers) and O
-// (head_dim columns).  With head_dim 128 the two O take 256 columns, so a step is 64 keys
-// there; then nothing shares columns and S of the next step is computed while the softmax
-// works on this one.  (128 keys with P written over S, as in attention_tc.cuh, make the
-// next S wait for P V: 4500 - 4900 cycles per 128 keys of both tiles, measured on prompts of 4096.)
+// TMEM (512 columns) holds, per query tile, the scores of a step (fp32, a column per key), the
+// probabilities (16 bits, half a column per key) and O (head_dim columns).  At head_dim 128 the
+// two O take 256 columns, so a step is 64 keys there, with two buffers of probabilities; then
+// nothing shares columns, S of the next step is computed while the softmax works on this one,
+// and no product is waited for.  Measured there, prompts of 3001 and 4096 tokens, 32 / 8 heads:
+// steps of 128 keys with P written over S, as in attention_tc.cuh, 286 us (the next S waits for
+// P V); one score buffer of 128 keys that the tiles take in turn, 250 - 258 us; this with
+// one issuing warp per tile 257 us, with one for S and one for P V, SPLIT_US us.
 template <int HD>
 struct TileSmem : AtcSmem<HD> {  // tile sizes and stages as there
   using B = AtcSmem<HD>;
-  static constexpr int KT = HD == 128 ? 64 : 128;
-  static constexpr int SUB = ATC_BN / KT;  // steps per loaded key tile
+  static constexpr bool SPLIT = HD == 128;        // S and P V issued by different warps
+  static constexpr int KT = HD == 128 ? 64 : 128;  // keys per step
+  static constexpr int SUB = ATC_BN / KT;          // steps per loaded key tile
   static constexpr int PBUF = HD == 128 ? 2 : 1;
+  // Warps: four softmax warps per query tile (their number modulo four is their TMEM
+  // quadrant), the loader, the MMA issuers, the cleaner.
+  static constexpr int LOADER = 4 * B::NT, ISSUER = LOADER + 1;
+  static constexpr int CLEANER = ISSUER + (SPLIT ? 2 : 1) * B::NT;
+  static constexpr int THREADS = 32 * (CLEANER + 1);
   __host__ __device__ static constexpr uint32_t s_col(int t) { return (uint32_t)(t * KT); }
   __host__ __device__ static constexpr uint32_t p_col(int t) { return (uint32_t)(B::NT * KT + t * PBUF * KT / 2); }
   __host__ __device__ static constexpr uint32_t o_col(int t) { return t == 0 ? B::TMEM_O0 : B::TMEM_O1; }
   static_assert(B::NT * (KT + PBUF * KT / 2) <= (int)B::TMEM_O0, "TMEM columns overlap");
-  static constexpr int BARS = 4 * B::QS + 5 * B::STAGES + 10 + 4 + 2;
+  static constexpr int BARS = 4 * B::QS + 5 * B::STAGES + 8 + 4 + 4 + 4;
   static constexpr int BAR_AT = B::Q_BYTES + B::KV_BYTES;
   static constexpr int SLOT_AT = BAR_AT + BARS * 8;  // TMEM base, abort flag
   static constexpr int INFO_AT = SLOT_AT + 16;       // [side][QS] items
@@ -84,7 +88,7 @@ constexpr int TILE_BUCKETS = 1024;
 
 __global__ void __launch_bounds__(TILE_PLAN_THREADS) tile_plan_kernel(const TileParams p, int nt, int grid) {
   __shared__ int s_pre[SRV_MAX_BATCH + 1];  // items before each sequence
-  __shared__ int s_n[SRV_MAX_BATCH], s_len[SRV_MAX_BATCH];
+  __shared__ int s_row0[SRV_MAX_BATCH], s_n[SRV_MAX_BATCH], s_len[SRV_MAX_BATCH];
   __shared__ int s_hist[TILE_BUCKETS];
   __shared__ int s_warp[32];
   __shared__ unsigned long long s_sum[2][32];  // key tiles of all items / of those in the last wave
@@ -102,6 +106,7 @@ __global__ void __launch_bounds__(TILE_PLAN_THREADS) tile_plan_kernel(const Tile
     const int b = 2 * tid + i;
     if (b < batch) {
       const SrvSeq q = srv_seq(p.s, b);
+      s_row0[b] = q.row0;
       s_n[b] = q.n;
       s_len[b] = q.len;
       cnt[i] = (q.n + item_tokens - 1) / item_tokens;
@@ -241,6 +246,9 @@ __global__ void __launch_bounds__(TILE_PLAN_THREADS) tile_plan_kernel(const Tile
   for (int e = tid; e < items; e += TILE_PLAN_THREADS) {
     TileEntry out{};
     out.q = locate(e, &out.b);
+    out.row0 = s_row0[out.b];
+    out.n = s_n[out.b];
+    out.len = s_len[out.b];
     const int t = tiles_of(out.b, out.q), n = pieces_of(e, t);
     int part = -1;
     if (n > 1) {
@@ -266,14 +274,14 @@ __global__ void __launch_bounds__(TILE_PLAN_THREADS) tile_plan_kernel(const Tile
 
 // -------------------------------------------------------------------------- attention
 template <int HD, bool BF16>
-__global__ void __launch_bounds__(tile_threads(tile_nt(HD)), 1)
+__global__ void __launch_bounds__(TileSmem<HD>::THREADS, 1)
     tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                 const __grid_constant__ CUtensorMap tmV, const TileParams p) {
   using SM = TileSmem<HD>;
   constexpr int STAGES = SM::STAGES;
   constexpr int NT = SM::NT;
   constexpr int QBUF = SM::QBUF;
-  constexpr int LOADER = 4 * NT, ISSUER = LOADER + 1, CLEANER = ISSUER + NT;
+  constexpr int LOADER = SM::LOADER, ISSUER = SM::ISSUER, CLEANER = SM::CLEANER;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t pad = (1024u - (raw & 1023u)) & 1023u;
@@ -289,12 +297,12 @@ __global__ void __launch_bounds__(tile_threads(tile_nt(HD)), 1)
   const uint32_t bar_v_ready = bar_v_full + 8 * STAGES;     // [STAGES] landed and cleaned
   const uint32_t bar_v_empty = bar_v_ready + 8 * STAGES;    // [STAGES]
   const uint32_t bar_s_full = bar_v_empty + 8 * STAGES;     // [side] ...
-  const uint32_t bar_p_full = bar_s_full + 16;
-  const uint32_t bar_o_full = bar_p_full + 16;
+  const uint32_t bar_p_full = bar_s_full + 16;              // [side][2] P buffer 0 / 1 written
+  const uint32_t bar_o_full = bar_p_full + 32;
   const uint32_t bar_o_free = bar_o_full + 16;
   const uint32_t bar_s_free = bar_o_free + 16;              // scores read by softmax
   const uint32_t bar_pv_done = bar_s_free + 16;             // [side][2] P V of P buffer 0 / 1 complete
-  const uint32_t bar_drain = bar_pv_done + 32;
+  const uint32_t bar_drain = bar_pv_done + 32;              // [issuer]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + SM::SLOT_AT);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   TileInfo* info = reinterpret_cast<TileInfo*>(smem + SM::INFO_AT);  // [side][QS]
@@ -312,8 +320,8 @@ __global__ void __launch_bounds__(tile_threads(tile_nt(HD)), 1)
     tma_prefetch_desc(&tmV);
     for (int i = 0; i < 2 * SM::QS; ++i) {
       mbar_init(bar_q_full + 8 * i, 1);
-      // The side's issuer and softmax warps, and for side 0 the cleaner.
-      mbar_init(bar_q_empty + 8 * i, i < SM::QS ? 6 : 5);
+      // The issuers, the softmax warps, and for side 0 the cleaner.
+      mbar_init(bar_q_empty + 8 * i, (SM::SPLIT ? 2 : 1) + 4 + (i < SM::QS ? 1 : 0));
     }
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(bar_k_full + 8 * i, 1);
@@ -324,14 +332,15 @@ __global__ void __launch_bounds__(tile_threads(tile_nt(HD)), 1)
     }
     for (int i = 0; i < 2; ++i) {  // softmax side: one arrival per warp
       mbar_init(bar_s_full + 8 * i, 1);
-      mbar_init(bar_p_full + 8 * i, 4);
+      mbar_init(bar_p_full + 16 * i, 4);
+      mbar_init(bar_p_full + 16 * i + 8, 4);
       mbar_init(bar_o_full + 8 * i, 1);
       mbar_init(bar_o_free + 8 * i, 4);
       mbar_init(bar_s_free + 8 * i, 4);
       mbar_init(bar_pv_done + 16 * i, 1);
       mbar_init(bar_pv_done + 16 * i + 8, 1);
-      mbar_init(bar_drain + 8 * i, 1);
     }
+    for (int i = 0; i < 4; ++i) mbar_init(bar_drain + 8 * i, 1);
     *abort_flag = 0;
     fence_barrier_init();
     fence_proxy_async_smem();
@@ -361,37 +370,63 @@ __global__ void __launch_bounds__(tile_threads(tile_nt(HD)), 1)
     bool ok = true;
     long kc = 0, vc = 0;  // K / V tiles issued
     int k = 0, sides = 0;  // items (including the final "no more items" marker), sides of it published
+    bool v_due = false;    // the V tile of the K tile loaded last
+    int v_c1 = 0, v_h = 0, v_page = 0;
     auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
       ok = __all_sync(FULL, srv_wait(bar, parity, abort_flag, limit));
       return ok;
     };
+    auto load_v = [&]() -> bool {
+      if (!v_due) return true;
+      v_due = false;
+      const int vs = (int)(vc % STAGES);
+      if (!wait(bar_v_empty + 8 * vs, (uint32_t)((vc / STAGES) & 1) ^ 1u)) return false;
+      if (lane == 0) mbar_arrive_expect_tx(bar_v_full + 8 * vs, SM::KV_TILE);
+      __syncwarp();
+      if (lane < boxes)
+        tma_load_4d(sV + vs * SM::KV_TILE + box_at, &tmV, bar_v_full + 8 * vs, box_x * SM::BOX_COLS, v_c1, v_h, v_page);
+      __syncwarp();
+      ++vc;
+      return true;
+    };
+    // The next item's number is taken while this one is loaded, its entry right after.
+    auto take = [&] { return lane == 0 ? atomicAdd(p.plan.counters, 1) : 0; };
+    auto fetch = [&](int it, int4* lo, int4* hi) {
+      if (it < n_items) {
+        const int4* e = reinterpret_cast<const int4*>(p.plan.entries + it / p.kv_heads);
+        *lo = e[0];
+        *hi = e[1];
+      }
+    };
+    int taken = take();
+    int it = __shfl_sync(FULL, taken, 0);
+    int4 lo{}, hi{};
+    fetch(it, &lo, &hi);
     for (;; ++k) {
-      int it = 0;
-      if (lane == 0) it = atomicAdd(p.plan.counters, 1);
-      it = __shfl_sync(FULL, it, 0);
       const bool stop = it >= n_items;
       TileInfo w{};
       w.n_kv = -1;
       if (!stop) {
-        const TileEntry e = p.plan.entries[it / p.kv_heads];
-        const SrvSeq s = srv_seq(p.s, e.b);
-        w.b = e.b;
-        w.q = e.q;
+        w.b = lo.x;
+        w.q = lo.y;
+        w.j0 = lo.z;
+        const int j1 = lo.w;
         w.h = it % p.kv_heads;
-        w.row0 = s.row0;
-        w.n = s.n;
-        w.len = s.len;
-        w.tok0 = e.q * NT * TOK;
-        w.j0 = e.j0;
-        w.part = e.part < 0 ? -1 : e.part + w.h;
+        w.part = hi.x < 0 ? -1 : hi.x + w.h;
+        w.row0 = hi.y;
+        w.n = hi.z;
+        w.len = hi.w;
+        w.tok0 = w.q * NT * TOK;
         w.n_kv = 0;
+        const SrvSeq s{w.row0, w.n, w.len};
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           const int t0 = w.tok0 + t * TOK;
           const int steps = max(1, (tile_kv_end(s, p.s.causal, t0, TOK) + SM::KT - 1) / SM::KT);
-          w.ns[t] = t0 < s.n ? max(0, min(steps, e.j1 * SM::SUB) - e.j0 * SM::SUB) : 0;
+          w.ns[t] = t0 < w.n ? max(0, min(steps, j1 * SM::SUB) - w.j0 * SM::SUB) : 0;
           w.n_kv = max(w.n_kv, (w.ns[t] + SM::SUB - 1) / SM::SUB);
         }
+        taken = take();
       }
       const int qb = k % QBUF;
       // Hand the item to a side: its query tile and the item's fields.
@@ -415,17 +450,17 @@ __global__ void __launch_bounds__(tile_threads(tile_nt(HD)), 1)
         return true;
       };
       sides = 0;
+      // K runs one tile ahead of V: a K stage is free as soon as its scores are computed, and
+      // waiting behind a V stage would make the next scores late.
       if (!publish(0)) break;
       for (int j = 0; j < w.n_kv; ++j) {
-        // K tile, then (with the item's first tile in between) the other side's queries, then
-        // the V tile.  Page numbers are fetched before the wait for the stage.
         const int slot = (w.j0 + j) * ATC_BN + piece * cr;
         int page = 0, c1 = w.row0 + slot;
-        if (paged) {
+        if (paged) {  // fetched before the wait for the stage
           page = lane < boxes && slot < w.len ? srv_page(p.s, w.b, slot) : p.s.num_pages;
           c1 = slot & ((1 << p.s.page_shift) - 1);
         }
-        const int ks = (int)(kc % STAGES), vs = (int)(vc % STAGES);
+        const int ks = (int)(kc % STAGES);
         if (!wait(bar_k_empty + 8 * ks, (uint32_t)((kc / STAGES) & 1) ^ 1u)) break;
         if (lane == 0) mbar_arrive_expect_tx(bar_k_full + 8 * ks, SM::KV_TILE);
         __syncwarp();
@@ -433,20 +468,20 @@ __global__ void __launch_bounds__(tile_threads(tile_nt(HD)), 1)
           tma_load_4d(sK + ks * SM::KV_TILE + box_at, &tmK, bar_k_full + 8 * ks, box_x * SM::BOX_COLS, c1, w.h, page);
         __syncwarp();
         ++kc;
+        if (!load_v()) break;  // the tile before
+        v_c1 = c1;
+        v_h = w.h;
+        v_page = page;
+        v_due = true;
         if (NT == 2 && j == 0 && !publish(1)) break;
-        if (!wait(bar_v_empty + 8 * vs, (uint32_t)((vc / STAGES) & 1) ^ 1u)) break;
-        if (lane == 0) mbar_arrive_expect_tx(bar_v_full + 8 * vs, SM::KV_TILE);
-        __syncwarp();
-        if (lane < boxes)
-          tma_load_4d(sV + vs * SM::KV_TILE + box_at, &tmV, bar_v_full + 8 * vs, box_x * SM::BOX_COLS, c1, w.h, page);
-        __syncwarp();
-        ++vc;
       }
-      if (!ok) break;
+      if (!ok || !load_v()) break;
       if (stop) {
         if (NT == 2) publish(1);
         break;
       }
+      it = __shfl_sync(FULL, taken, 0);
+      fetch(it, &lo, &hi);
     }
     if (!ok && lane == 0) {
       *abort_flag = 1;
@@ -464,20 +499,20 @@ __global__ void __launch_bounds__(tile_threads(tile_nt(HD)), 1)
     }
   } else if (warp < CLEANER && warp >= ISSUER) {
     // ------------------------------------------------------------ MMA issuers
-    // One warp per query tile, as in attention_tc.cuh: the whole warp runs the loop, one
-    // elected lane issues.
+    // As in attention_tc.cuh: the whole warp runs the loop, one elected lane issues.
     constexpr unsigned FULL = 0xffffffffu;
-    const int t = warp - ISSUER;
     constexpr uint32_t idesc_s = idesc_f16_f32(ATC_BM, SM::KT, 0, 0, BF16);
     constexpr uint32_t idesc_o = idesc_f16_f32(ATC_BM, HD, 0, 1, BF16);
     constexpr uint32_t v_step = HD == 32 ? (1024u >> 4) : (2048u >> 4);  // 16 keys
     constexpr uint32_t sub_bytes = SM::KT * SM::BOX_COLS * 2;            // a step's rows of a box
-    const uint32_t s_col = SM::s_col(t), p_col = SM::p_col(t), o_col = SM::o_col(t);
+    const int t = SM::SPLIT ? (warp - ISSUER) >> 1 : warp - ISSUER;
+    const bool does_s = !SM::SPLIT || ((warp - ISSUER) & 1) == 0;
+    const uint32_t s_col = tmem + SM::s_col(t), p_col = tmem + SM::p_col(t), o_col = tmem + SM::o_col(t);
     bool ok = true;
     bool issued = false;
-    long kvc = 0;                   // key tiles of all items so far
-    long k_seen = -1, v_seen = -1;  // highest K / V tile whose arrival this warp observed
-    long pc = 0, sfc = 0, oc = 0;   // p_full / s_free / o_free phases used
+    uint32_t kvc = 0;                // key tiles of all items so far
+    uint32_t k_seen = 0, v_seen = 0;  // K / V tiles whose arrival this warp observed
+    uint32_t pc = 0, sc = 0, oc = 0;  // steps whose P V / S this warp issued, items whose O it began
     auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
       if (!__all_sync(FULL, srv_wait(bar, parity, abort_flag, limit))) {
         ok = false;
@@ -486,80 +521,86 @@ __global__ void __launch_bounds__(tile_threads(tile_nt(HD)), 1)
       tc_fence_after();
       return true;
     };
-    auto ensure_k = [&](long idx) -> bool {
-      while (k_seen < idx) {
-        ++k_seen;
-        if (!wait(bar_k_full + 8 * (int)(k_seen % STAGES), (uint32_t)((k_seen / STAGES) & 1))) return false;
-      }
+    auto ensure_k = [&](uint32_t idx) -> bool {
+      for (; k_seen <= idx; ++k_seen)
+        if (!wait(bar_k_full + 8 * (k_seen % STAGES), (k_seen / STAGES) & 1)) return false;
       return true;
     };
-    auto ensure_v = [&](long idx) -> bool {
-      while (v_seen < idx) {
-        ++v_seen;
-        if (!wait(bar_v_ready + 8 * (int)(v_seen % STAGES), (uint32_t)((v_seen / STAGES) & 1))) return false;
-      }
+    auto ensure_v = [&](uint32_t idx) -> bool {
+      for (; v_seen <= idx; ++v_seen)
+        if (!wait(bar_v_ready + 8 * (v_seen % STAGES), (v_seen / STAGES) & 1)) return false;
+      return true;
+    };
+    // Whether step i is its key tile's last one of this side.
+    auto ends_tile = [](int i, int n) { return i % SM::SUB == SM::SUB - 1 || i + 1 == n; };
+    // S of step i (of n) into the side's score buffer, which the softmax has read.
+    auto do_s = [&](int i, int n, int qb) -> bool {
+      const uint32_t idx = kvc + i / SM::SUB;
+      if (sc > 0 && !wait(bar_s_free + 8 * t, (sc - 1) & 1)) return false;
+      if (!ensure_k(idx)) return false;
+      const uint32_t qaddr = sQ + (t * QBUF + qb) * SM::Q_TILE;
+      const uint32_t kaddr = sK + (idx % STAGES) * SM::KV_TILE + (uint32_t)(i % SM::SUB) * sub_bytes;
+#pragma unroll
+      for (int kk = 0; kk < HD / 16; ++kk)
+        mma_f16_ss_warp(s_col, atc_desc_qk<HD>(qaddr, kk), atc_desc_qk<HD>(kaddr, kk), idesc_s, kk > 0 ? 1u : 0u);
+      mma_commit_warp(bar_s_full + 8 * t);
+      if (ends_tile(i, n)) mma_commit_warp(bar_k_empty + 8 * (idx % STAGES));
+      if (i + 1 == n) mma_commit_warp(bar_q_empty + 8 * (t * SM::QS + qb));
+      issued = true;
+      ++sc;
+      return true;
+    };
+    // O += P V of step i.  The first of an item overwrites O, which the softmax has read.
+    auto do_pv = [&](int i, int n) -> bool {
+      const uint32_t idx = kvc + i / SM::SUB;
+      const uint32_t pb = pc % SM::PBUF;
+      if (!wait(bar_p_full + 16 * t + 8 * pb, (pc / SM::PBUF) & 1) || !ensure_v(idx)) return false;
+      if (i == 0 && !wait(bar_o_free + 8 * t, (oc++ & 1) ^ 1u)) return false;
+      const uint64_t vd = atc_desc_v<HD>(sV + (idx % STAGES) * SM::KV_TILE + (uint32_t)(i % SM::SUB) * sub_bytes);
+#pragma unroll
+      for (int kk = 0; kk < SM::KT / 16; ++kk)
+        mma_f16_ts_warp(o_col, p_col + pb * (SM::KT / 2) + (uint32_t)(kk * 8), vd + (uint64_t)(kk * v_step), idesc_o,
+                        (i > 0 || kk > 0) ? 1u : 0u);
+      mma_commit_warp(bar_pv_done + 16 * t + 8 * pb);
+      if (i + 1 == n) mma_commit_warp(bar_o_full + 8 * t);
+      if (ends_tile(i, n)) mma_commit_warp(bar_v_empty + 8 * (idx % STAGES));
+      issued = true;
+      ++pc;
       return true;
     };
     for (int k = 0; ok; ++k) {
       const int qb = k % QBUF;
+      const uint32_t q_empty = bar_q_empty + 8 * (t * SM::QS + qb);
       if (!wait(bar_q_full + 8 * (t * SM::QS + qb), (k / QBUF) & 1)) break;
       const TileInfo& wi = info[t * SM::QS + qb];
       const int n_kv = __shfl_sync(FULL, wi.n_kv, 0);
       if (n_kv < 0) break;  // no more items
       const int n = __shfl_sync(FULL, wi.ns[atc_query_tile<NT>(t, k)], 0);
-      const uint32_t qaddr = sQ + (t * QBUF + qb) * SM::Q_TILE;
-      // S of step i; the K stage is free after its last step.
-      auto issue_s = [&](int i) {
-        const long idx = kvc + i / SM::SUB;
-        const uint32_t kaddr = sK + (int)(idx % STAGES) * SM::KV_TILE + (uint32_t)(i % SM::SUB) * sub_bytes;
-#pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk)
-          mma_f16_ss_warp(tmem + s_col, atc_desc_qk<HD>(qaddr, kk), atc_desc_qk<HD>(kaddr, kk), idesc_s,
-                          kk > 0 ? 1u : 0u);
-        mma_commit_warp(bar_s_full + 8 * t);
-        if (i % SM::SUB == SM::SUB - 1 || i + 1 == n) mma_commit_warp(bar_k_empty + 8 * (int)(idx % STAGES));
-        issued = true;
-      };
-      if (n > 0) {
-        if (!ensure_k(kvc)) break;
-        issue_s(0);
-      }
-      for (int i = 0; i < n && ok; ++i, ++pc) {
-        // Next scores as soon as the softmax threads have read these (s_free).
-        if (i + 1 < n) {
-          if (!wait(bar_s_free + 8 * t, (uint32_t)(sfc++ & 1))) break;
-          if (!ensure_k(kvc + (i + 1) / SM::SUB)) break;
-          issue_s(i + 1);
+      if constexpr (SM::SPLIT) {
+        __syncwarp();
+        if (lane == 0 && (!does_s || n == 0)) mbar_arrive(q_empty);  // (S: with its last product)
+        for (int i = 0; i < n && ok; ++i)
+          if (!(does_s ? do_s(i, n, qb) : do_pv(i, n))) break;
+      } else {
+        if (n == 0 && lane == 0) mbar_arrive(q_empty);
+        __syncwarp();
+        // The next S as soon as the softmax has read this one's scores.
+        if (n > 0 && !do_s(0, n, qb)) break;
+        for (int i = 0; i < n && ok; ++i) {
+          if (i + 1 < n && !do_s(i + 1, n, qb)) break;
+          if (!do_pv(i, n)) break;
         }
-        if (!wait(bar_p_full + 8 * t, (uint32_t)(pc & 1))) break;
-        const long idx = kvc + i / SM::SUB;
-        if (!ensure_v(idx)) break;
-        // The first P V of an item overwrites O: the previous item's O must be read.
-        if (i == 0 && !wait(bar_o_free + 8 * t, (uint32_t)(oc++ & 1) ^ 1u)) break;
-        const uint32_t pb = (uint32_t)(pc % SM::PBUF);
-        const uint64_t vd =
-            atc_desc_v<HD>(sV + (int)(idx % STAGES) * SM::KV_TILE + (uint32_t)(i % SM::SUB) * sub_bytes);
-#pragma unroll
-        for (int kk = 0; kk < SM::KT / 16; ++kk)
-          mma_f16_ts_warp(tmem + o_col, tmem + p_col + pb * (SM::KT / 2) + (uint32_t)(kk * 8),
-                          vd + (uint64_t)(kk * v_step), idesc_o, (i > 0 || kk > 0) ? 1u : 0u);
-        mma_commit_warp(bar_pv_done + 16 * t + 8 * pb);
-        issued = true;
-        if (i + 1 == n) mma_commit_warp(bar_o_full + 8 * t);
-        if (i % SM::SUB == SM::SUB - 1 || i + 1 == n) mma_commit_warp(bar_v_empty + 8 * (int)(idx % STAGES));
       }
       // Key tiles that only the other side uses: released once they have landed.
       for (int j = (n + SM::SUB - 1) / SM::SUB; j < n_kv && ok; ++j) {
-        if (!ensure_k(kvc + j) || !ensure_v(kvc + j)) break;
+        if ((does_s && !ensure_k(kvc + j)) || ((!SM::SPLIT || !does_s) && !ensure_v(kvc + j))) break;
         if (lane == 0) {
-          mbar_arrive(bar_k_empty + 8 * (int)((kvc + j) % STAGES));
-          mbar_arrive(bar_v_empty + 8 * (int)((kvc + j) % STAGES));
+          if (does_s) mbar_arrive(bar_k_empty + 8 * ((kvc + j) % STAGES));
+          if (!SM::SPLIT || !does_s) mbar_arrive(bar_v_empty + 8 * ((kvc + j) % STAGES));
         }
         __syncwarp();
       }
-      if (!ok) break;
       kvc += n_kv;
-      mma_commit_warp(bar_q_empty + 8 * (t * SM::QS + qb));
     }
     if (!ok) {
       if (lane == 0) {
@@ -567,8 +608,8 @@ __global__ void __launch_bounds__(tile_threads(tile_nt(HD)), 1)
         report_status(p.s.status, SRV_DEV_TIMEOUT);
       }
       if (issued) {
-        mma_commit_warp(bar_drain + 8 * t);
-        srv_wait(bar_drain + 8 * t, 0, nullptr, limit);
+        mma_commit_warp(bar_drain + 8 * (warp - ISSUER));
+        srv_wait(bar_drain + 8 * (warp - ISSUER), 0, nullptr, limit);
       }
     }
   } else if (warp == CLEANER) {
@@ -650,7 +691,7 @@ __global__ void __launch_bounds__(tile_threads(tile_nt(HD)), 1)
     const uint32_t p_addr0 = tmem + lane_base + SM::p_col(t);
     const uint32_t o_addr = tmem + lane_base + SM::o_col(t);
     const float scale = p.scale_log2;
-    long c = 0;    // steps of all items so far (phase of s_full, P buffer)
+    long c = 0;    // steps of all items so far
     long ofc = 0;  // items with steps so far
     bool ok = true;
     // One arrival per warp, after every lane's reads and TMEM accesses.
@@ -707,10 +748,8 @@ __global__ void __launch_bounds__(tile_threads(tile_nt(HD)), 1)
         }
         tmem_wait_ld();
         // The scores are in registers: the buffer may take the next step's.
-        if (i + 1 < n) {
-          tc_fence_before();
-          arrive(bar_s_free + 8 * t);
-        }
+        tc_fence_before();
+        arrive(bar_s_free + 8 * t);
         const int k0 = key0 + i * KT;
         if (k0 + KT - 1 > first) {
           // Column e of this step is hidden when e > lim.
@@ -752,22 +791,21 @@ __global__ void __launch_bounds__(tile_threads(tile_nt(HD)), 1)
         // 32 keys' probabilities; one pair in four takes its exponentials from the FMA pipe
         // (the MUFU is the tighter one).
         auto exp_chunk = [&](int q) {
+          // Loop by loop, so that the MUFU's latencies overlap.
+          float2 x[16];
 #pragma unroll
-          for (int cc = 0; cc < 16; ++cc) {
-            const int e = q * 16 + cc;
-            const float2 x =
-                ffma2(make_float2(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1])), sc2, nb2);
-            float p0, p1;
-            if ((e & 3) == 3) {
-              const float2 y = exp2_fma2(x);
-              p0 = y.x;
-              p1 = y.y;
-            } else {
-              p0 = ex2_approx(x.x);
-              p1 = ex2_approx(x.y);
-            }
-            ps2[e & 1] = add2p(ps2[e & 1], pk2(p0, p1));
-            pk[q][cc] = srv_pack<BF16>(p0, p1);
+          for (int e = 0; e < 16; ++e)
+            x[e] = ffma2(make_float2(__uint_as_float(sv[32 * q + 2 * e]), __uint_as_float(sv[32 * q + 2 * e + 1])),
+                         sc2, nb2);
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if ((e & 3) != 3) x[e] = make_float2(ex2_approx(x[e].x), ex2_approx(x[e].y));
+#pragma unroll
+          for (int e = 3; e < 16; e += 4) x[e] = exp2_fma2(x[e]);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            ps2[e & 1] = add2p(ps2[e & 1], pk2(x[e].x, x[e].y));
+            pk[q][e] = srv_pack<BF16>(x[e].x, x[e].y);
           }
         };
         // The P buffer is free once the P V that used it last is complete; with one buffer
@@ -805,7 +843,9 @@ __global__ void __launch_bounds__(tile_threads(tile_nt(HD)), 1)
         }
         tmem_wait_st();
         tc_fence_before();
-        arrive(bar_p_full + 8 * t);
+        // A barrier per P buffer: the softmax may be a step ahead of P V, and a barrier that
+        // completed twice since it was looked at would read as not completed.
+        arrive(bar_p_full + 16 * t + 8 * (uint32_t)(c % SM::PBUF));
       }
       if (!ok) break;
       if (!srv_wait(bar_o_full + 8 * t, (uint32_t)(ofc++ & 1), abort_flag, limit)) {
