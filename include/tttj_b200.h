@@ -322,7 +322,7 @@ int tttj_attention_noalloc(const void* qkv, void* ctx, int qkv_rows, const uint8
  * gathers, eviction.  No counterpart in the reference (it runs whole sequences only).
  *
  * fp16 or bf16 (TTTJ_DTYPE_F16 / TTTJ_DTYPE_BF16) in and out, fp32 products, softmax
- * statistics and masses.  head_dim 32, 64, 128 or 256; group 1 .. 64; at most 2048
+ * statistics and masses.  head_dim 32, 64, 128 or 256; group 1 .. 64; at most 1024
  * sequences.  Rows are given by element strides, head_dim contiguous, all strides
  * positive multiples of 8, pointers 16-byte aligned; tokens x heads < 2^31.
  *

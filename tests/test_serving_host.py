@@ -38,7 +38,7 @@ def _refused(rc, text):
 @pytest.mark.parametrize("kw,text", [
     (dict(dtype=_lib.DTYPE_F32), "fp16 or bf16"), (dict(head_dim=48), "head_dim=48"), (dict(heads=9), "heads=9"),
     (dict(heads=130, kv_heads=2), "group"), (dict(kv_heads=0), "heads"), (dict(batch=0), "batch"),
-    (dict(batch=2049), "batch"), (dict(tokens=-1), "tokens"), (dict(tokens=1 << 29), "tokens"),
+    (dict(batch=1025), "batch"), (dict(tokens=-1), "tokens"), (dict(tokens=1 << 29), "tokens"),
     (dict(page_size=8), "page_size"), (dict(page_size=48), "page_size"), (dict(page_size=512), "page_size"),
     (dict(pages_per_seq=0), "pages_per_seq"), (dict(pages_per_seq=1 << 28), "pages_per_seq"),
     (dict(num_pages=0), "num_pages"), (dict(table_stride=7), "overlap"), (dict(seq_offsets=None), "seq_offsets"),

@@ -9,7 +9,7 @@
 
 namespace tttj {
 
-constexpr int SRV_MAX_BATCH = 2048;  // sequences of a call (prefix sums in shared memory)
+constexpr int SRV_MAX_BATCH = 1024;  // sequences of a call (prefix sums in shared memory)
 constexpr int SRV_MAX_GROUP = 64;    // query heads per key / value head
 constexpr int SRV_DEV_BAD_PAGE = 0x401;   // a live page-table entry outside the cache
 constexpr int SRV_DEV_BAD_LENS = 0x402;   // lengths or offsets outside the call's tensors
@@ -141,6 +141,7 @@ struct MassParams {
   float scale_log2;
   unsigned long long wait_limit_ns;
 };
+constexpr int MASS_TILE_ROWS = 80;  // query rows of a tile (MASS_ROWS)
 cudaError_t mass_launch(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const MassParams& p, int head_dim,
                         int bf16, int grid, cudaStream_t stream);
 

@@ -364,7 +364,7 @@ int tttj_cache_mass(const tttj_seqs* s, const tttj_rows* q, const float* lse, co
   p.kv_heads = s->kv_heads;
   p.group = s->heads / s->kv_heads;
   // Query tiles no larger than the tokens a sequence has: single tokens load one each.
-  p.tile_tokens = tile_tokens(s);
+  p.tile_tokens = MASS_TILE_ROWS / p.group;
   const int most = max_new > 0 && max_new < s->tokens ? max_new : s->tokens;
   if (most < p.tile_tokens) p.tile_tokens = most;
   p.scale_log2 = scale * 1.44269504088896341f;

@@ -9,12 +9,12 @@ template <int HD, bool BF16>
 cudaError_t launch(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const MassParams& p, int grid,
                    cudaStream_t stream) {
   auto kern = mass_kernel<HD, BF16>;
-  static_assert(MassSmem<HD>::FIXED + SRV_MAX_BATCH * (int)sizeof(SrvSeq) <= 232448,
+  static_assert(MassSmem<HD>::FIXED + SRV_MAX_BATCH * ((int)sizeof(SrvSeq) + 8) + 4 <= 232448,
                 "shared memory exceeds the 227 KB per-CTA limit");
-  const int smem = MassSmem<HD>::FIXED + p.s.batch * (int)sizeof(SrvSeq);
+  const int smem = MassSmem<HD>::FIXED + p.s.batch * ((int)sizeof(SrvSeq) + 8) + 4;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  return launch_pdl(kern, dim3(grid), dim3(MASS_THREADS), smem, stream, tm_q, tm_k, p);
+  return launch_pdl(kern, dim3(grid), dim3(mass_threads(MassSmem<HD>::NT)), smem, stream, tm_q, tm_k, p);
 }
 }  // namespace
 
