@@ -81,41 +81,35 @@ __global__ void __launch_bounds__(APPEND_THREADS, 5) append_kernel(const AppendP
 }
 
 // ------------------------------------------------------------------- evict
-// One cluster of 1 .. 8 blocks per (sequence, head); each block owns a contiguous range of
-// slots, whose masses and positions it holds in shared memory.  A radix selection over
-// an order-preserving integer image of the mass (digits of 11, 11 and 10 bits, counted in shared memory
-// and added up across the cluster) finds the keep-th largest value.  One ordered pass
-// then ranks the equal values, the holes (slots < keep that go) and the movers (slots >= keep
-// that stay); the i-th mover goes to the i-th hole, so as few rows move as can, and since
-// sources lie behind the budget and destinations in front of it, no move reads what
-// another writes.  All counts are integers: the result does not depend on the order in
-// which threads run.  Bound: for short caches latency (about twenty barriers), for long ones the bytes
-// of masses, positions and moved rows.
+// One cluster of 1 .. 8 blocks per (sequence, head); each warp owns a contiguous range of slots
+// and holds EVICT_HELD of them per thread in registers (a longer range's rest is read again
+// where it is needed).  The keep-th largest value is found two bits at a time: everyone
+// counts the values above three thresholds, the warps' counts meet in every block's shared
+// memory, 16 rounds of one barrier each.  (A radix selection with histograms in shared memory took
+// 77 thousand cycles of a cluster of 8 at 32768 slots, this SELECT.)  Then ballots rank the
+// equal values, the holes (slots < keep that go) and the movers (slots >= keep that stay); the
+// i-th mover goes to the i-th hole, so as few rows move as can, and since sources lie behind
+// the budget and destinations in front of it, no move reads what another writes.  All counts are
+// integers: the result does not depend on the order in which threads run.  Bound: for short
+// caches latency, for long ones the bytes of the moved rows.
 constexpr int EVICT_MAX_CLUSTER = 8;
-constexpr int EVICT_MAX_THREADS = 512;
-constexpr int EVICT_BINS = 2048;
-constexpr int EVICT_BATCH = 4;
-constexpr int EVICT_HELD_SLOTS = 24 * 1024;  // slots of one block held in shared memory (8 bytes each)
+constexpr int EVICT_MAX_THREADS = 1024;
+constexpr int EVICT_HELD = 8;
+constexpr int EVICT_BATCH = 2;  // moves of a thread whose rows are in flight
 
-// Unsigned image of a mass: larger mass, larger integer; -0 as +0, NaN lowest.
+// Unsigned image of a mass: larger mass, larger integer; -0 as +0, NaN lowest.  Never 0.
 __device__ __forceinline__ uint32_t evict_key(float mass) {
   if (mass != mass) return 0x007fffffu;  // the image of -inf
   const uint32_t u = __float_as_uint(mass + 0.f);
   return (u >> 31) ? ~u : (u | 0x80000000u);
 }
 
-struct EvictShared {
-  int hist[EVICT_BINS];   // counts of one digit (read by the whole cluster)
-  int total[4];           // newest position; equal, holes, movers of this block
-  int warp[2][32];
-  int digit, need;
-};
-
 __global__ void __launch_bounds__(EVICT_MAX_THREADS) evict_kernel(const EvictParams p, int cluster) {
-  extern __shared__ __align__(16) uint8_t s_dyn[];
-  __shared__ EvictShared sh;
+  // Three counts of every warp of the cluster, double-buffered.
+  __shared__ int4 s_cnt[2][EVICT_MAX_CLUSTER * EVICT_MAX_THREADS / 32];
   griddep_wait();
   griddep_launch();
+  constexpr unsigned FULL = 0xffffffffu;
   const int rank = cluster > 1 ? (int)cluster_ctarank() : 0;
   const int bh = blockIdx.x / cluster, b = bh / p.kv_heads;
   const int threads = blockDim.x, warps = threads >> 5, warp = warp_id(), lane = lane_id();
@@ -145,159 +139,173 @@ __global__ void __launch_bounds__(EVICT_MAX_THREADS) evict_kernel(const EvictPar
     }
     return;
   }
-  auto sync_all = [&] {
-    if (cluster > 1) cluster_sync_all(); else __syncthreads();
+  // This warp's slots.
+  const int all_warps = cluster * warps, my_warp = rank * warps + warp;
+  const int each = ((len + all_warps - 1) / all_warps + 31) & ~31;
+  const int w0 = (int)min((long)my_warp * each, (long)len), w1 = min(w0 + each, len);
+  float m[EVICT_HELD];
+  int ps[EVICT_HELD];
+#pragma unroll
+  for (int i = 0; i < EVICT_HELD; ++i) {
+    const int j = w0 + 32 * i + lane;
+    m[i] = j < w1 ? mass[j] : 0.f;
+    ps[i] = j < w1 ? pos[j] : INT32_MIN;
+  }
+  const int rest = w0 + 32 * EVICT_HELD;  // slots from here on are not held
+  int turn = 0;
+  // Every warp's three counts, to every warp of the cluster; returns the buffer they are in.
+  auto share = [&](int x, int y, int z) -> const int4* {
+    int4* buf = s_cnt[turn++ & 1];
+    if (cluster > 1) {
+      if (lane < cluster)
+        *static_cast<int4*>(__cluster_map_shared_rank(buf + my_warp, (unsigned)lane)) = make_int4(x, y, z, 0);
+      cluster_sync_all();
+    } else {
+      if (lane == 0) buf[my_warp] = make_int4(x, y, z, 0);
+      __syncthreads();
+    }
+    return buf;
   };
-  auto peer = [&](int* x, int r) -> int {
-    return cluster > 1 ? *static_cast<int*>(__cluster_map_shared_rank(x, (unsigned)r)) : *x;
-  };
-  // This block's slots, a multiple of 32 per warp.
-  const int each = ((len + cluster - 1) / cluster + 31) & ~31;
-  const int lo = min(rank * each, len), hi = min(lo + each, len);
-  const bool held = each <= EVICT_HELD_SLOTS;
-  float* s_mass = reinterpret_cast<float*>(s_dyn);
-  int* s_pos = reinterpret_cast<int*>(s_dyn) + (held ? each : 0);
   int newest = INT32_MIN;
-#pragma unroll 4
-  for (int j = lo + (int)threadIdx.x; j < hi; j += threads) {
-    const int x = pos[j];
-    const float m = held ? mass[j] : 0.f;
-    newest = max(newest, x);
-    if (held) {
-      s_mass[j - lo] = m;
-      s_pos[j - lo] = x;
-    }
+#pragma unroll
+  for (int i = 0; i < EVICT_HELD; ++i) newest = max(newest, ps[i]);
+  for (int j = rest + lane; j < w1; j += 32) newest = max(newest, pos[j]);
+  newest = __reduce_max_sync(FULL, newest);
+  if (cluster > 1) cluster_sync_all();  // every block has started: its shared memory may be written
+  {
+    const int4* c = share(newest, 0, 0);
+    for (int w = lane; w < all_warps; w += 32) newest = max(newest, c[w].x);
+    newest = __reduce_max_sync(FULL, newest);
   }
-  newest = __reduce_max_sync(0xffffffffu, newest);
-  if (lane == 0) sh.warp[0][warp] = newest;
-  for (int i = threadIdx.x; i < EVICT_BINS; i += threads) sh.hist[i] = 0;
-  __syncthreads();
-  if (warp == 0) {
-    newest = __reduce_max_sync(0xffffffffu, lane < warps ? sh.warp[0][lane] : INT32_MIN);
-    if (lane == 0) sh.total[0] = newest;
-  }
-  sync_all();
-  newest = INT32_MIN;
-  for (int r = 0; r < cluster; ++r) newest = max(newest, peer(&sh.total[0], r));
   const long edge = (long)newest - p.recent;  // positions behind it count as +inf
-  auto key_at = [&](int j) -> uint32_t {
-    const int x = held ? s_pos[j - lo] : pos[j];
-    return (long)x > edge ? 0xff800000u /* image of +inf */ : evict_key(held ? s_mass[j - lo] : mass[j]);
+  auto key_of = [&](float mass_j, int pos_j) {
+    return (long)pos_j > edge ? 0xff800000u /* image of +inf */ : evict_key(mass_j);
   };
-  uint32_t prefix = 0;
-  int need = keep;  // how many of the values that match the prefix so far are kept
+  uint32_t key[EVICT_HELD];
+#pragma unroll
+  for (int i = 0; i < EVICT_HELD; ++i) key[i] = w0 + 32 * i + lane < w1 ? key_of(m[i], ps[i]) : 0u;
+  // The keep-th largest value, two bits a round.
+  uint32_t cut = 0;
 #pragma unroll 1
-  for (int pass = 0; pass < 3; ++pass) {
-    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-    const int bits = pass == 2 ? 10 : 11;
-    for (int j = lo + (int)threadIdx.x; j < hi; j += threads) {
-      const uint32_t key = key_at(j);
-      if (pass == 0 || (key >> (shift + bits)) == (prefix >> (shift + bits)))
-        atomicAdd(&sh.hist[(key >> shift) & ((1u << bits) - 1)], 1);
+  for (int shift = 30; shift >= 0; shift -= 2) {
+    const uint32_t c1 = cut | (1u << shift), c2 = cut | (2u << shift), c3 = cut | (3u << shift);
+    int n1 = 0, n2 = 0, n3 = 0;
+#pragma unroll
+    for (int i = 0; i < EVICT_HELD; ++i) {
+      n1 += key[i] >= c1;
+      n2 += key[i] >= c2;
+      n3 += key[i] >= c3;
     }
-    sync_all();
-    // Largest digits first: thread t takes bins top - per t .. ; counts over the cluster.
-    const int per = (1 << bits) / threads;
-    const int first = (1 << bits) - 1 - per * (int)threadIdx.x;
-    int c[EVICT_BINS / 128], sum = 0;  // at least 128 threads
-#pragma unroll
-    for (int i = 0; i < EVICT_BINS / 128; ++i) c[i] = 0;
-    for (int r = 0; r < cluster; ++r) {
-#pragma unroll
-      for (int i = 0; i < EVICT_BINS / 128; ++i)
-        if (i < per) c[i] += peer(&sh.hist[first - i], r);
+    for (int j = rest + lane; j < w1; j += 32) {
+      const uint32_t x = key_of(mass[j], pos[j]);
+      n1 += x >= c1;
+      n2 += x >= c2;
+      n3 += x >= c3;
     }
-#pragma unroll
-    for (int i = 0; i < EVICT_BINS / 128; ++i) sum += c[i];
-    int inc = sum;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int o = __shfl_up_sync(0xffffffffu, inc, d);
-      if (lane >= d) inc += o;
+    const int4* c = share(__reduce_add_sync(FULL, n1), __reduce_add_sync(FULL, n2), __reduce_add_sync(FULL, n3));
+    n1 = n2 = n3 = 0;
+    for (int w = lane; w < all_warps; w += 32) {
+      const int4 v = c[w];
+      n1 += v.x;
+      n2 += v.y;
+      n3 += v.z;
     }
-    if (lane == 31) sh.warp[0][warp] = inc;
-    __syncthreads();
-    int above = inc - sum;
-    for (int w = 0; w < warp; ++w) above += sh.warp[0][w];
-    if (above < need && need <= above + sum) {
-#pragma unroll
-      for (int i = 0; i < EVICT_BINS / 128; ++i) {
-        if (i < per && above < need && need <= above + c[i]) {
-          sh.digit = first - i;
-          sh.need = need - above;
-        }
-        above += c[i];
-      }
-    }
-    sync_all();  // digit and need are there; every block has read this one's counts
-    prefix |= (uint32_t)sh.digit << shift;
-    need = sh.need;
-    for (int i = threadIdx.x; i < EVICT_BINS; i += threads) sh.hist[i] = 0;
-    __syncthreads();
+    n1 = __reduce_add_sync(FULL, n1);
+    n2 = __reduce_add_sync(FULL, n2);
+    n3 = __reduce_add_sync(FULL, n3);
+    cut = n3 >= keep ? c3 : n2 >= keep ? c2 : n1 >= keep ? c1 : cut;
   }
-  // Kept: key > prefix, and the first `need` slots with key == prefix.  Each warp owns a
-  // contiguous range; ranks by ballots.
-  const int per_warp = ((hi - lo + warps - 1) / warps + 31) & ~31;
-  const int w0 = min(lo + warp * per_warp, hi), w1 = min(w0 + per_warp, hi);
-  // Exclusive sum of one count per warp over the block (and the blocks before it).
-  auto offset = [&](int mine, int which) {
-    if (lane == 0) sh.warp[which & 1][warp] = mine;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      int t = 0;
-      for (int w = 0; w < warps; ++w) t += sh.warp[which & 1][w];
-      sh.total[which] = t;
+  // Kept: key > cut, and the first `need` slots with key == cut.
+  int above = 0, equal = 0;
+#pragma unroll
+  for (int i = 0; i < EVICT_HELD; ++i) {
+    above += key[i] > cut;
+    equal += key[i] == cut;
+  }
+  for (int j = rest + lane; j < w1; j += 32) {
+    const uint32_t x = key_of(mass[j], pos[j]);
+    above += x > cut;
+    equal += x == cut;
+  }
+  int equal0 = 0;  // equal values in the warps before
+  {
+    const int4* c = share(__reduce_add_sync(FULL, above), __reduce_add_sync(FULL, equal), 0);
+    above = 0;
+    for (int w = lane; w < all_warps; w += 32) {
+      above += c[w].x;
+      if (w < my_warp) equal0 += c[w].y;
     }
-    int at = 0;
-    for (int w = 0; w < warp; ++w) at += sh.warp[which & 1][w];
-    sync_all();
-    for (int r = 0; r < rank; ++r) at += peer(&sh.total[which], r);
-    return at;
-  };
-  int equal = 0;
-  for (int j = w0; j < w1; j += 32)
-    equal += __popc(__ballot_sync(0xffffffffu, j + lane < w1 && key_at(j + lane) == prefix));
-  const int equal0 = offset(equal, 1);
-  auto kept_at = [&](int j, int* rank_eq) {  // of slots j .. j + 31, a bit per lane
-    const uint32_t key = j + lane < w1 ? key_at(j + lane) : 0u;
-    const bool live = j + lane < w1;
-    const unsigned eq = __ballot_sync(0xffffffffu, live && key == prefix);
-    const bool kept = live && (key > prefix || (key == prefix && *rank_eq + __popc(eq & below) < need));
+    above = __reduce_add_sync(FULL, above);
+    equal0 = __reduce_add_sync(FULL, equal0);
+  }
+  const int need = keep - above;
+  // Which of the slots j .. j + 31 are kept, a bit per lane; `rank_eq`: equal values before them.
+  auto kept_of = [&](uint32_t x, int* rank_eq) {
+    const unsigned eq = __ballot_sync(FULL, x == cut);
+    const bool kept = x > cut || (x == cut && *rank_eq + __popc(eq & below) < need);
     *rank_eq += __popc(eq);
-    return __ballot_sync(0xffffffffu, kept);
+    return __ballot_sync(FULL, kept);
   };
   auto span = [&](int j) {  // lanes of slots j .. that are live, and of those the ones < keep
     const int n = w1 - j, f = keep - j;
-    const unsigned live = n >= 32 ? 0xffffffffu : (1u << n) - 1;
+    const unsigned live = n >= 32 ? FULL : n <= 0 ? 0u : (1u << n) - 1;
     return make_uint2(live, f >= 32 ? live : f <= 0 ? 0u : live & ((1u << f) - 1));
   };
-  int holes = 0, movers = 0, eq_rank = equal0;
-  for (int j = w0; j < w1; j += 32) {
-    const unsigned kept = kept_at(j, &eq_rank);
-    const uint2 sp = span(j);
-    holes += __popc(~kept & sp.y);
-    movers += __popc(kept & sp.x & ~sp.y);
+  auto key_rest = [&](int j) { return j + lane < w1 ? key_of(mass[j + lane], pos[j + lane]) : 0u; };
+  int holes = 0, movers = 0, rank_eq = equal0;
+  unsigned kept[EVICT_HELD];
+#pragma unroll
+  for (int i = 0; i < EVICT_HELD; ++i) {
+    kept[i] = kept_of(key[i], &rank_eq);
+    const uint2 sp = span(w0 + 32 * i);
+    holes += __popc(~kept[i] & sp.y);
+    movers += __popc(kept[i] & sp.x & ~sp.y);
   }
-  int hole0 = offset(holes, 2);
-  int mover0 = offset(movers, 3);
-  int n_moves = 0;
-  for (int r = 0; r < cluster; ++r) n_moves += peer(&sh.total[3], r);
-  int2* moves = p.moves + (long)bh * p.most_moves;
-  eq_rank = equal0;
-  for (int j = w0; j < w1; j += 32) {
-    const unsigned kept = kept_at(j, &eq_rank);
+  const int rank_rest = rank_eq;
+  for (int j = rest; j < w1; j += 32) {
+    const unsigned k = kept_of(key_rest(j), &rank_eq);
     const uint2 sp = span(j);
-    const unsigned hole = ~kept & sp.y, mover = kept & sp.x & ~sp.y, bit = 1u << lane;
-    if (hole & bit) moves[hole0 + __popc(hole & below)].y = j + lane;
-    if (mover & bit) moves[mover0 + __popc(mover & below)].x = j + lane;
-    if (kept & sp.y & bit) {
-      mass_out[j + lane] = held ? s_mass[j + lane - lo] : mass[j + lane];
-      pos_out[j + lane] = held ? s_pos[j + lane - lo] : pos[j + lane];
+    holes += __popc(~k & sp.y);
+    movers += __popc(k & sp.x & ~sp.y);
+  }
+  int hole0 = 0, mover0 = 0, n_moves = 0;
+  {
+    const int4* c = share(holes, movers, 0);
+    for (int w = lane; w < all_warps; w += 32) {
+      n_moves += c[w].y;
+      if (w < my_warp) {
+        hole0 += c[w].x;
+        mover0 += c[w].y;
+      }
     }
-    hole0 += __popc(hole);
-    mover0 += __popc(mover);
+    n_moves = __reduce_add_sync(FULL, n_moves);
+    hole0 = __reduce_add_sync(FULL, hole0);
+    mover0 = __reduce_add_sync(FULL, mover0);
   }
-  sync_all();  // the list is complete (and no block still reads another's shared memory)
+  int2* moves = p.moves + (long)bh * p.most_moves;
+  // The list, and the kept slots that stay in place.
+  auto list = [&](int j, unsigned k, float mass_j, int pos_j, int* hole_at, int* mover_at) {
+    const uint2 sp = span(j);
+    const unsigned hole = ~k & sp.y, mover = k & sp.x & ~sp.y, bit = 1u << lane;
+    if (hole & bit) moves[*hole_at + __popc(hole & below)].y = j + lane;
+    if (mover & bit) moves[*mover_at + __popc(mover & below)].x = j + lane;
+    if (k & sp.y & bit) {
+      mass_out[j + lane] = mass_j;
+      pos_out[j + lane] = pos_j;
+    }
+    *hole_at += __popc(hole);
+    *mover_at += __popc(mover);
+  };
+#pragma unroll
+  for (int i = 0; i < EVICT_HELD; ++i) list(w0 + 32 * i, kept[i], m[i], ps[i], &hole0, &mover0);
+  rank_eq = rank_rest;
+  for (int j = rest; j < w1; j += 32) {
+    const bool there = j + lane < w1;
+    const float mj = there ? mass[j + lane] : 0.f;
+    const int pj = there ? pos[j + lane] : 0;
+    list(j, kept_of(there ? key_of(mj, pj) : 0u, &rank_eq), mj, pj, &hole0, &mover0);
+  }
+  if (cluster > 1) cluster_sync_all(); else __syncthreads();  // the list is complete
   for (int i = me; i < n_moves; i += all) {
     const int2 mv = __ldcg(moves + i);
     mass_out[mv.y] = mass[mv.x];
@@ -358,17 +366,14 @@ cudaError_t append_launch(const AppendParams& p, int sms, cudaStream_t stream) {
 }
 
 cudaError_t evict_launch(const EvictParams& p, int sms, cudaStream_t stream) {
-  // Blocks per head: as many as keep at least 2048 slots each, while there are
-  // multiprocessors for them.  Threads: one per four slots or so.
+  // Blocks per head: while a block would have more than 1024 slots and two blocks per
+  // multiprocessor are not reached.  Threads: one per EVICT_HELD slots, 128 at least.
   const long bh = (long)p.s.batch * p.kv_heads;
   int cluster = 1;
-  while (cluster < EVICT_MAX_CLUSTER && p.cap / (2 * cluster) >= 2048 && bh * 2 * cluster <= 2 * sms) cluster *= 2;
-  const long each = ((p.cap + cluster - 1) / cluster + 31) & ~31l;
-  const int threads = each <= 1024 ? 128 : each <= 2048 ? 256 : EVICT_MAX_THREADS;
-  const int smem = each <= EVICT_HELD_SLOTS ? (int)each * 8 : EVICT_HELD_SLOTS * 8;
-  cudaError_t e = cudaFuncSetAttribute(evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return e;
-  return launch_pdl_cluster(evict_kernel, dim3((unsigned)(bh * cluster)), dim3(threads), smem, stream, cluster, p,
+  while (cluster < EVICT_MAX_CLUSTER && p.cap / cluster > 1024 && bh * 2 * cluster <= 2 * sms) cluster *= 2;
+  int threads = 128;
+  while (threads < EVICT_MAX_THREADS && (long)threads * EVICT_HELD * cluster < p.cap) threads *= 2;
+  return launch_pdl_cluster(evict_kernel, dim3((unsigned)(bh * cluster)), dim3(threads), 0, stream, cluster, p,
                             cluster);
 }
 
