@@ -143,12 +143,12 @@ __global__ void __launch_bounds__(EVICT_MAX_THREADS) evict_kernel(const EvictPar
   const int all_warps = cluster * warps, my_warp = rank * warps + warp;
   const int each = ((len + all_warps - 1) / all_warps + 31) & ~31;
   const int w0 = (int)min((long)my_warp * each, (long)len), w1 = min(w0 + each, len);
-  float m[EVICT_HELD];
+  uint32_t key[EVICT_HELD];
   int ps[EVICT_HELD];
 #pragma unroll
   for (int i = 0; i < EVICT_HELD; ++i) {
     const int j = w0 + 32 * i + lane;
-    m[i] = j < w1 ? mass[j] : 0.f;
+    key[i] = j < w1 ? evict_key(mass[j]) : 0u;
     ps[i] = j < w1 ? pos[j] : INT32_MIN;
   }
   const int rest = w0 + 32 * EVICT_HELD;  // slots from here on are not held
@@ -181,10 +181,11 @@ __global__ void __launch_bounds__(EVICT_MAX_THREADS) evict_kernel(const EvictPar
   auto key_of = [&](float mass_j, int pos_j) {
     return (long)pos_j > edge ? 0xff800000u /* image of +inf */ : evict_key(mass_j);
   };
-  uint32_t key[EVICT_HELD];
 #pragma unroll
-  for (int i = 0; i < EVICT_HELD; ++i) key[i] = w0 + 32 * i + lane < w1 ? key_of(m[i], ps[i]) : 0u;
-  // The keep-th largest value, two bits a round.
+  for (int i = 0; i < EVICT_HELD; ++i)
+    if (key[i] != 0u && (long)ps[i] > edge) key[i] = 0xff800000u;
+  // The keep-th largest value, two bits a round; done early once a threshold has exactly `keep`
+  // values at or above it.
   uint32_t cut = 0;
 #pragma unroll 1
   for (int shift = 30; shift >= 0; shift -= 2) {
@@ -213,6 +214,11 @@ __global__ void __launch_bounds__(EVICT_MAX_THREADS) evict_kernel(const EvictPar
     n1 = __reduce_add_sync(FULL, n1);
     n2 = __reduce_add_sync(FULL, n2);
     n3 = __reduce_add_sync(FULL, n3);
+    const int exact = n3 == keep ? 3 : n2 == keep ? 2 : n1 == keep ? 1 : 0;
+    if (exact != 0) {
+      cut = (cut | ((uint32_t)exact << shift)) - 1;  // all above it stay, no equal one does
+      break;
+    }
     cut = n3 >= keep ? c3 : n2 >= keep ? c2 : n1 >= keep ? c1 : cut;
   }
   // Kept: key > cut, and the first `need` slots with key == cut.
@@ -253,15 +259,13 @@ __global__ void __launch_bounds__(EVICT_MAX_THREADS) evict_kernel(const EvictPar
   };
   auto key_rest = [&](int j) { return j + lane < w1 ? key_of(mass[j + lane], pos[j + lane]) : 0u; };
   int holes = 0, movers = 0, rank_eq = equal0;
-  unsigned kept[EVICT_HELD];
 #pragma unroll
   for (int i = 0; i < EVICT_HELD; ++i) {
-    kept[i] = kept_of(key[i], &rank_eq);
+    const unsigned k = kept_of(key[i], &rank_eq);
     const uint2 sp = span(w0 + 32 * i);
-    holes += __popc(~kept[i] & sp.y);
-    movers += __popc(kept[i] & sp.x & ~sp.y);
+    holes += __popc(~k & sp.y);
+    movers += __popc(k & sp.x & ~sp.y);
   }
-  const int rank_rest = rank_eq;
   for (int j = rest; j < w1; j += 32) {
     const unsigned k = kept_of(key_rest(j), &rank_eq);
     const uint2 sp = span(j);
@@ -284,27 +288,23 @@ __global__ void __launch_bounds__(EVICT_MAX_THREADS) evict_kernel(const EvictPar
   }
   int2* moves = p.moves + (long)bh * p.most_moves;
   // The list, and the kept slots that stay in place.
-  auto list = [&](int j, unsigned k, float mass_j, int pos_j, int* hole_at, int* mover_at) {
+  auto list = [&](int j, uint32_t x) {
+    const unsigned k = kept_of(x, &rank_eq);
     const uint2 sp = span(j);
     const unsigned hole = ~k & sp.y, mover = k & sp.x & ~sp.y, bit = 1u << lane;
-    if (hole & bit) moves[*hole_at + __popc(hole & below)].y = j + lane;
-    if (mover & bit) moves[*mover_at + __popc(mover & below)].x = j + lane;
+    if (hole & bit) moves[hole0 + __popc(hole & below)].y = j + lane;
+    if (mover & bit) moves[mover0 + __popc(mover & below)].x = j + lane;
     if (k & sp.y & bit) {
-      mass_out[j + lane] = mass_j;
-      pos_out[j + lane] = pos_j;
+      mass_out[j + lane] = mass[j + lane];
+      pos_out[j + lane] = pos[j + lane];
     }
-    *hole_at += __popc(hole);
-    *mover_at += __popc(mover);
+    hole0 += __popc(hole);
+    mover0 += __popc(mover);
   };
+  rank_eq = equal0;
 #pragma unroll
-  for (int i = 0; i < EVICT_HELD; ++i) list(w0 + 32 * i, kept[i], m[i], ps[i], &hole0, &mover0);
-  rank_eq = rank_rest;
-  for (int j = rest; j < w1; j += 32) {
-    const bool there = j + lane < w1;
-    const float mj = there ? mass[j + lane] : 0.f;
-    const int pj = there ? pos[j + lane] : 0;
-    list(j, kept_of(there ? key_of(mj, pj) : 0u, &rank_eq), mj, pj, &hole0, &mover0);
-  }
+  for (int i = 0; i < EVICT_HELD; ++i) list(w0 + 32 * i, key[i]);
+  for (int j = rest; j < w1; j += 32) list(j, key_rest(j));
   if (cluster > 1) cluster_sync_all(); else __syncthreads();  // the list is complete
   for (int i = me; i < n_moves; i += all) {
     const int2 mv = __ldcg(moves + i);
