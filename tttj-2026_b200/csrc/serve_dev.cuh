@@ -80,6 +80,16 @@ __device__ __forceinline__ bool srv_nonfinite(uint32_t w) {
   constexpr uint32_t e = BF16 ? 0x7f80u : 0x7c00u;
   return (w & e) == e || ((w >> 16) & e) == e;
 }
+// z + w * 0 for two 16-bit floats.
+template <bool BF16>
+__device__ __forceinline__ uint32_t srv_fma_zero(uint32_t w, uint32_t z) {
+  uint32_t d;
+  if constexpr (BF16)
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(w), "r"(0u), "r"(z));
+  else
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(w), "r"(0u), "r"(z));
+  return d;
+}
 template <bool BF16>
 __device__ __forceinline__ float srv_to_float(uint32_t half_bits) {
   if constexpr (BF16) return __uint_as_float(half_bits << 16);

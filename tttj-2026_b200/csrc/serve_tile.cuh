@@ -27,6 +27,8 @@
 //
 // Every wait is bounded; a role that gives up records SRV_DEV_TIMEOUT and unwinds.
 #pragma once
+#include <type_traits>
+
 #include "attention_tc.cuh"
 #include "serve_dev.cuh"
 
@@ -389,7 +391,8 @@ __global__ void __launch_bounds__(TileSmem<HD>::THREADS, 1)
       ++vc;
       return true;
     };
-    // The next item's number is taken while this one is loaded, its entry right after.
+    // The next item's number is taken two tiles before this one is loaded (early enough to
+    // hide the counter's latency, late enough to go to a CTA that is free), its entry right after.
     auto take = [&] { return lane == 0 ? atomicAdd(p.plan.counters, 1) : 0; };
     auto fetch = [&](int it, int4* lo, int4* hi) {
       if (it < n_items) {
@@ -426,7 +429,6 @@ __global__ void __launch_bounds__(TileSmem<HD>::THREADS, 1)
           w.ns[t] = t0 < w.n ? max(0, min(steps, j1 * SM::SUB) - w.j0 * SM::SUB) : 0;
           w.n_kv = max(w.n_kv, (w.ns[t] + SM::SUB - 1) / SM::SUB);
         }
-        taken = take();
       }
       const int qb = k % QBUF;
       // Hand the item to a side: its query tile and the item's fields.
@@ -454,6 +456,7 @@ __global__ void __launch_bounds__(TileSmem<HD>::THREADS, 1)
       // waiting behind a V stage would make the next scores late.
       if (!publish(0)) break;
       for (int j = 0; j < w.n_kv; ++j) {
+        if (j == max(0, w.n_kv - 2)) taken = take();
         const int slot = (w.j0 + j) * ATC_BN + piece * cr;
         int page = 0, c1 = w.row0 + slot;
         if (paged) {  // fetched before the wait for the stage
@@ -639,24 +642,25 @@ __global__ void __launch_bounds__(TileSmem<HD>::THREADS, 1)
           const int keep = max(0, min(ATC_BN, wi.len - base));
           constexpr int ROW_BYTES = SM::BOX_COLS * 2;
           constexpr int CH = ROW_BYTES / 16;
-          bool odd = false;
+          uint32_t zero = 0;  // two sums of value x 0: NaN once a value was not finite
 #pragma unroll 1
           for (int x = 0; x < SM::NBOX; ++x) {
             const uint32_t vx = sV + vs * SM::KV_TILE + (uint32_t)(x * SM::BOX_BYTES);
-#pragma unroll 4
+#pragma unroll 8
             for (int i = lane; i < (p.s.causal ? keep * CH : 0); i += 32) {
               uint32_t w[4];
               asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                            : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
                            : "r"(vx + (uint32_t)(i * 16))
                            : "memory");
-              odd |= srv_nonfinite<BF16>(w[0]) | srv_nonfinite<BF16>(w[1]) | srv_nonfinite<BF16>(w[2]) |
-                     srv_nonfinite<BF16>(w[3]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) zero = srv_fma_zero<BF16>(w[e], zero);
             }
             for (int i = keep * CH + lane; i < ATC_BN * CH; i += 32)
               asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(vx + (uint32_t)(i * 16)), "r"(0u)
                            : "memory");
           }
+          const bool odd = srv_nonfinite<BF16>(zero);
           fence_proxy_async_smem();
           if (__any_sync(FULL, odd) && !noted) {
             noted = true;
@@ -730,6 +734,7 @@ __global__ void __launch_bounds__(TileSmem<HD>::THREADS, 1)
         continue;
       }
       const int row_lim = p.s.causal ? min(len - 1, first + rtok) : len - 1;
+      const int warp_lim_lo = __shfl_sync(0xffffffffu, row_lim, 0), warp_lim_hi = __shfl_sync(0xffffffffu, row_lim, 31);
       float m_run = -INFINITY;  // running max (log2 domain) used as the exp base
       float l_run = 0.f;
       for (int i = 0; i < n; ++i, ++c) {
@@ -750,21 +755,35 @@ __global__ void __launch_bounds__(TileSmem<HD>::THREADS, 1)
         // The scores are in registers: the buffer may take the next step's.
         tc_fence_before();
         arrive(bar_s_free + 8 * t);
-        const int k0 = key0 + i * KT;
-        if (k0 + KT - 1 > first) {
-          // Column e of this step is hidden when e > lim.
-          const int lim = row_lim - k0;
-#pragma unroll
-          for (int e = 0; e < KT; ++e)
-            if (e > lim) sv[e] = __float_as_uint(-INFINITY);
-        }
-        // Row max: independent chains of three-input maxima.
+        // 32 keys at a time: those that no row of the warp sees take no further part (on the
+        // diagonal half of them), those that some see are masked.  Column e of this step is
+        // hidden when e > lim; limits rise with the rows.
+        const int k0 = key0 + i * KT, lim = row_lim - k0, warp_hi = warp_lim_hi - k0, warp_lo = warp_lim_lo - k0;
+        const bool partly = KT - 1 > warp_lo;  // warp-uniform
         float pm[8];
+        if (!partly) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) pm[e] = __uint_as_float(sv[e]);
+          for (int e = 0; e < 8; ++e) pm[e] = __uint_as_float(sv[e]);
 #pragma unroll
-        for (int e = 8; e < KT; e += 2)
-          pm[(e >> 1) & 7] = srv_max3(pm[(e >> 1) & 7], __uint_as_float(sv[e]), __uint_as_float(sv[e + 1]));
+          for (int e = 8; e < KT; e += 2)
+            pm[(e >> 1) & 7] = srv_max3(pm[(e >> 1) & 7], __uint_as_float(sv[e]), __uint_as_float(sv[e + 1]));
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) pm[e] = -INFINITY;
+#pragma unroll
+          for (int q = 0; q < KT / 32; ++q) {
+            if (32 * q <= warp_hi) {
+              if (32 * q + 31 > warp_lo) {
+#pragma unroll
+                for (int e = 32 * q; e < 32 * q + 32; ++e)
+                  if (e > lim) sv[e] = __float_as_uint(-INFINITY);
+              }
+#pragma unroll
+              for (int e = 32 * q; e < 32 * q + 32; e += 2)
+                pm[(e >> 1) & 7] = srv_max3(pm[(e >> 1) & 7], __uint_as_float(sv[e]), __uint_as_float(sv[e + 1]));
+            }
+          }
+        }
         const float mx =
             srv_max3(srv_max3(pm[0], pm[1], pm[2]), srv_max3(pm[3], pm[4], pm[5]), srv_max3(pm[6], pm[7], pm[7]));
         const float m_tile = mx * scale;
@@ -787,41 +806,43 @@ __global__ void __launch_bounds__(TileSmem<HD>::THREADS, 1)
         const float base = !(m_tile < INFINITY) ? NAN : m_run == -INFINITY ? 0.f : m_run;
         const float2 sc2 = make_float2(scale, scale), nb2 = make_float2(-base, -base);
         unsigned long long ps2[2] = {0ull, 0ull};  // partial row sums, f32x2 pairs
-        uint32_t pk[KT / 32][16];
-        // 32 keys' probabilities; one pair in four takes its exponentials from the FMA pipe
-        // (the MUFU is the tighter one).
-        auto exp_chunk = [&](int q) {
-          // Loop by loop, so that the MUFU's latencies overlap.
-          float2 x[16];
+        const uint32_t p_addr = p_addr0 + (uint32_t)(c % SM::PBUF) * (KT / 2);
+        auto exponentials = [&](auto part) -> bool {
+          uint32_t pk[KT / 32][16];
+          // 32 keys' probabilities; one pair in four takes its exponentials from the FMA pipe
+          // (the MUFU is the tighter one).
+          auto chunk = [&](int q) {
+            if (decltype(part)::value && 32 * q > warp_hi) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-            x[e] = ffma2(make_float2(__uint_as_float(sv[32 * q + 2 * e]), __uint_as_float(sv[32 * q + 2 * e + 1])),
-                         sc2, nb2);
+              for (int e = 0; e < 16; ++e) pk[q][e] = 0u;
+              return;
+            }
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if ((e & 3) != 3) x[e] = make_float2(ex2_approx(x[e].x), ex2_approx(x[e].y));
+            for (int cc = 0; cc < 16; ++cc) {
+              const int e = q * 16 + cc;
+              const float2 x =
+                  ffma2(make_float2(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1])), sc2, nb2);
+              const float2 y = (e & 3) == 3 ? exp2_fma2(x) : make_float2(ex2_approx(x.x), ex2_approx(x.y));
+              ps2[e & 1] = add2p(ps2[e & 1], pk2(y.x, y.y));
+              pk[q][cc] = srv_pack<BF16>(y.x, y.y);
+            }
+          };
+          // The P buffer is free once the P V that used it last is complete; with one buffer
+          // that is the previous step's, so half of the exponentials come before the wait.
+          constexpr int EARLY = SM::PBUF == 1 ? ATC_P_EARLY : 0;
 #pragma unroll
-          for (int e = 3; e < 16; e += 4) x[e] = exp2_fma2(x[e]);
+          for (int q = 0; q < EARLY; ++q) chunk(q);
+          if (c >= SM::PBUF && !pv_done(c - SM::PBUF)) return false;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            ps2[e & 1] = add2p(ps2[e & 1], pk2(x[e].x, x[e].y));
-            pk[q][e] = srv_pack<BF16>(x[e].x, x[e].y);
+          for (int q = 0; q < KT / 32; ++q) {
+            if (q >= EARLY) chunk(q);
+            tmem_st_32x32b_x16(p_addr + (uint32_t)(q * 16), pk[q]);
           }
+          return true;
         };
-        // The P buffer is free once the P V that used it last is complete; with one buffer
-        // that is the previous step's, so half of the exponentials come before the wait.
-        constexpr int EARLY = SM::PBUF == 1 ? ATC_P_EARLY : 0;
-#pragma unroll
-        for (int q = 0; q < EARLY; ++q) exp_chunk(q);
-        if (c >= SM::PBUF && !pv_done(c - SM::PBUF)) {
+        if (!(partly ? exponentials(std::true_type{}) : exponentials(std::false_type{}))) {
           ok = false;
           break;
-        }
-        const uint32_t p_addr = p_addr0 + (uint32_t)(c % SM::PBUF) * (KT / 2);
-#pragma unroll
-        for (int q = 0; q < KT / 32; ++q) {
-          if (q >= EARLY) exp_chunk(q);
-          tmem_st_32x32b_x16(p_addr + (uint32_t)(q * 16), pk[q]);
         }
         const float2 rs2 = upk2(add2p(ps2[0], ps2[1]));
         l_run = l_run * alpha + (rs2.x + rs2.y);
@@ -875,6 +896,8 @@ __global__ void __launch_bounds__(TileSmem<HD>::THREADS, 1)
         if (live && p.lse != nullptr)
           p.lse[(long)token * p.heads + h * p.group + rhead] = srv_lse(m_run, l_run);
         uint16_t* out = static_cast<uint16_t*>(p.out);
+        // Where this row goes, -1: nowhere.
+        const long row_at = live ? (long)token * p.o_tok + (long)(h * p.group + rhead) * p.o_head : -1;
         if constexpr (SM::STAGED_EPI) {
           // The warp's 32 rows go through shared memory so that the stores cover whole
           // row segments (16-byte chunk j of row r staged at slot j ^ (r % NCH)).
@@ -910,15 +933,12 @@ __global__ void __launch_bounds__(TileSmem<HD>::THREADS, 1)
                          : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                          : "r"(a)
                          : "memory");
-            const int r2 = quad * 32 + rr;
-            const int tk = r2 / p.group, hd = r2 - tk * p.group;
-            if (tk < TOK && tok0 + tk < tokens)
-              *reinterpret_cast<uint4*>(out + (long)(token - rtok + tk) * p.o_tok +
-                                        (long)(h * p.group + hd) * p.o_head + j * 8) = v;
+            const long to = __shfl_sync(0xffffffffu, row_at, rr);
+            if (to >= 0) *reinterpret_cast<uint4*>(out + to + j * 8) = v;
           }
         } else {
           // Wide heads: each thread stores its own row, 64 bytes per 32 columns.
-          uint16_t* dst = out + (long)token * p.o_tok + (long)(h * p.group + rhead) * p.o_head;
+          uint16_t* dst = out + row_at;
 #pragma unroll 1
           for (int c = 0; c < HD / 32; ++c) {
             uint32_t o[32];
