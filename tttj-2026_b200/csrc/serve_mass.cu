@@ -14,7 +14,7 @@ cudaError_t launch(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const MassP
   const int smem = MassSmem<HD>::FIXED + p.s.batch * ((int)sizeof(SrvSeq) + 8) + 4;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  return launch_pdl(kern, dim3(grid), dim3(mass_threads(MassSmem<HD>::NT)), smem, stream, tm_q, tm_k, p);
+  return launch_pdl(kern, dim3(grid), dim3(MASS_THREADS), smem, stream, tm_q, tm_k, p);
 }
 }  // namespace
 

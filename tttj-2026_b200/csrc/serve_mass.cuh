@@ -11,9 +11,9 @@
 // that have work in turn (each computes the sequences' prefix sums itself), and share the
 // copying of the rest.  One warp loads K tiles (KBUF items ahead), another the query tiles with
 // their log-sum-exps (one warp for both made every item wait for page numbers and then for
-// log-sum-exps: 46 against 38 us at 32 sequences of 1000 - 4096 keys), one per key tile issues
-// its MMAs into three accumulators in turn, and two warpgroups per key tile add every other query
-// tile; their sums meet at the end of an item.
+// log-sum-exps: 46 against 38 us at 32 sequences of 1000 - 4096 keys), one issues
+// the MMAs into three accumulators per key tile in turn, and a warpgroup per accumulator adds, two keys per
+// thread; their sums meet at the end of an item.
 // For single tokens the bytes of K bound it; for chunks the exponentials and the products.
 #pragma once
 #include "attention_tc.cuh"
@@ -43,14 +43,14 @@ struct MassSmem {
   static constexpr int Q_BYTES = STAGES * Q_TILE;
   static constexpr int COLS = 4;                      // query tiles whose columns' data are held
   static constexpr int COL_BYTES = COLS * MASS_COLS * 8;    // (-lse, last key) of every query row
-  static constexpr int NBAR = 2 * KBUF + 2 * STAGES + 2 * COLS + 4 * MASS_BUFS + 2 + 8;
-  static constexpr int XCH_BYTES = NT * 2 * ATC_BM * 4;  // [tile][item parity][key] sums of the second warpgroup
+  static constexpr int NBAR = 2 * KBUF + 2 * STAGES + 2 * COLS + 2 * MASS_BUFS + 1 + 4;
+  static constexpr int XCH_BYTES = 2 * (MASS_BUFS - 1) * NT * ATC_BM * 4;  // [item parity][warpgroup][key] sums
   static constexpr int FIXED = K_BYTES + Q_BYTES + COL_BYTES + XCH_BYTES + NBAR * 8 + 16 + 1024;
 };
-// Warps: two warpgroups that add per key tile (each takes every other query tile, one accumulator
-// each), the key loader, the MMA issuers, the query loader.
-constexpr int mass_adders(int nt) { return 8 * nt; }
-constexpr int mass_threads(int nt) { return 32 * (mass_adders(nt) + 2 + nt); }
+// Warps: one warpgroup per accumulator that adds (both key tiles of an item, so the columns' data
+// and the bookkeeping serve two keys per thread), the key loader, the MMA issuer, the query loader.
+constexpr int MASS_ADDERS = 12;
+constexpr int MASS_THREADS = 32 * (MASS_ADDERS + 3);
 
 #ifndef MASS_FMA_PAIRS
 #define MASS_FMA_PAIRS 2
@@ -75,12 +75,12 @@ struct MassItem {
 };
 
 template <int HD, bool BF16>
-__global__ void __launch_bounds__(mass_threads(MassSmem<HD>::NT), 1)
+__global__ void __launch_bounds__(MASS_THREADS, 1)
     mass_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                 const MassParams p) {
   using SM = MassSmem<HD>;
   constexpr int NT = SM::NT;
-  constexpr int KEYS = mass_adders(NT), ISSUER = KEYS + 1, QUERIES = ISSUER + NT;  // warps
+  constexpr int KEYS = MASS_ADDERS, ISSUER = KEYS + 1, QUERIES = ISSUER + 1;  // warps
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   uint8_t* smem = smem_raw + ((1024u - (raw & 1023u)) & 1023u);
@@ -96,11 +96,11 @@ __global__ void __launch_bounds__(mass_threads(MassSmem<HD>::NT), 1)
   const uint32_t bar_q_empty = bar_q_full + 8 * SM::STAGES;  // [STAGES]
   const uint32_t bar_c_full = bar_q_empty + 8 * SM::STAGES;  // [COLS]
   const uint32_t bar_c_empty = bar_c_full + 8 * SM::COLS;    // [COLS]
-  const uint32_t bar_s_full = bar_c_empty + 8 * SM::COLS;    // [side][MASS_BUFS]
-  const uint32_t bar_s_free = bar_s_full + 16 * MASS_BUFS;   // [side][MASS_BUFS]
-  const uint32_t bar_x_full = bar_s_free + 16 * MASS_BUFS;               // [side][2] second warpgroup's sums
-  const uint32_t bar_x_free = bar_x_full + 32;               // [side][2] read by the first
-  const uint32_t bar_drain = bar_x_free + 32;                // [side]
+  const uint32_t bar_s_full = bar_c_empty + 8 * SM::COLS;    // [MASS_BUFS]
+  const uint32_t bar_s_free = bar_s_full + 8 * MASS_BUFS;    // [MASS_BUFS]
+  const uint32_t bar_x_full = bar_s_free + 8 * MASS_BUFS;   // [item parity] the other warpgroups' sums
+  const uint32_t bar_x_free = bar_x_full + 16;               // [item parity] read by the first
+  const uint32_t bar_drain = bar_x_free + 16;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + SM::K_BYTES + SM::Q_BYTES + SM::COL_BYTES + SM::XCH_BYTES +
                                                       SM::NBAR * 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -116,26 +116,25 @@ __global__ void __launch_bounds__(mass_threads(MassSmem<HD>::NT), 1)
     tma_prefetch_desc(&tmK);
     for (int i = 0; i < SM::KBUF; ++i) {
       mbar_init(bar_k_full + 8 * i, 1);
-      mbar_init(bar_k_empty + 8 * i, NT);
+      mbar_init(bar_k_empty + 8 * i, 1);
     }
     for (int i = 0; i < SM::STAGES; ++i) {
       mbar_init(bar_q_full + 8 * i, 1);
-      mbar_init(bar_q_empty + 8 * i, NT);
+      mbar_init(bar_q_empty + 8 * i, 1);
     }
     for (int i = 0; i < SM::COLS; ++i) {
       mbar_init(bar_c_full + 8 * i, 1);
-      mbar_init(bar_c_empty + 8 * i, 4 * NT);
+      mbar_init(bar_c_empty + 8 * i, 4);
     }
-    for (int i = 0; i < 2 * MASS_BUFS; ++i) {
+    for (int i = 0; i < MASS_BUFS; ++i) {
       mbar_init(bar_s_full + 8 * i, 1);
       mbar_init(bar_s_free + 8 * i, 4);
     }
-    for (int i = 0; i < 4; ++i) {
-      mbar_init(bar_x_full + 8 * i, 4);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar_x_full + 8 * i, 4 * (MASS_BUFS - 1));
       mbar_init(bar_x_free + 8 * i, 4);
     }
     mbar_init(bar_drain, 1);
-    mbar_init(bar_drain + 8, 1);
     *abort_flag = 0;
     fence_barrier_init();
     fence_proxy_async_smem();
@@ -211,21 +210,31 @@ __global__ void __launch_bounds__(mass_threads(MassSmem<HD>::NT), 1)
     const uint32_t dst = (uint32_t)(key / ATC_BM * SM::TILE + x * SM::BOX_BYTES + (key % ATC_BM) * SM::BOX_COLS * 2);
     bool ok = true;
     long kc = 0;
-    for (long r = 0, i; (i = item_at(r)) < items && ok; ++r) {
+    MassRing<SM::KBUF> kr;
+    // Page numbers are fetched an item ahead.
+    int slot = 0, page = p.s.num_pages, head = 0;
+    auto fetch = [&](long i) {
       const MassItem w = decode(i);
-      const int slot = w.k0 + key;
-      int page = p.s.num_pages;
-      if (lane < boxes && slot < w.q.len) page = srv_page(p.s, w.b, slot);
-      const int kb = (int)(kc % SM::KBUF);
-      ok = __all_sync(0xffffffffu, srv_wait(bar_k_empty + 8 * kb, (uint32_t)((kc / SM::KBUF) & 1) ^ 1u, abort_flag, limit));
+      slot = w.k0 + key;
+      head = w.h;
+      page = lane < boxes && slot < w.q.len ? srv_page(p.s, w.b, slot) : p.s.num_pages;
+    };
+    long i = item_at(0);
+    if (i < items) fetch(i);
+    for (long r = 1; i < items; ++r) {
+      const int use_slot = slot, use_page = page, use_head = head;
+      i = item_at(r);
+      if (i < items) fetch(i);
+      ok = __all_sync(0xffffffffu, srv_wait(bar_k_empty + 8 * kr.at, kr.parity ^ 1u, abort_flag, limit));
       if (!ok) break;
-      if (lane == 0) mbar_arrive_expect_tx(bar_k_full + 8 * kb, NT * SM::TILE);
+      if (lane == 0) mbar_arrive_expect_tx(bar_k_full + 8 * kr.at, NT * SM::TILE);
       __syncwarp();
       if (lane < boxes)
-        tma_load_4d(sK + kb * NT * SM::TILE + dst, &tmK, bar_k_full + 8 * kb, x * SM::BOX_COLS,
-                    slot & ((1 << p.s.page_shift) - 1), w.h, page);
+        tma_load_4d(sK + kr.at * NT * SM::TILE + dst, &tmK, bar_k_full + 8 * kr.at, x * SM::BOX_COLS,
+                    use_slot & ((1 << p.s.page_shift) - 1), use_head, use_page);
       __syncwarp();
       ++kc;
+      kr.next();
     }
     if (!ok && lane == 0) {
       *abort_flag = 1;
@@ -309,10 +318,11 @@ __global__ void __launch_bounds__(mass_threads(MassSmem<HD>::NT), 1)
       for (uint32_t j = qc > SM::STAGES ? qc - SM::STAGES : 0; j < qc; ++j)
         srv_wait(bar_q_full + 8 * (j % SM::STAGES), (j / SM::STAGES) & 1, nullptr, limit);
     }
-  } else if (warp >= ISSUER) {
-    // ------------------------------------------------------------ MMA issuers
+  } else if (warp == ISSUER) {
+    // ------------------------------------------------------------ MMA issuer
+    // One warp for both key tiles: with one each, the two warps' products interleave, end
+    // together, and the tensor core idles while both wait for their next operands.
     constexpr unsigned FULL = 0xffffffffu;
-    const int t = warp - ISSUER;
     bool ok = true, issued = false;
     MassRing<SM::KBUF> kr;
     MassRing<SM::STAGES> qr;
@@ -324,21 +334,25 @@ __global__ void __launch_bounds__(mass_threads(MassSmem<HD>::NT), 1)
     for (long r = 0, i; (i = item_at(r)) < items && ok; ++r) {
       const MassItem w = decode(i);
       if (!wait(bar_k_full + 8 * kr.at, kr.parity)) break;
-      const uint32_t kaddr = sK + (kr.at * NT + t) * SM::TILE;
+      const uint32_t kaddr = sK + kr.at * NT * SM::TILE;
+      int left = (w.q.n - w.first * TOK) * p.group;  // query rows from this tile on
       for (int s = 0; s < w.steps; ++s) {
-        const uint32_t buf = MASS_BUFS * t + sr.at;
-        if (!wait(bar_q_full + 8 * qr.at, qr.parity) || !wait(bar_s_free + 8 * buf, sr.parity ^ 1u)) break;
+        if (!wait(bar_q_full + 8 * qr.at, qr.parity) || !wait(bar_s_free + 8 * sr.at, sr.parity ^ 1u)) break;
         tc_fence_after();
-        const int rows = min(TOK, w.q.n - (w.first + s) * TOK) * p.group;
+        const int rows = min(TOK * p.group, left);
+        left -= TOK * p.group;
         const uint32_t idesc = idesc_f16_f32(ATC_BM, (rows + 15) / 16 * 16, 0, 0, BF16);
         const uint32_t qaddr = sQ + qr.at * SM::Q_TILE;
 #pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk) {
-          const uint64_t qd = HD == 32 ? desc_kmajor_sw64(qaddr) + (uint64_t)(2 * kk)
-                                       : desc_kmajor_sw128(qaddr + (uint32_t)((kk >> 2) * SM::Q_BOX)) + (uint64_t)(2 * (kk & 3));
-          mma_f16_ss_warp(tmem + (uint32_t)(buf * MASS_ROWS), atc_desc_qk<HD>(kaddr, kk), qd, idesc, kk > 0 ? 1u : 0u);
-        }
-        mma_commit_warp(bar_s_full + 8 * buf);
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int kk = 0; kk < HD / 16; ++kk) {
+            const uint64_t qd = HD == 32 ? desc_kmajor_sw64(qaddr) + (uint64_t)(2 * kk)
+                                         : desc_kmajor_sw128(qaddr + (uint32_t)((kk >> 2) * SM::Q_BOX)) + (uint64_t)(2 * (kk & 3));
+            mma_f16_ss_warp(tmem + (uint32_t)((MASS_BUFS * t + (int)sr.at) * MASS_ROWS),
+                            atc_desc_qk<HD>(kaddr + t * SM::TILE, kk), qd, idesc, kk > 0 ? 1u : 0u);
+          }
+        mma_commit_warp(bar_s_full + 8 * sr.at);
         mma_commit_warp(bar_q_empty + 8 * qr.at);
         issued = true;
         qr.next();
@@ -354,15 +368,15 @@ __global__ void __launch_bounds__(mass_threads(MassSmem<HD>::NT), 1)
         report_status(p.s.status, SRV_DEV_TIMEOUT);
       }
       if (issued) {
-        mma_commit_warp(bar_drain + 8 * t);
-        srv_wait(bar_drain + 8 * t, 0, nullptr, limit);
+        mma_commit_warp(bar_drain);
+        srv_wait(bar_drain, 0, nullptr, limit);
       }
     }
   } else {
     // ------------------------------------------------------------ adding warps
-    const int t = warp >> 3, u = (warp >> 2) & 1;  // key tile, query tiles of one parity
-    const int row = (warp & 3) * 32 + lane;
-    const uint32_t s_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t u = (uint32_t)warp >> 2;  // accumulator of this warpgroup: query tiles u, u + 3, ...
+    const int row = (warp & 3) * 32 + lane;  // key of each tile
+    const uint32_t s_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16) + u * MASS_ROWS;
     const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
     // Slots behind the items: copied while the first keys are on their way.
     if (p.out != p.mass) {
@@ -371,100 +385,119 @@ __global__ void __launch_bounds__(mass_threads(MassSmem<HD>::NT), 1)
         const SrvSeq q = s_seq[r / p.kv_heads];
         const long from = q.n > 0 ? (long)(q.len + ITEM_KEYS - 1) / ITEM_KEYS * ITEM_KEYS : 0;
 #pragma unroll 4
-        for (long j = from + threadIdx.x; j < p.cap; j += 32 * mass_adders(NT)) p.out[r * p.cap + j] = p.mass[r * p.cap + j];
+        for (long j = from + threadIdx.x; j < p.cap; j += 32 * MASS_ADDERS) p.out[r * p.cap + j] = p.mass[r * p.cap + j];
       }
     }
     bool ok = true;
-    uint32_t parity = 0;  // of the query tiles of earlier items
-    uint32_t xc = 0;      // items whose sums the two warpgroups exchanged
+    uint32_t xc = 0;  // items whose sums the warpgroups exchanged
     MassRing<SM::COLS> cr;
     MassRing<MASS_BUFS> sr;
     for (long r = 0, i; (i = item_at(r)) < items && ok; ++r) {
       const MassItem w = decode(i);
-      const int tile0 = w.k0 + t * ATC_BM;
-      const int key = tile0 + row;
+      const int key = w.k0 + row;  // and key + 128 of the second tile
       const long at = ((long)w.b * p.kv_heads + w.h) * p.cap + key;
-      // One query tile: its warpgroup writes the result; more: the first does, with both sums.
+      // One query tile: its warpgroup writes the result; more: the first does, with all sums.
       const bool alone = w.steps == 1;
-      const bool writes = alone ? parity == (uint32_t)u : u == 0;
-      const float old = writes && key < p.cap ? p.mass[at] : 0.f;
-      unsigned long long acc[4] = {0ull, 0ull, 0ull, 0ull};
-      for (int s = 0; s < w.steps; ++s, cr.next(), sr.next(), parity ^= 1) {
-        if (parity != (uint32_t)u) continue;
-        const uint32_t ct = cr.at, buf = MASS_BUFS * t + sr.at;
-        const uint32_t s_addr = s_base + buf * MASS_ROWS;
+      const bool writes = alone ? sr.at == u : u == 0;
+      float old[NT];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) old[t] = writes && key + t * ATC_BM < p.cap ? p.mass[at + t * ATC_BM] : 0.f;
+      unsigned long long acc[NT][4];
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[t][e] = 0ull;
+      for (int s = 0; s < w.steps; ++s, cr.next(), sr.next()) {
+        if (sr.at != u) continue;
         const int tok0 = (w.first + s) * TOK;
         const int rows = min(TOK, w.q.n - tok0) * p.group;
-        // Some row of this tile does not see some key of this one.
-        const bool partly = tile0 + ATC_BM - 1 > w.q.len - w.q.n + tok0;
-        if (!srv_wait(bar_c_full + 8 * ct, cr.parity, abort_flag, limit) ||
-            !srv_wait(bar_s_full + 8 * buf, sr.parity, abort_flag, limit)) {
+        // Some row of this tile does not see some key of the item.
+        const bool partly = w.k0 + ITEM_KEYS - 1 > w.q.len - w.q.n + tok0;
+        if (!srv_wait(bar_c_full + 8 * cr.at, cr.parity, abort_flag, limit) ||
+            !srv_wait(bar_s_full + 8 * u, sr.parity, abort_flag, limit)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        const float* nl = s_lse + ct * MASS_COLS;
-        const int* lim = s_lim + ct * MASS_COLS;
-        auto add = [&](auto& v, int c0) {
-          constexpr int N = sizeof(v) / 8;  // pairs
-          float2 x[N];
+        const float* nl = s_lse + cr.at * MASS_COLS;
+        const int* lim = s_lim + cr.at * MASS_COLS;
+#pragma unroll 1
+        for (int c0 = 0; c0 < rows; c0 += 16) {
+          uint32_t v[NT][16];
 #pragma unroll
-          for (int c = 0; c < N; c += 2) {
-            const float4 l4 = *reinterpret_cast<const float4*>(nl + c0 + 2 * c);
-            x[c] = ffma2(make_float2(__uint_as_float(v[2 * c]), __uint_as_float(v[2 * c + 1])), sc2, make_float2(l4.x, l4.y));
-            x[c + 1] = ffma2(make_float2(__uint_as_float(v[2 * c + 2]), __uint_as_float(v[2 * c + 3])), sc2, make_float2(l4.z, l4.w));
-          }
-          if (partly || c0 + 2 * N > rows) {
+          for (int t = 0; t < NT; ++t)
+            tmem_ld_32x32b_x16(s_addr + (uint32_t)(t * MASS_BUFS * MASS_ROWS + c0), v[t]);
+          float4 l4[4];
 #pragma unroll
-            for (int c = 0; c < N; c += 2) {
+          for (int c = 0; c < 4; ++c) l4[c] = *reinterpret_cast<const float4*>(nl + c0 + 4 * c);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) tmem_wait_ld_of(v[t]);
+          float2 x[NT][8];
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              x[t][2 * c] = ffma2(make_float2(__uint_as_float(v[t][4 * c]), __uint_as_float(v[t][4 * c + 1])), sc2,
+                                  make_float2(l4[c].x, l4[c].y));
+              x[t][2 * c + 1] = ffma2(make_float2(__uint_as_float(v[t][4 * c + 2]), __uint_as_float(v[t][4 * c + 3])),
+                                      sc2, make_float2(l4[c].z, l4[c].w));
+            }
+          if (partly || c0 + 16 > rows) {
+#pragma unroll
+            for (int c = 0; c < 8; c += 2) {
               const int4 m4 = *reinterpret_cast<const int4*>(lim + c0 + 2 * c);
-              x[c] = make_float2(key <= m4.x ? ex2_approx(x[c].x) : 0.f, key <= m4.y ? ex2_approx(x[c].y) : 0.f);
-              x[c + 1] = make_float2(key <= m4.z ? ex2_approx(x[c + 1].x) : 0.f, key <= m4.w ? ex2_approx(x[c + 1].y) : 0.f);
+#pragma unroll
+              for (int t = 0; t < NT; ++t) {
+                const int k = key + t * ATC_BM;
+                x[t][c] = make_float2(k <= m4.x ? ex2_approx(x[t][c].x) : 0.f, k <= m4.y ? ex2_approx(x[t][c].y) : 0.f);
+                x[t][c + 1] = make_float2(k <= m4.z ? ex2_approx(x[t][c + 1].x) : 0.f,
+                                          k <= m4.w ? ex2_approx(x[t][c + 1].y) : 0.f);
+              }
             }
           } else {
             // Of every eight pairs, MASS_FMA_PAIRS take their exponentials from the FMA pipe.
 #pragma unroll
-            for (int c = 0; c < N; ++c)
-              x[c] = (c * MASS_FMA_PAIRS) % 8 < MASS_FMA_PAIRS ? exp2_fine2(x[c]) : make_float2(ex2_approx(x[c].x), ex2_approx(x[c].y));
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+              for (int c = 0; c < 8; ++c)
+                x[t][c] = (c * MASS_FMA_PAIRS) % 8 < MASS_FMA_PAIRS ? exp2_fine2(x[t][c])
+                                                                   : make_float2(ex2_approx(x[t][c].x), ex2_approx(x[t][c].y));
           }
 #pragma unroll
-          for (int c = 0; c < N; ++c) acc[c & 3] = add2p(acc[c & 3], pk2(x[c].x, x[c].y));
-        };
-#pragma unroll 1
-        for (int c0 = 0; c0 < min(rows, 64); c0 += 32) {
-          uint32_t v[32];
-          tmem_ld_32x32b_x32(s_addr + (uint32_t)c0, v);
-          tmem_wait_ld_of(v);
-          add(v, c0);
-        }
-        if (rows > 64) {
-          uint32_t v[16];
-          tmem_ld_32x32b_x16(s_addr + 64, v);
-          tmem_wait_ld_of(v);
-          add(v, 64);
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int c = 0; c < 8; ++c) acc[t][c & 3] = add2p(acc[t][c & 3], pk2(x[t][c].x, x[t][c].y));
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(bar_s_free + 8 * buf);
-          mbar_arrive(bar_c_empty + 8 * ct);
+          mbar_arrive(bar_s_free + 8 * u);
+          mbar_arrive(bar_c_empty + 8 * cr.at);
         }
       }
       if (!ok) break;
-      const float2 a = upk2(add2p(add2p(acc[0], acc[1]), add2p(acc[2], acc[3])));
-      float sum = a.x + a.y;
+      float sum[NT];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const float2 a = upk2(add2p(add2p(acc[t][0], acc[t][1]), add2p(acc[t][2], acc[t][3])));
+        sum[t] = a.x + a.y;
+      }
       if (!alone) {
-        // The second warpgroup hands its sum over, through one of two buffers in turn.
-        const uint32_t xb = 2 * t + (xc & 1), turn = xc >> 1;
-        float* x = s_xch + xb * ATC_BM + row;
-        if (u == 1) {
+        // The other warpgroups hand their sums to the first, through one of two buffers in turn.
+        const uint32_t xb = xc & 1, turn = xc >> 1;
+        float* x = s_xch + xb * (MASS_BUFS - 1) * ITEM_KEYS + row;
+        if (u != 0) {
           if (turn > 0 && !srv_wait(bar_x_free + 8 * xb, (turn - 1) & 1, abort_flag, limit)) ok = false;
-          *x = sum;
+#pragma unroll
+          for (int t = 0; t < NT; ++t) x[(u - 1) * ITEM_KEYS + t * ATC_BM] = sum[t];
           __syncwarp();
           if (lane == 0) mbar_arrive(bar_x_full + 8 * xb);
         } else {
           if (!srv_wait(bar_x_full + 8 * xb, turn & 1, abort_flag, limit)) ok = false;
-          sum += *x;
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int o = 0; o < MASS_BUFS - 1; ++o) sum[t] += x[o * ITEM_KEYS + t * ATC_BM];
           __syncwarp();
           if (lane == 0) mbar_arrive(bar_x_free + 8 * xb);
         }
@@ -472,7 +505,13 @@ __global__ void __launch_bounds__(mass_threads(MassSmem<HD>::NT), 1)
         if (!ok) break;
         ++xc;
       }
-      if (writes && key < p.cap) p.out[at] = key < w.q.len ? old + sum : old;
+      if (writes) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const int k = key + t * ATC_BM;
+          if (k < p.cap) p.out[at + t * ATC_BM] = k < w.q.len ? old[t] + sum[t] : old[t];
+        }
+      }
     }
     if (!ok) {
       *abort_flag = 1;
