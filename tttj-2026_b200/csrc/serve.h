@@ -102,6 +102,7 @@ struct TileEntry {    // one item of every key/value head
 static_assert(sizeof(TileEntry) == 32, "entries are read as two 16-byte words");
 struct TileJoin {     // an entry whose keys were split
   int b, q, pieces, part;  // piece i of head h is slot part + i * kv_heads + h
+  int row0, n, pad[2];     // of the sequence
 };
 struct TilePlan {     // in the workspace, rebuilt by every call
   int* counters;      // [4]: items taken, entries, joins, items to redo

@@ -17,7 +17,7 @@ cudaError_t launch(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUten
   if (e != cudaSuccess) return e;
   e = launch_pdl(kern, dim3(grid), dim3(TileSmem<HD>::THREADS), smem, stream, tm_q, tm_k, tm_v, p);
   if (e != cudaSuccess) return e;
-  return launch_pdl(tile_join_kernel<HD, BF16>, dim3(4 * grid), dim3(32 * TILE_JOIN_WARPS), 0, stream, p);
+  return launch_pdl(tile_join_kernel<HD, BF16>, dim3(8 * grid), dim3(32 * TILE_JOIN_WARPS), 0, stream, p);
 }
 }  // namespace
 

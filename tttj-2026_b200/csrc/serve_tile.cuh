@@ -210,7 +210,8 @@ __global__ void __launch_bounds__(TILE_PLAN_THREADS) tile_plan_kernel(const Tile
   };
   auto pieces_of = [&](int e, int t) {
     const int c = e >= whole ? min(most, most_rest) : most;
-    return (t + c - 1) / c;
+    // A whole item a little above the fair share costs less than its pieces' joining.
+    return e < whole && t <= most + most / 4 ? 1 : (t + c - 1) / c;
   };
   auto bucket = [&](int len) { return TILE_BUCKETS - min(len, TILE_BUCKETS); };  // longest first
   for (int e = tid; e < items; e += TILE_PLAN_THREADS) {
@@ -255,7 +256,7 @@ __global__ void __launch_bounds__(TILE_PLAN_THREADS) tile_plan_kernel(const Tile
     int part = -1;
     if (n > 1) {
       part = atomicAdd(&s_parts, n * p.kv_heads);
-      p.plan.joins[atomicAdd(&s_joins, 1)] = TileJoin{out.b, out.q, n, part};
+      p.plan.joins[atomicAdd(&s_joins, 1)] = TileJoin{out.b, out.q, n, part, out.row0, out.n, {0, 0}};
     }
     const int at = add_to(bucket((t + n - 1) / n), n);
     for (int i = 0; i < n; ++i) {
@@ -996,6 +997,28 @@ __device__ __forceinline__ void tile_store_row(const TileParams& p, int token, i
 
 constexpr int TILE_JOIN_WARPS = 8;
 
+// This lane's HD / 32 neighbouring values of a row.
+template <int HD>
+__device__ __forceinline__ void tile_load_part(const float* row, float (&o)[HD / 32]) {
+  const float* at = row + lane_id() * (HD / 32);
+  if constexpr (HD == 32) {
+    o[0] = *at;
+  } else if constexpr (HD == 64) {
+    const float2 v = *reinterpret_cast<const float2*>(at);
+    o[0] = v.x;
+    o[1] = v.y;
+  } else {
+#pragma unroll
+    for (int x = 0; x < HD / 32; x += 4) {
+      const float4 v = *reinterpret_cast<const float4*>(at + x);
+      o[x] = v.x;
+      o[x + 1] = v.y;
+      o[x + 2] = v.z;
+      o[x + 3] = v.w;
+    }
+  }
+}
+
 // One row key by key, hidden keys left out: for items in which a hidden value is infinite
 // or NaN.
 template <int HD, bool BF16>
@@ -1056,35 +1079,55 @@ __global__ void __launch_bounds__(32 * TILE_JOIN_WARPS) tile_join_kernel(const T
   const int redo = min(p.plan.counters[3], 2 * p.plan.most_entries * p.kv_heads);
   const int lane = lane_id();
   const long w0 = (long)blockIdx.x * TILE_JOIN_WARPS + warp_id(), step = (long)gridDim.x * TILE_JOIN_WARPS;
-  for (long i = w0; i < (long)joins * p.kv_heads * ROWS; i += step) {
-    const int r = (int)(i % ROWS);
-    const int h = (int)(i / ROWS % p.kv_heads);
-    const TileJoin e = p.plan.joins[i / ROWS / p.kv_heads];
-    const int rtok = (r % ATC_BM) / p.group, g = (r % ATC_BM) - rtok * p.group;
-    const int tok = (e.q * NT + r / ATC_BM) * p.tile_tokens + rtok;
-    const SrvSeq s = srv_seq(p.s, e.b);
-    if (rtok >= p.tile_tokens || tok >= s.n) continue;
+  // Four rows per warp at a time, their loads in flight together.
+  constexpr int R = 4;
+  for (long i = w0; i < (long)joins * p.kv_heads * (ROWS / R); i += step) {
+    const int r0 = (int)(i % (ROWS / R)) * R;
+    const int h = (int)(i / (ROWS / R) % p.kv_heads);
+    const TileJoin e = p.plan.joins[i / (ROWS / R) / p.kv_heads];
+    const int tok0 = (e.q * NT + r0 / ATC_BM) * p.tile_tokens;
+    if ((r0 % ATC_BM) / p.group >= p.tile_tokens || tok0 + (r0 % ATC_BM) / p.group >= e.n) continue;
     bool noted = false;
     for (int c = 0; c < redo; ++c)
       noted |= p.plan.redo[3 * c] == e.b && p.plan.redo[3 * c + 1] == e.q && p.plan.redo[3 * c + 2] == h;
     if (noted) continue;
-    auto at = [&](int piece) { return ((long)e.part + (long)piece * p.kv_heads + h) * ROWS + r; };
-    float top = -INFINITY;
-    for (int c = lane; c < e.pieces; c += 32) top = fmaxf(top, p.part_ml[at(c)].x);
+    auto at = [&](int piece) { return ((long)e.part + (long)piece * p.kv_heads + h) * ROWS + r0; };
+    float top[R], sum[R], acc[R][HD / 32];
 #pragma unroll
-    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    float acc[HD / 32], sum = 0.f;
+    for (int x = 0; x < R; ++x) {
+      top[x] = -INFINITY;
+      sum[x] = 0.f;
 #pragma unroll
-    for (int x = 0; x < HD / 32; ++x) acc[x] = 0.f;
-    for (int c = 0; c < e.pieces; ++c) {
-      const float2 ml = p.part_ml[at(c)];
-      const float f = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - top);
-      sum += ml.y * f;
-      if (ml.x == -INFINITY && ml.y == 0.f) continue;  // nothing was stored for it
-#pragma unroll
-      for (int x = 0; x < HD / 32; ++x) acc[x] += p.part_o[at(c) * HD + lane * (HD / 32) + x] * f;
+      for (int y = 0; y < HD / 32; ++y) acc[x][y] = 0.f;
     }
-    tile_store_row<HD, BF16>(p, s.row0 + tok, h * p.group + g, acc, sum == 0.f ? 0.f : 1.f / sum, top, sum);
+    for (int c = 0; c < e.pieces; ++c) {
+#pragma unroll
+      for (int x = 0; x < R; ++x) top[x] = fmaxf(top[x], p.part_ml[at(c) + x].x);
+    }
+    for (int c = 0; c < e.pieces; ++c) {
+      float2 ml[R];
+      float o[R][HD / 32];
+#pragma unroll
+      for (int x = 0; x < R; ++x) {
+        ml[x] = p.part_ml[at(c) + x];
+        tile_load_part<HD>(p.part_o + (at(c) + x) * HD, o[x]);  // (rows of empty pieces hold anything)
+      }
+#pragma unroll
+      for (int x = 0; x < R; ++x) {
+        const float f = ml[x].x == -INFINITY ? 0.f : ex2_approx(ml[x].x - top[x]);
+        sum[x] += ml[x].y * f;
+        const bool none = ml[x].x == -INFINITY && ml[x].y == 0.f;
+#pragma unroll
+        for (int y = 0; y < HD / 32; ++y) acc[x][y] += none ? 0.f : o[x][y] * f;
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < R; ++x) {
+      const int rtok = (r0 % ATC_BM + x) / p.group, g = r0 % ATC_BM + x - rtok * p.group;
+      if (rtok < p.tile_tokens && tok0 + rtok < e.n)
+        tile_store_row<HD, BF16>(p, e.row0 + tok0 + rtok, h * p.group + g, acc[x], sum[x] == 0.f ? 0.f : 1.f / sum[x],
+                                 top[x], sum[x]);
+    }
   }
   // Items with a hidden infinite or NaN value (left out above where they were also cut).
   for (long i = w0; i < (long)redo * ROWS; i += step) {
