@@ -235,7 +235,6 @@ def test_cache_attention_rows_that_see_nothing():
 def test_cache_attention_nonfinite_values_reach_only_rows_that_see_them(new):
     lens = [131, 80]
     c = Cache(lens, 2, 128, 16, torch.bfloat16, 8)
-    last = cache_rows  # noqa: F841
     j = 129  # seen by the last two new tokens of the first sequence only
     c.v[c.table[0, j // 16].long(), j % 16, 1, 77] = math.nan
     c.v[c.table[0, (j + 1) // 16].long(), (j + 1) % 16, 0, 3] = -math.inf
@@ -533,6 +532,244 @@ def test_cache_mass_of_no_tokens_copies():
     lse = torch.zeros(0, 4, device=DEV)
     got = ops.cache_mass(q, lse, c.k, c.table, lengths_to_offsets([0]), c.lens, mass)
     assert torch.equal(got, mass)
+
+
+# --------------------------------------------------------------------- edges of every call
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d,new", [(64, [60, 50]), (128, [60, 50]), (128, [2, 3])])
+def test_hidden_largest_values_do_not_count(dtype, d, new):
+    """The type's largest number as a value that only the last token sees."""
+    lens = [131, 80]
+    c = Cache(lens, 2, d, 16, dtype, 8)
+    for b, m in enumerate(lens):
+        c.v[c.table[b, (m - 1) // 16].long(), (m - 1) % 16] = torch.finfo(dtype).max
+    q = torch.randn(sum(new), 8, d, device=DEV, generator=_gen(5)).to(dtype)
+    out, lse = ops.cache_attention(q, c.k, c.v, c.table, lengths_to_offsets(new), c.lens, return_lse=True)
+    at = 0
+    for b, (n, m) in enumerate(zip(new, lens)):
+        s = slice(at, at + n - 1)  # all rows but the last, against keys without the last
+        _check(out[s], lse[s], q[s], cache_rows(c.k, c.table, b, m)[:-1], cache_rows(c.v, c.table, b, m)[:-1], n - 1,
+               m - 1, d**-0.5)
+        at += n
+
+
+@pytest.mark.parametrize("offsets", [[0, 40, 0, 40], [40, 40, 20, 0], [0, 1 << 30, -(1 << 30), 40]])
+def test_offsets_that_do_not_rise_are_contained(offsets):
+    """Results are nobody's, the status says so, and nothing outside the call is touched."""
+    c = Cache([48, 64, 33], 2, 64, 16, torch.float16, 8)
+    rows = torch.randn(60, 8, 64, device=DEV, generator=_gen(5)).half()
+    q, k, v = rows[10:50], rows[10:50, :2], rows[10:50, 2:4]
+    off = torch.tensor(offsets, dtype=torch.int32, device=DEV)
+    big = torch.full((60, 8, 64), 7.0, dtype=torch.float16, device=DEV)
+    mass = torch.ones(3, 2, c.table.shape[1] * 16, device=DEV)
+    lse = torch.zeros(40, 8, device=DEV)
+    kc, vc = c.k.clone(), c.v.clone()
+    for call in (lambda s: ops.prompt_attention(q, k, v, off, out=big[10:50], status=s),
+                 lambda s: ops.cache_attention(q, c.k, c.v, c.table, off, c.lens, out=big[10:50], status=s),
+                 lambda s: ops.cache_attention(q, c.k, c.v, c.table, off, c.lens, out=big[10:50], max_new=1, status=s),
+                 lambda s: ops.cache_mass(q, lse, c.k, c.table, off, c.lens, mass, status=s),
+                 lambda s: ops.cache_append(k, v, kc, vc, c.table, off, c.lens, status=s)):
+        status = torch.zeros(1, dtype=torch.int32, device=DEV)
+        call(status)
+        assert int(status) == 0x402
+    assert bool((big[:10] == 7).all()) and bool((big[50:] == 7).all())
+
+
+def test_batches_of_padding_only():
+    """Rows, but no sequence with tokens: outputs stay, masses are copied."""
+    c = Cache([48, 64], 2, 64, 16, torch.float16, 8)
+    q = torch.randn(70, 8, 64, device=DEV, generator=_gen(5)).half()
+    k = q[:, :2]
+    off, out = lengths_to_offsets([0, 0]), torch.full((70, 8, 64), 7.0, dtype=torch.float16, device=DEV)
+    mass = torch.rand(2, 2, c.table.shape[1] * 16, device=DEV)
+    before = c.k.clone()
+    ops.prompt_attention(q, k, k, off, out=out)
+    ops.cache_attention(q, c.k, c.v, c.table, off, c.lens, out=out)
+    ops.cache_attention(q, c.k, c.v, c.table, off, c.lens, out=out, max_new=1)
+    ops.cache_append(k, k, c.k, c.v, c.table, off, c.lens)
+    assert bool((out == 7).all())
+    assert torch.equal(c.k.view(torch.int16), before.view(torch.int16))
+    assert torch.equal(ops.cache_mass(q, torch.zeros(70, 8, device=DEV), c.k, c.table, off, c.lens, mass), mass)
+
+
+@pytest.mark.parametrize("new", [[1, 2, 1], [30, 1, 65]])
+def test_padded_cache_batches_and_strided_outputs(new):
+    lens = [90, 333, 70]
+    c = Cache(lens, 2, 64, 16, torch.bfloat16, 8)
+    t = sum(new)
+    q = torch.randn(t + 9, 4, 64, device=DEV, generator=_gen(5)).bfloat16()
+    q[t:] = math.nan
+    big = torch.full((t + 9, 6, 80), 7.0, dtype=torch.bfloat16, device=DEV)
+    off = lengths_to_offsets(new)
+    ws = torch.empty(ops.serve_workspace_bytes(5, t + 100, 4, 2, 64), dtype=torch.uint8, device=DEV)
+    out, lse = ops.cache_attention(q, c.k, c.v, c.table, off, c.lens, max_new=max(new), out=big[:, 1:5, 8:72],
+                                   return_lse=True, workspace=ws)
+    _check_cache(out[:t], lse[:t], q, c, new, lens, 0.125)
+    keep = torch.ones_like(big, dtype=torch.bool)
+    keep[:t, 1:5, 8:72] = False
+    assert bool((big[keep] == 7).all())
+    lse[t:] = math.nan
+    mass = torch.rand(3, 2, c.table.shape[1] * 16, device=DEV)
+    _check_mass(ops.cache_mass(q, lse, c.k, c.table, off, c.lens, mass), mass, q, lse, c, new, lens, 0.125)
+    want = c.k.clone()
+    kn = torch.randn(t + 9, 2, 64, device=DEV, generator=_gen(6)).bfloat16()
+    kn[t:] = math.nan
+    ops.cache_append(kn, kn, c.k, c.v, c.table, off, c.lens)
+    at = 0
+    for b, (n, m) in enumerate(zip(new, lens)):
+        for i in range(n):
+            j = m - n + i
+            want[c.table[b, j // 16].long(), j % 16] = kn[at + i]
+        at += n
+    assert torch.equal(c.k.view(torch.int16), want.view(torch.int16))
+
+
+def test_pages_shared_by_sequences():
+    """A common prefix: two tables list the same pages, one lists a page twice."""
+    c = Cache([96, 96, 96], 2, 64, 16, torch.float16, 8)
+    c.table[1, :4] = c.table[0, :4]
+    c.table[2, 3] = c.table[2, 1]
+    lens = [96, 90, 96]
+    c.lens = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    for new in ([1, 1, 1], [20, 40, 1]):
+        q = torch.randn(sum(new), 4, 64, device=DEV, generator=_gen(5)).half()
+        off = lengths_to_offsets(new)
+        out, lse = ops.cache_attention(q, c.k, c.v, c.table, off, c.lens, max_new=max(new), return_lse=True)
+        _check_cache(out, lse, q, c, new, lens, 0.125)
+        mass = torch.rand(3, 2, c.table.shape[1] * 16, device=DEV)
+        _check_mass(ops.cache_mass(q, lse, c.k, c.table, off, c.lens, mass), mass, q, lse, c, new, lens, 0.125)
+
+
+def test_the_most_sequences():
+    g = torch.Generator().manual_seed(3)
+    new = torch.randint(0, 4, (1024,), generator=g).tolist()
+    lens = [n + int(x) for n, x in zip(new, torch.randint(0, 40, (1024,), generator=g))]
+    new[1000], lens[1000] = 40, 70
+    c = Cache(lens, 1, 32, 16, torch.float16, 8)
+    q = torch.randn(sum(new), 2, 32, device=DEV, generator=_gen(5)).half()
+    off = lengths_to_offsets(new)
+    for hint in (1, 40):
+        out, lse = ops.cache_attention(q, c.k, c.v, c.table, off, c.lens, max_new=hint, return_lse=True)
+        _check_cache(out, lse, q, c, new, lens, 32**-0.5)
+    mass = torch.rand(1024, 1, c.table.shape[1] * 16, device=DEV)
+    _check_mass(ops.cache_mass(q, lse, c.k, c.table, off, c.lens, mass), mass, q, lse, c, new, lens, 32**-0.5)
+    pos = torch.arange(mass.shape[2], device=DEV, dtype=torch.int32).expand(mass.shape).contiguous()
+    _check_evict(c, mass, pos, lens, 9, 2)
+    out, lse = ops.prompt_attention(q, q[:, :1], q[:, 1:], off, return_lse=True)
+    at = 0
+    for n in new[:200] + [0]:
+        s = slice(at, at + n)
+        if n:
+            _check(out[s], lse[s], q[s], q[s, :1], q[s, 1:], n, n, 32**-0.5)
+        at += n
+
+
+def test_calls_at_the_same_time():
+    """Two streams, each with its own calls; results as alone."""
+    def work(seed):
+        c = Cache([700, 300, 1500], 2, 128, 32, torch.bfloat16, seed)
+        new = [200, 1, 90]
+        q = torch.randn(sum(new), 8, 128, device=DEV, generator=_gen(seed)).bfloat16()
+        off = lengths_to_offsets(new)
+        mass = torch.rand(3, 2, c.table.shape[1] * 32, device=DEV, generator=_gen(seed))
+        pos = torch.arange(mass.shape[2], device=DEV, dtype=torch.int32).expand(mass.shape).contiguous()
+
+        def run():
+            out, lse = ops.cache_attention(q, c.k, c.v, c.table, off, c.lens, max_new=200, return_lse=True)
+            one = ops.cache_attention(q[:3], c.k, c.v, c.table, lengths_to_offsets([1, 1, 1]), c.lens, max_new=1)
+            m = ops.cache_mass(q, lse, c.k, c.table, off, c.lens, mass)
+            own_k, own_v = c.k.clone(), c.v.clone()
+            m2, p2, l2 = ops.cache_evict(m, pos, own_k, own_v, c.table, c.lens, 256, recent=16)
+            pr = ops.prompt_attention(q, q[:, :2], q[:, 2:4], off)
+            return out, lse, one, m, m2, p2, l2, pr, own_k.view(torch.int16), own_v.view(torch.int16)
+        return run
+
+    runs = [work(1), work(2)]
+    want = [r() for r in runs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(5):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(runs[i]())
+    torch.cuda.synchronize()
+    for i in range(2):
+        for g in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(want[i], g))
+
+
+def test_captured_chunks_mass_and_eviction_follow_new_lengths():
+    kv, heads, d, page, cap = 2, 8, 64, 16, 256
+    c = Cache([cap] * 3, kv, d, page, torch.float16, 3)
+    off = lengths_to_offsets([100, 20, 30])
+    q = torch.zeros(150, heads, d, dtype=torch.float16, device=DEV)
+    mass = torch.zeros(3, kv, cap, device=DEV)
+    pos = torch.arange(cap, device=DEV, dtype=torch.int32).expand(3, kv, cap).contiguous()
+    ws = torch.empty(ops.serve_workspace_bytes(3, 150, heads, kv, d), dtype=torch.uint8, device=DEV)
+
+    def step():
+        out, lse = ops.cache_attention(q, c.k, c.v, c.table, off, c.lens, return_lse=True, workspace=ws)
+        prompt = ops.prompt_attention(q, q[:, :kv], q[:, kv:2 * kv], off, workspace=ws)
+        m = ops.cache_mass(q, lse, c.k, c.table, off, c.lens, mass)
+        return out, lse, prompt, m, *ops.cache_evict(m, pos, c.k, c.v, c.table, c.lens, 64, recent=8)
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for i, (new, lens) in enumerate([([100, 20, 30], [100, 256, 31]), ([1, 0, 140], [1, 77, 200]), ([5, 3, 2], [5, 3, 256])]):
+        g = _gen(20 + i)
+        q.copy_(torch.randn(q.shape, device=DEV, generator=g))
+        mass.copy_(torch.rand(mass.shape, device=DEV, generator=g))
+        c.lens.copy_(torch.tensor(lens))
+        off.copy_(lengths_to_offsets(new))
+        c.k.copy_(torch.randn(c.k.shape, device=DEV, generator=g))
+        c.v.copy_(torch.randn(c.v.shape, device=DEV, generator=g))
+        k0, v0 = c.k.clone(), c.v.clone()
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed, k1, v1 = [x.clone() for x in got], c.k.clone(), c.v.clone()
+        c.k.copy_(k0), c.v.copy_(v0)
+        t = sum(new)
+        _check_cache(replayed[0][:t], replayed[1][:t], q, c, new, lens, 0.125)
+        _check_mass(replayed[3], mass, q, replayed[1], c, new, lens, 0.125)
+        for j, (a, b) in enumerate(zip(replayed, step())):
+            assert torch.equal(a[:t], b[:t]) if j < 3 else torch.equal(a, b)
+        assert torch.equal(k1, c.k) and torch.equal(v1, c.v)
+
+
+def test_requires_grad_and_wide_integers():
+    c = Cache([20, 30], 2, 64, 16, torch.float16, 8)
+    q = torch.randn(2, 4, 64, device=DEV, generator=_gen(5)).half()
+    off = lengths_to_offsets([1, 1])
+    for name in ("q", "k", "v", "out"):
+        args = dict(q=q, k=q[:, :2], v=q[:, 2:], out=torch.empty_like(q))
+        args[name] = args[name].clone().requires_grad_()
+        with pytest.raises(ValueError, match="inference only"):
+            ops.prompt_attention(args["q"], args["k"], args["v"], off, out=args["out"])
+        with torch.no_grad():
+            ops.prompt_attention(args["q"], args["k"], args["v"], off, out=args["out"])
+    with pytest.raises(ValueError, match="inference only"):
+        ops.cache_attention(q, c.k, c.v.clone().requires_grad_(), c.table, off, c.lens)
+    mass = torch.rand(2, 2, c.table.shape[1] * 16, device=DEV)
+    with pytest.raises(ValueError, match="inference only"):
+        ops.cache_mass(q, torch.zeros(2, 4, device=DEV), c.k, c.table, off, c.lens, mass.clone().requires_grad_())
+    pos = torch.arange(mass.shape[2], device=DEV, dtype=torch.int32).expand(mass.shape).contiguous()
+    for keep, recent in ((2**32 + 1, 0), (2**31, 2**31)):
+        _check_evict(c, mass, pos, [20, 30], keep, recent)
+    for keep, recent in ((0, 0), (-(2**32) + 3, 0), (4, 5), (2**33, 2**34), (4, -1)):
+        with pytest.raises(ValueError, match="keep"):
+            ops.cache_evict(mass, pos, c.k, c.v, c.table, c.lens, keep, recent=recent)
+    want = ops.cache_attention(q, c.k, c.v, c.table, off, c.lens)
+    assert torch.equal(want, ops.cache_attention(q, c.k, c.v, c.table, off, c.lens, max_new=2**40))
+    with pytest.raises(ValueError, match="max_new"):
+        ops.cache_attention(q, c.k, c.v, c.table, off, c.lens, max_new=-1)
+    with pytest.raises(ValueError, match="1-D"):
+        ops.cache_attention(q, c.k, c.v, c.table, off, c.lens, workspace=torch.empty(2, 1 << 24, dtype=torch.uint8, device=DEV))
 
 
 # ---------------------------------------------------------------------------- all together

@@ -81,6 +81,18 @@ def test_evict_arguments_refused(kw, text):
     _refused(_evict(_seqs(), **kw), text)
 
 
+@pytest.mark.parametrize("kw,text", [
+    (dict(q=_rows(tok=0)), "q strides"), (dict(q=_rows(data=A + 8)), "q must be 16-byte"), (dict(lse=None), "null"),
+    (dict(kc=_pages(slot=0)), "k_cache strides"), (dict(mass=None), "null"), (dict(out=None), "null"),
+    (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(max_new=-1), "max_new"),
+    (dict(s=_seqs(batch=1025)), "batch"), (dict(s=_seqs(cache_lens=None)), "cache_lens"),
+])
+def test_mass_arguments_refused(kw, text):
+    a = dict(s=_seqs(), q=_rows(), lse=A, kc=_pages(), mass=A, out=A, max_new=0, scale=0.125) | kw
+    _refused(_lib.lib().tttj_cache_mass(ctypes.byref(a["s"]), a["q"], a["lse"], a["kc"], a["mass"], a["out"],
+                                        a["max_new"], a["scale"], None), text)
+
+
 def test_packed_arguments_have_the_c_layout():
     seqs = [A, 2 * A, 3 * A, 1 << 40, *range(1, 10), 4 * A]
     assert ops._pack_seqs(*seqs) == bytes(_lib.TttjSeqs(*seqs))
@@ -119,3 +131,5 @@ def test_wrappers_refuse_before_any_launch():
         ops.cache_append(k, k, cache[0], cache, off, off, off)
     with pytest.raises(ValueError, match="k_cache"):
         ops.cache_evict(cache, cache, cache[0], cache, off, off, 4)
+    with pytest.raises(ValueError, match="k_cache"):
+        ops.cache_mass(q, q, cache[0], off, off, off, q)

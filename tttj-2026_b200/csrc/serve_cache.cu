@@ -40,6 +40,9 @@ __global__ void __launch_bounds__(APPEND_THREADS, 5) append_kernel(const AppendP
     s_page[threadIdx.x] = page;
     s_first[threadIdx.x] = (p.seen != nullptr ? p.seen[lo] : q.len) - q.n + (t - q.row0);
   }
+  // Tokens look at their own sequence only: offsets that do not rise are found here.
+  if (p.s.status != nullptr && blockIdx.x == 0)
+    for (int b = threadIdx.x; b < p.s.batch; b += APPEND_THREADS) srv_seq(p.s, b);
   __syncthreads();
   const int per_head = p.head_dim / 8, per_tensor = p.kv_heads * per_head;
   const int groups = APPEND_THREADS / lanes, group = threadIdx.x / lanes;
@@ -86,7 +89,7 @@ __global__ void __launch_bounds__(APPEND_THREADS, 5) append_kernel(const AppendP
 // where it is needed).  The keep-th largest value is found two bits at a time: everyone
 // counts the values above three thresholds, the warps' counts meet in every block's shared
 // memory, 16 rounds of one barrier each.  (A radix selection with histograms in shared memory took
-// 77 thousand cycles of a cluster of 8 at 32768 slots, this SELECT.)  Then ballots rank the
+// 77 thousand cycles of a cluster of 8 at 32768 slots, this 23 thousand.)  Then ballots rank the
 // equal values, the holes (slots < keep that go) and the movers (slots >= keep that stay); the
 // i-th mover goes to the i-th hole, so as few rows move as can, and since sources lie behind
 // the budget and destinations in front of it, no move reads what another writes.  All counts are

@@ -52,9 +52,7 @@ struct MassSmem {
 constexpr int MASS_ADDERS = 12;
 constexpr int MASS_THREADS = 32 * (MASS_ADDERS + 3);
 
-#ifndef MASS_FMA_PAIRS
-#define MASS_FMA_PAIRS 2
-#endif
+constexpr int MASS_FMA_PAIRS = 2;  // of eight pairs of exponentials, those on the FMA pipe
 
 // Position in a ring of N stages: index and phase parity, without divisions.
 template <int N>

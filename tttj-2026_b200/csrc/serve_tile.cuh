@@ -12,9 +12,9 @@
 //                     longest items first.  An item is NT query tiles of one head.  Items
 //                     that would leave CTAs idle -- those of a last, partial wave, and any
 //                     longer than a CTA's fair share -- are cut along the keys.
-//   tile_kernel       persistent CTAs (1 per SM) of 12 warps take items in turn: a TMA
-//                     loader, one MMA-issuing warp and four softmax warps per query tile
-//                     (one thread per row), and a warp that prepares V tiles; running
+//   tile_kernel       persistent CTAs (1 per SM) take items in turn: a TMA loader; per query
+//                     tile four softmax warps (one thread per row) and one MMA-issuing warp,
+//                     at head_dim 128 two; and a warp that prepares V tiles; running
 //                     statistics in fp32, O rescaled only when a row's maximum grew by
 //                     more than 2^8.
 //   tile_join_kernel  joins the pieces of cut items in the order of their keys.
@@ -49,7 +49,7 @@ static_assert(sizeof(TileInfo) <= 64, "item info slot is 64 bytes");
 // and no product is waited for.  Measured there, prompts of 3001 and 4096 tokens, 32 / 8 heads:
 // steps of 128 keys with P written over S, as in attention_tc.cuh, 286 us (the next S waits for
 // P V); one score buffer of 128 keys that the tiles take in turn, 250 - 258 us; this with
-// one issuing warp per tile 257 us, with one for S and one for P V, SPLIT_US us.
+// one issuing warp per tile 257 us, with one for S and one for P V, 251 us.
 template <int HD>
 struct TileSmem : AtcSmem<HD> {  // tile sizes and stages as there
   using B = AtcSmem<HD>;
@@ -811,7 +811,8 @@ __global__ void __launch_bounds__(TileSmem<HD>::THREADS, 1)
         auto exponentials = [&](auto part) -> bool {
           uint32_t pk[KT / 32][16];
           // 32 keys' probabilities; one pair in four takes its exponentials from the FMA pipe
-          // (the MUFU is the tighter one).
+          // (the MUFU is the tighter one), but not where keys are hidden: exp2_fma2 ends at
+          // 2^-126, and a hidden key's probability has to be 0.
           auto chunk = [&](int q) {
             if (decltype(part)::value && 32 * q > warp_hi) {
 #pragma unroll
@@ -823,7 +824,8 @@ __global__ void __launch_bounds__(TileSmem<HD>::THREADS, 1)
               const int e = q * 16 + cc;
               const float2 x =
                   ffma2(make_float2(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1])), sc2, nb2);
-              const float2 y = (e & 3) == 3 ? exp2_fma2(x) : make_float2(ex2_approx(x.x), ex2_approx(x.y));
+              const float2 y = !decltype(part)::value && (e & 3) == 3 ? exp2_fma2(x)
+                                                                     : make_float2(ex2_approx(x.x), ex2_approx(x.y));
               ps2[e & 1] = add2p(ps2[e & 1], pk2(y.x, y.y));
               pk[q][cc] = srv_pack<BF16>(y.x, y.y);
             }
@@ -875,7 +877,7 @@ __global__ void __launch_bounds__(TileSmem<HD>::THREADS, 1)
         break;
       }
       tc_fence_after();
-      // A row that saw no key: exp2_fma2 leaves 2^-126 where the exponential of -inf is 0.
+      // A row of nothing but scores of -inf: exp2_fma2 leaves 2^-126 where their exponential is 0.
       if (m_run == -INFINITY && l_run == l_run) l_run = 0.f;
       if (part >= 0) {
         // A piece: raw sums, joined later.

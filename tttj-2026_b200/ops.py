@@ -150,6 +150,8 @@ def _serve_rows(what: str, name: str, t: torch.Tensor, shape: tuple, dtype: torc
     tok, head, one = t.stride()
     if one != 1:
         raise ValueError(f"{what}: head_dim of {name} must be contiguous")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what}: inference only ({name} requires a gradient)")
     return _pack_rows(t.data_ptr(), tok, head)
 
 
@@ -166,6 +168,8 @@ def _serve_pages(what: str, name: str, t: torch.Tensor, shape: tuple, dtype: tor
     page, slot, head, one = t.stride()
     if one != 1:
         raise ValueError(f"{what}: head_dim of {name} must be contiguous")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what}: inference only ({name} requires a gradient)")
     return _pack_pages(t.data_ptr(), page, slot, head)
 
 
@@ -175,8 +179,6 @@ def _serve_type(what: str, t: torch.Tensor) -> int:
         raise ValueError(f"{what}: dtype {t.dtype} unsupported (float16, bfloat16)")
     if not t.is_cuda:
         raise ValueError(f"{what}: tensors must be on a CUDA device")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{what}: inference only (no gradient)")
     return dtype
 
 
@@ -220,8 +222,9 @@ def serve_workspace_bytes(batch: int, tokens: int, heads: int, kv_heads: int, he
 def _serve_workspace(what: str, workspace: Optional[torch.Tensor], nbytes: int, device: torch.device) -> torch.Tensor:
     if workspace is None:
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
-    if workspace.dtype != torch.uint8 or workspace.device != device or not workspace.is_contiguous():
-        raise ValueError(f"{what}: workspace must be a contiguous uint8 tensor on {device}")
+    if workspace.dtype != torch.uint8 or workspace.device != device or workspace.dim() != 1 or \
+            not workspace.is_contiguous():
+        raise ValueError(f"{what}: workspace must be a contiguous 1-D uint8 tensor on {device}")
     return workspace
 
 
@@ -288,7 +291,7 @@ def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     lse = torch.empty((tokens, heads), dtype=torch.float32, device=device) if return_lse else None
     ws = _serve_workspace(what, workspace, _serve_workspace_bytes(batch, tokens, kind, heads, kv_heads, d), device)
     rc = _call(device, _lib.lib().tttj_cache_attention, s, rq, ck, cv, ro, lse.data_ptr() if return_lse else None,
-               max_new or 0, d ** -0.5 if scale is None else scale, ws.data_ptr(), ws.shape[0])
+               min(max_new or 0, tokens), d ** -0.5 if scale is None else scale, ws.data_ptr(), ws.shape[0])
     if rc:
         _lib.check(rc, what)
     return (out, lse) if return_lse else out
@@ -298,6 +301,8 @@ def _slot_tensor(what: str, name: str, t: torch.Tensor, dtype: torch.dtype, shap
     if t.dtype != dtype or t.shape != shape or t.device != device or not t.is_contiguous():
         raise ValueError(f"{what}: {name} must be a contiguous {dtype} tensor {list(shape)} "
                          f"(sequences, kv_heads, slots) on {device}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what}: inference only ({name} requires a gradient)")
     return t.data_ptr()
 
 
@@ -353,6 +358,9 @@ def cache_evict(mass: torch.Tensor, positions: torch.Tensor, k_cache: torch.Tens
     s, cap = _cache_seqs(what, None, batch, 0, kind, kv_heads, k_cache, page_table, cache_lens, status, device)
     ck = _serve_pages(what, "k_cache", k_cache, pages, dtype, device)
     cv = _serve_pages(what, "v_cache", v_cache, pages, dtype, device)
+    if keep <= 0 or not 0 <= recent <= keep:
+        raise ValueError(f"{what}: keep={keep} must be positive, recent={recent} in 0 .. keep")
+    keep, recent = min(keep, cap), min(recent, cap)  # (the C arguments have 32 bits)
     slots = (batch, kv_heads, cap)
     ms = _slot_tensor(what, "mass", mass, torch.float32, slots, device)
     pos = _slot_tensor(what, "positions", positions, torch.int32, slots, device)
@@ -400,7 +408,7 @@ def cache_mass(q: torch.Tensor, lse: torch.Tensor, k_cache: torch.Tensor, page_t
     mo = _slot_tensor(what, "out", out, torch.float32, slots, device)
     rq = _serve_rows(what, "q", q, rows, dtype, device)
     ck = _serve_pages(what, "k_cache", k_cache, pages, dtype, device)
-    rc = _call(device, _lib.lib().tttj_cache_mass, s, rq, lse.data_ptr(), ck, ms, mo, max_new or 0,
+    rc = _call(device, _lib.lib().tttj_cache_mass, s, rq, lse.data_ptr(), ck, ms, mo, min(max_new or 0, tokens),
                d ** -0.5 if scale is None else scale)
     if rc:
         _lib.check(rc, what)
