@@ -53,10 +53,10 @@ static_assert(sizeof(TileInfo) <= 64, "item info slot is 64 bytes");
 template <int HD>
 struct TileSmem : AtcSmem<HD> {  // tile sizes and stages as there
   using B = AtcSmem<HD>;
-  static constexpr bool SPLIT = HD == 128;        // S and P V issued by different warps
-  static constexpr int KT = HD == 128 ? 64 : 128;  // keys per step
+  static constexpr bool SPLIT = HD != 256;        // S and P V issued by different warps
+  static constexpr int KT = HD == 256 ? 128 : 64;  // keys per step
   static constexpr int SUB = ATC_BN / KT;          // steps per loaded key tile
-  static constexpr int PBUF = HD == 128 ? 2 : 1;
+  static constexpr int PBUF = HD == 256 ? 1 : 2;
   // Warps: four softmax warps per query tile (their number modulo four is their TMEM
   // quadrant), the loader, the MMA issuers, the cleaner.
   static constexpr int LOADER = 4 * B::NT, ISSUER = LOADER + 1;
@@ -541,6 +541,9 @@ __global__ void __launch_bounds__(TileSmem<HD>::THREADS, 1)
     auto do_s = [&](int i, int n, int qb) -> bool {
       const uint32_t idx = kvc + i / SM::SUB;
       if (sc > 0 && !wait(bar_s_free + 8 * t, (sc - 1) & 1)) return false;
+      // With two P buffers the softmax writes a step's P without a wait of its own: these scores
+      // come after the P V that used the buffer last.
+      if (SM::PBUF == 2 && sc >= 2 && !wait(bar_pv_done + 16 * t + 8 * (sc & 1), ((sc - 2) / 2) & 1)) return false;
       if (!ensure_k(idx)) return false;
       const uint32_t qaddr = sQ + (t * QBUF + qb) * SM::Q_TILE;
       const uint32_t kaddr = sK + (idx % STAGES) * SM::KV_TILE + (uint32_t)(i % SM::SUB) * sub_bytes;
@@ -803,49 +806,40 @@ __global__ void __launch_bounds__(TileSmem<HD>::THREADS, 1)
             rescale = true;  // warp-uniform
           }
         }
-        // A NaN or +inf score makes the whole row NaN (exp2_fma2 alone would lose it).
-        const float base = !(m_tile < INFINITY) ? NAN : m_run == -INFINITY ? 0.f : m_run;
+        const float base = m_run == -INFINITY ? 0.f : m_run;
         const float2 sc2 = make_float2(scale, scale), nb2 = make_float2(-base, -base);
         unsigned long long ps2[2] = {0ull, 0ull};  // partial row sums, f32x2 pairs
         const uint32_t p_addr = p_addr0 + (uint32_t)(c % SM::PBUF) * (KT / 2);
-        auto exponentials = [&](auto part) -> bool {
-          uint32_t pk[KT / 32][16];
-          // 32 keys' probabilities; one pair in four takes its exponentials from the FMA pipe
-          // (the MUFU is the tighter one), but not where keys are hidden: exp2_fma2 ends at
-          // 2^-126, and a hidden key's probability has to be 0.
-          auto chunk = [&](int q) {
-            if (decltype(part)::value && 32 * q > warp_hi) {
+        uint32_t pk[KT / 32][16];
+        auto chunk = [&](int q) {  // 32 keys' probabilities
+          if (32 * q > warp_hi) {
 #pragma unroll
-              for (int e = 0; e < 16; ++e) pk[q][e] = 0u;
-              return;
-            }
-#pragma unroll
-            for (int cc = 0; cc < 16; ++cc) {
-              const int e = q * 16 + cc;
-              const float2 x =
-                  ffma2(make_float2(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1])), sc2, nb2);
-              const float2 y = !decltype(part)::value && (e & 3) == 3 ? exp2_fma2(x)
-                                                                     : make_float2(ex2_approx(x.x), ex2_approx(x.y));
-              ps2[e & 1] = add2p(ps2[e & 1], pk2(y.x, y.y));
-              pk[q][cc] = srv_pack<BF16>(y.x, y.y);
-            }
-          };
-          // The P buffer is free once the P V that used it last is complete; with one buffer
-          // that is the previous step's, so half of the exponentials come before the wait.
-          constexpr int EARLY = SM::PBUF == 1 ? ATC_P_EARLY : 0;
-#pragma unroll
-          for (int q = 0; q < EARLY; ++q) chunk(q);
-          if (c >= SM::PBUF && !pv_done(c - SM::PBUF)) return false;
-#pragma unroll
-          for (int q = 0; q < KT / 32; ++q) {
-            if (q >= EARLY) chunk(q);
-            tmem_st_32x32b_x16(p_addr + (uint32_t)(q * 16), pk[q]);
+            for (int e = 0; e < 16; ++e) pk[q][e] = 0u;
+            return;
           }
-          return true;
+#pragma unroll
+          for (int cc = 0; cc < 16; ++cc) {
+            const int e = q * 16 + cc;
+            const float2 x = ffma2(make_float2(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1])), sc2, nb2);
+            const float2 y = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+            ps2[e & 1] = add2p(ps2[e & 1], pk2(y.x, y.y));
+            pk[q][cc] = srv_pack<BF16>(y.x, y.y);
+          }
         };
-        if (!(partly ? exponentials(std::true_type{}) : exponentials(std::false_type{}))) {
+        // The P buffer is free once the P V that used it last is complete.  With one buffer
+        // that is the previous step's, so half of the exponentials come before the wait;
+        // with two the issuer waited.
+        constexpr int EARLY = SM::PBUF == 1 ? KT / 64 : 0;
+#pragma unroll
+        for (int q = 0; q < EARLY; ++q) chunk(q);
+        if (SM::PBUF == 1 && c >= 1 && !pv_done(c - 1)) {
           ok = false;
           break;
+        }
+#pragma unroll
+        for (int q = 0; q < KT / 32; ++q) {
+          if (q >= EARLY) chunk(q);
+          tmem_st_32x32b_x16(p_addr + (uint32_t)(q * 16), pk[q]);
         }
         const float2 rs2 = upk2(add2p(ps2[0], ps2[1]));
         l_run = l_run * alpha + (rs2.x + rs2.y);
@@ -877,8 +871,6 @@ __global__ void __launch_bounds__(TileSmem<HD>::THREADS, 1)
         break;
       }
       tc_fence_after();
-      // A row of nothing but scores of -inf: exp2_fma2 leaves 2^-126 where their exponential is 0.
-      if (m_run == -INFINITY && l_run == l_run) l_run = 0.f;
       if (part >= 0) {
         // A piece: raw sums, joined later.
         float* dst = p.part_o + prow * HD;
