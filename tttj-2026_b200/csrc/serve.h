@@ -105,10 +105,11 @@ struct TileJoin {     // an entry whose keys were split
   int row0, n, pad[2];     // of the sequence
 };
 struct TilePlan {     // in the workspace, rebuilt by every call
-  int* counters;      // [4]: items taken, entries, joins, items to redo
+  int* counters;      // [4]: items taken, entries, joins, notes of rows that are not finite
   TileEntry* entries; // [most_entries]
   TileJoin* joins;    // [most_entries]
-  int* redo;          // [2 * most_entries * kv_heads][3]: b, q, h
+  int4* redo;         // [most_redo]: b, q, h, warp of the item (32 rows)
+  int most_redo;
   int most_entries;
   int most_parts;     // partial-result slots
 };
@@ -119,6 +120,7 @@ struct TileParams {
   CacheView k, v;      // the same (prompts: page 0)
   void* out;
   long o_tok, o_head;
+  int o_wide;          // rows of out are 32-byte aligned
   float* lse;
   int heads, kv_heads, group, tile_tokens;
   float scale_log2;

@@ -152,7 +152,7 @@ constexpr int kStepMostRows = 16;
 // Workspace of either attention kernel.
 struct ServeWs {
   size_t part_o, part_ml, entries, joins, redo, counters, total;
-  int most_entries, most_parts;
+  int most_entries, most_parts, most_redo;
 };
 int tile_tokens(const tttj_seqs* s) { return ATC_BM / (s->heads / s->kv_heads); }
 ServeWs step_ws(const tttj_seqs* s) {
@@ -167,13 +167,16 @@ ServeWs tile_ws(const tttj_seqs* s) {
   ServeWs w{};
   // Bounds of tile_plan_kernel: cut items leave at most 4 pieces per CTA (and one per head).
   w.most_parts = 4 * kMostSms + s->kv_heads;
-  w.most_entries = s->tokens / (tile_nt(s->head_dim) * tile_tokens(s)) + s->batch + w.most_parts;
+  const int items = s->tokens / (tile_nt(s->head_dim) * tile_tokens(s)) + s->batch;  // of a key/value head
+  w.most_entries = items + w.most_parts;
+  const long notes = (long)items * s->kv_heads * 4 * tile_nt(s->head_dim);  // one per softmax warp of an item
+  w.most_redo = (int)(notes < (1l << 30) ? notes : 1l << 30);
   const size_t rows = (size_t)w.most_parts * tile_nt(s->head_dim) * ATC_BM;
   w.counters = 0;
   w.entries = up(16);
   w.joins = w.entries + up((size_t)w.most_entries * sizeof(TileEntry));
   w.redo = w.joins + up((size_t)w.most_entries * sizeof(TileJoin));
-  w.part_ml = w.redo + up((size_t)w.most_entries * s->kv_heads * 2 * 3 * 4);
+  w.part_ml = w.redo + up((size_t)w.most_redo * sizeof(int4));
   w.part_o = w.part_ml + up(rows * 8);
   w.total = w.part_o + up(rows * s->head_dim * 4);
   return w;
@@ -244,6 +247,7 @@ int attention(const char* what, const tttj_seqs* s, const tttj_rows* q, const Ca
   p.out = const_cast<void*>(out->data);
   p.o_tok = out->token_stride;
   p.o_head = out->head_stride;
+  p.o_wide = reinterpret_cast<uintptr_t>(out->data) % 32 == 0 && out->token_stride % 16 == 0 && out->head_stride % 16 == 0;
   p.lse = lse;
   p.heads = s->heads;
   p.kv_heads = s->kv_heads;
@@ -253,7 +257,8 @@ int attention(const char* what, const tttj_seqs* s, const tttj_rows* q, const Ca
   p.plan.counters = reinterpret_cast<int*>(base + w.counters);
   p.plan.entries = reinterpret_cast<TileEntry*>(base + w.entries);
   p.plan.joins = reinterpret_cast<TileJoin*>(base + w.joins);
-  p.plan.redo = reinterpret_cast<int*>(base + w.redo);
+  p.plan.redo = reinterpret_cast<int4*>(base + w.redo);
+  p.plan.most_redo = w.most_redo;
   p.plan.most_entries = w.most_entries;
   p.plan.most_parts = w.most_parts;
   p.part_o = reinterpret_cast<float*>(base + w.part_o);

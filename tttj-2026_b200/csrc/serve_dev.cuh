@@ -74,6 +74,13 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* tmap, uint
       : "memory");
 }
 
+// 32 bytes, 32-byte aligned.
+__device__ __forceinline__ void srv_st_v8(void* to, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+
 // Whether one of the two 16-bit floats of a word is infinite or NaN.
 template <bool BF16>
 __device__ __forceinline__ bool srv_nonfinite(uint32_t w) {

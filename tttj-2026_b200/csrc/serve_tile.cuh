@@ -20,10 +20,12 @@
 //   tile_join_kernel  joins the pieces of cut items in the order of their keys.
 //
 // Hidden keys.  Scores of keys a row does not see are replaced by -inf.  Their values still
-// meet P = 0 in the product, and 0 x NaN is NaN: V rows behind the last key are zeroed in
-// shared memory, and a tile that some row sees only in part is searched for infinite or NaN
-// values while the softmax works on its scores.  Where one is found the item is noted, and
-// the joining kernel computes its rows again, one warp per row, key by key.
+// meet P = 0 in the product, and 0 x NaN is NaN.  V rows behind the last key (stale pages, the
+// next sequence) are zeroed in shared memory.  For the others the result is looked at: a row
+// that is not finite may owe it to a value that it does not see, so the joining kernel searches
+// its hidden values, and where one is not finite computes the row again, key by key.
+// (Searching every V tile on the diagonal for such values took a warp 2000 cycles per tile,
+// in which the tile's product waited: prompts of 128 - 256 tokens.)
 //
 // Every wait is bounded; a role that gives up records SRV_DEV_TIMEOUT and unwinds.
 #pragma once
@@ -70,8 +72,7 @@ struct TileSmem : AtcSmem<HD> {  // tile sizes and stages as there
   static constexpr int BAR_AT = B::Q_BYTES + B::KV_BYTES;
   static constexpr int SLOT_AT = BAR_AT + BARS * 8;  // TMEM base, abort flag
   static constexpr int INFO_AT = SLOT_AT + 16;       // [side][QS] items
-  static constexpr int EPI_AT = (INFO_AT + 2 * B::QS * 64 + 127) / 128 * 128;
-  static constexpr int ALL = EPI_AT + B::EPI_BYTES + 1024;
+  static constexpr int ALL = INFO_AT + 2 * B::QS * 64 + 1024;
 };
 
 constexpr int TILE_MIN_PIECE = 4;  // key tiles (512 keys) a cut piece has at least
@@ -309,7 +310,6 @@ __global__ void __launch_bounds__(TileSmem<HD>::THREADS, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + SM::SLOT_AT);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   TileInfo* info = reinterpret_cast<TileInfo*>(smem + SM::INFO_AT);  // [side][QS]
-  const uint32_t sEpi = sQ + SM::EPI_AT;
 
   const int warp = warp_id();
   const int lane = lane_id();
@@ -621,9 +621,7 @@ __global__ void __launch_bounds__(TileSmem<HD>::THREADS, 1)
     }
   } else if (warp == CLEANER) {
     // ------------------------------------------------------------ cleaner
-    // Sees every V tile before the products do: rows behind the last key become zeros, and
-    // a tile that some row of the item sees only in part is searched for values that a
-    // product with P = 0 would not hide.
+    // Sees every V tile before the products do: rows behind the last key become zeros.
     constexpr unsigned FULL = 0xffffffffu;
     bool ok = true;
     long vc = 0;
@@ -635,48 +633,20 @@ __global__ void __launch_bounds__(TileSmem<HD>::THREADS, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_q_empty + 8 * qb);
       if (wi.n_kv < 0) break;  // no more items
-      const int all_see = p.s.causal ? wi.len - wi.n + wi.tok0 + 1 : wi.len;
-      bool noted = false;
       for (int j = 0; j < wi.n_kv; ++j, ++vc) {
         const int vs = (int)(vc % STAGES);
         ok = __all_sync(FULL, srv_wait(bar_v_full + 8 * vs, (uint32_t)((vc / STAGES) & 1), abort_flag, limit));
         if (!ok) break;
-        const int base = (wi.j0 + j) * ATC_BN;
-        if (base + ATC_BN > all_see) {
-          const int keep = max(0, min(ATC_BN, wi.len - base));
-          constexpr int ROW_BYTES = SM::BOX_COLS * 2;
-          constexpr int CH = ROW_BYTES / 16;
-          uint32_t zero = 0;  // two sums of value x 0: NaN once a value was not finite
-#pragma unroll 1
+        const int keep = wi.len - (wi.j0 + j) * ATC_BN;
+        if (keep < ATC_BN) {
+          constexpr int CH = SM::BOX_COLS * 2 / 16;  // 16-byte chunks of a row of a box
           for (int x = 0; x < SM::NBOX; ++x) {
             const uint32_t vx = sV + vs * SM::KV_TILE + (uint32_t)(x * SM::BOX_BYTES);
-#pragma unroll 8
-            for (int i = lane; i < (p.s.causal ? keep * CH : 0); i += 32) {
-              uint32_t w[4];
-              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                           : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                           : "r"(vx + (uint32_t)(i * 16))
-                           : "memory");
-#pragma unroll
-              for (int e = 0; e < 4; ++e) zero = srv_fma_zero<BF16>(w[e], zero);
-            }
-            for (int i = keep * CH + lane; i < ATC_BN * CH; i += 32)
+            for (int i = max(0, keep) * CH + lane; i < ATC_BN * CH; i += 32)
               asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(vx + (uint32_t)(i * 16)), "r"(0u)
                            : "memory");
           }
-          const bool odd = srv_nonfinite<BF16>(zero);
           fence_proxy_async_smem();
-          if (__any_sync(FULL, odd) && !noted) {
-            noted = true;
-            if (lane == 0) {
-              const int at = atomicAdd(p.plan.counters + 3, 1);
-              if (at < 2 * p.plan.most_entries * p.kv_heads) {
-                p.plan.redo[3 * at] = wi.b;
-                p.plan.redo[3 * at + 1] = wi.q;
-                p.plan.redo[3 * at + 2] = wi.h;
-              }
-            }
-          }
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(bar_v_ready + 8 * vs);
@@ -724,7 +694,7 @@ __global__ void __launch_bounds__(TileSmem<HD>::THREADS, 1)
       if (wi.n_kv < 0) break;  // no more items
       const int tq = atc_query_tile<NT>(t, k);
       const int n = tq == 0 ? wi.ns[0] : wi.ns[1];
-      const int key0 = wi.j0 * ATC_BN, len = wi.len, part = wi.part, h = wi.h;
+      const int key0 = wi.j0 * ATC_BN, len = wi.len, part = wi.part, h = wi.h, b = wi.b, qi = wi.q;
       const int tok0 = wi.tok0 + tq * TOK;  // first token of the tile
       const int tokens = wi.n;
       const int token = wi.row0 + tok0 + rtok;   // packed row of this thread's token
@@ -890,67 +860,36 @@ __global__ void __launch_bounds__(TileSmem<HD>::THREADS, 1)
         const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
         if (live && p.lse != nullptr)
           p.lse[(long)token * p.heads + h * p.group + rhead] = srv_lse(m_run, l_run);
-        uint16_t* out = static_cast<uint16_t*>(p.out);
-        // Where this row goes, -1: nowhere.
-        const long row_at = live ? (long)token * p.o_tok + (long)(h * p.group + rhead) * p.o_head : -1;
-        if constexpr (SM::STAGED_EPI) {
-          // The warp's 32 rows go through shared memory so that the stores cover whole
-          // row segments (16-byte chunk j of row r staged at slot j ^ (r % NCH)).
-          constexpr int NCH = SM::EPI_ROW / 16;
-          const uint32_t stage = sEpi + (uint32_t)(warp * 32 * SM::EPI_ROW);
-#pragma unroll
-          for (int c = 0; c < HD / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld_32x32b_x32(o_addr + (uint32_t)(c * 32), o);
-            tmem_wait_ld();
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const int j = c * 4 + q;
-              const uint32_t a = stage + (uint32_t)(lane * SM::EPI_ROW + ((j ^ (lane % NCH)) << 4));
-              uint32_t w[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                w[e] = srv_pack<BF16>(__uint_as_float(o[8 * q + 2 * e]) * inv, __uint_as_float(o[8 * q + 2 * e + 1]) * inv);
-              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(w[0]), "r"(w[1]), "r"(w[2]),
-                           "r"(w[3])
-                           : "memory");
-            }
-          }
-          __syncwarp();
-          constexpr int RPI = 32 / NCH;  // rows per store instruction
-          const int j = lane % NCH;
-#pragma unroll
-          for (int it = 0; it < 32 / RPI; ++it) {
-            const int rr = it * RPI + lane / NCH;
-            const uint32_t a = stage + (uint32_t)(rr * SM::EPI_ROW + ((j ^ (rr % NCH)) << 4));
-            uint4 v;
-            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                         : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                         : "r"(a)
-                         : "memory");
-            const long to = __shfl_sync(0xffffffffu, row_at, rr);
-            if (to >= 0) *reinterpret_cast<uint4*>(out + to + j * 8) = v;
-          }
-        } else {
-          // Wide heads: each thread stores its own row, 64 bytes per 32 columns.
-          uint16_t* dst = out + row_at;
+        // Every thread stores its own row, a whole 32-byte sector at a time where rows are aligned
+        // for that.  (Through shared memory, so that a warp's stores cover whole rows: 127 against
+        // 123 us at 256 prompts of 128 - 256 tokens, head_dim 64.)
+        uint16_t* dst = static_cast<uint16_t*>(p.out) + (long)token * p.o_tok + (long)(h * p.group + rhead) * p.o_head;
+        uint32_t odd = 0;  // two sums of result x 0: NaN once one was not finite
 #pragma unroll 1
-          for (int c = 0; c < HD / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld_32x32b_x32(o_addr + (uint32_t)(c * 32), o);
-            tmem_wait_ld();
-            if (live) {
+        for (int c = 0; c < HD / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld_32x32b_x32(o_addr + (uint32_t)(c * 32), o);
+          tmem_wait_ld();
+          if (live) {
+            uint32_t w[16];
 #pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                uint32_t w[4];
+            for (int e = 0; e < 16; ++e) {
+              w[e] = srv_pack<BF16>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
+              odd = srv_fma_zero<BF16>(w[e], odd);
+            }
+            if (p.o_wide) {
+              srv_st_v8(dst + c * 32, w);
+              srv_st_v8(dst + c * 32 + 16, w + 8);
+            } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  w[e] = srv_pack<BF16>(__uint_as_float(o[8 * q + 2 * e]) * inv,
-                                        __uint_as_float(o[8 * q + 2 * e + 1]) * inv);
-                *reinterpret_cast<uint4*>(dst + c * 32 + q * 8) = make_uint4(w[0], w[1], w[2], w[3]);
-              }
+              for (int e = 0; e < 16; e += 4)
+                *reinterpret_cast<uint4*>(dst + c * 32 + 2 * e) = make_uint4(w[e], w[e + 1], w[e + 2], w[e + 3]);
             }
           }
+        }
+        if (p.s.causal && __any_sync(0xffffffffu, srv_nonfinite<BF16>(odd)) && lane == 0) {
+          const int at = atomicAdd(p.plan.counters + 3, 1);
+          if (at < p.plan.most_redo) p.plan.redo[at] = make_int4(b, qi, h, tq * 4 + quad);
         }
       }
       tc_fence_before();
@@ -1013,8 +952,19 @@ __device__ __forceinline__ void tile_load_part(const float* row, float (&o)[HD /
   }
 }
 
-// One row key by key, hidden keys left out: for items in which a hidden value is infinite
-// or NaN.
+// Where key j of a head lies, in elements; false: on no page.
+__device__ __forceinline__ bool tile_locate(const TileParams& p, const CacheView& c, const SrvSeq& s, int b, int kvh,
+                                            int j, long* at) {
+  if (p.s.table == nullptr) {
+    *at = (long)(s.row0 + j) * c.slot + kvh * c.head;
+    return true;
+  }
+  const int page = srv_page(p.s, b, j), in = j & ((1 << p.s.page_shift) - 1);
+  *at = page * c.page + in * c.slot + kvh * c.head;
+  return page < p.s.num_pages;
+}
+
+// One row key by key, hidden keys left out.
 template <int HD, bool BF16>
 __device__ void tile_redo_row(const TileParams& p, const SrvSeq& s, int b, int tok, int kvh, int g) {
   const int lane = lane_id();
@@ -1030,18 +980,10 @@ __device__ void tile_redo_row(const TileParams& p, const SrvSeq& s, int b, int t
   const int keys = p.s.causal ? min(s.len, s.len - s.n + tok + 1) : s.len;
   for (int j = 0; j < keys; ++j) {
     long at_k, at_v;
-    bool there = true;
-    if (p.s.table != nullptr) {
-      const int page = srv_page(p.s, b, j), in = j & ((1 << p.s.page_shift) - 1);
-      there = page < p.s.num_pages;
-      at_k = page * p.k.page + in * p.k.slot;
-      at_v = page * p.v.page + in * p.v.slot;
-    } else {
-      at_k = (long)(s.row0 + j) * p.k.slot;
-      at_v = (long)(s.row0 + j) * p.v.slot;
-    }
-    const uint16_t* kr = static_cast<const uint16_t*>(p.k.data) + at_k + kvh * p.k.head + lane * E;
-    const uint16_t* vr = static_cast<const uint16_t*>(p.v.data) + at_v + kvh * p.v.head + lane * E;
+    tile_locate(p, p.v, s, b, kvh, j, &at_v);
+    const bool there = tile_locate(p, p.k, s, b, kvh, j, &at_k);
+    const uint16_t* kr = static_cast<const uint16_t*>(p.k.data) + at_k + lane * E;
+    const uint16_t* vr = static_cast<const uint16_t*>(p.v.data) + at_v + lane * E;
     float dot = 0.f;
     if (there)
 #pragma unroll
@@ -1064,13 +1006,35 @@ __device__ void tile_redo_row(const TileParams& p, const SrvSeq& s, int b, int t
   tile_store_row<HD, BF16>(p, token, head, acc, l == 0.f ? 0.f : 1.f / l, m, l);
 }
 
+// A row whose result is not finite: again, if a value that it does not see, among those that
+// its tile's products read, is not finite.
 template <int HD, bool BF16>
-__global__ void __launch_bounds__(32 * TILE_JOIN_WARPS) tile_join_kernel(const TileParams p) {
+__device__ __noinline__ void tile_mend_row(const TileParams& p, int b, int tok0, int rtok, int kvh, int g) {
+  constexpr int E = HD / 32;
+  const SrvSeq s = srv_seq(p.s, b);
+  const int tok = tok0 + rtok;
+  if (tok >= s.n) return;
+  const int end = tile_kv_tiles(tile_kv_end(s, 1, tok0, p.tile_tokens)) * ATC_BN;
+  bool odd = false;
+#pragma unroll 4
+  for (int j = max(0, s.len - s.n + tok + 1); j < min(s.len, end); ++j) {
+    long at;
+    if (tile_locate(p, p.v, s, b, kvh, j, &at)) {
+      const uint16_t* v = static_cast<const uint16_t*>(p.v.data) + at + lane_id() * E;
+#pragma unroll
+      for (int i = 0; i < E; ++i) odd |= srv_nonfinite<BF16>(v[i]);
+    }
+  }
+  if (__any_sync(0xffffffffu, odd)) tile_redo_row<HD, BF16>(p, s, b, tok, kvh, g);
+}
+
+template <int HD, bool BF16>
+__global__ void __launch_bounds__(32 * TILE_JOIN_WARPS) tile_join_kernel(const __grid_constant__ TileParams p) {
   constexpr int NT = AtcSmem<HD>::NT;
   constexpr int ROWS = NT * ATC_BM;
   griddep_wait();
   const int joins = p.plan.counters[2];
-  const int redo = min(p.plan.counters[3], 2 * p.plan.most_entries * p.kv_heads);
+  const int redo = min(p.plan.counters[3], p.plan.most_redo);
   const int lane = lane_id();
   const long w0 = (long)blockIdx.x * TILE_JOIN_WARPS + warp_id(), step = (long)gridDim.x * TILE_JOIN_WARPS;
   // Four rows per warp at a time, their loads in flight together.
@@ -1081,10 +1045,6 @@ __global__ void __launch_bounds__(32 * TILE_JOIN_WARPS) tile_join_kernel(const T
     const TileJoin e = p.plan.joins[i / (ROWS / R) / p.kv_heads];
     const int tok0 = (e.q * NT + r0 / ATC_BM) * p.tile_tokens;
     if ((r0 % ATC_BM) / p.group >= p.tile_tokens || tok0 + (r0 % ATC_BM) / p.group >= e.n) continue;
-    bool noted = false;
-    for (int c = 0; c < redo; ++c)
-      noted |= p.plan.redo[3 * c] == e.b && p.plan.redo[3 * c + 1] == e.q && p.plan.redo[3 * c + 2] == h;
-    if (noted) continue;
     auto at = [&](int piece) { return ((long)e.part + (long)piece * p.kv_heads + h) * ROWS + r0; };
     float top[R], sum[R], acc[R][HD / 32];
 #pragma unroll
@@ -1115,23 +1075,30 @@ __global__ void __launch_bounds__(32 * TILE_JOIN_WARPS) tile_join_kernel(const T
         for (int y = 0; y < HD / 32; ++y) acc[x][y] += none ? 0.f : o[x][y] * f;
       }
     }
+    unsigned odd = 0;  // rows that are not finite
 #pragma unroll
     for (int x = 0; x < R; ++x) {
       const int rtok = (r0 % ATC_BM + x) / p.group, g = r0 % ATC_BM + x - rtok * p.group;
-      if (rtok < p.tile_tokens && tok0 + rtok < e.n)
+      if (rtok < p.tile_tokens && tok0 + rtok < e.n) {
         tile_store_row<HD, BF16>(p, e.row0 + tok0 + rtok, h * p.group + g, acc[x], sum[x] == 0.f ? 0.f : 1.f / sum[x],
                                  top[x], sum[x]);
+#pragma unroll
+        for (int y = 0; y < HD / 32; ++y) odd |= fabsf(acc[x][y]) < INFINITY ? 0u : 1u << x;
+      }
+    }
+    odd = p.s.causal ? __reduce_or_sync(0xffffffffu, odd) : 0;
+    for (; odd != 0; odd &= odd - 1) {
+      const int r = r0 % ATC_BM + __ffs(odd) - 1, rtok = r / p.group;
+      tile_mend_row<HD, BF16>(p, e.b, tok0, rtok, h, r - rtok * p.group);
     }
   }
-  // Items with a hidden infinite or NaN value (left out above where they were also cut).
-  for (long i = w0; i < (long)redo * ROWS; i += step) {
-    const int* e = p.plan.redo + 3 * (i / ROWS);
-    const int r = (int)(i % ROWS);
-    const int rtok = (r % ATC_BM) / p.group, g = (r % ATC_BM) - rtok * p.group;
-    const int tok = (e[1] * NT + r / ATC_BM) * p.tile_tokens + rtok;
-    const SrvSeq s = srv_seq(p.s, e[0]);
-    if (rtok >= p.tile_tokens || tok >= s.n) continue;
-    tile_redo_row<HD, BF16>(p, s, e[0], tok, e[2], g);
+  // Rows of whole items, 32 per note.
+  for (long i = w0; i < (long)redo * 32; i += step) {
+    const int4 e = p.plan.redo[i / 32];
+    const int r = (e.w & 3) * 32 + (int)(i % 32);
+    const int rtok = r / p.group;
+    if (rtok < p.tile_tokens)
+      tile_mend_row<HD, BF16>(p, e.x, (e.y * NT + e.w / 4) * p.tile_tokens, rtok, e.z, r - rtok * p.group);
   }
 }
 
