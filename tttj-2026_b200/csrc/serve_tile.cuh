@@ -164,17 +164,32 @@ __global__ void __launch_bounds__(TILE_PLAN_THREADS) tile_plan_kernel(const Tile
     s.len = s_len[b];
     return tile_kv_tiles(tile_kv_end(s, p.s.causal, q * item_tokens, item_tokens));
   };
+  // Item e: sequence, item of the sequence, key tiles.  A thread's first is found once.
+  struct Item {
+    int b, q, t;
+  };
+  auto find = [&](int e) {
+    Item i;
+    i.q = locate(e, &i.b);
+    i.t = tiles_of(i.b, i.q);
+    return i;
+  };
+  Item own{};
+  if (tid < items) own = find(tid);
+  auto item = [&](int e) { return e == tid ? own : find(e); };
+  // Quotients in 32 bits where they fit: a 64-bit division is a few hundred cycles of latency.
+  auto share = [&](unsigned long long x) {  // of all heads' x per CTA, rounded up
+    x = x * p.kv_heads + grid - 1;
+    return x >> 32 ? (int)(x / grid) : (int)((unsigned)x / (unsigned)grid);
+  };
   // Whole waves of items stay whole; with at least four waves the last one is short
   // against the rest.  Which items are cut depends on their number alone, not on the
   // order in which threads run: results repeat exactly.
-  const long all_items = (long)items * p.kv_heads;
-  const long waves = all_items / grid;
-  const int whole = waves >= 4 ? items : (int)(waves * grid / p.kv_heads);
+  const bool many = (long)items * p.kv_heads >= 4l * grid;
+  const int whole = many ? items : items * p.kv_heads / grid * grid / p.kv_heads;
   unsigned long long sum = 0, rest = 0;
   for (int e = tid; e < items; e += TILE_PLAN_THREADS) {
-    int b;
-    const int q = locate(e, &b);
-    const int t = tiles_of(b, q);
+    const int t = item(e).t;
     sum += t;
     if (e >= whole) rest += t;
   }
@@ -195,8 +210,7 @@ __global__ void __launch_bounds__(TILE_PLAN_THREADS) tile_plan_kernel(const Tile
     sum += __shfl_xor_sync(0xffffffffu, sum, d);
     rest += __shfl_xor_sync(0xffffffffu, rest, d);
   }
-  const int most = (int)max((long)(sum * p.kv_heads + grid - 1) / grid, (long)TILE_MIN_PIECE);
-  const int most_rest = (int)max((long)(rest * p.kv_heads + grid - 1) / grid, (long)TILE_MIN_PIECE);
+  const int most = max(share(sum), TILE_MIN_PIECE), most_rest = max(share(rest), TILE_MIN_PIECE);
   // Adds n to a bucket, returns what it held: lanes of one bucket share one atomic.
   auto add_to = [&](int at, int n) {
     const unsigned active = __activemask();
@@ -212,14 +226,12 @@ __global__ void __launch_bounds__(TILE_PLAN_THREADS) tile_plan_kernel(const Tile
   auto pieces_of = [&](int e, int t) {
     const int c = e >= whole ? min(most, most_rest) : most;
     // A whole item a little above the fair share costs less than its pieces' joining.
-    return e < whole && t <= most + most / 4 ? 1 : (t + c - 1) / c;
+    return t <= (e < whole ? most + most / 4 : c) ? 1 : (t + c - 1) / c;
   };
   auto bucket = [&](int len) { return TILE_BUCKETS - min(len, TILE_BUCKETS); };  // longest first
   for (int e = tid; e < items; e += TILE_PLAN_THREADS) {
-    int b;
-    const int q = locate(e, &b);
-    const int t = tiles_of(b, q), n = pieces_of(e, t);
-    add_to(bucket((t + n - 1) / n), n);
+    const int t = item(e).t, n = pieces_of(e, t);
+    add_to(bucket(n == 1 ? t : (t + n - 1) / n), n);
   }
   __syncthreads();
   {
@@ -249,22 +261,24 @@ __global__ void __launch_bounds__(TILE_PLAN_THREADS) tile_plan_kernel(const Tile
   __syncthreads();
   for (int e = tid; e < items; e += TILE_PLAN_THREADS) {
     TileEntry out{};
-    out.q = locate(e, &out.b);
+    const Item i = item(e);
+    out.b = i.b;
+    out.q = i.q;
     out.row0 = s_row0[out.b];
     out.n = s_n[out.b];
     out.len = s_len[out.b];
-    const int t = tiles_of(out.b, out.q), n = pieces_of(e, t);
+    const int t = i.t, n = pieces_of(e, t);
     int part = -1;
     if (n > 1) {
       part = atomicAdd(&s_parts, n * p.kv_heads);
       p.plan.joins[atomicAdd(&s_joins, 1)] = TileJoin{out.b, out.q, n, part, out.row0, out.n, {0, 0}};
     }
-    const int at = add_to(bucket((t + n - 1) / n), n);
-    for (int i = 0; i < n; ++i) {
-      out.j0 = (int)((long)t * i / n);
-      out.j1 = (int)((long)t * (i + 1) / n);
-      out.part = n > 1 ? part + i * p.kv_heads : -1;
-      p.plan.entries[at + i] = out;
+    const int at = add_to(bucket(n == 1 ? t : (t + n - 1) / n), n);
+    for (int x = 0; x < n; ++x) {
+      out.j0 = n == 1 ? 0 : (int)((long)t * x / n);
+      out.j1 = n == 1 ? t : (int)((long)t * (x + 1) / n);
+      out.part = n > 1 ? part + x * p.kv_heads : -1;
+      p.plan.entries[at + x] = out;
     }
   }
   __syncthreads();
@@ -1009,7 +1023,7 @@ __device__ void tile_redo_row(const TileParams& p, const SrvSeq& s, int b, int t
 // A row whose result is not finite: again, if a value that it does not see, among those that
 // its tile's products read, is not finite.
 template <int HD, bool BF16>
-__device__ __noinline__ void tile_mend_row(const TileParams& p, int b, int tok0, int rtok, int kvh, int g) {
+__device__ __forceinline__ void tile_mend_row(const TileParams& p, int b, int tok0, int rtok, int kvh, int g) {
   constexpr int E = HD / 32;
   const SrvSeq s = srv_seq(p.s, b);
   const int tok = tok0 + rtok;
