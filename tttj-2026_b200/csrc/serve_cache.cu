@@ -88,8 +88,8 @@ __global__ void __launch_bounds__(APPEND_THREADS, 5) append_kernel(const AppendP
 // and holds EVICT_HELD of them per thread in registers (a longer range's rest is read again
 // where it is needed).  The keep-th largest value is found two bits at a time: everyone
 // counts the values above three thresholds, the warps' counts meet in every block's shared
-// memory, 16 rounds of one barrier each.  (A radix selection with histograms in shared memory took
-// 77 thousand cycles of a cluster of 8 at 32768 slots, this 23 thousand.)  Then ballots rank the
+// memory, 16 rounds of one barrier each.  (A radix selection with histograms in shared memory: 123
+// against 50 us in all, 16 heads of 20000 - 32768 slots.)  Then ballots rank the
 // equal values, the holes (slots < keep that go) and the movers (slots >= keep that stay); the
 // i-th mover goes to the i-th hole, so as few rows move as can, and since sources lie behind
 // the budget and destinations in front of it, no move reads what another writes.  All counts are

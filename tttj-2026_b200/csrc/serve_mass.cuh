@@ -2,7 +2,7 @@
 // the probabilities exp(scale q k_j - lse) that the new tokens' queries gave to it.
 //
 // Keys stay, queries stream: S^T = K Q^T on the tensor cores with 128 keys as the rows of
-// the accumulator and up to 128 query rows (token x group + head) as its columns, so a
+// the accumulator and up to 80 query rows (token x group + head) as its columns, so a
 // thread owns one key and adds its row of exponentials in registers -- no reduction across
 // threads, no atomics, a fixed order.  The log-sum-exp of the attention makes every
 // probability independent of the others, so one pass suffices.
@@ -52,7 +52,7 @@ struct MassSmem {
 constexpr int MASS_ADDERS = 12;
 constexpr int MASS_THREADS = 32 * (MASS_ADDERS + 3);
 
-constexpr int MASS_FMA_PAIRS = 2;  // of eight pairs of exponentials, those on the FMA pipe
+constexpr int MASS_FMA_PAIRS = 2;  // of eight pairs of exponentials, those on the FMA pipe (0 or 1: 2 % slower)
 
 // Position in a ring of N stages: index and phase parity, without divisions.
 template <int N>

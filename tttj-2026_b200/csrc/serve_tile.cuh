@@ -45,13 +45,20 @@ struct TileInfo {  // one decoded item, in shared memory
 static_assert(sizeof(TileInfo) <= 64, "item info slot is 64 bytes");
 
 // TMEM (512 columns) holds, per query tile, the scores of a step (fp32, a column per key), the
-// probabilities (16 bits, half a column per key) and O (head_dim columns).  At head_dim 128 the
-// two O take 256 columns, so a step is 64 keys there, with two buffers of probabilities; then
-// nothing shares columns, S of the next step is computed while the softmax works on this one,
-// and no product is waited for.  Measured there, prompts of 3001 and 4096 tokens, 32 / 8 heads:
-// steps of 128 keys with P written over S, as in attention_tc.cuh, 286 us (the next S waits for
-// P V); one score buffer of 128 keys that the tiles take in turn, 250 - 258 us; this with
-// one issuing warp per tile 257 us, with one for S and one for P V, 251 us.
+// probabilities (16 bits, half a column per key) and O (head_dim columns).  Up to head_dim 128
+// a step is 64 keys, with two buffers of probabilities: nothing shares columns, S of the next step
+// is computed while the softmax works on this one, and the softmax waits for no product.
+// Measured at head_dim 128, prompts of 3001 and 4096 tokens, 32 / 8 heads: steps of 128 keys with P
+// written over S, as in attention_tc.cuh, 286 us (the next S waits for P V); one score buffer of
+// 128 keys that the tiles take in turn 250 - 258; steps of 64 with one issuing warp per tile
+// 257, with one for S and one for P V 251; the wait for the P buffer moved to the issuer 227
+// against 233; no exponentials on the FMA pipe 223 (a quarter: 227, 3/8: 233, 1/2: 242; issue
+// slots are as scarce as the MUFU); scores read twice from TMEM in rolled loops, S double-buffered
+// and P over it, 244 against 215.  At head_dim 64, 256 prompts of 128 - 256 tokens: steps of 128
+// keys 150 us, of 64 keys 127.  At head_dim 256 (one query tile per item) steps of 128 keys and one
+// buffer of P: 111 against 182 us, prompts of 3000 and 4096 tokens, 8 / 2 heads.
+// What bounds it: with nearly all products left out the same prompts take 186 us, so the
+// softmax warps do, two per scheduler, 57 % of the MUFU's rate; the tensor pipe is half busy.
 template <int HD>
 struct TileSmem : AtcSmem<HD> {  // tile sizes and stages as there
   using B = AtcSmem<HD>;
@@ -743,7 +750,7 @@ __global__ void __launch_bounds__(TileSmem<HD>::THREADS, 1)
         // The scores are in registers: the buffer may take the next step's.
         tc_fence_before();
         arrive(bar_s_free + 8 * t);
-        // 32 keys at a time: those that no row of the warp sees take no further part (on the
+        // 32 keys at a time: those that no row of the warp sees take no part (on the
         // diagonal half of them), those that some see are masked.  Column e of this step is
         // hidden when e > lim; limits rise with the rows.
         const int k0 = key0 + i * KT, lim = row_lim - k0, warp_hi = warp_lim_hi - k0, warp_lo = warp_lim_lo - k0;
