@@ -276,7 +276,6 @@ __global__ void __launch_bounds__(STEP_THREADS, step_ctas_per_sm(HD))
             }
           }
           __syncwarp();
-          __syncwarp();
           odd = __any_sync(0xffffffffu, odd);
           fence_proxy_async_smem();  // before the ring's next TMA write of these bytes
         }
@@ -305,34 +304,34 @@ __global__ void __launch_bounds__(STEP_THREADS, step_ctas_per_sm(HD))
             o[i][3] *= alpha[1];
           }
         }
-                  if (odd) {
-                    for (int key = 0; key < 16; ++key) {
-        #pragma unroll
-                      for (int i = 0; i < HD / 8; ++i) {
-                        uint32_t w;
-                        asm volatile("ld.shared.b32 %0, [%1];"
-                                     : "=r"(w)
-                                     : "r"(at(sv, warp * 16 + key, i) + (lane & 3) * 4)
-                                     : "memory");
-        #pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                          const float v = srv_to_float<BF16>((w >> (16 * x)) & 0xffffu);
-                          if (!isfinite(v)) {
-                            if (k0 + key <= lim[0]) o[i][x] += v;
-                            if (k0 + key <= lim[1]) o[i][2 + x] += v;
-                          }
-                        }
-                      }
-                    }
-                    __syncwarp();
-                    for (int i = lane; i < 16 * (HD / 2); i += 32) {
-                      const uint32_t a = at(sv, warp * 16 + i / (HD / 2), (i % (HD / 2)) / 4) + (i % 4) * 4;
-                      uint32_t w;
-                      asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(a) : "memory");
-                      if (srv_nonfinite<BF16>(w & 0xffffu)) w &= 0xffff0000u;
-                      if (srv_nonfinite<BF16>(w & 0xffff0000u)) w &= 0xffffu;
-                      asm volatile("st.shared.b32 [%0], %1;" ::"r"(a), "r"(w) : "memory");
-                    }
+        if (odd) {
+          for (int key = 0; key < 16; ++key) {
+#pragma unroll
+            for (int i = 0; i < HD / 8; ++i) {
+              uint32_t w;
+              asm volatile("ld.shared.b32 %0, [%1];"
+                           : "=r"(w)
+                           : "r"(at(sv, warp * 16 + key, i) + (lane & 3) * 4)
+                           : "memory");
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                const float v = srv_to_float<BF16>((w >> (16 * x)) & 0xffffu);
+                if (!isfinite(v)) {
+                  if (k0 + key <= lim[0]) o[i][x] += v;
+                  if (k0 + key <= lim[1]) o[i][2 + x] += v;
+                }
+              }
+            }
+          }
+          __syncwarp();
+          for (int i = lane; i < 16 * (HD / 2); i += 32) {
+            const uint32_t a = at(sv, warp * 16 + i / (HD / 2), (i % (HD / 2)) / 4) + (i % 4) * 4;
+            uint32_t w;
+            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(a) : "memory");
+            if (srv_nonfinite<BF16>(w & 0xffffu)) w &= 0xffff0000u;
+            if (srv_nonfinite<BF16>(w & 0xffff0000u)) w &= 0xffffu;
+            asm volatile("st.shared.b32 [%0], %1;" ::"r"(a), "r"(w) : "memory");
+          }
           __syncwarp();
           fence_proxy_async_smem();
         }
