@@ -8,7 +8,8 @@ Public surface:
   * make_optimized_transformer(model) -> nn.Module with forward(x, valid_token_mask)
   * TransformerConfig, TransformerParameters (weights container with the reference
     organizer model's module tree)
-  * ops: per-kernel wrappers (linear, layernorm, attention)
+  * ops: per-kernel wrappers (linear, layernorm, attention) and the serving operators
+    (prompt_attention, cache_append, cache_attention, cache_mass, cache_evict)
   * cases: the reference's 14 benchmark cases (IMPLEMENTED_CASES,
     case_number_for_model), all served by make_optimized_transformer
   * sharding: batch data parallelism (LPT shards, one process per GPU or one

@@ -3,7 +3,8 @@
 Each wrapper checks dtype, shape, contiguity and device (the reference's
 TORCH_CHECK conventions, kernels/csrc/case14_softmax.cpp:18-35) and launches on the
 current CUDA stream.  They exist for parity tests and for callers composing their
-own layer; the forward of ``B200Transformer`` runs the same kernels from C.
+own layer; the forward of ``B200Transformer`` runs the same kernels from C.  The serving
+operators at the end (prompts with grouped heads, a paged key/value cache) stand beside it.
 """
 from __future__ import annotations
 
