@@ -220,6 +220,15 @@ def serve_workspace_bytes(batch: int, tokens: int, heads: int, kv_heads: int, he
     return n
 
 
+def _serve_out(what: str, out: Optional[torch.Tensor], q: torch.Tensor) -> tuple:
+    """The output [tokens, heads, head_dim], made contiguous if not given, and its tttj_rows."""
+    if out is not None:
+        return out, _serve_rows(what, "out", out, q.shape, q.dtype, q.device)
+    _, heads, d = q.shape
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    return out, _pack_rows(out.data_ptr(), heads * d, d)
+
+
 def _serve_workspace(what: str, workspace: Optional[torch.Tensor], nbytes: int, device: torch.device) -> torch.Tensor:
     if workspace is None:
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
@@ -247,14 +256,13 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_offs
     tokens, heads, d = q.shape
     kv_heads = k.shape[1]
     batch, off = _serve_offsets(what, seq_offsets, device)
-    if out is None:
-        out = torch.empty((tokens, heads, d), dtype=dtype, device=device)
     rows, kv_rows = (tokens, heads, d), (tokens, kv_heads, d)
+    out, ro = _serve_out(what, out, q)
     s = _pack_seqs(off, 0, 0, 0, batch, tokens, 0, 0, 0, kind, heads, kv_heads, d,
                    0 if status is None else _serve_ints(what, "status", status, 1, device))
     rq, rk = _serve_rows(what, "q", q, rows, dtype, device), _serve_rows(what, "k", k, kv_rows, dtype, device)
-    rv, ro = _serve_rows(what, "v", v, kv_rows, dtype, device), _serve_rows(what, "out", out, rows, dtype, device)
-    lse = torch.empty((tokens, heads), dtype=torch.float32, device=device) if return_lse else None
+    rv = _serve_rows(what, "v", v, kv_rows, dtype, device)
+    lse = q.new_empty((tokens, heads), dtype=torch.float32) if return_lse else None
     ws = _serve_workspace(what, workspace, _serve_workspace_bytes(batch, tokens, kind, heads, kv_heads, d), device)
     rc = _call(device, _lib.lib().tttj_prompt_attention, s, rq, rk, rv, ro, lse.data_ptr() if return_lse else None,
                1 if causal else 0, d ** -0.5 if scale is None else scale, ws.data_ptr(), ws.shape[0])
@@ -283,13 +291,11 @@ def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         raise ValueError(f"{what}: the cache has head_dim {pages[3]}, q {d}")
     batch, off = _serve_offsets(what, seq_offsets, device)
     s, _ = _cache_seqs(what, off, batch, tokens, kind, heads, k_cache, page_table, cache_lens, status, device)
-    if out is None:
-        out = torch.empty((tokens, heads, d), dtype=dtype, device=device)
-    rows = (tokens, heads, d)
-    rq, ro = _serve_rows(what, "q", q, rows, dtype, device), _serve_rows(what, "out", out, rows, dtype, device)
+    out, ro = _serve_out(what, out, q)
+    rq = _serve_rows(what, "q", q, (tokens, heads, d), dtype, device)
     ck = _serve_pages(what, "k_cache", k_cache, pages, dtype, device)
     cv = _serve_pages(what, "v_cache", v_cache, pages, dtype, device)
-    lse = torch.empty((tokens, heads), dtype=torch.float32, device=device) if return_lse else None
+    lse = q.new_empty((tokens, heads), dtype=torch.float32) if return_lse else None
     ws = _serve_workspace(what, workspace, _serve_workspace_bytes(batch, tokens, kind, heads, kv_heads, d), device)
     rc = _call(device, _lib.lib().tttj_cache_attention, s, rq, ck, cv, ro, lse.data_ptr() if return_lse else None,
                min(max_new or 0, tokens), d ** -0.5 if scale is None else scale, ws.data_ptr(), ws.shape[0])
