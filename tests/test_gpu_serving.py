@@ -244,6 +244,21 @@ def test_cache_attention_nonfinite_values_reach_only_rows_that_see_them(new):
     _check_cache(out, lse, q, c, new, lens, 128**-0.5, rows=True)
 
 
+@pytest.mark.parametrize("new", [3, 150])
+@pytest.mark.parametrize("d", [32, 64, 128, 256])
+def test_cache_attention_nonfinite_values_in_split_keys(d, new):
+    """As above where one sequence's keys are shared out between CTAs: hidden values in the last
+    part, one that every row sees in the first."""
+    lens = [9001]
+    c = Cache(lens, 2, d, 64, torch.float16, 8)
+    for j, h, x in ((8999, 0, math.nan), (9000, 1, math.inf)):
+        c.v[c.table[0, j // 64].long(), j % 64, h, 5] = x
+    c.v[c.table[0, 1].long(), 3, 1, 7] = -math.inf
+    q = torch.randn(new, 8, d, device=DEV, generator=_gen(5)).half()
+    out, lse = ops.cache_attention(q, c.k, c.v, c.table, lengths_to_offsets([new]), c.lens, return_lse=True)
+    _check_cache(out, lse, q, c, [new], lens, d**-0.5, rows=True)
+
+
 def test_cache_attention_wrong_pages_and_lengths_are_contained():
     """Page numbers outside the cache stand for zeros, lengths for the table's slots."""
     lens = [100, 64, 30]
