@@ -58,7 +58,7 @@ static_assert(sizeof(TileInfo) <= 64, "item info slot is 64 bytes");
 // keys 150 us, of 64 keys 127.  At head_dim 256 (one query tile per item) steps of 128 keys and one
 // buffer of P: 111 against 182 us, prompts of 3000 and 4096 tokens, 8 / 2 heads.
 // What bounds it: with nearly all products left out the same prompts take 186 us, so the
-// softmax warps do, two per scheduler, 57 % of the MUFU's rate; the tensor pipe is half busy.
+// softmax warps do, two per scheduler; MUFU and tensor pipe are 51 % busy each.
 template <int HD>
 struct TileSmem : AtcSmem<HD> {  // tile sizes and stages as there
   using B = AtcSmem<HD>;
