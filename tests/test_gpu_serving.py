@@ -458,6 +458,21 @@ def test_cache_evict_special_masses():
     _check_evict(c, mass, pos, lens, 128, 16)
 
 
+@pytest.mark.parametrize("keep", [99, 100, 101, 159, 160, 161])
+def test_cache_evict_cut_beside_zero(keep):
+    """100 positive masses, 60 zeros of either sign, 40 negative ones, in any order."""
+    lens = [200, 200]
+    c, mass, pos = _evict_case(lens, 2, 64, 16, torch.float16, 9)
+    g = _gen(4)
+    for b in range(2):
+        for h in range(2):
+            row = torch.rand(200, device=DEV, generator=g) + 0.1
+            row[100:160] = torch.where(torch.rand(60, device=DEV, generator=g) < 0.5, 0.0, -0.0)
+            row[160:] *= -1
+            mass[b, h, :200] = row[torch.randperm(200, device=DEV, generator=g)]
+    _check_evict(c, mass, pos, lens, keep, 0)
+
+
 @pytest.mark.parametrize("length", [40000, 70000])
 def test_cache_evict_long(length):
     """Longer than what the selection holds in shared memory, and just below."""

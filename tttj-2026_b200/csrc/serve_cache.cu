@@ -88,9 +88,9 @@ __global__ void __launch_bounds__(APPEND_THREADS, 5) append_kernel(const AppendP
 // and holds EVICT_HELD of them per thread in registers (a longer range's rest is read again
 // where it is needed).  The keep-th largest value is found two bits at a time: everyone
 // counts the values above three thresholds, the warps' counts meet in every block's shared
-// memory, 16 rounds of one barrier each.  (A radix selection with histograms in shared memory: 123
-// against 50 us in all, 16 heads of 20000 - 32768 slots.)  Then ballots rank the
-// equal values, the holes (slots < keep that go) and the movers (slots >= keep that stay); the
+// memory, at most 17 rounds of one barrier each, about 2000 cycles.  (A radix selection with
+// histograms in shared memory: 123 against 50 us in all, 16 heads of 20000 - 32768 slots.)
+// Then ballots rank the equal values, the holes (slots < keep that go) and the movers (slots >= keep that stay); the
 // i-th mover goes to the i-th hole, so as few rows move as can, and since sources lie behind
 // the budget and destinations in front of it, no move reads what another writes.  All counts are
 // integers: the result does not depend on the order in which threads run.  Bound: for short
@@ -187,26 +187,40 @@ __global__ void __launch_bounds__(EVICT_MAX_THREADS) evict_kernel(const EvictPar
 #pragma unroll
   for (int i = 0; i < EVICT_HELD; ++i)
     if (key[i] != 0u && (long)ps[i] > edge) key[i] = 0xff800000u;
-  // The keep-th largest value, two bits a round; done early once a threshold has exactly `keep`
-  // values at or above it.
+  // The keep-th largest value.  First whether it is zero, as where more slots than go have
+  // gathered nothing (64 x 8 heads of 1025 - 1152 slots, a tenth of them zero: 26 against 34 us,
+  // since no threshold separates equal values).  Then two bits a round; done early once a
+  // threshold has exactly `keep` values at or above it.
+  constexpr uint32_t ZERO = 0x80000000u;  // the image of 0
+  static_assert(32 * EVICT_HELD < 1024, "counts of a warp take ten bits");
   uint32_t cut = 0;
 #pragma unroll 1
-  for (int shift = 30; shift >= 0; shift -= 2) {
-    const uint32_t c1 = cut | (1u << shift), c2 = cut | (2u << shift), c3 = cut | (3u << shift);
-    int n1 = 0, n2 = 0, n3 = 0;
+  for (int shift = 32; shift >= 0; shift -= 2) {
+    const bool first = shift == 32;
+    const uint32_t c1 = first ? ZERO : cut | (1u << shift), c2 = first ? ZERO + 1 : cut | (2u << shift),
+                   c3 = first ? 0xc0000000u : cut | (3u << shift);
+    unsigned packed = 0;  // live values at or above each threshold, ten bits each
 #pragma unroll
     for (int i = 0; i < EVICT_HELD; ++i) {
-      n1 += key[i] >= c1;
-      n2 += key[i] >= c2;
-      n3 += key[i] >= c3;
+      packed += key[i] >= c1 ? 1u : 0u;
+      packed += key[i] >= c2 ? 1u << 10 : 0u;
+      packed += key[i] >= c3 ? 1u << 20 : 0u;
     }
-    for (int j = rest + lane; j < w1; j += 32) {
-      const uint32_t x = key_of(mass[j], pos[j]);
-      n1 += x >= c1;
-      n2 += x >= c2;
-      n3 += x >= c3;
+    packed = __reduce_add_sync(FULL, packed);
+    int n1 = packed & 1023, n2 = packed >> 10 & 1023, n3 = packed >> 20;
+    if (rest < w1) {
+      int m1 = 0, m2 = 0, m3 = 0;
+      for (int j = rest + lane; j < w1; j += 32) {
+        const uint32_t x = key_of(mass[j], pos[j]);
+        m1 += x >= c1;
+        m2 += x >= c2;
+        m3 += x >= c3;
+      }
+      n1 += __reduce_add_sync(FULL, m1);
+      n2 += __reduce_add_sync(FULL, m2);
+      n3 += __reduce_add_sync(FULL, m3);
     }
-    const int4* c = share(__reduce_add_sync(FULL, n1), __reduce_add_sync(FULL, n2), __reduce_add_sync(FULL, n3));
+    const int4* c = share(n1, n2, n3);
     n1 = n2 = n3 = 0;
     for (int w = lane; w < all_warps; w += 32) {
       const int4 v = c[w];
@@ -217,6 +231,17 @@ __global__ void __launch_bounds__(EVICT_MAX_THREADS) evict_kernel(const EvictPar
     n1 = __reduce_add_sync(FULL, n1);
     n2 = __reduce_add_sync(FULL, n2);
     n3 = __reduce_add_sync(FULL, n3);
+    if (first) {
+      if (n1 >= keep && n2 < keep) {
+        cut = ZERO;
+        break;
+      }
+      if (n2 >= keep) {  // the first two bits are known
+        cut = n3 >= keep ? c3 : ZERO;
+        shift = 30;
+      }
+      continue;
+    }
     const int exact = n3 == keep ? 3 : n2 == keep ? 2 : n1 == keep ? 1 : 0;
     if (exact != 0) {
       cut = (cut | ((uint32_t)exact << shift)) - 1;  // all above it stay, no equal one does
