@@ -137,6 +137,17 @@ def test_prompt_attention_nonfinite_values_reach_only_rows_that_see_them(d, dtyp
         at += n
 
 
+@pytest.mark.parametrize("d", [64, 128])
+def test_prompt_attention_a_channel_of_nan_values(d):
+    """Every row sees a NaN in one channel, and hides others: that channel is NaN, no other is."""
+    q, k, v = _prompt([1500], 4, 2, d, torch.float16, 12)
+    v[:, 1, 5] = math.nan
+    out, lse = ops.prompt_attention(q, k, v, lengths_to_offsets([1500]), return_lse=True)
+    assert bool(torch.isnan(out[:, 2:, 5]).all())
+    v[:, 1, 5], out[:, 2:, 5] = 0, 0
+    _check(out, lse, q, k, v, 1500, 1500, d**-0.5)
+
+
 # -------------------------------------------------------------------------- paged cache
 class Cache:
     def __init__(self, lens, kv, d, page, dtype, seed, spare=5, heads_first=False, extra_pages=0):

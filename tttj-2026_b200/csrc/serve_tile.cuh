@@ -985,9 +985,9 @@ __device__ __forceinline__ bool tile_locate(const TileParams& p, const CacheView
   return page < p.s.num_pages;
 }
 
-// One row key by key, hidden keys left out.
+// The columns `need` (a bit per column of this lane) of one row key by key, hidden keys left out.
 template <int HD, bool BF16>
-__device__ void tile_redo_row(const TileParams& p, const SrvSeq& s, int b, int tok, int kvh, int g) {
+__device__ void tile_redo_row(const TileParams& p, const SrvSeq& s, int b, int tok, int kvh, int g, unsigned need) {
   const int lane = lane_id();
   constexpr int E = HD / 32;
   const int token = s.row0 + tok, head = kvh * p.group + g;
@@ -1000,6 +1000,12 @@ __device__ void tile_redo_row(const TileParams& p, const SrvSeq& s, int b, int t
   }
   const int keys = p.s.causal ? min(s.len, s.len - s.n + tok + 1) : s.len;
   for (int j = 0; j < keys; ++j) {
+    if (j % 32 == 0) {  // a NaN in sight settles its column
+      bool open = false;
+#pragma unroll
+      for (int i = 0; i < E; ++i) open |= (need >> i & 1) != 0 && acc[i] == acc[i];
+      if (!__any_sync(0xffffffffu, open)) break;
+    }
     long at_k, at_v;
     tile_locate(p, p.v, s, b, kvh, j, &at_v);
     const bool there = tile_locate(p, p.k, s, b, kvh, j, &at_k);
@@ -1024,11 +1030,16 @@ __device__ void tile_redo_row(const TileParams& p, const SrvSeq& s, int b, int t
       if (there) acc[i] = fmaf(e, srv_to_float<BF16>(vr[i]), acc[i]);
     }
   }
-  tile_store_row<HD, BF16>(p, token, head, acc, l == 0.f ? 0.f : 1.f / l, m, l);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  uint16_t* out = static_cast<uint16_t*>(p.out) + (long)token * p.o_tok + (long)head * p.o_head + lane * E;
+#pragma unroll
+  for (int i = 0; i < E; ++i)
+    if (need >> i & 1) out[i] = (uint16_t)srv_pack<BF16>(acc[i] * inv, 0.f);
 }
 
-// A row whose result is not finite: again, if a value that it does not see, among those that
-// its tile's products read, is not finite.
+// A row whose result is not finite: again in the columns in which a value that it does not see,
+// among those that its tile's products read, is not finite.  (The log-sum-exp owes nothing to
+// values.)
 template <int HD, bool BF16>
 __device__ __forceinline__ void tile_mend_row(const TileParams& p, int b, int tok0, int rtok, int kvh, int g) {
   constexpr int E = HD / 32;
@@ -1036,17 +1047,17 @@ __device__ __forceinline__ void tile_mend_row(const TileParams& p, int b, int to
   const int tok = tok0 + rtok;
   if (tok >= s.n) return;
   const int end = tile_kv_tiles(tile_kv_end(s, 1, tok0, p.tile_tokens)) * ATC_BN;
-  bool odd = false;
+  unsigned need = 0;
 #pragma unroll 4
   for (int j = max(0, s.len - s.n + tok + 1); j < min(s.len, end); ++j) {
     long at;
     if (tile_locate(p, p.v, s, b, kvh, j, &at)) {
       const uint16_t* v = static_cast<const uint16_t*>(p.v.data) + at + lane_id() * E;
 #pragma unroll
-      for (int i = 0; i < E; ++i) odd |= srv_nonfinite<BF16>(v[i]);
+      for (int i = 0; i < E; ++i) need |= srv_nonfinite<BF16>(v[i]) ? 1u << i : 0u;
     }
   }
-  if (__any_sync(0xffffffffu, odd)) tile_redo_row<HD, BF16>(p, s, b, tok, kvh, g);
+  if (__any_sync(0xffffffffu, need != 0)) tile_redo_row<HD, BF16>(p, s, b, tok, kvh, g, need);
 }
 
 template <int HD, bool BF16>
