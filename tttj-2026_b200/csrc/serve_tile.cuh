@@ -23,14 +23,12 @@
 // meet P = 0 in the product, and 0 x NaN is NaN.  V rows behind the last key (stale pages, the
 // next sequence) are zeroed in shared memory.  For the others the result is looked at: a row
 // that is not finite may owe it to a value that it does not see, so the joining kernel searches
-// its hidden values, and where one is not finite computes the row again, key by key.
+// its hidden values, and computes the columns in which one is not finite again, key by key.
 // (Searching every V tile on the diagonal for such values took a warp 2000 cycles per tile,
 // in which the tile's product waited: prompts of 128 - 256 tokens.)
 //
 // Every wait is bounded; a role that gives up records SRV_DEV_TIMEOUT and unwinds.
 #pragma once
-#include <type_traits>
-
 #include "attention_tc.cuh"
 #include "serve_dev.cuh"
 
