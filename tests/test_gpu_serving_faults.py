@@ -1,0 +1,48 @@
+"""GPU: serving operators, calls that went wrong once: tokens behind the table, tensors with
+gradients or tangents, weights outside fp32's range, calls of two threads, device waits that
+give up, a captured step that carries its own state.  Tolerances as in test_gpu_serving.py."""
+import math
+
+import pytest
+import torch
+
+from serving_reference import cache_rows, lengths_to_offsets
+from test_gpu_serving import Cache, _check, _gen
+from tttj_2026_b200 import ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+# -------------------------------------------------------------------------------- append
+@pytest.mark.parametrize("with_seen", [False, True])
+@pytest.mark.parametrize("length", [65, 66, 67, 1 << 30, 2**31 - 1])
+def test_append_keeps_live_slots_when_a_length_exceeds_the_table(length, with_seen):
+    """64 slots, three new tokens: those whose slot is not in the table are dropped, and no slot in
+    front of the new tokens changes."""
+    new, lens = [3, 1], [length, 64]
+    c = Cache([64, 64], 2, 64, 16, torch.float16, 3)
+    c.lens = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    want_k, want_v = c.k.clone(), c.v.clone()
+    k = torch.randn(4, 2, 64, device=DEV, generator=_gen(1)).half()
+    pos = torch.full((2, 2, 64), 77, dtype=torch.int32, device=DEV)
+    mass = torch.full((2, 2, 64), 5.0, device=DEV)
+    want_pos, want_mass = pos.clone(), mass.clone()
+    seen = torch.tensor([1000, 2000], dtype=torch.int32, device=DEV) if with_seen else None
+    at = 0
+    for b, (n, m) in enumerate(zip(new, lens)):
+        for i in range(n):
+            slot = m - n + i
+            if slot < 64:
+                page = c.table[b, slot // 16].long()
+                want_k[page, slot % 16], want_v[page, slot % 16] = k[at + i], k[at + i] + 1
+                want_pos[b, :, slot] = (1000 * (b + 1) if with_seen else m) - n + i
+                want_mass[b, :, slot] = 0
+        at += n
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    ops.cache_append(k, k + 1, c.k, c.v, c.table, lengths_to_offsets(new), c.lens, positions=pos, mass=mass, seen=seen,
+                     status=status)
+    assert int(status) == 0x402
+    assert torch.equal(c.k.view(torch.int16), want_k.view(torch.int16))
+    assert torch.equal(c.v.view(torch.int16), want_v.view(torch.int16))
+    assert torch.equal(pos, want_pos) and torch.equal(mass, want_mass)

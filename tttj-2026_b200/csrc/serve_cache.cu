@@ -32,13 +32,17 @@ __global__ void __launch_bounds__(APPEND_THREADS, 5) append_kernel(const AppendP
       if (p.s.seq_off[mid] <= t) lo = mid; else hi = mid - 1;
     }
     const SrvSeq q = srv_seq(p.s, lo);
-    const int slot = q.len - q.n + (t - q.row0);
+    // The slot by the length as it was given: with the clamped one, the tokens of a sequence that
+    // has outgrown its table would land on the live slots at the table's end.
+    const int len = p.s.lens[lo];
+    const long slot = (long)len - q.n + (t - q.row0);
     int page = p.s.num_pages;
-    if (t >= q.row0 && t < q.row0 + q.n && slot >= 0) page = srv_page(p.s, lo, slot);
+    if (t >= q.row0 && t < q.row0 + q.n && slot >= 0 && slot < (long)p.s.pages_per_seq << p.s.page_shift)
+      page = srv_page(p.s, lo, (int)slot);
     s_b[threadIdx.x] = lo;
-    s_slot[threadIdx.x] = slot;
+    s_slot[threadIdx.x] = (int)slot;
     s_page[threadIdx.x] = page;
-    s_first[threadIdx.x] = (p.seen != nullptr ? p.seen[lo] : q.len) - q.n + (t - q.row0);
+    s_first[threadIdx.x] = (p.seen != nullptr ? p.seen[lo] : len) - q.n + (t - q.row0);
   }
   // Tokens look at their own sequence only: offsets that do not rise are found here.
   if (p.s.status != nullptr && blockIdx.x == 0)
