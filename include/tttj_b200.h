@@ -379,8 +379,9 @@ int tttj_cache_attention(const tttj_seqs* s, const tttj_rows* q, const tttj_page
  * [batch][kv_heads][pages_per_seq * page_size], contiguous) a new slot's position becomes
  * seen[b] - n + i (seen: tokens the sequence has had, new ones included; NULL =
  * cache_lens, which differ once tokens were evicted) and its mass 0.  Here cache_lens is not
- * clamped: new tokens whose slot is not in the table are dropped, the slots in it stay as they
- * are. */
+ * clamped: new tokens whose slot is not in the table (behind its end, or in front of its first
+ * slot where len < n) are dropped, the slots in it stay as they are, and `status` records
+ * TTTJ_DEV_BAD_LENS. */
 int tttj_cache_append(const tttj_seqs* s, const tttj_rows* k, const tttj_rows* v,
                       const tttj_pages* k_cache, const tttj_pages* v_cache, int32_t* positions,
                       float* mass, const int32_t* seen, void* stream);

@@ -46,3 +46,14 @@ def test_append_keeps_live_slots_when_a_length_exceeds_the_table(length, with_se
     assert torch.equal(c.k.view(torch.int16), want_k.view(torch.int16))
     assert torch.equal(c.v.view(torch.int16), want_v.view(torch.int16))
     assert torch.equal(pos, want_pos) and torch.equal(mass, want_mass)
+
+
+def test_append_says_that_it_dropped_tokens_before_the_first_slot():
+    c = Cache([64, 64], 2, 64, 16, torch.float16, 3)
+    k = torch.randn(6, 2, 64, device=DEV, generator=_gen(1)).half()
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    for lens, want in (([4, 2], 0), ([3, 2], 0x402), ([4, 0], 0x402), ([4, -1], 0x402)):
+        status.zero_()
+        c.lens = torch.tensor(lens, dtype=torch.int32, device=DEV)
+        ops.cache_append(k, k, c.k, c.v, c.table, lengths_to_offsets([4, 2]), c.lens, status=status)
+        assert int(status) == want, lens

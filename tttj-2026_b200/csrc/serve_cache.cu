@@ -37,8 +37,12 @@ __global__ void __launch_bounds__(APPEND_THREADS, 5) append_kernel(const AppendP
     const int len = p.s.lens[lo];
     const long slot = (long)len - q.n + (t - q.row0);
     int page = p.s.num_pages;
-    if (t >= q.row0 && t < q.row0 + q.n && slot >= 0 && slot < (long)p.s.pages_per_seq << p.s.page_shift)
-      page = srv_page(p.s, lo, (int)slot);
+    if (t >= q.row0 && t < q.row0 + q.n) {
+      if (slot >= 0 && slot < (long)p.s.pages_per_seq << p.s.page_shift)
+        page = srv_page(p.s, lo, (int)slot);
+      else
+        report_status(p.s.status, SRV_DEV_BAD_LENS);
+    }
     s_b[threadIdx.x] = lo;
     s_slot[threadIdx.x] = (int)slot;
     s_page[threadIdx.x] = page;

@@ -322,7 +322,8 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     With ``positions`` (int32) / ``mass`` (fp32), both [B, kv_heads, P * page_size], a new
     slot's position becomes seen[b] - n + i and its mass 0; ``seen`` int32 [B] counts the tokens
     of each sequence, new ones included (default cache_lens; they differ once tokens were
-    evicted).  New tokens whose slot would not be in the table are dropped."""
+    evicted).  New tokens whose slot would not be in the table are dropped, and ``status`` says
+    so (TTTJ_DEV_BAD_LENS)."""
     what = "cache_append"
     if k.dim() != 3 or k_cache.dim() != 4:
         raise ValueError(f"{what}: k must be [tokens, kv_heads, head_dim], k_cache [pages, page_size, kv_heads, head_dim]")
