@@ -2,6 +2,7 @@
 gradients or tangents, weights outside fp32's range, calls of two threads, device waits that
 give up, a captured step that carries its own state.  Tolerances as in test_gpu_serving.py."""
 import math
+import threading
 
 import pytest
 import torch
@@ -57,3 +58,48 @@ def test_append_says_that_it_dropped_tokens_before_the_first_slot():
         c.lens = torch.tensor(lens, dtype=torch.int32, device=DEV)
         ops.cache_append(k, k, c.k, c.v, c.table, lengths_to_offsets([4, 2]), c.lens, status=status)
         assert int(status) == want, lens
+
+
+# ------------------------------------------------------------------------------- threads
+@pytest.mark.parametrize("op", ["attend", "mass"])
+def test_two_threads_with_batches_of_different_sizes(op, monkeypatch):
+    """Calls need shared memory by their number of sequences: neither thread's launch may depend on
+    the other's."""
+    recorded = []
+    real = ops._call
+
+    def record(device, fn, *args):
+        recorded.append((fn, args))
+        return real(device, fn, *args)
+
+    monkeypatch.setattr(ops, "_call", record)
+    kept = []
+    for batch in (1, 1024):
+        c = Cache([17] * batch, 1, 64, 32, torch.float16, batch)
+        q = torch.randn(batch, 2, 64, device=DEV, generator=_gen(5)).half()
+        off = lengths_to_offsets([1] * batch)
+        mass, lse = torch.zeros(batch, 1, c.table.shape[1] * 32, device=DEV), torch.zeros(batch, 2, device=DEV)
+        ws = torch.empty(ops.serve_workspace_bytes(batch, batch, 2, 1, 64), dtype=torch.uint8, device=DEV)
+        if op == "mass":
+            out = ops.cache_mass(q, lse, c.k, c.table, off, c.lens, mass, max_new=1)
+        else:
+            out = ops.cache_attention(q, c.k, c.v, c.table, off, c.lens, max_new=1, workspace=ws)
+        kept.append((c, q, off, mass, lse, ws, out))
+    torch.cuda.synchronize()
+    failed = [0, 0]
+
+    def loop(i):
+        torch.cuda.set_device(0)
+        fn, args = recorded[i]
+        stream = torch.cuda.Stream()
+        for _ in range(300):
+            for _ in range(100):
+                failed[i] += fn(*args, stream.cuda_stream) != 0
+            stream.synchronize()
+
+    threads = [threading.Thread(target=loop, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert failed == [0, 0]

@@ -9,10 +9,12 @@ template <int HD, bool BF16>
 cudaError_t launch(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const MassParams& p, int grid,
                    cudaStream_t stream) {
   auto kern = mass_kernel<HD, BF16>;
-  static_assert(MassSmem<HD>::FIXED + SRV_MAX_BATCH * ((int)sizeof(SrvSeq) + 8) + 4 <= 232448,
-                "shared memory exceeds the 227 KB per-CTA limit");
   const int smem = MassSmem<HD>::FIXED + p.s.batch * ((int)sizeof(SrvSeq) + 8) + 4;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  // The most that any call needs, for every call: the limit is the kernel's, and a call of another
+  // thread must not lower it between here and the launch.
+  constexpr int most = MassSmem<HD>::FIXED + SRV_MAX_BATCH * ((int)sizeof(SrvSeq) + 8) + 4;
+  static_assert(most <= 232448, "shared memory exceeds the 227 KB per-CTA limit");
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
   if (e != cudaSuccess) return e;
   return launch_pdl(kern, dim3(grid), dim3(MASS_THREADS), smem, stream, tm_q, tm_k, p);
 }

@@ -11,8 +11,11 @@ cudaError_t launch(const CUtensorMap& tm_k, const CUtensorMap& tm_v, const StepP
   const int prefix = (p.s.batch + 1) * (int)sizeof(long);
   const int smem = StepSmem<HD>::FIXED + prefix;
   auto kern = step_kernel<HD, BF16>;
-  static_assert(StepSmem<HD>::FIXED + (SRV_MAX_BATCH + 1) * 8 <= 232448, "shared memory exceeds the 227 KB per-CTA limit");
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  // The limit is the kernel's, not the launch's: set to the most that any call needs, so that a
+  // call of another thread does not lower it between here and the launch.
+  constexpr int most = StepSmem<HD>::FIXED + (SRV_MAX_BATCH + 1) * (int)sizeof(long);
+  static_assert(most <= 232448, "shared memory exceeds the 227 KB per-CTA limit");
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
   if (e != cudaSuccess) return e;
   e = launch_pdl(kern, dim3(grid), dim3(STEP_THREADS), smem, stream, tm_k, tm_v, p);
   if (e != cudaSuccess) return e;
