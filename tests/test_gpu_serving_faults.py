@@ -60,6 +60,44 @@ def test_append_says_that_it_dropped_tokens_before_the_first_slot():
         assert int(status) == want, lens
 
 
+# ----------------------------------------------------------------------------- gradients
+def _call_all(q, k, lse, c, mass):
+    """Every operator, as a list of (name, call of its floating-point tensors, those tensors)."""
+    off = lengths_to_offsets([1, 1])
+    pos = torch.arange(mass.shape[2], device=DEV, dtype=torch.int32).expand(mass.shape).contiguous()
+    return [
+        ("prompt", lambda a: ops.prompt_attention(a[0], a[1], a[2], off, out=a[3]), [q, k, k, torch.empty_like(q)]),
+        ("attend", lambda a: ops.cache_attention(a[0], a[1], a[2], c.table, off, c.lens, out=a[3]),
+         [q, c.k, c.v, torch.empty_like(q)]),
+        ("append", lambda a: ops.cache_append(a[0], a[1], a[2], a[3], c.table, off, c.lens, mass=a[4]),
+         [k, k, c.k.clone(), c.v.clone(), mass.clone()]),
+        ("mass", lambda a: ops.cache_mass(a[0], a[1], a[2], c.table, off, c.lens, a[3], out=a[4]),
+         [q, lse, c.k, mass, mass.clone()]),
+        ("evict", lambda a: ops.cache_evict(a[0], pos, a[1], a[2], c.table, c.lens, 16),
+         [mass, c.k.clone(), c.v.clone()]),
+    ]
+
+
+def _grad_inputs():
+    c = Cache([20, 30], 2, 64, 16, torch.float16, 8)
+    q = torch.randn(2, 4, 64, device=DEV, generator=_gen(5)).half()
+    lse = torch.zeros(2, 4, device=DEV)
+    mass = torch.rand(2, 2, c.table.shape[1] * 16, device=DEV)
+    return q, q[:, :2], lse, c, mass
+
+
+def test_every_tensor_with_a_gradient_is_refused():
+    for name, call, tensors in _call_all(*_grad_inputs()):
+        call(tensors)
+        for i in range(len(tensors)):
+            a = [t.clone() for t in tensors]
+            a[i].requires_grad_()
+            with pytest.raises(ValueError, match="inference only"):
+                call(a)
+            with torch.no_grad():
+                call(a)
+
+
 # ------------------------------------------------------------------------------- threads
 @pytest.mark.parametrize("op", ["attend", "mass"])
 def test_two_threads_with_batches_of_different_sizes(op, monkeypatch):

@@ -409,6 +409,8 @@ def cache_mass(q: torch.Tensor, lse: torch.Tensor, k_cache: torch.Tensor, page_t
     s, cap = _cache_seqs(what, off, batch, tokens, kind, heads, k_cache, page_table, cache_lens, status, device)
     if lse.dtype != torch.float32 or lse.shape != rows[:2] or lse.device != device or not lse.is_contiguous():
         raise ValueError(f"{what}: lse must be a contiguous float32 tensor [{tokens}, {heads}] on {device}")
+    if lse.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what}: inference only (lse requires a gradient)")
     slots = (batch, pages[2], cap)
     ms = _slot_tensor(what, "mass", mass, torch.float32, slots, device)
     if out is None:
