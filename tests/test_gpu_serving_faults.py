@@ -98,6 +98,20 @@ def test_every_tensor_with_a_gradient_is_refused():
                 call(a)
 
 
+def test_every_tensor_with_a_tangent_is_refused():
+    """Forward-mode derivatives would be dropped silently."""
+    fwd = torch.autograd.forward_ad
+    for name, call, tensors in _call_all(*_grad_inputs()):
+        for i in range(len(tensors)):
+            with fwd.dual_level():
+                a = list(tensors)
+                a[i] = fwd.make_dual(tensors[i].clone(), torch.ones_like(tensors[i]))
+                with pytest.raises(ValueError, match="inference only"):
+                    call(a)
+                call(tensors)  # no tangent: served
+        call(tensors)
+
+
 # ------------------------------------------------------------------------------- threads
 @pytest.mark.parametrize("op", ["attend", "mass"])
 def test_two_threads_with_batches_of_different_sizes(op, monkeypatch):

@@ -14,6 +14,7 @@ import struct
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from . import _lib
 
@@ -125,7 +126,8 @@ def selftest_wait_timeout(status: torch.Tensor, limit_ns: int) -> None:
 #   CUDA graphs and replayed with new ones.  They are bounds-checked there; ``status`` (int32
 #   [1], zeroed by the caller) records a wrong one (include/tttj_b200.h, TTTJ_DEV_BAD_*).
 # * Launches go to the current stream of the tensors' device, whichever device is current.
-# * Inference only: tensors that require gradients are refused while gradients are enabled.
+# * Inference only: tensors that require gradients are refused while gradients are enabled, and
+#   tensors that carry a forward-mode tangent.
 
 _SERVE_DTYPES = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
 # tttj_rows, tttj_pages and tttj_seqs of include/tttj_b200.h as bytes in C layout: a decode
@@ -144,6 +146,14 @@ def _call(device: torch.device, fn, *args) -> int:
         return fn(*args, torch._C._cuda_getCurrentRawStream(index))
 
 
+def _refuse_gradient(what: str, name: str, t: torch.Tensor) -> None:
+    """Raise if a derivative of ``t`` is wanted: the operators would drop it silently."""
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what}: inference only ({name} requires a gradient)")
+    if _forward_ad._current_level >= 0 and _forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{what}: inference only ({name} carries a forward-mode tangent)")
+
+
 def _serve_rows(what: str, name: str, t: torch.Tensor, shape: tuple, dtype: torch.dtype, device: torch.device) -> bytes:
     if t.shape != shape or t.dtype != dtype or t.device != device:
         raise ValueError(f"{what}: {name} must be [tokens, heads, head_dim] = {list(shape)}, {dtype} on {device}, "
@@ -151,8 +161,8 @@ def _serve_rows(what: str, name: str, t: torch.Tensor, shape: tuple, dtype: torc
     tok, head, one = t.stride()
     if one != 1:
         raise ValueError(f"{what}: head_dim of {name} must be contiguous")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{what}: inference only ({name} requires a gradient)")
+    if t.requires_grad or _forward_ad._current_level >= 0:
+        _refuse_gradient(what, name, t)
     return _pack_rows(t.data_ptr(), tok, head)
 
 
@@ -169,8 +179,8 @@ def _serve_pages(what: str, name: str, t: torch.Tensor, shape: tuple, dtype: tor
     page, slot, head, one = t.stride()
     if one != 1:
         raise ValueError(f"{what}: head_dim of {name} must be contiguous")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{what}: inference only ({name} requires a gradient)")
+    if t.requires_grad or _forward_ad._current_level >= 0:
+        _refuse_gradient(what, name, t)
     return _pack_pages(t.data_ptr(), page, slot, head)
 
 
@@ -308,8 +318,8 @@ def _slot_tensor(what: str, name: str, t: torch.Tensor, dtype: torch.dtype, shap
     if t.dtype != dtype or t.shape != shape or t.device != device or not t.is_contiguous():
         raise ValueError(f"{what}: {name} must be a contiguous {dtype} tensor {list(shape)} "
                          f"(sequences, kv_heads, slots) on {device}")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{what}: inference only ({name} requires a gradient)")
+    if t.requires_grad or _forward_ad._current_level >= 0:
+        _refuse_gradient(what, name, t)
     return t.data_ptr()
 
 
@@ -409,8 +419,8 @@ def cache_mass(q: torch.Tensor, lse: torch.Tensor, k_cache: torch.Tensor, page_t
     s, cap = _cache_seqs(what, off, batch, tokens, kind, heads, k_cache, page_table, cache_lens, status, device)
     if lse.dtype != torch.float32 or lse.shape != rows[:2] or lse.device != device or not lse.is_contiguous():
         raise ValueError(f"{what}: lse must be a contiguous float32 tensor [{tokens}, {heads}] on {device}")
-    if lse.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{what}: inference only (lse requires a gradient)")
+    if lse.requires_grad or _forward_ad._current_level >= 0:
+        _refuse_gradient(what, "lse", lse)
     slots = (batch, pages[2], cap)
     ms = _slot_tensor(what, "mass", mass, torch.float32, slots, device)
     if out is None:
