@@ -112,6 +112,44 @@ def test_every_tensor_with_a_tangent_is_refused():
         call(tensors)
 
 
+# ---------------------------------------------------------------------------------- mass
+@pytest.mark.parametrize("shift", [0.0, 5.0, 40.0, 86.0, 88.0, 95.0, 400.0, -60.0, -300.0])
+def test_mass_far_from_the_log_sum_exp(shift):
+    """One row after the other (each column of the accumulator) has an lse that lies `shift` below its
+    largest score, the others' weights are zero: weights grow up to fp32's overflow, and to
+    infinity beyond; weights of zero leave a mass of zero."""
+    d, n, m, heads = 64, 3, 900, 16
+    c = Cache([m], 2, d, 16, torch.float16, 8)
+    q = torch.randn(n, heads, d, device=DEV, generator=_gen(5)).half()
+    off = lengths_to_offsets([n])
+    k = cache_rows(c.k, c.table, 0, m).double()
+    s = torch.einsum("nhd,mhd->nhm", q.double(), k.repeat_interleave(heads // 2, 1)) * d**-0.5
+    hidden = torch.ones(n, m, dtype=torch.bool, device=DEV).triu(m - n + 1)
+    s.masked_fill_(hidden[:, None], -math.inf)
+    sa = torch.einsum("nhd,mhd->nhm", q.double().abs(), k.abs().repeat_interleave(heads // 2, 1)) * d**-0.5
+    zeros = torch.zeros(1, 2, c.table.shape[1] * 16, device=DEV)
+    big = torch.finfo(torch.float32).max
+    for i in range(n):
+        for h in range(heads):
+            lse = torch.full((n, heads), 1e4, device=DEV)
+            lse[i, h] = s[i, h].max() - shift
+            got = ops.cache_mass(q, lse, c.k, c.table, off, c.lens, zeros)[0, :, :m].double()
+            assert bool((got[1 - h // 8] == 0).all())
+            got, g = got[h // 8], lse[i, h].double()
+            want = torch.exp(s[i, h] - g)
+            # its score's error (an fp32 sum of d products), the exponent's roundings, and what is
+            # too small for a normal number
+            rel = d * 2.0**-24 * sa[i, h] + 2.0**-21 * (1 + torch.nan_to_num(s[i, h].abs(), posinf=0) + g.abs())
+            tol = want * rel + 2.0**-125
+            assert not bool(torch.isnan(got).any())
+            assert bool(torch.isposinf(got)[want - tol > big].all())
+            fits = want + tol < big
+            err = (got - want).abs()
+            assert bool((err <= tol)[fits].all()), f"{float((err / tol)[fits].max()):.2f} times the tolerance"
+            if shift == -300.0:
+                assert bool((got == 0).all())
+
+
 # ------------------------------------------------------------------------------- threads
 @pytest.mark.parametrize("op", ["attend", "mass"])
 def test_two_threads_with_batches_of_different_sizes(op, monkeypatch):

@@ -110,26 +110,30 @@ __device__ __forceinline__ float srv_max3(float a, float b, float c) {
   return d;
 }
 
-// 2^x for a pair of x <= 8 on the FMA pipe, as exp2_fma2 but as exact as ex2.approx (degree
-// 5: max relative error 2.1e-7 in fp32 Horner arithmetic, coefficients fitted for this library
-// by a Remez exchange on the relative error) and NaN for NaN: 2^j multiplies, since adding it into
-// the bits of a NaN would give a number.
+// 2^x for a pair on the FMA pipe, as exp2_fma2 but as exact as ex2.approx (degree 5: max relative
+// error 2.1e-7 in fp32 Horner arithmetic, coefficients fitted for this library by a Remez exchange
+// on the relative error) and for every x: infinity where 2^x is none, 0 below 2^-125.5, NaN for
+// NaN (2^j multiplies, since adding it into the bits of a NaN would give a number).  The
+// polynomial is twice 2^f and the scale 2^(j-1), a normal number for j = rint(x) up to 128 and 0
+// for j = -126, to which x is clamped from below.
 __device__ __forceinline__ float2 exp2_fine2(float2 x) {
   float a, b;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(a) : "f"(x.x), "f"(-126.0f));
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(b) : "f"(x.y), "f"(-126.0f));
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(a) : "f"(a), "f"(128.0f));
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(b) : "f"(b), "f"(128.0f));
   const unsigned long long xm = pk2(a, b);
   const unsigned long long magic = pk2(12582912.0f, 12582912.0f);
   const unsigned long long t = add2p(xm, magic);  // rint(x) in the low mantissa bits
   const unsigned long long f = sub2p(xm, sub2p(t, magic));
-  unsigned long long p = fma2p(f, pk2(1.327647245e-03f, 1.327647245e-03f), pk2(9.675540961e-03f, 9.675540961e-03f));
-  p = fma2p(f, p, pk2(5.550713092e-02f, 5.550713092e-02f));
-  p = fma2p(f, p, pk2(2.402212024e-01f, 2.402212024e-01f));
-  p = fma2p(f, p, pk2(6.931469440e-01f, 6.931469440e-01f));
-  p = fma2p(f, p, pk2(1.000000119e+00f, 1.000000119e+00f));
+  unsigned long long p = fma2p(f, pk2(2.655294490e-03f, 2.655294490e-03f), pk2(1.9351081922e-02f, 1.9351081922e-02f));
+  p = fma2p(f, p, pk2(1.1101426184e-01f, 1.1101426184e-01f));
+  p = fma2p(f, p, pk2(4.804424048e-01f, 4.804424048e-01f));
+  p = fma2p(f, p, pk2(1.386293888e+00f, 1.386293888e+00f));
+  p = fma2p(f, p, pk2(2.000000238e+00f, 2.000000238e+00f));
   const float2 tf = upk2(t);
-  return upk2(mul2p(p, pk2(__int_as_float((__float_as_int(tf.x) << 23) + 0x3f800000),
-                           __int_as_float((__float_as_int(tf.y) << 23) + 0x3f800000))));
+  return upk2(mul2p(p, pk2(__int_as_float((__float_as_int(tf.x) << 23) + 0x3f000000),
+                           __int_as_float((__float_as_int(tf.y) << 23) + 0x3f000000))));
 }
 
 // tmem_wait_ld for a load whose registers are first used after other work: naming them keeps
