@@ -15,6 +15,8 @@
 //   * a run that does not cover a row block's whole key range leaves (max, sum, O) in
 //     the workspace, and a second small kernel joins the runs of each row in order.
 #pragma once
+#include <math_constants.h>
+
 #include "serve_dev.cuh"
 
 namespace tttj {
@@ -196,6 +198,7 @@ __global__ void __launch_bounds__(STEP_THREADS, step_ctas_per_sm(HD))
   const float scale = p.scale_log2;
   long it = 0;
   bool first_run = true;
+  bool ok = true;  // false for good once a wait gave up (warp-uniform)
   for (long u = u0; u < u1;) {
     const StepRun r = step_run(p, pre, u, u1);
     const int rows = r.q.n * p.group;
@@ -224,13 +227,14 @@ __global__ void __launch_bounds__(STEP_THREADS, step_ctas_per_sm(HD))
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
     // Slots from here on are hidden from some row of the block (or from all).
     const int all_see = p.s.causal ? r.q.len - r.q.n + 1 : r.q.len;
-    bool ok = true;
 
-    for (int t = r.t0; t < r.t1; ++t, ++it) {
+    for (int t = r.t0; ok && t < r.t1; ++t, ++it) {
       const int st = (int)(it % SM::STAGES);
-      ok = srv_wait(bar_full + 8 * st, (uint32_t)((it / SM::STAGES) & 1), abort_flag, p.wait_limit_ns);
-      if (!__all_sync(0xffffffffu, ok)) {
-        ok = false;
+      ok = __all_sync(0xffffffffu, srv_wait(bar_full + 8 * st, (uint32_t)((it / SM::STAGES) & 1), abort_flag,
+                                            p.wait_limit_ns));
+      if (!ok) {
+        *abort_flag = 1;
+        if (lane == 0) report_status(p.s.status, SRV_DEV_TIMEOUT);
         break;
       }
       const int k0 = t * STEP_KEYS + warp * 16;  // this warp's 16 keys
@@ -357,10 +361,19 @@ __global__ void __launch_bounds__(STEP_THREADS, step_ctas_per_sm(HD))
       if (lane == 0) mbar_arrive(bar_empty + 8 * st);
     }
     if (!ok) {
-      // A wait gave up: the other consumers see the flag and leave at their next wait;
-      // nobody reaches the barriers below for this run.
-      *abort_flag = 1;
-      if (lane == 0) report_status(p.s.status, SRV_DEV_TIMEOUT);
+      // A wait gave up, here or in a run before.  This warp waits for no tile any more (and frees no
+      // stage: the producer and the other consumers see the flag, or give up in turn), but it
+      // takes part in the barriers of every run that is left, with NaN for its share: no row whose
+      // keys were not all read looks like a result.
+#pragma unroll
+      for (int i = 0; i < HD / 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][e] = CUDART_NAN_F;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        m[e] = 0.f;
+        l[e] = CUDART_NAN_F;
+      }
     }
 
     // Join the four warps: common maximum per row, then their outputs added quarter by
@@ -437,7 +450,6 @@ __global__ void __launch_bounds__(STEP_THREADS, step_ctas_per_sm(HD))
     sync4();
     first_run = false;
     u += r.t1 - r.t0;
-    if (!ok) it += r.t1 - r.t0;  // keep the stage count; the next wait returns at once
   }
 }
 
