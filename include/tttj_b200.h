@@ -359,6 +359,16 @@ typedef struct tttj_seqs {
 #define TTTJ_DEV_BAD_LENS 0x402    /* status: lengths or offsets outside the call's tensors */
 #define TTTJ_DEV_SERVE_TIMEOUT 0x403 /* status: a bounded device wait gave up */
 
+/* A wait that gave up (2 s) is also noted in a word of the device that every serving call looks
+ * at without synchronising: the next one on that device returns TTTJ_ERR_DEVICE_TIMEOUT once and
+ * launches nothing; the results of the call that gave up are invalid.  tttj_serve_status
+ * synchronises the current device, reads the word and clears it (replayed graphs, the last call):
+ * *device_status = 0 when healthy. */
+int tttj_serve_status(int* device_status);
+/* Failure-detection self test: a kernel's bounded wait on nothing gives up after limit_ns (at most
+ * 1 s) and is reported as a serving kernel reports it, in *status (nullable) too. */
+int tttj_serve_selftest_timeout(int32_t* status, uint64_t limit_ns, void* stream);
+
 /* out = softmax(scale q k^T) v inside every sequence (causal: token i sees tokens <= i),
  * lse (nullable) [tokens][heads] = log sum exp of the scaled scores.  The workspace
  * (tttj_serve_workspace_bytes with cache_lens = NULL; 256-byte aligned, any contents) must

@@ -2,7 +2,10 @@
 gradients or tangents, weights outside fp32's range, calls of two threads, device waits that
 give up, a captured step that carries its own state.  Tolerances as in test_gpu_serving.py."""
 import math
+import subprocess
+import sys
 import threading
+from pathlib import Path
 
 import pytest
 import torch
@@ -193,3 +196,61 @@ def test_two_threads_with_batches_of_different_sizes(op, monkeypatch):
     for t in threads:
         t.join()
     assert failed == [0, 0]
+
+
+# --------------------------------------------------------------------- failure detection
+@pytest.mark.parametrize("which", range(5))
+@pytest.mark.parametrize("with_status", [False, True])
+def test_a_wait_that_gave_up_is_reported_by_the_next_call(which, with_status):
+    """A 2 ms wait on nothing, reported as a kernel's would be: the next call raises once and launches
+    nothing, the one after it is served."""
+    name, call, tensors = _call_all(*_grad_inputs())[which]
+    want = call(tensors)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    ops.serve_selftest_timeout(torch.device(DEV), status=status if with_status else None)
+    torch.cuda.synchronize()
+    assert int(status) == (0x403 if with_status else 0)
+    before = [t.clone() for t in tensors]
+    with pytest.raises(RuntimeError, match="timed out"):
+        call(tensors)
+    torch.cuda.synchronize()
+    for a, b in zip(before, tensors):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8)), name
+    got = call(tensors)
+    if name in ("prompt", "attend"):
+        assert torch.equal(got, want)
+
+
+def test_serve_status_raises_once():
+    assert ops.serve_status(torch.device(DEV)) == 0
+    ops.serve_selftest_timeout(torch.device(DEV))
+    with pytest.raises(RuntimeError, match="timed out"):
+        ops.serve_status(torch.device(DEV))
+    assert ops.serve_status(torch.device(DEV)) == 0
+    with pytest.raises(ValueError, match="1 s"):
+        ops.serve_selftest_timeout(torch.device(DEV), limit_ns=10**10)
+
+
+def test_first_call_of_a_process_under_capture():
+    """The device's word is made by the first call, which may be a captured one."""
+    code = """
+import torch, optimized_transformer
+from tttj_2026_b200 import ops
+g = torch.Generator(device="cuda").manual_seed(1)
+kc = torch.randn(8, 16, 2, 64, device="cuda", generator=g).half()
+q = torch.randn(2, 4, 64, device="cuda", generator=g).half()
+table = torch.arange(8, device="cuda", dtype=torch.int32).view(2, 4)
+off = torch.tensor([0, 1, 2], device="cuda", dtype=torch.int32)
+lens = torch.tensor([30, 64], device="cuda", dtype=torch.int32)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = ops.cache_attention(q, kc, kc, table, off, lens, max_new=1)
+graph.replay()
+torch.cuda.synchronize()
+assert torch.equal(out, ops.cache_attention(q, kc, kc, table, off, lens, max_new=1))
+print("served")
+"""
+    root = Path(__file__).resolve().parent.parent
+    res = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert res.returncode == 0 and "served" in res.stdout, res.stderr[-2000:]

@@ -103,6 +103,8 @@ _SIGNATURES = {
     ),
     "tttj_plan_path": (_c.c_int, [_vp]),
     "tttj_serve_workspace_bytes": (_c.c_size_t, [_vp]),
+    "tttj_serve_status": (_c.c_int, [_vp]),
+    "tttj_serve_selftest_timeout": (_c.c_int, [_vp, _c.c_uint64, _vp]),
     "tttj_prompt_attention": (
         _c.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _c.c_int, _c.c_float, _vp, _c.c_size_t, _vp]
     ),

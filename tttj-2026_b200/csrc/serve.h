@@ -29,6 +29,7 @@ struct SrvSeqs {
   int tokens;          // rows allocated in q / out
   int causal;
   int* status;         // device status word (nullable)
+  int* timeout_host;   // the device's pinned word (serve_capi.cu); null where nothing waits
 };
 
 struct SrvSeq {
@@ -177,5 +178,8 @@ struct EvictParams {
   int most_moves;
 };
 cudaError_t evict_launch(const EvictParams& p, int sms, cudaStream_t stream);
+
+// One bounded wait on a barrier that nothing arrives on, reported like any other.
+cudaError_t serve_selftest_launch(const SrvSeqs& s, unsigned long long limit_ns, cudaStream_t stream);
 
 }  // namespace tttj

@@ -1,7 +1,7 @@
 // Paged key/value cache: append of new tokens, eviction by gathered attention mass.
 #include "common.cuh"
 #include "launch.h"
-#include "serve.h"
+#include "serve_dev.cuh"
 
 namespace tttj {
 
@@ -386,7 +386,20 @@ __global__ void __launch_bounds__(EVICT_MAX_THREADS) evict_kernel(const EvictPar
   }
 }
 
+// ---------------------------------------------------------------- failure detection
+__global__ void serve_selftest_kernel(const SrvSeqs s, unsigned long long limit_ns) {
+  __shared__ __align__(8) uint64_t bar;
+  mbar_init(smem_u32(&bar), 1);
+  fence_barrier_init();
+  if (!srv_wait(smem_u32(&bar), 0, nullptr, limit_ns)) srv_report_timeout(s);
+}
+
 }  // namespace
+
+cudaError_t serve_selftest_launch(const SrvSeqs& s, unsigned long long limit_ns, cudaStream_t stream) {
+  serve_selftest_kernel<<<1, 1, 0, stream>>>(s, limit_ns);
+  return cudaGetLastError();
+}
 
 cudaError_t append_launch(const AppendParams& p, int sms, cudaStream_t stream) {
   const long pieces = 2l * p.kv_heads * (p.head_dim / 8);

@@ -2,6 +2,8 @@
 // tensor maps and launches.  Nothing here reads device memory or synchronises.
 #include <math.h>
 
+#include <atomic>
+
 #include "capi_util.h"
 #include "serve.h"
 
@@ -136,11 +138,48 @@ int q_map(CUtensorMap* m, const char* what, const tttj_seqs* s, const tttj_rows*
   return TTTJ_OK;
 }
 
-int sm_count_here(int* sms) {
+// A pinned word per device, written by a kernel whose bounded wait gave up and read by the
+// device's next call, without synchronising.  Allocated at the first call, which may be under
+// stream capture; kept until the process ends.
+constexpr int kMostDevices = 64;
+std::atomic<int*> g_timeout_words[kMostDevices];
+
+int timeout_word(int dev, int** word) {
+  if (dev < 0 || dev >= kMostDevices) return capi_fail(TTTJ_ERR_CUDA, "device %d out of range", dev);
+  *word = g_timeout_words[dev].load(std::memory_order_acquire);
+  if (*word) return TTTJ_OK;
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  CAPI_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+  void* fresh = nullptr;
+  const cudaError_t e = cudaHostAlloc(&fresh, sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable);
+  if (e == cudaSuccess) {
+    *static_cast<volatile int*>(fresh) = 0;
+    int* first = nullptr;  // another thread's first call may have been faster: its word then
+    *word = g_timeout_words[dev].compare_exchange_strong(first, static_cast<int*>(fresh), std::memory_order_acq_rel)
+                ? static_cast<int*>(fresh)
+                : first;
+  }
+  const cudaError_t back = cudaThreadExchangeStreamCaptureMode(&mode);
+  CAPI_CUDA(e);
+  CAPI_CUDA(back);
+  return TTTJ_OK;
+}
+
+// The current device of a call that is about to launch: its multiprocessors and its word.  An
+// earlier call's wait that gave up is reported here, once.
+int device_here(const char* what, int* sms, int** word) {
   int dev = 0;
   CAPI_CUDA(cudaGetDevice(&dev));
   *sms = capi_sm_count(dev);
   if (*sms <= 0) return capi_fail(TTTJ_ERR_CUDA, "no multiprocessor count");
+  TRY(timeout_word(dev, word));
+  if (*static_cast<volatile int*>(*word) != 0) {
+    const int v = __atomic_exchange_n(*word, 0, __ATOMIC_ACQ_REL);
+    if (v != 0)
+      return capi_fail(TTTJ_ERR_DEVICE_TIMEOUT,
+                       "%s: a device wait of an earlier serving call on this device timed out (status 0x%x); that "
+                       "call's results are invalid", what, v);
+  }
   return TTTJ_OK;
 }
 
@@ -202,8 +241,8 @@ int attention(const char* what, const tttj_seqs* s, const tttj_rows* q, const Ca
   if (reinterpret_cast<uintptr_t>(workspace) & (kAlign - 1))
     return capi_fail(TTTJ_ERR_INVALID, "%s: workspace must be 256-byte aligned", what);
   TRY(check_scale(what, scale));
-  int sms = 0;
-  TRY(sm_count_here(&sms));
+  int sms = 0, *timeout = nullptr;
+  TRY(device_here(what, &sms, &timeout));
   if (sms > kMostSms) sms = kMostSms;
   const bool step = step_runs(s, cache, max_new);
   const int keys = step ? STEP_KEYS : ATC_BN;
@@ -219,6 +258,7 @@ int attention(const char* what, const tttj_seqs* s, const tttj_rows* q, const Ca
     const ServeWs w = step_ws(s);
     StepParams p{};
     p.s = seqs_of(s, cache, causal);
+    p.s.timeout_host = timeout;
     p.q = q->data;
     p.q_tok = q->token_stride;
     p.q_head = q->head_stride;
@@ -239,6 +279,7 @@ int attention(const char* what, const tttj_seqs* s, const tttj_rows* q, const Ca
   const ServeWs w = tile_ws(s);
   TileParams p{};
   p.s = seqs_of(s, cache, causal);
+  p.s.timeout_host = timeout;
   p.q = q->data;
   p.q_tok = q->token_stride;
   p.q_head = q->head_stride;
@@ -335,8 +376,8 @@ int tttj_cache_append(const tttj_seqs* s, const tttj_rows* k, const tttj_rows* v
   p.positions = positions;
   p.mass = mass;
   p.seen = seen;
-  int sms = 0;
-  TRY(sm_count_here(&sms));
+  int sms = 0, *timeout = nullptr;
+  TRY(device_here(what, &sms, &timeout));
   CAPI_CUDA(append_launch(p, sms, static_cast<cudaStream_t>(stream)));
   return TTTJ_OK;
 }
@@ -357,10 +398,11 @@ int tttj_cache_mass(const tttj_seqs* s, const tttj_rows* q, const float* lse, co
       CAPI_CUDA(cudaMemcpyAsync(mass_out, mass, (size_t)s->batch * s->kv_heads * cap * 4, cudaMemcpyDeviceToDevice, st));
     return TTTJ_OK;
   }
-  int sms = 0;
-  TRY(sm_count_here(&sms));
+  int sms = 0, *timeout = nullptr;
+  TRY(device_here(what, &sms, &timeout));
   MassParams p{};
   p.s = seqs_of(s, true, 1);
+  p.s.timeout_host = timeout;
   p.lse = lse;
   p.mass = mass;
   p.out = mass_out;
@@ -379,6 +421,29 @@ int tttj_cache_mass(const tttj_seqs* s, const tttj_rows* q, const float* lse, co
   TRY(kv_map(&tm_k, what, s, k_cache->data, k_cache->page_stride, k_cache->slot_stride, k_cache->head_stride,
              s->page_size, s->num_pages, s->page_size < ATC_BM ? s->page_size : ATC_BM));
   CAPI_CUDA(mass_launch(tm_q, tm_k, p, s->head_dim, s->dtype == TTTJ_DTYPE_BF16, sms, st));
+  return TTTJ_OK;
+}
+
+int tttj_serve_status(int* device_status) {
+  if (!device_status) return capi_fail(TTTJ_ERR_INVALID, "serve_status: null argument");
+  int dev = 0, *word = nullptr;
+  CAPI_CUDA(cudaGetDevice(&dev));
+  TRY(timeout_word(dev, &word));
+  CAPI_CUDA(cudaDeviceSynchronize());
+  *device_status = __atomic_exchange_n(word, 0, __ATOMIC_ACQ_REL);
+  if (*device_status != 0)
+    return capi_fail(TTTJ_ERR_DEVICE_TIMEOUT, "serving: a device wait timed out (status 0x%x)", *device_status);
+  return TTTJ_OK;
+}
+
+int tttj_serve_selftest_timeout(int32_t* status, uint64_t limit_ns, void* stream) {
+  if (limit_ns > 1000000000ull) return capi_fail(TTTJ_ERR_INVALID, "serve_selftest: limit above 1 s");
+  int dev = 0;
+  SrvSeqs s{};
+  s.status = status;
+  CAPI_CUDA(cudaGetDevice(&dev));
+  TRY(timeout_word(dev, &s.timeout_host));
+  CAPI_CUDA(serve_selftest_launch(s, limit_ns, static_cast<cudaStream_t>(stream)));
   return TTTJ_OK;
 }
 
@@ -430,8 +495,8 @@ int tttj_cache_evict(const tttj_seqs* s, const tttj_pages* k_cache, const tttj_p
   p.cap = (long)s->pages_per_seq * s->page_size;
   p.most_moves = evict_most_moves(s, keep);
   p.moves = reinterpret_cast<int2*>(workspace);
-  int sms = 0;
-  TRY(sm_count_here(&sms));
+  int sms = 0, *timeout = nullptr;
+  TRY(device_here(what, &sms, &timeout));
   CAPI_CUDA(evict_launch(p, sms, static_cast<cudaStream_t>(stream)));
   return TTTJ_OK;
 }

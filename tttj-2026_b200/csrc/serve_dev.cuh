@@ -24,6 +24,12 @@ __device__ __forceinline__ bool srv_wait(uint32_t bar, uint32_t parity, volatile
   }
 }
 
+// A wait gave up: the call's status word, and the word that the device's next call looks at.
+__device__ __forceinline__ void srv_report_timeout(const SrvSeqs& s) {
+  report_status(s.status, SRV_DEV_TIMEOUT);
+  if (s.timeout_host != nullptr) *reinterpret_cast<volatile int*>(s.timeout_host) = SRV_DEV_TIMEOUT;
+}
+
 template <bool BF16>
 __device__ __forceinline__ uint32_t srv_pack(float a, float b) {
   if constexpr (BF16) {

@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(MASS_THREADS, 1)
     }
     if (!ok && lane == 0) {
       *abort_flag = 1;
-      report_status(p.s.status, SRV_DEV_TIMEOUT);
+      srv_report_timeout(p.s);
       for (long j = kc > SM::KBUF ? kc - SM::KBUF : 0; j < kc; ++j)
         srv_wait(bar_k_full + 8 * (int)(j % SM::KBUF), (uint32_t)((j / SM::KBUF) & 1), nullptr, limit);
     }
@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(MASS_THREADS, 1)
     }
     if (!ok && lane == 0) {
       *abort_flag = 1;
-      report_status(p.s.status, SRV_DEV_TIMEOUT);
+      srv_report_timeout(p.s);
       for (uint32_t j = qc > SM::STAGES ? qc - SM::STAGES : 0; j < qc; ++j)
         srv_wait(bar_q_full + 8 * (j % SM::STAGES), (j / SM::STAGES) & 1, nullptr, limit);
     }
@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(MASS_THREADS, 1)
     if (!ok) {
       if (lane == 0) {
         *abort_flag = 1;
-        report_status(p.s.status, SRV_DEV_TIMEOUT);
+        srv_report_timeout(p.s);
       }
       if (issued) {
         mma_commit_warp(bar_drain);
@@ -513,7 +513,7 @@ __global__ void __launch_bounds__(MASS_THREADS, 1)
     }
     if (!ok) {
       *abort_flag = 1;
-      report_status(p.s.status, SRV_DEV_TIMEOUT);
+      srv_report_timeout(p.s);
     }
   }
 

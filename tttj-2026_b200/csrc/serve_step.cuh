@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(STEP_THREADS, step_ctas_per_sm(HD))
     }
     if (!ok && lane == 0) {
       *abort_flag = 1;
-      report_status(p.s.status, SRV_DEV_TIMEOUT);
+      srv_report_timeout(p.s);
     }
     // Issued loads land before the CTA may exit.
     if (!ok)
@@ -234,7 +234,7 @@ __global__ void __launch_bounds__(STEP_THREADS, step_ctas_per_sm(HD))
                                             p.wait_limit_ns));
       if (!ok) {
         *abort_flag = 1;
-        if (lane == 0) report_status(p.s.status, SRV_DEV_TIMEOUT);
+        if (lane == 0) srv_report_timeout(p.s);
         break;
       }
       const int k0 = t * STEP_KEYS + warp * 16;  // this warp's 16 keys

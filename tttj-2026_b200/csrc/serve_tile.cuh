@@ -508,7 +508,7 @@ __global__ void __launch_bounds__(TileSmem<HD>::THREADS, 1)
     }
     if (!ok && lane == 0) {
       *abort_flag = 1;
-      report_status(p.s.status, SRV_DEV_TIMEOUT);
+      srv_report_timeout(p.s);
       // Let issued loads land before the CTA can exit.
       for (long j = kc > STAGES ? kc - STAGES : 0; j < kc; ++j)
         srv_wait(bar_k_full + 8 * (int)(j % STAGES), (uint32_t)((j / STAGES) & 1), nullptr, limit);
@@ -631,7 +631,7 @@ __global__ void __launch_bounds__(TileSmem<HD>::THREADS, 1)
     if (!ok) {
       if (lane == 0) {
         *abort_flag = 1;
-        report_status(p.s.status, SRV_DEV_TIMEOUT);
+        srv_report_timeout(p.s);
       }
       if (issued) {
         mma_commit_warp(bar_drain + 8 * (warp - ISSUER));
@@ -673,7 +673,7 @@ __global__ void __launch_bounds__(TileSmem<HD>::THREADS, 1)
     }
     if (!ok && lane == 0) {
       *abort_flag = 1;
-      report_status(p.s.status, SRV_DEV_TIMEOUT);
+      srv_report_timeout(p.s);
     }
   } else if (warp < 4 * NT) {
     // ------------------------------------------------------------ softmax
@@ -916,7 +916,7 @@ __global__ void __launch_bounds__(TileSmem<HD>::THREADS, 1)
     }
     if (!ok) {
       *abort_flag = 1;
-      report_status(p.s.status, SRV_DEV_TIMEOUT);
+      srv_report_timeout(p.s);
     }
   }
 

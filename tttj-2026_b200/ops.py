@@ -125,6 +125,8 @@ def selftest_wait_timeout(status: torch.Tensor, limit_ns: int) -> None:
 # * Lengths, offsets and page numbers are read on the device only: calls can be captured into
 #   CUDA graphs and replayed with new ones.  They are bounds-checked there; ``status`` (int32
 #   [1], zeroed by the caller) records a wrong one (include/tttj_b200.h, TTTJ_DEV_BAD_*).
+# * A device wait that gave up (2 s; status TTTJ_DEV_SERVE_TIMEOUT) makes the next call on the device
+#   raise RuntimeError, with or without ``status``; ``serve_status`` asks for it.
 # * Launches go to the current stream of the tensors' device, whichever device is current.
 # * Inference only: tensors that require gradients are refused while gradients are enabled, and
 #   tensors that carry a forward-mode tangent.
@@ -228,6 +230,26 @@ def serve_workspace_bytes(batch: int, tokens: int, heads: int, kv_heads: int, he
     if n == 0:
         _lib.check(_lib.TTTJ_ERR_INVALID, "serve_workspace_bytes")
     return n
+
+
+def serve_status(device: torch.device) -> int:
+    """Synchronise ``device`` and raise RuntimeError if a bounded wait of a serving kernel gave up
+    there (returns 0 when healthy).  Without this call the device's next serving call raises
+    instead; replayed graphs make none."""
+    with torch.cuda.device(device):
+        v = ctypes.c_int(0)
+        _lib.check(_lib.lib().tttj_serve_status(ctypes.byref(v)), "serve_status")
+    return 0
+
+
+def serve_selftest_timeout(device: torch.device, limit_ns: int = 2_000_000, status: Optional[torch.Tensor] = None) -> None:
+    """Failure-detection self test: a bounded device wait on nothing gives up after ``limit_ns`` and
+    reports as a serving kernel's would, so that the next serving call on ``device`` raises
+    RuntimeError.  No GPU fault is involved."""
+    device = torch.device(device)
+    stat = None if status is None else _serve_ints("serve_selftest", "status", status, 1, device)
+    with torch.cuda.device(device):
+        _lib.check(_lib.lib().tttj_serve_selftest_timeout(stat, int(limit_ns), _stream(device)), "serve_selftest")
 
 
 def _serve_out(what: str, out: Optional[torch.Tensor], q: torch.Tensor) -> tuple:
