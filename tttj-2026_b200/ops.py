@@ -148,12 +148,11 @@ def _call(device: torch.device, fn, *args) -> int:
         return fn(*args, torch._C._cuda_getCurrentRawStream(index))
 
 
-def _refuse_gradient(what: str, name: str, t: torch.Tensor) -> None:
-    """Raise if a derivative of ``t`` is wanted: the operators would drop it silently."""
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{what}: inference only ({name} requires a gradient)")
-    if _forward_ad._current_level >= 0 and _forward_ad.unpack_dual(t).tangent is not None:
-        raise ValueError(f"{what}: inference only ({name} carries a forward-mode tangent)")
+def _refuse_tangents(what: str, **tensors: Optional[torch.Tensor]) -> None:
+    """Inside a forward-mode level: raise if a tensor carries a tangent, which would be dropped."""
+    for name, t in tensors.items():
+        if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError(f"{what}: inference only ({name} carries a forward-mode tangent)")
 
 
 def _serve_rows(what: str, name: str, t: torch.Tensor, shape: tuple, dtype: torch.dtype, device: torch.device) -> bytes:
@@ -163,8 +162,8 @@ def _serve_rows(what: str, name: str, t: torch.Tensor, shape: tuple, dtype: torc
     tok, head, one = t.stride()
     if one != 1:
         raise ValueError(f"{what}: head_dim of {name} must be contiguous")
-    if t.requires_grad or _forward_ad._current_level >= 0:
-        _refuse_gradient(what, name, t)
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what}: inference only ({name} requires a gradient)")
     return _pack_rows(t.data_ptr(), tok, head)
 
 
@@ -181,8 +180,8 @@ def _serve_pages(what: str, name: str, t: torch.Tensor, shape: tuple, dtype: tor
     page, slot, head, one = t.stride()
     if one != 1:
         raise ValueError(f"{what}: head_dim of {name} must be contiguous")
-    if t.requires_grad or _forward_ad._current_level >= 0:
-        _refuse_gradient(what, name, t)
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what}: inference only ({name} requires a gradient)")
     return _pack_pages(t.data_ptr(), page, slot, head)
 
 
@@ -284,6 +283,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_offs
     what = "prompt_attention"
     if q.dim() != 3 or k.dim() != 3:
         raise ValueError(f"{what}: q and k must be [tokens, heads, head_dim]")
+    if _forward_ad._current_level >= 0:
+        _refuse_tangents(what, q=q, k=k, v=v, out=out)
     dtype, device, kind = q.dtype, q.device, _serve_type(what, q)
     tokens, heads, d = q.shape
     kv_heads = k.shape[1]
@@ -315,6 +316,8 @@ def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     what = "cache_attention"
     if q.dim() != 3 or k_cache.dim() != 4:
         raise ValueError(f"{what}: q must be [tokens, heads, head_dim], k_cache [pages, page_size, kv_heads, head_dim]")
+    if _forward_ad._current_level >= 0:
+        _refuse_tangents(what, q=q, k_cache=k_cache, v_cache=v_cache, out=out)
     dtype, device, kind = q.dtype, q.device, _serve_type(what, q)
     tokens, heads, d = q.shape
     pages = k_cache.shape
@@ -340,8 +343,8 @@ def _slot_tensor(what: str, name: str, t: torch.Tensor, dtype: torch.dtype, shap
     if t.dtype != dtype or t.shape != shape or t.device != device or not t.is_contiguous():
         raise ValueError(f"{what}: {name} must be a contiguous {dtype} tensor {list(shape)} "
                          f"(sequences, kv_heads, slots) on {device}")
-    if t.requires_grad or _forward_ad._current_level >= 0:
-        _refuse_gradient(what, name, t)
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what}: inference only ({name} requires a gradient)")
     return t.data_ptr()
 
 
@@ -359,6 +362,8 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     what = "cache_append"
     if k.dim() != 3 or k_cache.dim() != 4:
         raise ValueError(f"{what}: k must be [tokens, kv_heads, head_dim], k_cache [pages, page_size, kv_heads, head_dim]")
+    if _forward_ad._current_level >= 0:
+        _refuse_tangents(what, k=k, v=v, k_cache=k_cache, v_cache=v_cache, mass=mass)
     dtype, device, kind = k.dtype, k.device, _serve_type(what, k)
     tokens, kv_heads, d = rows = k.shape
     pages = k_cache.shape
@@ -392,6 +397,8 @@ def cache_evict(mass: torch.Tensor, positions: torch.Tensor, k_cache: torch.Tens
     what = "cache_evict"
     if k_cache.dim() != 4 or cache_lens.dim() != 1 or cache_lens.shape[0] < 1:
         raise ValueError(f"{what}: k_cache must be [pages, page_size, kv_heads, head_dim], cache_lens [sequences]")
+    if _forward_ad._current_level >= 0:
+        _refuse_tangents(what, mass=mass, k_cache=k_cache, v_cache=v_cache)
     dtype, device, kind = k_cache.dtype, k_cache.device, _serve_type(what, k_cache)
     pages = k_cache.shape
     batch, kv_heads = cache_lens.shape[0], pages[2]
@@ -432,6 +439,8 @@ def cache_mass(q: torch.Tensor, lse: torch.Tensor, k_cache: torch.Tensor, page_t
     what = "cache_mass"
     if q.dim() != 3 or k_cache.dim() != 4:
         raise ValueError(f"{what}: q must be [tokens, heads, head_dim], k_cache [pages, page_size, kv_heads, head_dim]")
+    if _forward_ad._current_level >= 0:
+        _refuse_tangents(what, q=q, lse=lse, k_cache=k_cache, mass=mass, out=out)
     dtype, device, kind = q.dtype, q.device, _serve_type(what, q)
     tokens, heads, d = rows = q.shape
     pages = k_cache.shape
@@ -441,8 +450,8 @@ def cache_mass(q: torch.Tensor, lse: torch.Tensor, k_cache: torch.Tensor, page_t
     s, cap = _cache_seqs(what, off, batch, tokens, kind, heads, k_cache, page_table, cache_lens, status, device)
     if lse.dtype != torch.float32 or lse.shape != rows[:2] or lse.device != device or not lse.is_contiguous():
         raise ValueError(f"{what}: lse must be a contiguous float32 tensor [{tokens}, {heads}] on {device}")
-    if lse.requires_grad or _forward_ad._current_level >= 0:
-        _refuse_gradient(what, "lse", lse)
+    if lse.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what}: inference only (lse requires a gradient)")
     slots = (batch, pages[2], cap)
     ms = _slot_tensor(what, "mass", mass, torch.float32, slots, device)
     if out is None:
