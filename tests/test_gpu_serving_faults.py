@@ -254,3 +254,61 @@ print("served")
     root = Path(__file__).resolve().parent.parent
     res = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
     assert res.returncode == 0 and "served" in res.stdout, res.stderr[-2000:]
+
+
+# --------------------------------------------------------------------- a captured step
+def test_a_captured_step_carries_its_state():
+    """Evict, append, attend, gather in one graph, as INTEGRATION.md shows it: eviction makes new
+    tensors, so the step ends by copying them into those that the next replay reads.  Replays follow
+    the same steps run one by one on tensors of their own, bit for bit."""
+    heads, kv, d, page, per, keep, recent = 8, 2, 64, 16, 6, 40, 6
+    lens0 = [90, 12, 41]
+    b, cap = len(lens0), per * page
+    gen = _gen(7)
+    kc = torch.randn(b * per, page, kv, d, device=DEV, generator=gen).half()
+    vc = torch.randn(b * per, page, kv, d, device=DEV, generator=gen).half()
+    table = torch.randperm(b * per, device=DEV, generator=gen).to(torch.int32).view(b, per)
+    lens = torch.tensor(lens0, dtype=torch.int32, device=DEV)
+    live = torch.arange(cap, device=DEV)[None, None] < lens[:, None, None]
+    mass = torch.where(live, torch.rand(b, kv, cap, device=DEV, generator=gen), 0.0)
+    pos = torch.where(live, torch.arange(cap, device=DEV)[None, None].expand(b, kv, cap), -1).to(torch.int32).contiguous()
+    seen, off = lens.clone(), lengths_to_offsets([1] * b)
+    q = torch.zeros(b, heads, d, dtype=torch.float16, device=DEV)
+    k, v = torch.zeros(b, kv, d, dtype=torch.float16, device=DEV), torch.zeros(b, kv, d, dtype=torch.float16, device=DEV)
+
+    def step():
+        m, p, n = ops.cache_evict(mass, pos, kc, vc, table, lens, keep, recent=recent)
+        mass.copy_(m), pos.copy_(p), lens.copy_(n + 1), seen.add_(1)
+        ops.cache_append(k, v, kc, vc, table, off, lens, positions=pos, mass=mass, seen=seen)
+        out, lse = ops.cache_attention(q, kc, vc, table, off, lens, max_new=1, return_lse=True)
+        ops.cache_mass(q, lse, kc, table, off, lens, mass, max_new=1, out=mass)
+        return out, lse
+
+    state = (mass, pos, lens, seen, kc, vc)
+    start = [x.clone() for x in state]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got, got_lse = step()
+    for x, y in zip(state, start):
+        x.copy_(y)
+    m, p, n, s, k2, v2 = [x.clone() for x in start]
+    for i in range(60):  # past the budget, and every sequence evicts
+        for x in (q, k, v):
+            x.copy_(torch.randn(x.shape, device=DEV, generator=gen))
+        graph.replay()
+        m, p, n = ops.cache_evict(m, p, k2, v2, table, n, keep, recent=recent)
+        n, s = n + 1, s + 1
+        ops.cache_append(k, v, k2, v2, table, off, n, positions=p, mass=m, seen=s)
+        out, lse = ops.cache_attention(q, k2, v2, table, off, n, max_new=1, return_lse=True)
+        ops.cache_mass(q, lse, k2, table, off, n, m, max_new=1, out=m)
+        assert torch.equal(got, out) and torch.equal(got_lse, lse), i
+        for x, y in zip(state, (m, p, n, s, k2, v2)):
+            assert torch.equal(x, y), i
+    assert n.tolist() == [keep + 1] * b
+    assert s.tolist() == [x + 60 for x in lens0]
+    assert ops.serve_status(torch.device(DEV)) == 0

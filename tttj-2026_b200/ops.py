@@ -393,7 +393,9 @@ def cache_evict(mass: torch.Tensor, positions: torch.Tensor, k_cache: torch.Tens
     lower slot; NaN counts as -inf).  Kept slots behind the budget move into the freed ones in
     front of it, the i-th into the i-th, in both caches (whose pages must be the sequence's own);
     all others keep their place, so the cache is no longer in the tokens' order.  Returns new
-    (mass, positions, cache_lens): 0 and -1 behind the new lengths min(len, keep)."""
+    (mass, positions, cache_lens): 0 and -1 behind the new lengths min(len, keep).  A captured call
+    reads the tensors that it was captured with: copy the returned ones into them for the next
+    replay."""
     what = "cache_evict"
     if k_cache.dim() != 4 or cache_lens.dim() != 1 or cache_lens.shape[0] < 1:
         raise ValueError(f"{what}: k_cache must be [pages, page_size, kv_heads, head_dim], cache_lens [sequences]")
