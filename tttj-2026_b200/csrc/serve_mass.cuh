@@ -411,11 +411,10 @@ __global__ void __launch_bounds__(MASS_THREADS, 1)
         const int rows = min(TOK, w.q.n - tok0) * p.group;
         // Some row of this tile does not see some key of the item.
         const bool partly = w.k0 + ITEM_KEYS - 1 > w.q.len - w.q.n + tok0;
-        if (!srv_wait(bar_c_full + 8 * cr.at, cr.parity, abort_flag, limit) ||
-            !srv_wait(bar_s_full + 8 * u, sr.parity, abort_flag, limit)) {
-          ok = false;
-          break;
-        }
+        // All lanes give up together (the __syncwarp below has no limit).
+        ok = __all_sync(0xffffffffu, srv_wait(bar_c_full + 8 * cr.at, cr.parity, abort_flag, limit) &&
+                                         srv_wait(bar_s_full + 8 * u, sr.parity, abort_flag, limit));
+        if (!ok) break;
         tc_fence_after();
         const float* nl = s_lse + cr.at * MASS_COLS;
         const int* lim = s_lim + cr.at * MASS_COLS;

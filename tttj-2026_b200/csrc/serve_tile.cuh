@@ -691,6 +691,11 @@ __global__ void __launch_bounds__(TileSmem<HD>::THREADS, 1)
     long c = 0;    // steps of all items so far
     long ofc = 0;  // items with steps so far
     bool ok = true;
+    // All lanes give up together: one that left alone would leave the others waiting for it in the
+    // next warp-wide instruction, without a limit.
+    auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
+      return __all_sync(0xffffffffu, srv_wait(bar, parity, abort_flag, limit));
+    };
     // One arrival per warp, after every lane's reads and TMEM accesses.
     auto arrive = [&](uint32_t bar) {
       __syncwarp();
@@ -698,14 +703,13 @@ __global__ void __launch_bounds__(TileSmem<HD>::THREADS, 1)
     };
     // P V of step i of this side complete: phase i / PBUF of its buffer's barrier.
     auto pv_done = [&](long i) -> bool {
-      const bool fine = srv_wait(bar_pv_done + 16 * t + 8 * (uint32_t)(i % SM::PBUF),
-                                 (uint32_t)((i / SM::PBUF) & 1), abort_flag, limit);
+      const bool fine = wait(bar_pv_done + 16 * t + 8 * (uint32_t)(i % SM::PBUF), (uint32_t)((i / SM::PBUF) & 1));
       tc_fence_after();
       return fine;
     };
     for (int k = 0; ok; ++k) {
       const int qb = k % QBUF;
-      if (!srv_wait(bar_q_full + 8 * (t * SM::QS + qb), (uint32_t)((k / QBUF) & 1), abort_flag, limit)) {
+      if (!wait(bar_q_full + 8 * (t * SM::QS + qb), (uint32_t)((k / QBUF) & 1))) {
         ok = false;
         break;
       }
@@ -731,7 +735,7 @@ __global__ void __launch_bounds__(TileSmem<HD>::THREADS, 1)
       float m_run = -INFINITY;  // running max (log2 domain) used as the exp base
       float l_run = 0.f;
       for (int i = 0; i < n; ++i, ++c) {
-        if (!srv_wait(bar_s_full + 8 * t, (uint32_t)(c & 1), abort_flag, limit)) {
+        if (!wait(bar_s_full + 8 * t, (uint32_t)(c & 1))) {
           ok = false;
           break;
         }
@@ -855,7 +859,7 @@ __global__ void __launch_bounds__(TileSmem<HD>::THREADS, 1)
         arrive(bar_p_full + 16 * t + 8 * (uint32_t)(c % SM::PBUF));
       }
       if (!ok) break;
-      if (!srv_wait(bar_o_full + 8 * t, (uint32_t)(ofc++ & 1), abort_flag, limit)) {
+      if (!wait(bar_o_full + 8 * t, (uint32_t)(ofc++ & 1))) {
         ok = false;
         break;
       }
