@@ -1,4 +1,5 @@
-// Attention of few query rows (single tokens, short drafts) over many keys.
+// Causal attention of few query rows (single tokens, short drafts) over the many keys of a
+// paged cache.
 //
 // For each sequence, key/value head and block of 16 query rows (row = new token x group
 // + head of the group): O = softmax(scale q K^T) V over the slots a row may see.  What
@@ -28,7 +29,9 @@ struct StepSmem {
   static constexpr int ROW_BYTES = BOX_COLS * 2;
   static constexpr int BOX_BYTES = STEP_KEYS * ROW_BYTES;
   static constexpr int TILE = STEP_KEYS * HD * 2;
-  // About 96 KB in flight per CTA (192 KB per SM) hides the HBM latency.
+  // About 96 KB in flight per CTA hides the HBM latency: 64 KB at head_dim 32, 192 KB at 256 (one CTA
+  // per SM).  Two CTAs per SM fit with it, at head_dim 128 up to about 890 sequences: with more,
+  // the prefix sums leave room for one at a time, and half the bytes are in flight.
   static constexpr int STAGES = HD == 256 ? 3 : HD == 128 ? 3 : HD == 64 ? 6 : 8;
   static constexpr int OSTRIDE = HD + 8;  // floats; rows 8 banks apart
   static constexpr int RING = STAGES * 2 * TILE;
@@ -146,11 +149,10 @@ __global__ void __launch_bounds__(STEP_THREADS, step_ctas_per_sm(HD))
   const long per = step_per_cta(total, gridDim.x);
   const long u0 = (long)blockIdx.x * per;
   const long u1 = min(total, u0 + per);
-  const bool paged = p.s.table != nullptr;
 
   if (warp == 4) {
     // ------------------------------------------------------------ producer
-    const int cr = paged ? min(STEP_KEYS, 1 << p.s.page_shift) : STEP_KEYS;
+    const int cr = min(STEP_KEYS, 1 << p.s.page_shift);
     const int chunks = STEP_KEYS / cr;
     const int boxes = chunks * SM::NBOX * 2;  // <= 32
     const int kv = lane & 1, box = (lane >> 1) % SM::NBOX, chunk = (lane >> 1) / SM::NBOX;
@@ -161,12 +163,8 @@ __global__ void __launch_bounds__(STEP_THREADS, step_ctas_per_sm(HD))
       const StepRun r = step_run(p, pre, u, u1);
       for (int t = r.t0; t < r.t1; ++t, ++it) {
         const int slot = t * STEP_KEYS + chunk * cr;
-        int page = 0, c1 = r.q.row0 + slot;
-        if (paged) {
-          page = p.s.num_pages;
-          if (lane < boxes && slot < r.q.len) page = srv_page(p.s, r.b, slot);
-          c1 = slot & ((1 << p.s.page_shift) - 1);
-        }
+        const int page = lane < boxes && slot < r.q.len ? srv_page(p.s, r.b, slot) : p.s.num_pages;
+        const int c1 = slot & ((1 << p.s.page_shift) - 1);
         const int st = (int)(it % SM::STAGES);
         ok = srv_wait(bar_empty + 8 * st, (uint32_t)((it / SM::STAGES) & 1) ^ 1u, abort_flag,
                        p.wait_limit_ns);
@@ -210,7 +208,7 @@ __global__ void __launch_bounds__(STEP_THREADS, step_ctas_per_sm(HD))
       const int row = r.rb * STEP_ROWS + (lane >> 2) + 8 * e;
       const int tok = row / p.group, g = row - tok * p.group;
       const bool live = row < rows;
-      lim[e] = !live ? -1 : p.s.causal ? r.q.len - r.q.n + tok : r.q.len - 1;
+      lim[e] = live ? r.q.len - r.q.n + tok : -1;
       const long at = ((long)(r.q.row0 + (live ? tok : 0)) * p.q_tok +
                        (long)(r.h * p.group + (live ? g : 0)) * p.q_head) / 2 + (lane & 3);
 #pragma unroll
@@ -226,7 +224,7 @@ __global__ void __launch_bounds__(STEP_THREADS, step_ctas_per_sm(HD))
       for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
     // Slots from here on are hidden from some row of the block (or from all).
-    const int all_see = p.s.causal ? r.q.len - r.q.n + 1 : r.q.len;
+    const int all_see = r.q.len - r.q.n + 1;
 
     for (int t = r.t0; ok && t < r.t1; ++t, ++it) {
       const int st = (int)(it % SM::STAGES);
