@@ -52,7 +52,9 @@ struct MassSmem {
 constexpr int MASS_ADDERS = 12;
 constexpr int MASS_THREADS = 32 * (MASS_ADDERS + 3);
 
-constexpr int MASS_FMA_PAIRS = 2;  // of eight pairs of exponentials, those on the FMA pipe (0 or 1: 2 % slower)
+// Of eight pairs of exponentials, those on the FMA pipe (4 chunks of 300 - 512 tokens over 2000 -
+// 8192 keys, 32 / 8 heads x 128: none 106.5 us, one 104.0, two 105.9).
+constexpr int MASS_FMA_PAIRS = 1;
 
 // Position in a ring of N stages: index and phase parity, without divisions.
 template <int N>
