@@ -10,7 +10,7 @@ from pathlib import Path
 import pytest
 import torch
 
-from serving_reference import cache_rows, lengths_to_offsets
+from serving_reference import attention_rows, cache_rows, lengths_to_offsets
 from test_gpu_serving import Cache, _check, _gen
 from tttj_2026_b200 import ops
 
@@ -312,3 +312,45 @@ def test_a_captured_step_carries_its_state():
     assert n.tolist() == [keep + 1] * b
     assert s.tolist() == [x + 60 for x in lens0]
     assert ops.serve_status(torch.device(DEV)) == 0
+
+
+# ---------------------------------------------------------------- log-sum-exps, many prompts
+@pytest.mark.parametrize("d", [32, 64, 128, 256])
+def test_log_sum_exp_of_rows_that_see_a_nan(d):
+    """NaN for a row whose scores hold one, on every path, split keys among them; a number elsewhere."""
+    def check(lse, q, k, n, m):
+        _, want = attention_rows(q, k, torch.zeros_like(k), n, m, d**-0.5)
+        assert torch.equal(torch.isnan(lse), torch.isnan(want))
+        assert torch.equal(torch.isneginf(lse.double()), torch.isneginf(want))
+        assert 0 < int(torch.isnan(want).sum()) < want.numel()
+
+    q = torch.randn(200, 4, d, device=DEV, generator=_gen(5)).half()
+    k = torch.randn(200, 2, d, device=DEV, generator=_gen(6)).half()
+    for at in (3, 130, 199):
+        bad = k.clone()
+        bad[at, 1, 0] = math.nan
+        _, lse = ops.prompt_attention(q, bad, k, lengths_to_offsets([200]), return_lse=True)
+        check(lse, q, bad, 200, 200)
+    for m in (300, 9001):
+        for n in (3, 150):
+            for back in (0, 1, 100):
+                c = Cache([m], 2, d, 16, torch.float16, 8)
+                slot = m - n if back == 100 else m - 1 - back
+                c.k[c.table[0, slot // 16].long(), slot % 16, 1, 2] = math.nan
+                qn = q[:n]
+                _, lse = ops.cache_attention(qn, c.k, c.v, c.table, lengths_to_offsets([n]), c.lens, return_lse=True)
+                check(lse, qn, cache_rows(c.k, c.table, 0, m), n, m)
+
+
+def test_every_prompt_of_the_most_sequences():
+    g = torch.Generator().manual_seed(3)
+    new = torch.randint(0, 4, (1024,), generator=g).tolist()
+    new[1000], new[1023], new[600] = 40, 130, 0
+    q = torch.randn(sum(new), 4, 32, device=DEV, generator=_gen(5)).half()
+    out, lse = ops.prompt_attention(q[:, :2], q[:, 2:3], q[:, 3:], lengths_to_offsets(new), return_lse=True)
+    at = 0
+    for n in new:
+        s = slice(at, at + n)
+        if n:
+            _check(out[s], lse[s], q[s, :2], q[s, 2:3], q[s, 3:], n, n, 32**-0.5)
+        at += n
