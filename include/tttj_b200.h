@@ -336,7 +336,8 @@ int tttj_attention_noalloc(const void* qkv, void* ctx, int qkv_rows, const uint8
  * on the device: offsets and lengths are clamped to the call's tensors, an entry of the
  * page table outside the cache stands for a page of zeros (nothing is written to it),
  * and `status` (nullable) records TTTJ_DEV_BAD_LENS / TTTJ_DEV_BAD_PAGE.  Infinite or NaN
- * values reach only rows that see them. */
+ * values reach only rows that see them; an infinite value in sight whose probability, rounded to
+ * the tensors' type, is 0 gives NaN. */
 typedef struct tttj_rows { /* [tokens][heads][head_dim] */
   const void* data;
   int64_t token_stride, head_stride;

@@ -185,7 +185,12 @@ int device_here(const char* what, int* sms, int** word) {
 
 constexpr int kMostSms = 160;  // multiprocessors that a call uses at most (workspace sizes)
 // Sequences of at most this many query rows per key/value head (new tokens x group) run on
-// the few-row kernel, chunks of more on the tile kernel.
+// the few-row kernel, chunks of more on the tile kernel: one mma tile of rows reads the keys once,
+// two read them twice.  Measured, few-row against tile kernel, bf16, us: 64 sequences of 4096 keys, 8
+// key/value heads x 128: 16 rows 183 / 230-238, 24 rows 341 / 245, 64 rows 668 / 262; 64 of 2048, 4
+// x 64: 16 rows 33 / 63, 32 rows 55 / 62, 48 rows 75 / 63.  Calls too small to fill the device stay
+// faster on the few-row kernel beyond the limit (8 of 8192, 4 x 128: 48 rows 49 / 70, 64 rows 72 / 69;
+// 4 of 1000, 4 x 64: 128 rows 15 / 23), but the host does not know the lengths.
 constexpr int kStepMostRows = 16;
 
 // Workspace of either attention kernel.

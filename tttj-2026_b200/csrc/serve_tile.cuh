@@ -13,8 +13,8 @@
 //                     that would leave CTAs idle -- those of a last, partial wave, and any
 //                     longer than a CTA's fair share -- are cut along the keys.
 //   tile_kernel       persistent CTAs (1 per SM) take items in turn: a TMA loader; per query
-//                     tile four softmax warps (one thread per row) and one MMA-issuing warp,
-//                     at head_dim 128 two; and a warp that prepares V tiles; running
+//                     tile four softmax warps (one thread per row) and two MMA-issuing warps
+//                     (one at head_dim 256); and a warp that prepares V tiles; running
 //                     statistics in fp32, O rescaled only when a row's maximum grew by
 //                     more than 2^8.
 //   tile_join_kernel  joins the pieces of cut items in the order of their keys.

@@ -388,9 +388,9 @@ def cache_evict(mass: torch.Tensor, positions: torch.Tensor, k_cache: torch.Tens
                 status: Optional[torch.Tensor] = None):
     """Evict down to ``keep`` slots per sequence and key/value head, those of least mass.
 
-    mass fp32 and positions int32 [B, kv_heads, P * page_size].  Slots whose position is among
-    the head's ``recent`` newest stay; of the others the largest masses (equal ones: the
-    lower slot; NaN counts as -inf).  Kept slots behind the budget move into the freed ones in
+    mass fp32 and positions int32 [B, kv_heads, P * page_size].  The slots of the largest masses
+    stay (equal ones: the lower slot; NaN counts as -inf); those whose position is among the
+    head's ``recent`` newest count as +inf.  Kept slots behind the budget move into the freed ones in
     front of it, the i-th into the i-th, in both caches (whose pages must be the sequence's own);
     all others keep their place, so the cache is no longer in the tokens' order.  Returns new
     (mass, positions, cache_lens): 0 and -1 behind the new lengths min(len, keep).  A captured call
