@@ -238,7 +238,6 @@ __global__ void __launch_bounds__(MASS_THREADS, 1)
     }
     if (!ok && lane == 0) {
       *abort_flag = 1;
-      srv_report_timeout(p.s);
       for (long j = kc > SM::KBUF ? kc - SM::KBUF : 0; j < kc; ++j)
         srv_wait(bar_k_full + 8 * (int)(j % SM::KBUF), (uint32_t)((j / SM::KBUF) & 1), nullptr, limit);
     }
@@ -314,7 +313,6 @@ __global__ void __launch_bounds__(MASS_THREADS, 1)
     }
     if (!ok && lane == 0) {
       *abort_flag = 1;
-      srv_report_timeout(p.s);
       for (uint32_t j = qc > SM::STAGES ? qc - SM::STAGES : 0; j < qc; ++j)
         srv_wait(bar_q_full + 8 * (j % SM::STAGES), (j / SM::STAGES) & 1, nullptr, limit);
     }
@@ -363,10 +361,7 @@ __global__ void __launch_bounds__(MASS_THREADS, 1)
       kr.next();
     }
     if (!ok) {
-      if (lane == 0) {
-        *abort_flag = 1;
-        srv_report_timeout(p.s);
-      }
+      if (lane == 0) *abort_flag = 1;
       if (issued) {
         mma_commit_warp(bar_drain);
         srv_wait(bar_drain, 0, nullptr, limit);
@@ -512,14 +507,12 @@ __global__ void __launch_bounds__(MASS_THREADS, 1)
         }
       }
     }
-    if (!ok) {
-      *abort_flag = 1;
-      srv_report_timeout(p.s);
-    }
+    if (!ok) *abort_flag = 1;
   }
 
   tc_fence_before();
   __syncthreads();
+  if (threadIdx.x == 0 && *abort_flag) srv_report_timeout(p.s);
   if (warp == ISSUER) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);

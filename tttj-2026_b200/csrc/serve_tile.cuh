@@ -508,7 +508,6 @@ __global__ void __launch_bounds__(TileSmem<HD>::THREADS, 1)
     }
     if (!ok && lane == 0) {
       *abort_flag = 1;
-      srv_report_timeout(p.s);
       // Let issued loads land before the CTA can exit.
       for (long j = kc > STAGES ? kc - STAGES : 0; j < kc; ++j)
         srv_wait(bar_k_full + 8 * (int)(j % STAGES), (uint32_t)((j / STAGES) & 1), nullptr, limit);
@@ -629,10 +628,7 @@ __global__ void __launch_bounds__(TileSmem<HD>::THREADS, 1)
       kvc += n_kv;
     }
     if (!ok) {
-      if (lane == 0) {
-        *abort_flag = 1;
-        srv_report_timeout(p.s);
-      }
+      if (lane == 0) *abort_flag = 1;
       if (issued) {
         mma_commit_warp(bar_drain + 8 * (warp - ISSUER));
         srv_wait(bar_drain + 8 * (warp - ISSUER), 0, nullptr, limit);
@@ -671,10 +667,7 @@ __global__ void __launch_bounds__(TileSmem<HD>::THREADS, 1)
         if (lane == 0) mbar_arrive(bar_v_ready + 8 * vs);
       }
     }
-    if (!ok && lane == 0) {
-      *abort_flag = 1;
-      srv_report_timeout(p.s);
-    }
+    if (!ok && lane == 0) *abort_flag = 1;
   } else if (warp < 4 * NT) {
     // ------------------------------------------------------------ softmax
     constexpr int KT = SM::KT;
@@ -918,14 +911,12 @@ __global__ void __launch_bounds__(TileSmem<HD>::THREADS, 1)
       tc_fence_before();
       arrive(bar_o_free + 8 * t);
     }
-    if (!ok) {
-      *abort_flag = 1;
-      srv_report_timeout(p.s);
-    }
+    if (!ok) *abort_flag = 1;
   }
 
   tc_fence_before();
   __syncthreads();
+  if (threadIdx.x == 0 && *abort_flag) srv_report_timeout(p.s);
   if (warp == ISSUER) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
