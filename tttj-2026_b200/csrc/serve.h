@@ -11,6 +11,9 @@ namespace tttj {
 
 constexpr int SRV_MAX_BATCH = 1024;  // sequences of a call (prefix sums in shared memory)
 constexpr int SRV_MAX_GROUP = 64;    // query heads per key / value head
+// How long a device wait may take.  A constant: as a field beside timeout_host it made the
+// parameters longer, and a short prompt's three launches 0.7 us slower.
+constexpr unsigned long long SRV_WAIT_LIMIT_NS = TTTJ_WAIT_LIMIT_NS;
 constexpr int SRV_DEV_BAD_PAGE = 0x401;   // a live page-table entry outside the cache
 constexpr int SRV_DEV_BAD_LENS = 0x402;   // lengths or offsets outside the call's tensors
 constexpr int SRV_DEV_TIMEOUT = 0x403;    // a bounded device wait gave up
@@ -29,7 +32,6 @@ struct SrvSeqs {
   int tokens;          // rows allocated in q / out
   int causal;
   int* status;         // device status word (nullable)
-  int* timeout_host;   // the device's pinned word (serve_capi.cu); null where nothing waits
 };
 
 struct SrvSeq {
@@ -83,7 +85,7 @@ struct StepParams {
   float scale_log2;
   float* part_o;       // [2 * grid][STEP_ROWS][head_dim] partial outputs
   float2* part_ml;     // [2 * grid][STEP_ROWS] their (max, sum)
-  unsigned long long wait_limit_ns;
+  int* timeout_host;   // the device's pinned word (serve_capi.cu)
 };
 constexpr int STEP_ROWS = 16;   // query rows of one mma tile
 constexpr int STEP_KEYS = 64;   // keys per pipeline stage
@@ -128,7 +130,7 @@ struct TileParams {
   TilePlan plan;
   float* part_o;       // [most_parts][NT * 128][head_dim]
   float2* part_ml;     // [most_parts][NT * 128]
-  unsigned long long wait_limit_ns;
+  int* timeout_host;   // the device's pinned word (serve_capi.cu)
 };
 constexpr int tile_nt(int hd) { return hd == 256 ? 1 : 2; }
 cudaError_t tile_launch(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v,
@@ -143,7 +145,7 @@ struct MassParams {
   long cap;
   int heads, kv_heads, group, tile_tokens;
   float scale_log2;
-  unsigned long long wait_limit_ns;
+  int* timeout_host;   // the device's pinned word (serve_capi.cu)
 };
 constexpr int MASS_TILE_ROWS = 80;  // query rows of a tile (MASS_ROWS)
 cudaError_t mass_launch(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const MassParams& p, int head_dim,
@@ -180,6 +182,6 @@ struct EvictParams {
 cudaError_t evict_launch(const EvictParams& p, int sms, cudaStream_t stream);
 
 // One bounded wait on a barrier that nothing arrives on, reported like any other.
-cudaError_t serve_selftest_launch(const SrvSeqs& s, unsigned long long limit_ns, cudaStream_t stream);
+cudaError_t serve_selftest_launch(int* status, int* timeout_host, unsigned long long limit_ns, cudaStream_t stream);
 
 }  // namespace tttj

@@ -389,17 +389,17 @@ __global__ void __launch_bounds__(EVICT_MAX_THREADS) evict_kernel(const EvictPar
 }
 
 // ---------------------------------------------------------------- failure detection
-__global__ void serve_selftest_kernel(const SrvSeqs s, unsigned long long limit_ns) {
+__global__ void serve_selftest_kernel(int* status, int* timeout_host, unsigned long long limit_ns) {
   __shared__ __align__(8) uint64_t bar;
   mbar_init(smem_u32(&bar), 1);
   fence_barrier_init();
-  if (!srv_wait(smem_u32(&bar), 0, nullptr, limit_ns)) srv_report_timeout(s);
+  if (!srv_wait(smem_u32(&bar), 0, nullptr, limit_ns)) srv_report_timeout(status, timeout_host);
 }
 
 }  // namespace
 
-cudaError_t serve_selftest_launch(const SrvSeqs& s, unsigned long long limit_ns, cudaStream_t stream) {
-  serve_selftest_kernel<<<1, 1, 0, stream>>>(s, limit_ns);
+cudaError_t serve_selftest_launch(int* status, int* timeout_host, unsigned long long limit_ns, cudaStream_t stream) {
+  serve_selftest_kernel<<<1, 1, 0, stream>>>(status, timeout_host, limit_ns);
   return cudaGetLastError();
 }
 

@@ -263,7 +263,6 @@ int attention(const char* what, const tttj_seqs* s, const tttj_rows* q, const Ca
     const ServeWs w = step_ws(s);
     StepParams p{};
     p.s = seqs_of(s, cache, causal);
-    p.s.timeout_host = timeout;
     p.q = q->data;
     p.q_tok = q->token_stride;
     p.q_head = q->head_stride;
@@ -277,14 +276,13 @@ int attention(const char* what, const tttj_seqs* s, const tttj_rows* q, const Ca
     p.scale_log2 = scale_log2;
     p.part_o = reinterpret_cast<float*>(base + w.part_o);
     p.part_ml = reinterpret_cast<float2*>(base + w.part_ml);
-    p.wait_limit_ns = TTTJ_WAIT_LIMIT_NS;
+    p.timeout_host = timeout;
     CAPI_CUDA(step_launch(tm_k, tm_v, p, s->head_dim, bf16, sms * step_ctas_per_sm(s->head_dim), stream));
     return TTTJ_OK;
   }
   const ServeWs w = tile_ws(s);
   TileParams p{};
   p.s = seqs_of(s, cache, causal);
-  p.s.timeout_host = timeout;
   p.q = q->data;
   p.q_tok = q->token_stride;
   p.q_head = q->head_stride;
@@ -309,7 +307,7 @@ int attention(const char* what, const tttj_seqs* s, const tttj_rows* q, const Ca
   p.plan.most_parts = w.most_parts;
   p.part_o = reinterpret_cast<float*>(base + w.part_o);
   p.part_ml = reinterpret_cast<float2*>(base + w.part_ml);
-  p.wait_limit_ns = TTTJ_WAIT_LIMIT_NS;
+  p.timeout_host = timeout;
   CUtensorMap tm_q;
   TRY(q_map(&tm_q, what, s, q, p.tile_tokens));
   CAPI_CUDA(tile_launch(tm_q, tm_k, tm_v, p, s->head_dim, bf16, sms, stream));
@@ -407,7 +405,6 @@ int tttj_cache_mass(const tttj_seqs* s, const tttj_rows* q, const float* lse, co
   TRY(device_here(what, &sms, &timeout));
   MassParams p{};
   p.s = seqs_of(s, true, 1);
-  p.s.timeout_host = timeout;
   p.lse = lse;
   p.mass = mass;
   p.out = mass_out;
@@ -420,7 +417,7 @@ int tttj_cache_mass(const tttj_seqs* s, const tttj_rows* q, const float* lse, co
   const int most = max_new > 0 && max_new < s->tokens ? max_new : s->tokens;
   if (most < p.tile_tokens) p.tile_tokens = most;
   p.scale_log2 = scale * 1.44269504088896341f;
-  p.wait_limit_ns = TTTJ_WAIT_LIMIT_NS;
+  p.timeout_host = timeout;
   CUtensorMap tm_q, tm_k;
   TRY(q_map(&tm_q, what, s, q, p.tile_tokens));
   TRY(kv_map(&tm_k, what, s, k_cache->data, k_cache->page_stride, k_cache->slot_stride, k_cache->head_stride,
@@ -443,12 +440,10 @@ int tttj_serve_status(int* device_status) {
 
 int tttj_serve_selftest_timeout(int32_t* status, uint64_t limit_ns, void* stream) {
   if (limit_ns > 1000000000ull) return capi_fail(TTTJ_ERR_INVALID, "serve_selftest: limit above 1 s");
-  int dev = 0;
-  SrvSeqs s{};
-  s.status = status;
+  int dev = 0, *word = nullptr;
   CAPI_CUDA(cudaGetDevice(&dev));
-  TRY(timeout_word(dev, &s.timeout_host));
-  CAPI_CUDA(serve_selftest_launch(s, limit_ns, static_cast<cudaStream_t>(stream)));
+  TRY(timeout_word(dev, &word));
+  CAPI_CUDA(serve_selftest_launch(status, word, limit_ns, static_cast<cudaStream_t>(stream)));
   return TTTJ_OK;
 }
 

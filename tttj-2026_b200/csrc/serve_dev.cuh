@@ -25,9 +25,9 @@ __device__ __forceinline__ bool srv_wait(uint32_t bar, uint32_t parity, volatile
 }
 
 // A wait gave up: the call's status word, and the word that the device's next call looks at.
-__device__ __forceinline__ void srv_report_timeout(const SrvSeqs& s) {
-  report_status(s.status, SRV_DEV_TIMEOUT);
-  if (s.timeout_host != nullptr) *reinterpret_cast<volatile int*>(s.timeout_host) = SRV_DEV_TIMEOUT;
+__device__ __forceinline__ void srv_report_timeout(int* status, int* timeout_host) {
+  report_status(status, SRV_DEV_TIMEOUT);
+  *reinterpret_cast<volatile int*>(timeout_host) = SRV_DEV_TIMEOUT;
 }
 
 template <bool BF16>

@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(MASS_THREADS, 1)
   int* s_pre = reinterpret_cast<int*>(s_seq + p.s.batch);    // [batch + 1] items of a head before each place
   int* s_order = s_pre + p.s.batch + 1;                       // [batch] sequence at each place
   const int warp = warp_id(), lane = lane_id();
-  const uint64_t limit = p.wait_limit_ns;
+  constexpr uint64_t limit = SRV_WAIT_LIMIT_NS;
   const int TOK = p.tile_tokens;
 
   if (threadIdx.x == 0) {
@@ -512,7 +512,7 @@ __global__ void __launch_bounds__(MASS_THREADS, 1)
 
   tc_fence_before();
   __syncthreads();
-  if (threadIdx.x == 0 && *abort_flag) srv_report_timeout(p.s);
+  if (threadIdx.x == 0 && *abort_flag) srv_report_timeout(p.s.status, p.timeout_host);
   if (warp == ISSUER) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);

@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(STEP_THREADS, step_ctas_per_sm(HD))
         const int c1 = slot & ((1 << p.s.page_shift) - 1);
         const int st = (int)(it % SM::STAGES);
         ok = srv_wait(bar_empty + 8 * st, (uint32_t)((it / SM::STAGES) & 1) ^ 1u, abort_flag,
-                       p.wait_limit_ns);
+                       SRV_WAIT_LIMIT_NS);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         const uint32_t bar = bar_full + 8 * st;
@@ -181,13 +181,13 @@ __global__ void __launch_bounds__(STEP_THREADS, step_ctas_per_sm(HD))
     }
     if (!ok && lane == 0) {
       *abort_flag = 1;
-      srv_report_timeout(p.s);
+      srv_report_timeout(p.s.status, p.timeout_host);
     }
     // Issued loads land before the CTA may exit.
     if (!ok)
       for (long j = it > SM::STAGES ? it - SM::STAGES : 0; j < it; ++j)
         srv_wait(bar_full + 8 * (int)(j % SM::STAGES), (uint32_t)((j / SM::STAGES) & 1), nullptr,
-                  p.wait_limit_ns);
+                  SRV_WAIT_LIMIT_NS);
     return;
   }
 
@@ -229,10 +229,10 @@ __global__ void __launch_bounds__(STEP_THREADS, step_ctas_per_sm(HD))
     for (int t = r.t0; ok && t < r.t1; ++t, ++it) {
       const int st = (int)(it % SM::STAGES);
       ok = __all_sync(0xffffffffu, srv_wait(bar_full + 8 * st, (uint32_t)((it / SM::STAGES) & 1), abort_flag,
-                                            p.wait_limit_ns));
+                                            SRV_WAIT_LIMIT_NS));
       if (!ok) {
         *abort_flag = 1;
-        if (lane == 0) srv_report_timeout(p.s);
+        if (lane == 0) srv_report_timeout(p.s.status, p.timeout_host);
         break;
       }
       const int k0 = t * STEP_KEYS + warp * 16;  // this warp's 16 keys

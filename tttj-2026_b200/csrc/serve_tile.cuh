@@ -332,7 +332,7 @@ __global__ void __launch_bounds__(TileSmem<HD>::THREADS, 1)
 
   const int warp = warp_id();
   const int lane = lane_id();
-  const uint64_t limit = p.wait_limit_ns;
+  constexpr uint64_t limit = SRV_WAIT_LIMIT_NS;
   const int TOK = p.tile_tokens;
   const bool paged = p.s.table != nullptr;
 
@@ -916,7 +916,7 @@ __global__ void __launch_bounds__(TileSmem<HD>::THREADS, 1)
 
   tc_fence_before();
   __syncthreads();
-  if (threadIdx.x == 0 && *abort_flag) srv_report_timeout(p.s);
+  if (threadIdx.x == 0 && *abort_flag) srv_report_timeout(p.s.status, p.timeout_host);
   if (warp == ISSUER) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
